@@ -54,6 +54,29 @@ class FfnBlockWeights(ctypes.Structure):
     ]
 
 
+class HeadRows(ctypes.Structure):
+    """gw_head_rows: heads of token rows inside a projection's output."""
+    _fields_ = [("input", c_void_p), ("input_stride", c_uint64), ("output", c_void_p), ("output_stride", c_uint64),
+                ("weight", c_void_p), ("heads", c_uint32), ("normalize", c_int)]
+
+
+class Rotary(ctypes.Structure):
+    """gw_rotary: rotation by position."""
+    _fields_ = [("inverse_frequencies", c_void_p), ("width", c_uint32), ("interleaved", c_int)]
+
+
+class KvCache(ctypes.Structure):
+    """gw_kv_cache: a paged cache of E4M3 keys and values with a scale for every page and head."""
+    _fields_ = [("k_data", c_void_p), ("v_data", c_void_p), ("k_scales", c_void_p), ("v_scales", c_void_p),
+                ("pages", c_uint32), ("kv_heads", c_uint32), ("page_tokens", c_uint32), ("head_dim", c_uint32)]
+
+
+class Sequences(ctypes.Structure):
+    """gw_sequences: rows, lengths and pages of a step's sequences."""
+    _fields_ = [("row_offsets", c_void_p), ("context_lengths", c_void_p), ("page_table", c_void_p),
+                ("page_table_stride", c_uint32), ("sequences", c_uint32), ("rows", c_uint32), ("max_rows", c_uint32)]
+
+
 class ExpertWeights(ctypes.Structure):
     """gw_expert_weights (mirrors sm120::ExpertWeights, moe.cuh:11-13)."""
     _fields_ = [("gate", Projection), ("up", Projection), ("down", Projection)]
@@ -187,6 +210,13 @@ _SIGNATURES = {
     "gw_moe_host_runner_streams": (c_int, [c_void_p, POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p)]),
     "gw_moe_host_runner_h2d_bytes": (c_uint64, [c_void_p]),
     "gw_moe_host_runner_d2h_bytes": (c_uint64, [c_void_p]),
+    "gw_qk_norm_rotary_bf16": (c_int, [POINTER(HeadRows), POINTER(HeadRows), c_uint32, c_uint32, c_void_p, POINTER(Rotary), c_float,
+                                       c_void_p]),
+    "gw_kv_cache_append": (c_int, [POINTER(KvCache), POINTER(Sequences), POINTER(HeadRows), POINTER(HeadRows), POINTER(HeadRows),
+                                   c_void_p, POINTER(Rotary), c_float, c_void_p]),
+    "gw_paged_attention_scratch_bytes": (c_size_t, [POINTER(KvCache), POINTER(Sequences), c_uint32]),
+    "gw_paged_attention_bf16": (c_int, [POINTER(KvCache), POINTER(Sequences), c_void_p, c_uint64, c_uint32, c_float, c_uint32,
+                                        c_void_p, c_uint64, c_void_p, c_size_t, c_void_p]),
     "gw_debug_kernel_error": (c_uint32, []),
     "gw_debug_launch_count": (c_uint64, []),
     "gw_debug_gemm_profile": (c_int, [c_void_p]),

@@ -135,7 +135,8 @@ uint32_t gw_debug_kernel_error(void) {
   if (value != 0) zero_now(word, sizeof(value));
   // the allocation-free linear reports into a word of its own (it may not use the allocated one)
   const uint32_t built_in = take_static_scratch_error();
-  return value != 0 ? value : built_in;
+  const uint32_t append = take_head_rows_error(), attention = take_paged_attention_error();
+  return value != 0 ? value : built_in != 0 ? built_in : append != 0 ? append : attention;
 }
 
 uint64_t gw_debug_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }

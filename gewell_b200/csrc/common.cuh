@@ -49,6 +49,9 @@ void note_launch(unsigned kernels = 1);
 // Error word of the allocation-free linear (static_scratch.cu) on the current GPU, cleared on read;
 // 0 when that entry point has not run on this GPU.
 uint32_t take_static_scratch_error();
+// The same of the cache append (head_rows.cu) and of the attention over it (paged_attention.cu), which take no set-up call.
+uint32_t take_head_rows_error();
+uint32_t take_paged_attention_error();
 
 constexpr size_t scale_storage_bytes(size_t rows, size_t width) {
   return ((rows + 127) / 128) * ((width + 63) / 64) * 512;

@@ -1,0 +1,630 @@
+// Heads of queries, keys and values between the Q | K | V projection and attention: RMS norm of every head, rotation by
+// position, and keys and values rounded to E4M3 into the pages of a cache.
+//
+// A head is D values.  LPH lanes of a warp take one (D = 128: two heads a warp); a lane has 4 V values from the head's first
+// half and the 4 V values that lie half a head behind them, so that with a half-split rotation of the whole head both
+// elements of a pair, and with neighbouring pairs too, are in one lane's registers.  A half-split rotation of a part of the
+// head fetches its partners through shared memory.
+//
+//   y_i = n_i cos a - n_j sin a,  y_j = n_j cos a + n_i sin a,  a = position * f,  n = x * rsqrt(mean(x^2) + eps) * w
+//
+// The angle in turns, position * (f / 2 pi), is formed and reduced to [-1/2, 1/2] in 64 bits: in 32 bits position 250000 at
+// f = 1 would be off by 0.01 rad.  What is left goes to the hardware's sine and cosine (absolute error 2^-21, against BF16's
+// 2^-9 and E4M3's 2^-4 at the end); everything else is FP32 and is rounded once.
+#include <algorithm>
+#include <string>
+
+#include "common.cuh"
+#include "paged.h"
+
+using namespace gw;
+
+namespace {
+
+__device__ uint32_t g_head_rows_error;       // first report since it was last taken
+
+__device__ __forceinline__ void report(uint32_t code) { atomicCAS(&g_head_rows_error, 0u, code); }
+
+enum Rotation { kNone, kWhole, kNeighbours, kPart };
+
+struct Rotary {
+  const float* frequencies;
+  uint32_t width;
+  int kind;
+};
+
+struct Heads {
+  const bf16* input;
+  uint64_t input_stride;
+  bf16* output;
+  uint64_t output_stride;
+  const bf16* weight;
+  uint32_t heads;
+  int normalize;
+};
+
+// 4 V neighbouring BF16 values
+template <int V>
+struct Raw {
+  uint2 bits[V];
+  __device__ __forceinline__ void load(const bf16* p) {
+    if constexpr (V == 1) {
+      bits[0] = *reinterpret_cast<const uint2*>(p);
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      bits[0] = make_uint2(v.x, v.y);
+      bits[1] = make_uint2(v.z, v.w);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int j = 0; j < V; ++j) bits[j] = make_uint2(0, 0);
+  }
+  __device__ __forceinline__ void unpack(float* f) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      f[4 * j] = __uint_as_float(bits[j].x << 16);
+      f[4 * j + 1] = __uint_as_float(bits[j].x & 0xffff0000u);
+      f[4 * j + 2] = __uint_as_float(bits[j].y << 16);
+      f[4 * j + 3] = __uint_as_float(bits[j].y & 0xffff0000u);
+    }
+  }
+};
+
+// A lane's share of the rotation: turns per position of its pairs.
+template <int V>
+struct Turns {
+  static constexpr int E = 4 * V;
+  double per_position[E];
+  __device__ __forceinline__ void load(const Rotary& r, uint32_t lane_at, uint32_t half, bool active) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      // kWhole: pair (at + e, at + e + half).  kNeighbours: E / 2 pairs of the first half, then E / 2 of the second.
+      const uint32_t pair = r.kind == kWhole ? lane_at + e : e < E / 2 ? lane_at / 2 + e : (half + lane_at) / 2 + (e - E / 2);
+      const bool used = active && r.kind != kNone && r.kind != kPart && 2 * pair < r.width;
+      per_position[e] = used ? double(r.frequencies[pair]) * 0.15915494309189535 : 0.0;     // 1 / 2 pi
+    }
+  }
+};
+
+__device__ __forceinline__ void sine_cosine(double turns, float& s, float& c) {
+  const float angle = float(turns - rint(turns)) * 6.283185307179586F;
+  __sincosf(angle, &s, &c);
+}
+
+template <int V>
+__device__ __forceinline__ void angles(const Turns<V>& t, int position, float* s, float* c) {
+#pragma unroll
+  for (int e = 0; e < 4 * V; ++e) sine_cosine(t.per_position[e] * double(position), s[e], c[e]);
+}
+
+__device__ __forceinline__ void turn(float& a, float& b, float s, float c) {
+  const float x = a;
+  a = fmaf(-b, s, x * c);
+  b = fmaf(x, s, b * c);
+}
+
+// lo / hi: a lane's values of the head's halves, in place.  `stage`: half-split rotation of a part goes through 2 * half
+// floats of shared memory that belong to these LPH lanes.
+template <int V>
+__device__ __forceinline__ void rotate(const Rotary& r, float* lo, float* hi, const float* s, const float* c, int position, uint32_t at,
+                                       uint32_t half, bool active, float* stage) {
+  constexpr int E = 4 * V;
+  if (r.kind == kWhole) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) turn(lo[e], hi[e], s[e], c[e]);
+  } else if (r.kind == kNeighbours) {
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) {
+      turn(lo[2 * e], lo[2 * e + 1], s[e], c[e]);
+      turn(hi[2 * e], hi[2 * e + 1], s[E / 2 + e], c[E / 2 + e]);
+    }
+  } else if (r.kind == kPart) {
+    __syncwarp();
+    if (active) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        stage[at + e] = lo[e];
+        stage[half + at + e] = hi[e];
+      }
+    }
+    __syncwarp();
+    if (active) {
+      const uint32_t pairs = r.width / 2;
+#pragma unroll
+      for (int e = 0; e < 2 * E; ++e) {
+        const uint32_t i = e < E ? at + e : half + at + (e - E);
+        if (i >= r.width) continue;
+        float& mine = e < E ? lo[e] : hi[e - E];
+        const bool first = i < pairs;
+        const uint32_t pair = first ? i : i - pairs;
+        const float other = stage[first ? i + pairs : pair];
+        float sine, cosine;
+        sine_cosine(double(r.frequencies[pair]) * 0.15915494309189535 * double(position), sine, cosine);
+        mine = first ? fmaf(-other, sine, mine * cosine) : fmaf(other, sine, mine * cosine);
+      }
+    }
+  }
+}
+
+template <int LPH, int E>
+__device__ __forceinline__ float inverse_rms(const float* lo, const float* hi, float inverse_width, float epsilon) {
+  float sum = 0.F;
+#pragma unroll
+  for (int e = 0; e < E; ++e) sum = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], sum));
+#pragma unroll
+  for (int m = LPH / 2; m; m /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+  return rsqrtf(fmaf(sum, inverse_width, epsilon));
+}
+
+// ---------------------------------------------------------------------------
+// queries and keys, BF16 to BF16
+// ---------------------------------------------------------------------------
+struct NormRotary {
+  Heads query, key;                    // key.heads == 0: none
+  uint32_t rows, width, per_task;      // heads that a task takes
+  uint32_t query_tasks, tasks;         // of a row
+  const int32_t* positions;            // or NULL: those of the batch
+  gw_sequences batch;
+  Rotary rotary;
+  float epsilon;
+};
+
+// Position of a row in its sequence; false: no sequence has it.
+__device__ __forceinline__ bool position_in_batch(const gw_sequences& b, uint32_t row, int& position) {
+  uint32_t low = 0, high = b.sequences;                    // the last sequence that starts at or before the row
+  while (low + 1 < high) {
+    const uint32_t middle = (low + high) / 2;
+    if (b.row_offsets[middle] <= int(row)) low = middle; else high = middle;
+  }
+  const SequenceRows s = sequence_rows(b, low);
+  position = s.context - s.count + int(row) - s.first;
+  return int(row) >= s.first && int(row) < s.first + s.count;
+}
+
+constexpr int kNormWarps = 4;
+
+template <int LPH, int V>
+__global__ void __launch_bounds__(32 * kNormWarps) qk_norm_rotary_kernel(NormRotary a) {
+  constexpr int E = 4 * V, kSide = 32 / LPH;
+  __shared__ float stage[kNormWarps][kSide * LPH * 2 * E];
+  griddep_enter();
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, group = lane / LPH, at = lane % LPH * E, half = a.width / 2;
+  const uint32_t task = blockIdx.x * kNormWarps + warp;
+  const uint32_t row = task / a.tasks, part = task % a.tasks;
+  if (row >= a.rows) return;
+  const bool is_key = part >= a.query_tasks;
+  const Heads& h = is_key ? a.key : a.query;
+  const uint32_t first = (is_key ? part - a.query_tasks : part) * a.per_task, last = min(first + a.per_task, h.heads);
+  int position = 0;
+  if (a.positions != nullptr) position = a.positions[row];
+  else if (a.batch.sequences && !position_in_batch(a.batch, row, position)) return;
+  const bool inside = at < half;
+  float s[E], c[E], weight_lo[E], weight_hi[E];
+  {
+    Turns<V> turns;
+    turns.load(a.rotary, at, half, inside);
+    angles(turns, position, s, c);
+  }
+  const bool weighted = h.weight != nullptr;
+#pragma unroll
+  for (int e = 0; e < E; ++e) weight_lo[e] = weight_hi[e] = 1.F;
+  if (weighted && inside) {
+    Raw<V> raw;
+    raw.load(h.weight + at);
+    raw.unpack(weight_lo);
+    raw.load(h.weight + half + at);
+    raw.unpack(weight_hi);
+  }
+  const float inverse_width = 1.F / float(a.width);
+  for (uint32_t head = first; head < last; head += kSide) {
+    const bool active = inside && head + group < last;
+    const size_t place = size_t(head + group) * a.width + at;
+    float lo[E], hi[E];
+    Raw<V> raw_lo, raw_hi;
+    raw_lo.clear();
+    raw_hi.clear();
+    if (active) {
+      const bf16* from = h.input + size_t(row) * h.input_stride + place;
+      raw_lo.load(from);
+      raw_hi.load(from + half);
+    }
+    raw_lo.unpack(lo);
+    raw_hi.unpack(hi);
+    const float inverse = h.normalize ? inverse_rms<LPH, E>(lo, hi, inverse_width, a.epsilon) : 1.F;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      lo[e] = lo[e] * inverse * weight_lo[e];
+      hi[e] = hi[e] * inverse * weight_hi[e];
+    }
+    rotate<V>(a.rotary, lo, hi, s, c, position, at, half, active, stage[warp] + group * LPH * 2 * E);
+    if (active) {
+      uint32_t out_lo[2 * V], out_hi[2 * V];
+#pragma unroll
+      for (int e = 0; e < 2 * V; ++e) {
+        const __nv_bfloat162 l = __floats2bfloat162_rn(lo[2 * e], lo[2 * e + 1]), u = __floats2bfloat162_rn(hi[2 * e], hi[2 * e + 1]);
+        out_lo[e] = *reinterpret_cast<const uint32_t*>(&l);
+        out_hi[e] = *reinterpret_cast<const uint32_t*>(&u);
+      }
+      bf16* to = h.output + size_t(row) * h.output_stride + place;
+      if constexpr (V == 1) {
+        *reinterpret_cast<uint2*>(to) = make_uint2(out_lo[0], out_lo[1]);
+        *reinterpret_cast<uint2*>(to + half) = make_uint2(out_hi[0], out_hi[1]);
+      } else {
+        *reinterpret_cast<uint4*>(to) = make_uint4(out_lo[0], out_lo[1], out_lo[2], out_lo[3]);
+        *reinterpret_cast<uint4*>(to + half) = make_uint4(out_hi[0], out_hi[1], out_hi[2], out_hi[3]);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// keys and values into pages
+// ---------------------------------------------------------------------------
+struct Append {
+  gw_kv_cache cache;
+  gw_sequences batch;
+  Heads key, value;
+  const int32_t* positions;
+  Rotary rotary;
+  float epsilon;
+};
+
+// What the call brings to one page of one sequence.
+struct Segment {
+  int row, count, slot, position;      // first row, rows, slot and position of the first
+  int page;                            // -1: nothing to do
+};
+
+__device__ __forceinline__ uint32_t segments_of(const SequenceRows& s, uint32_t page_tokens) {
+  const int first = max(0, s.context - s.count);
+  return s.count == 0 || s.context <= first ? 0 : uint32_t(s.context - 1) / page_tokens - uint32_t(first) / page_tokens + 1;
+}
+
+__device__ __forceinline__ Segment segment_at(const Append& a, uint32_t sequence, const SequenceRows& s, uint32_t which) {
+  const uint32_t page_tokens = a.cache.page_tokens;
+  const int begin = s.context - s.count, first = max(0, begin);
+  const uint32_t ordinal = uint32_t(first) / page_tokens + which;
+  const int low = max(first, int(ordinal * page_tokens)), high = min(int64_t(s.context), int64_t(ordinal + 1) * page_tokens);
+  Segment g{s.first + low - begin, high - low, int(uint32_t(low) % page_tokens), low, -1};
+  if (ordinal < a.batch.page_table_stride) {
+    const int page = a.batch.page_table[size_t(sequence) * a.batch.page_table_stride + ordinal];
+    if (page >= 0 && uint32_t(page) < a.cache.pages) g.page = page;
+  }
+  if (g.page < 0) report(0xa1000000u | (sequence & 0xffffffu));
+  return g;
+}
+
+// The block's segment: number blockIdx.x over all sequences, found by a scan over their counts.
+template <int THREADS>
+__device__ __forceinline__ Segment find_segment(const Append& a) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ uint32_t totals[WARPS];
+  __shared__ Segment found;
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, wanted = blockIdx.x;
+  if (threadIdx.x == 0) found.page = -1;
+  uint32_t before = 0;
+  for (uint32_t base = 0; base < a.batch.sequences; base += THREADS) {
+    const uint32_t s = base + threadIdx.x;
+    SequenceRows rows{0, 0, 0, false};
+    if (s < a.batch.sequences) {
+      rows = sequence_rows(a.batch, s);
+      if (rows.bad && blockIdx.x == 0) report(0xa2000000u | (s & 0xffffffu));
+    }
+    const uint32_t mine = segments_of(rows, a.cache.page_tokens);
+    uint32_t sum = mine;
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) {
+      const uint32_t other = __shfl_up_sync(0xffffffffu, sum, m);
+      if (lane >= uint32_t(m)) sum += other;
+    }
+    if (lane == 31) totals[warp] = sum;
+    __syncthreads();
+    uint32_t low = before + sum - mine, all = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (uint32_t(w) < warp) low += totals[w];
+      all += totals[w];
+    }
+    if (wanted >= low && wanted - low < mine) found = segment_at(a, s, rows, wanted - low);
+    before += all;
+    __syncthreads();
+    if (wanted < before) break;
+  }
+  return found;
+}
+
+// Smallest power of two, 2^-64 or more, with which `loudest` (finite) fits: 448 = 1.75 * 2^8 is the largest code.
+__device__ __forceinline__ float page_scale(float loudest) {
+  const uint32_t bits = __float_as_uint(loudest), fraction = bits & 0x7fffffu;
+  const int exponent = int(bits >> 23) - 8 + (fraction > 0x600000u);
+  return __uint_as_float(uint32_t(max(exponent, 127 - 64)) << 23);
+}
+
+__device__ __forceinline__ float finite_size(float v) {
+  const float size = fabsf(v);
+  return size <= 3.4028234e38F ? size : 0.F;         // not of infinities and NaN
+}
+
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  return uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3)) |
+         uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16;
+}
+
+__device__ __forceinline__ uint32_t softer(uint32_t codes, float ratio) {
+  uint32_t out = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const __half2 pair(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(codes >> (8 * i)), __NV_E4M3));
+    const float2 f = __half22float2(pair);
+    out |= uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(f.x * ratio, f.y * ratio), __NV_SATFINITE, __NV_E4M3)) << (8 * i);
+  }
+  return out;
+}
+
+// One block: the call's tokens of one page, one KV head, keys or values.  W warps take tokens in T rounds; a token's raw values
+// stay in registers between the search for the loudest element and the rounding, which norms and rotates again (T > 1).
+template <int LPH, int V, int W, int T>
+__global__ void __launch_bounds__(32 * W) kv_append_kernel(Append a) {
+  constexpr int E = 4 * V, kSide = 32 / LPH;
+  __shared__ float stage[W][kSide * LPH * 2 * E];
+  __shared__ float loudest_of[W];
+  griddep_enter();
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, group = lane / LPH, at = lane % LPH * E;
+  const uint32_t width = LPH * 2 * E, half = width / 2;
+  const uint32_t head = blockIdx.y % a.cache.kv_heads;
+  const bool is_key = blockIdx.y < a.cache.kv_heads;
+  Segment g;
+  if constexpr (W == 1) {                                  // one row a sequence
+    const SequenceRows s = sequence_rows(a.batch, blockIdx.x);
+    if (s.bad && threadIdx.x == 0) report(0xa2000000u | (blockIdx.x & 0xffffffu));
+    if (segments_of(s, a.cache.page_tokens) == 0) return;
+    g = segment_at(a, blockIdx.x, s, 0);
+  } else {
+    g = find_segment<32 * W>(a);
+  }
+  if (g.page < 0) return;
+  const Heads& h = is_key ? a.key : a.value;
+  Rotary rotary = a.rotary;
+  if (!is_key) rotary.kind = kNone;
+
+  Raw<V> raw_lo[T], raw_hi[T];
+  int position[T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    const int token = (t * W + warp) * kSide + group;
+    position[t] = 0;
+    raw_lo[t].clear();
+    raw_hi[t].clear();
+    if (token < g.count) {
+      const bf16* from = h.input + size_t(g.row + token) * h.input_stride + size_t(head) * width + at;
+      raw_lo[t].load(from);
+      raw_hi[t].load(from + half);
+      position[t] = a.positions != nullptr ? a.positions[g.row + token] : g.position + token;
+    }
+  }
+  float weight_lo[E], weight_hi[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) weight_lo[e] = weight_hi[e] = 1.F;
+  if (h.weight != nullptr) {
+    Raw<V> raw;
+    raw.load(h.weight + at);
+    raw.unpack(weight_lo);
+    raw.load(h.weight + half + at);
+    raw.unpack(weight_hi);
+  }
+  Turns<V> turns;
+  turns.load(rotary, at, half, true);
+
+  const auto finished = [&](int t, float* lo, float* hi) {
+    raw_lo[t].unpack(lo);
+    raw_hi[t].unpack(hi);
+    const float inverse = h.normalize ? inverse_rms<LPH, E>(lo, hi, 1.F / float(width), a.epsilon) : 1.F;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      lo[e] = lo[e] * inverse * weight_lo[e];
+      hi[e] = hi[e] * inverse * weight_hi[e];
+    }
+    if (rotary.kind != kNone) {
+      float s[E], c[E];
+      if (rotary.kind != kPart) angles(turns, position[t], s, c);
+      rotate<V>(rotary, lo, hi, s, c, position[t], at, half, true, stage[warp] + group * LPH * 2 * E);
+    }
+  };
+
+  float loudest = 0.F, lo[E], hi[E];
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    if ((t * W + warp) * kSide >= uint32_t(g.count)) break;          // the same for the whole warp
+    finished(t, lo, hi);
+    if ((t * W + warp) * kSide + group < uint32_t(g.count))
+#pragma unroll
+      for (int e = 0; e < E; ++e) loudest = fmaxf(loudest, fmaxf(finite_size(lo[e]), finite_size(hi[e])));
+  }
+#pragma unroll
+  for (int m = 16; m; m /= 2) loudest = fmaxf(loudest, __shfl_xor_sync(0xffffffffu, loudest, m));
+  float* scale_at = (is_key ? a.cache.k_scales : a.cache.v_scales) + size_t(g.page) * a.cache.kv_heads + head;
+  float old = g.slot > 0 ? *scale_at : 0.F;
+  if (!(old > 0.F && old <= 3.4028234e38F)) old = 0.F;
+  if constexpr (W > 1) {
+    if (lane == 0) loudest_of[warp] = loudest;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) loudest = fmaxf(loudest, loudest_of[w]);
+  } else {
+    __syncwarp();
+  }
+  const float scale = fmaxf(old, page_scale(loudest)), inverse_scale = __frcp_rn(scale);
+  if (threadIdx.x == 0) *scale_at = scale;
+
+  uint8_t* page = static_cast<uint8_t*>(is_key ? a.cache.k_data : a.cache.v_data) +
+                  (size_t(g.page) * a.cache.kv_heads + head) * a.cache.page_tokens * width;
+  if (g.slot > 0 && scale > old) {                         // a louder token than the page had
+    const float ratio = old * inverse_scale;
+    uint4* codes = reinterpret_cast<uint4*>(page);
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < uint32_t(g.slot) * width / 16; i += 32 * W) {
+      uint4 v = codes[i];
+      v = make_uint4(softer(v.x, ratio), softer(v.y, ratio), softer(v.z, ratio), softer(v.w, ratio));
+      codes[i] = v;
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    if ((t * W + warp) * kSide >= uint32_t(g.count)) break;
+    if (T > 1) finished(t, lo, hi);
+    const uint32_t token = (t * W + warp) * kSide + group;
+    if (token >= uint32_t(g.count)) continue;
+    uint8_t* to = page + size_t(g.slot + token) * width + at;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      lo[e] *= inverse_scale;
+      hi[e] *= inverse_scale;
+    }
+    if constexpr (V == 1) {
+      *reinterpret_cast<uint32_t*>(to) = e4m3x4(lo[0], lo[1], lo[2], lo[3]);
+      *reinterpret_cast<uint32_t*>(to + half) = e4m3x4(hi[0], hi[1], hi[2], hi[3]);
+    } else {
+      *reinterpret_cast<uint2*>(to) = make_uint2(e4m3x4(lo[0], lo[1], lo[2], lo[3]), e4m3x4(lo[4], lo[5], lo[6], lo[7]));
+      *reinterpret_cast<uint2*>(to + half) = make_uint2(e4m3x4(hi[0], hi[1], hi[2], hi[3]), e4m3x4(hi[4], hi[5], hi[6], hi[7]));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+gw_status check_heads(const gw_head_rows* h, bool has_output, uint32_t width, const std::string& what) {
+  if (!h || !h->input || h->heads == 0 || h->heads > 1024 || !is_aligned16(h->input) || (h->weight && !is_aligned16(h->weight)))
+    return fail(GW_INVALID_ARGUMENT, what + " requires 1 to 1024 heads, 16-byte aligned inputs and weights");
+  if (h->input_stride % 8 != 0 || h->input_stride < uint64_t(h->heads) * width)
+    return fail(GW_INVALID_ARGUMENT, what + " requires row strides divisible by 8 that hold all heads");
+  if (has_output && (!h->output || !is_aligned16(h->output) || h->output_stride % 8 != 0 || h->output_stride < uint64_t(h->heads) * width ||
+                     (h->output == h->input && h->output_stride != h->input_stride)))
+    return fail(GW_INVALID_ARGUMENT, what + " requires a 16-byte aligned output with a row stride divisible by 8 (in place: the input's)");
+  return GW_OK;
+}
+
+gw_status check_rotary(const gw_rotary* r, uint32_t width, const std::string& what, Rotary* rotary) {
+  *rotary = Rotary{nullptr, 0, kNone};
+  if (!r || r->width == 0) return GW_OK;
+  if (!r->inverse_frequencies || r->width % 2 != 0 || r->width > width)
+    return fail(GW_INVALID_ARGUMENT, what + " requires inverse frequencies and an even rotated width within the head");
+  *rotary = Rotary{r->inverse_frequencies, r->width, r->interleaved ? kNeighbours : r->width == width ? kWhole : kPart};
+  return GW_OK;
+}
+
+Heads heads_of(const gw_head_rows& h) {
+  return Heads{static_cast<const bf16*>(h.input), h.input_stride, static_cast<bf16*>(h.output), h.output_stride,
+               static_cast<const bf16*>(h.weight), h.heads, h.normalize};
+}
+
+cudaError_t launch_norm_rotary(NormRotary a, cudaStream_t stream) {
+  const int lanes = a.width <= 64 ? 8 : a.width <= 128 ? 16 : 32;
+  a.per_task = 32 / lanes;
+  a.query_tasks = (a.query.heads + a.per_task - 1) / a.per_task;
+  a.tasks = a.query_tasks + (a.key.heads + a.per_task - 1) / a.per_task;
+  const uint64_t tasks = uint64_t(a.rows) * a.tasks;
+  if (tasks > 0xffffffffull - 64) return cudaErrorInvalidValue;
+  const auto kernel = a.width <= 64    ? qk_norm_rotary_kernel<8, 1>
+                      : a.width <= 128 ? qk_norm_rotary_kernel<16, 1>
+                      : a.width <= 256 ? qk_norm_rotary_kernel<32, 1>
+                                       : qk_norm_rotary_kernel<32, 2>;
+  return launch_pdl(kernel, uint32_t((tasks + kNormWarps - 1) / kNormWarps), 32 * kNormWarps, stream, a);
+}
+
+template <int LPH, int V>
+cudaError_t launch_append(const Append& a, cudaStream_t stream) {
+  const uint32_t page = a.cache.page_tokens, most = std::min(page, a.batch.max_rows), sequences = a.batch.sequences;
+  constexpr uint32_t kSide = 32 / LPH;
+  const dim3 heads(1, 2 * a.cache.kv_heads);
+  if (a.batch.max_rows == 1) return launch_pdl(kv_append_kernel<LPH, V, 1, 1>, dim3(sequences, heads.y), 32, stream, a);
+  // a sequence of n rows touches at most 1 + (n + page - 2) / page pages
+  const uint64_t bound = std::min(uint64_t(sequences) * (1 + (a.batch.max_rows + page - 2) / page),
+                                  sequences + (uint64_t(a.batch.rows) + uint64_t(sequences) * (page - 2)) / page);
+  const dim3 grid(uint32_t(bound), heads.y);
+  if (most <= 4 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 4, 1>, grid, 128, stream, a);
+  if (most <= 16 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 16, 1>, grid, 512, stream, a);
+  if (most <= 32 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 16, 2>, grid, 512, stream, a);
+  if (most <= 64 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 16, 4>, grid, 512, stream, a);
+  return launch_pdl(kv_append_kernel<LPH, V, 16, 8>, grid, 512, stream, a);
+}
+
+}  // namespace
+
+uint32_t gw::take_head_rows_error() {
+  uint32_t value = 0;
+  if (cudaMemcpyFromSymbol(&value, g_head_rows_error, sizeof(value)) != cudaSuccess) return 0xFFFFFFFDu;
+  const uint32_t none = 0;
+  if (value != 0 && cudaMemcpyToSymbol(g_head_rows_error, &none, sizeof(none)) != cudaSuccess) return 0xFFFFFFFDu;
+  return value;
+}
+
+extern "C" {
+
+gw_status gw_qk_norm_rotary_bf16(const gw_head_rows* query, const gw_head_rows* key, uint32_t rows, uint32_t head_dim,
+                                 const int32_t* positions, const gw_rotary* rotary, float epsilon, void* stream) {
+  clear_error();
+  if (rows == 0) return GW_OK;
+  const std::string what = "norm and rotation of queries and keys";
+  if (head_dim == 0 || head_dim > 512 || head_dim % (head_dim <= 256 ? 8 : 16) != 0 || rows > (1u << 24))
+    return fail(GW_INVALID_ARGUMENT, what + " requires a head width divisible by 8 (beyond 256: by 16) of at most 512 and at most 2^24 rows");
+  NormRotary a{};
+  if (gw_status s = check_heads(query, true, head_dim, what); s != GW_OK) return s;
+  a.query = heads_of(*query);
+  if (key) {
+    if (gw_status s = check_heads(key, true, head_dim, what); s != GW_OK) return s;
+    a.key = heads_of(*key);
+  }
+  if (gw_status s = check_rotary(rotary, head_dim, what, &a.rotary); s != GW_OK) return s;
+  if (a.rotary.kind != kNone && !positions) return fail(GW_INVALID_ARGUMENT, what + " requires positions");
+  if (!(epsilon >= 0.F)) return fail(GW_INVALID_ARGUMENT, what + " requires an epsilon of 0 or more");
+  a.rows = rows;
+  a.width = head_dim;
+  a.positions = positions;
+  a.epsilon = epsilon;
+  GW_CUDA_CHECK(launch_norm_rotary(a, as_stream(stream)), what);
+  return GW_OK;
+}
+
+gw_status gw_kv_cache_append(const gw_kv_cache* cache, const gw_sequences* batch, const gw_head_rows* key,
+                             const gw_head_rows* value, const gw_head_rows* query, const int32_t* positions,
+                             const gw_rotary* rotary, float epsilon, void* stream) {
+  clear_error();
+  const std::string what = "cache append";
+  if (gw_status s = check_cache(cache, "cache append"); s != GW_OK) return s;
+  if (gw_status s = check_batch(batch, "cache append"); s != GW_OK) return s;
+  if (batch->rows == 0 || batch->sequences == 0) return GW_OK;
+  const uint32_t width = cache->head_dim;
+  if (gw_status s = check_heads(key, false, width, what); s != GW_OK) return s;
+  if (gw_status s = check_heads(value, false, width, what); s != GW_OK) return s;
+  if (key->heads != cache->kv_heads || value->heads != cache->kv_heads)
+    return fail(GW_INVALID_ARGUMENT, what + " requires keys and values of the cache's heads");
+  Append a{};
+  if (gw_status s = check_rotary(rotary, width, what, &a.rotary); s != GW_OK) return s;
+  if (!(epsilon >= 0.F)) return fail(GW_INVALID_ARGUMENT, what + " requires an epsilon of 0 or more");
+  NormRotary q{};
+  if (query) {
+    if (gw_status s = check_heads(query, true, width, what); s != GW_OK) return s;
+    q.query = heads_of(*query);
+    q.rows = batch->rows;
+    q.width = width;
+    q.positions = positions;
+    q.batch = *batch;
+    q.rotary = a.rotary;
+    q.epsilon = epsilon;
+  }
+  a.cache = *cache;
+  a.batch = *batch;
+  a.key = heads_of(*key);
+  a.value = heads_of(*value);
+  a.positions = positions;
+  a.epsilon = epsilon;
+  const cudaStream_t s = as_stream(stream);
+  if (query) GW_CUDA_CHECK(launch_norm_rotary(q, s), "cache append (queries)");
+  const auto launch = width == 128 ? &launch_append<16, 1> : width == 256 ? &launch_append<32, 1> : &launch_append<32, 2>;
+  GW_CUDA_CHECK(launch(a, s), what);
+  return GW_OK;
+}
+
+}  // extern "C"

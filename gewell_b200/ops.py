@@ -718,6 +718,142 @@ class FfnBlock:
             self._block = None
 
 
+# --------------------------------------------------------------------------- attention between the projections
+
+def _on_current(device):
+    """The launches go to the current device, so the tensors have to lie there."""
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise _lib.GewellInvalidArgument(f"tensors on {device}: the current CUDA device's are wanted")
+    return device
+
+
+class KvCache:
+    """A paged cache of keys and values in 8 bits over the caller's tensors: E4M3 codes [pages, kv_heads, page_tokens,
+    head_dim] (torch.uint8 or torch.float8_e4m3fn) and FP32 scales [pages, kv_heads], contiguous."""
+
+    def __init__(self, k_data: torch.Tensor, v_data: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor):
+        for name, data, scales in (("keys", k_data, k_scales), ("values", v_data, v_scales)):
+            if data.dim() != 4 or data.dtype not in (torch.uint8, torch.float8_e4m3fn) or not data.is_contiguous():
+                raise _lib.GewellInvalidArgument(f"{name}: contiguous E4M3 codes [pages, kv_heads, page_tokens, head_dim] are wanted")
+            if scales.dtype != torch.float32 or scales.shape != data.shape[:2] or not scales.is_contiguous():
+                raise _lib.GewellInvalidArgument(f"{name}: contiguous FP32 scales [pages, kv_heads] are wanted")
+            if data.shape != k_data.shape or data.device != k_data.device or scales.device != k_data.device:
+                raise _lib.GewellInvalidArgument("keys and values have one shape and lie on one device")
+        self.k_data, self.v_data, self.k_scales, self.v_scales = k_data, v_data, k_scales, v_scales
+        self.pages, self.kv_heads, self.page_tokens, self.head_dim = k_data.shape
+        self.device = k_data.device
+        self._struct = _lib.KvCache(_ptr(k_data), _ptr(v_data), _ptr(k_scales), _ptr(v_scales), *k_data.shape)
+        self._ref = ctypes.byref(self._struct)
+
+
+class SequenceBatch:
+    """The sequences of a step: int32 tensors row_offsets [sequences + 1], context_lengths [sequences] (with the step's own rows)
+    and page_table [sequences, entries]; `rows` token rows in the step's arrays, at most `max_rows` of one sequence."""
+
+    def __init__(self, row_offsets: torch.Tensor, context_lengths: torch.Tensor, page_table: torch.Tensor, rows: int, max_rows: int):
+        for name, t, dim in (("row_offsets", row_offsets, 1), ("context_lengths", context_lengths, 1), ("page_table", page_table, 2)):
+            if t.dtype != torch.int32 or t.dim() != dim or t.stride(-1) != 1 or t.device != row_offsets.device:
+                raise _lib.GewellInvalidArgument(f"{name}: int32 with neighbouring elements, all three on one device")
+        count = context_lengths.shape[0]
+        if row_offsets.shape[0] != count + 1 or page_table.shape[0] != count or page_table.stride(0) < page_table.shape[1]:
+            raise _lib.GewellInvalidArgument("row_offsets has one entry more than there are sequences, page_table a row for each")
+        self.row_offsets, self.context_lengths, self.page_table = row_offsets, context_lengths, page_table
+        self.rows, self.max_rows, self.device = rows, max_rows, row_offsets.device
+        stride = page_table.stride(0) if count > 1 else max(1, page_table.shape[1])
+        self._struct = _lib.Sequences(_ptr(row_offsets), _ptr(context_lengths), _ptr(page_table), stride, count, rows, max_rows)
+        self._ref = ctypes.byref(self._struct)
+
+
+def _head_rows(x: torch.Tensor, weight, normalize: bool, y=None, rows=None):
+    """gw_head_rows of x [rows, heads, head_dim]."""
+    for t in (x,) if y is None else (x, y):
+        if t.dim() != 3 or t.dtype != torch.bfloat16 or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+            raise _lib.GewellInvalidArgument("heads are BF16 [rows, heads, head_dim], a row's heads side by side")
+    if y is not None and (y.shape != x.shape or y.device != x.device):
+        raise _lib.GewellInvalidArgument("the output has its input's shape and device")
+    if rows is not None and x.shape[0] < rows:
+        raise _lib.GewellInvalidArgument(f"{x.shape[0]} rows of heads for {rows} token rows")
+    if weight is not None and (weight.dtype != torch.bfloat16 or weight.shape != x.shape[2:] or not weight.is_contiguous() or weight.device != x.device):
+        raise _lib.GewellInvalidArgument("a head norm's weight is BF16 [head_dim]")
+    single = x.shape[0] <= 1
+    return _lib.HeadRows(x.data_ptr(), x.shape[1] * x.shape[2] if single else x.stride(0), _ptr(y),
+                         0 if y is None else y.shape[1] * y.shape[2] if single else y.stride(0), _ptr(weight), x.shape[1], int(normalize))
+
+
+def _rotary(frequencies, interleaved: bool, device):
+    if frequencies is None:
+        return None
+    if frequencies.dtype != torch.float32 or frequencies.dim() != 1 or not frequencies.is_contiguous() or frequencies.device != device:
+        raise _lib.GewellInvalidArgument("inverse frequencies are FP32 [width / 2]")
+    return ctypes.byref(_lib.Rotary(frequencies.data_ptr(), 2 * frequencies.shape[0], int(interleaved)))
+
+
+def _check_positions(positions, rows: int, device):
+    if positions.dtype != torch.int32 or positions.dim() != 1 or positions.shape[0] < rows or not positions.is_contiguous() or positions.device != device:
+        raise _lib.GewellInvalidArgument("positions are int32 [rows]")
+
+
+def qk_norm_rotary(query: torch.Tensor, key, query_weight, key_weight, positions: torch.Tensor, frequencies, epsilon: float = 1e-6,
+                   interleaved: bool = False, query_out=None, key_out=None, stream=None):
+    """RMS norm of every head of query [rows, heads, head_dim] and key [rows, kv_heads, head_dim] (or None; rows of a joined
+    projection will do) and rotation by position, in one launch; returns (query_out, key_out)."""
+    _on_current(query.device)
+    rows = query.shape[0]
+    query_out = torch.empty(query.shape, dtype=torch.bfloat16, device=query.device) if query_out is None else query_out
+    q = _head_rows(query, query_weight, True, query_out)
+    k = None
+    if key is not None:
+        if key.shape[0] != rows or key.shape[2] != query.shape[2] or key.device != query.device:
+            raise _lib.GewellInvalidArgument("queries and keys have the same rows and head width")
+        key_out = torch.empty(key.shape, dtype=torch.bfloat16, device=key.device) if key_out is None else key_out
+        k = ctypes.byref(_head_rows(key, key_weight, True, key_out))
+    _check_positions(positions, rows, query.device)
+    _check(_library().gw_qk_norm_rotary_bf16(ctypes.byref(q), k, rows, query.shape[2], positions.data_ptr(),
+                                             _rotary(frequencies, interleaved, query.device), epsilon, _stream(stream)))
+    return query_out, key_out
+
+
+def kv_cache_append(cache: KvCache, batch: SequenceBatch, key: torch.Tensor, value: torch.Tensor, key_weight=None,
+                    normalize_key: bool = True, normalize_value: bool = True, frequencies=None, interleaved: bool = False,
+                    positions=None, query=None, query_weight=None, query_out=None, epsilon: float = 1e-6, stream=None):
+    """Keys and values [rows, kv_heads, head_dim] of a step into their pages: norms, rotation of the keys, quantisation.  With
+    `query` [rows, heads, head_dim] its heads are normed and rotated in the same call; returns query_out then, else None."""
+    device = _on_current(cache.device)
+    for x in (key, value, query):
+        if x is not None and (x.device != device or x.shape[-1] != cache.head_dim):
+            raise _lib.GewellInvalidArgument("heads have the cache's width and lie on its device")
+    if batch.device != device:
+        raise _lib.GewellInvalidArgument("the batch lies on the cache's device")
+    k = _head_rows(key, key_weight, normalize_key, None, batch.rows)
+    v = _head_rows(value, None, normalize_value, None, batch.rows)
+    q = None
+    if query is not None:
+        query_out = torch.empty(query.shape, dtype=torch.bfloat16, device=device) if query_out is None else query_out
+        q = ctypes.byref(_head_rows(query, query_weight, True, query_out, batch.rows))
+    if positions is not None:
+        _check_positions(positions, batch.rows, device)
+    _check(_library().gw_kv_cache_append(cache._ref, batch._ref, ctypes.byref(k), ctypes.byref(v), q, _ptr(positions),
+                                         _rotary(frequencies, interleaved, device), epsilon, _stream(stream)))
+    return query_out if query is not None else None
+
+
+def paged_attention(cache: KvCache, batch: SequenceBatch, query: torch.Tensor, scale: float, window: int = 0, y=None, scratch=None,
+                    stream=None):
+    """Attention of query [rows, heads, head_dim] over the cache, which holds the step's own tokens already; BF16 [rows, heads,
+    head_dim] (rows behind the last sequence are not written).  `scratch`: uint8 that later calls on the same stream may share (allocated for the call if None)."""
+    device = _on_current(cache.device)
+    y = torch.empty(query.shape, dtype=torch.bfloat16, device=device) if y is None else y
+    q = _head_rows(query, None, False, y, batch.rows)
+    if query.device != device or batch.device != device or query.shape[2] != cache.head_dim:
+        raise _lib.GewellInvalidArgument("queries have the cache's head width; queries, batch and cache lie on one device")
+    lib = _library()
+    if scratch is None:
+        scratch = torch.empty(max(256, lib.gw_paged_attention_scratch_bytes(cache._ref, batch._ref, q.heads)), dtype=torch.uint8, device=device)
+    _check(lib.gw_paged_attention_bf16(cache._ref, batch._ref, q.input, q.input_stride, q.heads, scale, window, q.output, q.output_stride,
+                                       scratch.data_ptr(), scratch.numel(), _stream(stream)))
+    return y
+
+
 def gather_rows(x, index, divisor: int, rows: int, stream=None):
     out = torch.empty((rows, x.shape[1]), dtype=torch.bfloat16, device=x.device)
     _check(_library().gw_gather_rows_bf16(_ptr(x), _ptr(index), divisor, rows, x.shape[1], _ptr(out), _stream(stream)))

@@ -336,6 +336,91 @@ gw_status gw_qkv_projector_run(gw_qkv_projector* projector, const gw_projection*
 size_t gw_qkv_projector_bytes(const gw_qkv_projector* projector);
 void gw_qkv_projector_destroy(gw_qkv_projector* projector);
 
+/* ------------------------------------------------------------------------- */
+/* Attention between the Q | K | V projection and the output projection       */
+/* ------------------------------------------------------------------------- */
+
+/* Heads of token rows inside a projection's output: head h of row r is the `head_dim` BF16 values from
+ * input + r * input_stride + h * head_dim on (stride in elements, so a slice of a joined Q | K | V row will do).
+ * normalize != 0: RMS norm over the head; weight (BF16 [head_dim] or NULL) multiplies what the norm left.
+ * output / output_stride: where the result goes, likewise (not used for keys and values that go to a cache).
+ * Pointers 16-byte aligned, strides divisible by 8. */
+typedef struct gw_head_rows {
+  const void* input;
+  uint64_t input_stride;
+  void* output;
+  uint64_t output_stride;
+  const void* weight;
+  uint32_t heads;
+  int normalize;
+} gw_head_rows;
+
+/* Rotation by position: pair i of the first `width` elements of a head turns by position * inverse_frequencies[i]
+ * (FP32 [width / 2] on the device; zeros leave pairs as they are).  Pairs are (i, i + width / 2), or (2 i, 2 i + 1) where
+ * `interleaved`; elements behind `width` stay.  The angle is exact up to the rounding of its remainder, also far into a context. */
+typedef struct gw_rotary {
+  const float* inverse_frequencies;
+  uint32_t width;
+  int interleaved;
+} gw_rotary;
+
+/* Norm of every query and key head and their rotation, one launch: y = rotate(x * rsqrt(mean(x^2) + epsilon) * weight) in
+ * FP32, rounded to BF16 once.  (The norms that Executor::project_qkv of the reference ends with, models/gemma4/31b/sm120/
+ * executor.cuh:1218-1247, and the rotation behind them.)  key NULL: queries alone; rotary NULL: no rotation.  positions: int32
+ * [rows], at least 0.  head_dim divisible by 8, at most 512.  output may be input (same stride).  rows == 0 is a no-op. */
+gw_status gw_qk_norm_rotary_bf16(const gw_head_rows* query, const gw_head_rows* key, uint32_t rows, uint32_t head_dim,
+                                 const int32_t* positions, const gw_rotary* rotary, float epsilon, void* stream);
+
+/* A paged cache of keys and values in 8 bits, in the caller's memory: E4M3 codes [pages, kv_heads, page_tokens, head_dim]
+ * (16-byte aligned) and an FP32 scale for every page and head [pages, kv_heads], for keys and for values.  What a code stands for
+ * is code * scale.  page_tokens 16, 32, 64 or 128; head_dim 128, 256 or 512; pages * kv_heads * page_tokens below 2^31. */
+typedef struct gw_kv_cache {
+  void* k_data;
+  void* v_data;
+  float* k_scales;
+  float* v_scales;
+  uint32_t pages, kv_heads, page_tokens, head_dim;
+} gw_kv_cache;
+
+/* The sequences of one step, on the device.  Sequence s has the token rows row_offsets[s] .. row_offsets[s + 1] - 1 of the step
+ * and, with them, context_lengths[s] tokens; its row i of n is the token at position context_lengths[s] - n + i, which lies in
+ * page page_table[s * page_table_stride + position / page_tokens].  Only entries of pages that the call needs are read.
+ * rows: token rows that the step's arrays have (rows behind the last sequence are left as they are); max_rows: at least the rows
+ * of the sequence with the most.  A position below 0 (a context shorter than its rows, as batches are padded) is no token: nothing
+ * is appended for it, and it sees nothing.  Offsets outside 0 .. rows, sequences of more than max_rows rows, positions behind the
+ * page table and page numbers outside the cache are not followed: those tokens are left out and gw_debug_kernel_error() reports
+ * 0xa....... . */
+typedef struct gw_sequences {
+  const int32_t* row_offsets;     /* [sequences + 1] */
+  const int32_t* context_lengths; /* [sequences] */
+  const int32_t* page_table;      /* [sequences, page_table_stride] */
+  uint32_t page_table_stride, sequences, rows, max_rows;
+} gw_sequences;
+
+/* Keys and values of the step's rows into their pages, keys normed and rotated and values normed on the way (each as its
+ * gw_head_rows says; both have the cache's heads).  A page's scale is the smallest power of two (at least 2^-64) with which its
+ * loudest finite element fits E4M3; where a page had tokens before the call and a louder one comes, their codes are rounded
+ * again to the new scale; a page that the call begins at its first slot starts anew.  Codes round to nearest even; infinities become
+ * the largest code.  Slots behind a page's last token are not touched.  A page belongs to one sequence of the step (pages that
+ * several sequences share may only be full ones).
+ * query (or NULL) is normed and rotated into its output as by gw_qk_norm_rotary_bf16.  positions (or NULL): int32 [rows] for the
+ * rotation in place of the positions in the sequences.  rotary NULL: no rotation. */
+gw_status gw_kv_cache_append(const gw_kv_cache* cache, const gw_sequences* batch, const gw_head_rows* key,
+                             const gw_head_rows* value, const gw_head_rows* query, const int32_t* positions,
+                             const gw_rotary* rotary, float epsilon, void* stream);
+
+/* Attention of the step's query rows over the cache (which holds the step's own tokens already): head h of `heads` reads KV head
+ * h / (heads / kv_heads); the query at position p sees the positions max(0, p - window + 1) .. p (window 0: 0 .. p).
+ * output = sum softmax(scale * q . k) v over what it sees, BF16; a row that sees nothing is 0.  Scores, softmax and sums in FP32;
+ * products of the codes themselves: queries and probabilities enter as two E4M3 parts with a shared power of two for every 32
+ * elements, which hold 8 significant bits.  A NaN in a cached value reaches every query of its KV head that reads the same 128
+ * tokens.  query and output: rows of [heads, head_dim] with strides in elements, 16-byte aligned, strides divisible by 8.
+ * heads / kv_heads at most 64.  scratch: gw_paged_attention_scratch_bytes bytes, 256-byte aligned (not kept between calls). */
+size_t gw_paged_attention_scratch_bytes(const gw_kv_cache* cache, const gw_sequences* batch, uint32_t heads);
+gw_status gw_paged_attention_bf16(const gw_kv_cache* cache, const gw_sequences* batch, const void* query_bf16,
+                                  uint64_t query_stride, uint32_t heads, float scale, uint32_t window, void* output_bf16,
+                                  uint64_t output_stride, void* scratch, size_t scratch_capacity, void* stream);
+
 /* The joins the 31B loader makes in place after uploading a layer (Weights, weights.cuh:146-223), so
  * that the joined forms above apply.  Both rewrite device memory on `stream` and update the
  * projections' pointers; *joined = 0 and nothing changes when the group does not qualify.

@@ -1,0 +1,283 @@
+"""Attention over a paged 8-bit cache against its definition in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import attention as oat
+from tests.attention_helpers import Batch, f64, random_cache, sequence_values, to_device
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def gw():
+    import gewell_b200
+    return gewell_b200
+
+
+def queries(rows, heads, dim, seed, std=1.0):
+    return (torch.randn((rows, heads, dim), generator=torch.Generator().manual_seed(seed)) * std).bfloat16().cuda()
+
+
+def assert_rows(got, q, batch, cache, scale, window, rows_of=None, what=""):
+    """Every row of `rows_of` (default: all sequences' rows) against the oracle.
+
+    With A = sum p |v|: the output's rounding is 2^-8 |o|.  A probability in two E4M3 parts is off by 2^-4 * 2^-4 = 2^-8 of it, and
+    2^-11 for the half-precision value they are cut from; below 2^-17 of the largest of 32 it is lost, 32 * 2^-17 = 2^-12 of that one.
+    A query element in two parts is exact down to 2^-13 of the loudest of its 32, and off by half a step of 2^-13 of it, 2^-14 at most
+    (2^-18 where its second part is scaled on its own), below; the score is then off by e = 2^-14 * |scale| * max |q| * sum |k_d| at most, which
+    changes a probability by 2 e (numerator and sum).  FP32 sums of a few thousand terms stay below 2^-12 of A."""
+    for s, (n, length) in enumerate(batch.sequences):
+        if n == 0:
+            continue
+        k, v = (sequence_values(batch, c, s) for c in cache)
+        low = int(batch.row_offsets[s])
+        picked = range(n) if rows_of is None else sorted({i % n for i in rows_of})
+        for i in picked:
+            position = length - n + i
+            exact, size = oat.attention(f64(q[low + i:low + i + 1]), k, v, scale, position, window)
+            begin = max(0, position - window + 1) if window else 0
+            seen = k[:, begin:position + 1]
+            loudest = float(q[low + i].abs().max())
+            e = 2.0 ** -14 * abs(scale) * loudest * (np.abs(seen).sum(axis=2).max() if position >= 0 else 0.0)
+            bound = 2.0 ** -8 * np.abs(exact) + (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -12 + 2.0 ** -12 + 2 * e) * size + 1e-30
+            error = np.abs(f64(got[low + i:low + i + 1]) - exact)
+            assert (error <= bound).all(), f"{what} sequence {s} row {i}: {float((error / bound).max())} of the bound"
+
+
+def check(gw, sequences, heads, kv_heads, dim, page, window=0, seed=0, scale=None, std=1.5, rows_of=None, extra_rows=0, spread=2.0):
+    batch = Batch(sequences, page, seed, extra_rows=extra_rows)
+    host = random_cache(batch, kv_heads, dim, seed + 1, spread=spread)
+    q = queries(batch.rows, heads, dim, seed + 2, std)
+    scale = dim ** -0.5 if scale is None else scale
+    y = torch.full(q.shape, 7.0, dtype=torch.bfloat16).cuda()
+    got = gw.paged_attention(to_device(gw, host), batch.device(gw), q, scale, window=window, y=y)
+    torch.cuda.synchronize()
+    assert gw.kernel_error() == 0
+    assert (got[int(batch.row_offsets[-1]):] == 7.0).all()
+    assert_rows(got, q, batch, host, scale, window, rows_of, f"{heads}/{kv_heads} x {dim}, page {page}, window {window}:")
+
+
+LAYOUTS = [(16, 8, 256), (16, 2, 512), (8, 2, 128), (6, 2, 128), (7, 7, 256), (16, 1, 128), (2, 2, 512)]
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", LAYOUTS)
+@pytest.mark.parametrize("page", [16, 128])
+def test_decode(gw, heads, kv_heads, dim, page):
+    check(gw, [(1, 1), (1, 2), (1, 127), (1, 128), (1, 129), (0, 50), (1, 700), (1, 31)], heads, kv_heads, dim, page, seed=page)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("window", [1, 5, 128, 200])
+def test_decode_window(gw, page, window):
+    check(gw, [(1, 1), (1, 300), (1, 128), (1, 133), (1, 900)], 8, 4, 256, page, window=window, seed=window)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", LAYOUTS)
+def test_drafts(gw, heads, kv_heads, dim):
+    check(gw, [(3, 3), (5, 700), (2, 130), (4, 128), (1, 64), (0, 0), (5, 257)], heads, kv_heads, dim, 32, seed=5, extra_rows=3)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", LAYOUTS)
+@pytest.mark.parametrize("window", [0, 100])
+def test_prompt(gw, heads, kv_heads, dim, window):
+    check(gw, [(200, 200), (130, 517), (64, 64), (1, 90), (77, 141)], heads, kv_heads, dim, 64, window=window, seed=6,
+          rows_of=[0, 1, 40, 63, 64, 100, 129, 199])
+
+
+def test_many_query_heads_of_one_cache_head(gw):
+    check(gw, [(1, 200), (3, 150)], 64, 1, 128, 16, seed=8)
+    check(gw, [(1, 200), (40, 150)], 33, 1, 256, 16, seed=9, rows_of=[0, 17, 39])
+
+
+def test_one_long_sequence(gw):
+    check(gw, [(1, 20011)], 4, 2, 256, 64, seed=10)
+    check(gw, [(1, 9999)], 16, 2, 512, 128, seed=11)
+    check(gw, [(2, 5000), (1, 3)], 8, 8, 128, 16, seed=12)
+
+
+@pytest.mark.parametrize("std,scale", [(40.0, 1.0), (1e-3, 1.0), (3.0, -0.3), (1.0, 0.0), (300.0, 0.5)])
+def test_sharp_and_flat_scores(gw, std, scale):
+    check(gw, [(1, 600), (3, 333), (70, 400)], 8, 2, 128, 32, seed=13, std=std, scale=scale, rows_of=[0, 1, 2, 69])
+
+
+def test_pages_of_very_different_loudness(gw):
+    check(gw, [(1, 700), (5, 256), (80, 300)], 4, 2, 256, 16, seed=14, spread=10.0, scale=1e-3, rows_of=[0, 4, 79])
+
+
+def test_one_loud_token_among_many_quiet_ones(gw):
+    """A token that takes half of the sum and thousands that share the other half: their probabilities lie 2^-13 and less below
+    the largest, and their values point the other way."""
+    dim, tokens, page = 128, 12000, 64
+    batch = Batch([(1, tokens)], page, 15)
+    (k, ks), (v, vs) = random_cache(batch, 1, dim, 16, garbage=False)
+    ks[:], vs[:] = 1.0, 1.0
+    values = oat.e4m3_values()
+    one = int(np.flatnonzero(values == 1.0)[0])
+    minus = int(np.flatnonzero(values == -1.0)[0])
+    k[:], v[:] = 0, minus
+    for place in (0, 5000, tokens - 1):
+        kk, vv = k.copy(), v.copy()
+        kk[batch.table[0, place // page], 0, place % page] = one
+        vv[batch.table[0, place // page], 0, place % page] = one
+        q = torch.full((1, 2, dim), 1.0, dtype=torch.bfloat16).cuda()
+        scale = np.log(tokens) / dim
+        got = gw.paged_attention(to_device(gw, [(kk, ks), (vv, vs)]), batch.device(gw), q, float(scale))
+        assert_rows(got, q, batch, [(kk, ks), (vv, vs)], float(np.float32(scale)), 0)
+
+
+def test_scores_that_rise_along_the_sequence(gw):
+    """Every tile of tokens louder than all before it, by far more than one power of two, and the other way round."""
+    dim, tokens, page = 256, 1500, 32
+    batch = Batch([(1, tokens), (150, tokens)], page, 17)
+    for sign in (1.0, -1.0):
+        (k, ks), (v, vs) = random_cache(batch, 2, dim, 18, garbage=False, spread=0.0)
+        ones = int(np.flatnonzero(oat.e4m3_values() == 1.0)[0])
+        k[:] = ones
+        for s in range(2):
+            for page_at, page_number in enumerate(batch.table[s, :-(-tokens // page)]):
+                ks[page_number] = np.float32(sign * (page_at + 1) * 0.02) if sign > 0 else np.float32((50 - page_at) * 0.02)
+        q = queries(batch.rows, 4, dim, 19, 1.0) * 0 + 1.0
+        got = gw.paged_attention(to_device(gw, [(k, ks), (v, vs)]), batch.device(gw), q, 1.0)
+        assert_rows(got, q, batch, [(k, ks), (v, vs)], 1.0, 0, rows_of=[0, 149])
+
+
+def test_rows_without_a_token_are_zero(gw):
+    """Padding of a batch: rows of a sequence that has fewer tokens than rows."""
+    batch = Batch([(3, 1), (2, 0), (1, 20), (4, -5)], 16, 20)
+    host = random_cache(batch, 2, 128, 21)
+    q = queries(batch.rows, 4, 128, 22)
+    for std in (1.0,):
+        got = gw.paged_attention(to_device(gw, host), batch.device(gw), q, 0.1, y=torch.full(q.shape, 3.0, dtype=torch.bfloat16).cuda())
+        assert gw.kernel_error() == 0
+        assert (got[:2] == 0).all() and (got[3:5] == 0).all() and (got[6:] == 0).all()
+        rest = Batch([(3, 1), (2, 0), (1, 20), (4, -5)], 16, 20)
+        rest.sequences = [(0, 0), (0, 0), (1, 20), (0, 0)]
+        assert_rows(got, q, rest, host, 0.1, 0)
+        k, v = (sequence_values(batch, c, 0) for c in host)
+        exact, size = oat.attention(f64(q[2:3]), k, v, 0.1, 0)
+        assert (np.abs(f64(got[2:3]) - exact) <= 2.0 ** -7 * (np.abs(exact) + size)).all()
+
+
+def test_strided_rows_and_the_same_inputs_twice(gw):
+    """Queries and outputs inside wider rows; two runs give the same bits."""
+    batch = Batch([(1, 1500), (90, 300), (5, 70)], 32, 23)
+    host = random_cache(batch, 2, 256, 24)
+    cache, held = to_device(gw, host), batch.device(gw)
+    wide = torch.randn((batch.rows, 3, 8 * 256), generator=torch.Generator().manual_seed(25)).bfloat16().cuda()
+    q = wide[:, 1].unflatten(1, (8, 256))
+    out = torch.full((batch.rows, 2, 8 * 256), 5.0, dtype=torch.bfloat16).cuda()
+    got = gw.paged_attention(cache, held, q, 0.06, y=out[:, 1].unflatten(1, (8, 256)))
+    assert (out[:, 0] == 5.0).all()
+    assert_rows(got, q, batch, host, 0.06, 0, rows_of=[0, 44, 89])
+    again = gw.paged_attention(cache, held, q.contiguous(), 0.06)
+    assert torch.equal(again, got)
+
+
+def test_bad_pages_are_left_out(gw):
+    """A page number outside the cache, and a context that reaches behind the page table: those tokens do not count, and it is reported."""
+    batch = Batch([(1, 100), (20, 90)], 16, 26)
+    host = random_cache(batch, 1, 128, 27, garbage=False)
+    q = queries(batch.rows, 2, 128, 28)
+    for bad in (-1, batch.pages, 2 ** 30):
+        broken = Batch([(1, 100), (20, 90)], 16, 26)
+        broken.table[0, 2] = bad
+        got = gw.paged_attention(to_device(gw, host), broken.device(gw), q, 0.1)
+        assert gw.kernel_error() >> 24 == 0xa1
+        k, v = (np.delete(sequence_values(batch, c, 0), np.arange(32, 48), axis=1) for c in host)
+        exact, size = oat.attention(f64(q[:1]), k, v, 0.1, 83)
+        assert (np.abs(f64(got[:1]) - exact) <= 2.0 ** -7 * (np.abs(exact) + size)).all()
+    short = batch.device(gw)
+    short = gw.SequenceBatch(short.row_offsets, short.context_lengths, short.page_table[:, :5].contiguous(), batch.rows, batch.max_rows)
+    got = gw.paged_attention(to_device(gw, host), short, q, 0.1)
+    assert gw.kernel_error() >> 24 == 0xa1
+    k, v = (sequence_values(batch, c, 0)[:, :80] for c in host)
+    exact, size = oat.attention(f64(q[:1]), k, v, 0.1, 79)
+    assert (np.abs(f64(got[:1]) - exact) <= 2.0 ** -7 * (np.abs(exact) + size)).all()
+
+
+def test_captured_replayed_with_other_lengths_and_beside_another(gw):
+    """One graph serves later steps: lengths and pages are read on the device.  Two graphs with scratch of their own run at once."""
+    steps = [[(1, 40), (1, 700), (1, 3)], [(1, 41), (1, 1900), (1, 300)], [(1, 1), (1, 2), (0, 0)]]
+    batches = [Batch(s, 32, 29) for s in steps]
+    largest = max(b.pages for b in batches)
+    entries = max(b.table.shape[1] for b in batches)
+    q = queries(3, 8, 256, 30)
+    hosts = []
+    for b in batches:
+        b.pages, wide = largest, np.full((3, entries), -1, dtype=np.int32)
+        wide[:, :b.table.shape[1]] = b.table
+        b.table = wide
+        hosts.append(random_cache(b, 4, 256, 31))
+    caches = [to_device(gw, hosts[0]) for _ in range(2)]
+    held = [batches[0].device(gw) for _ in range(2)]
+    outs = [torch.empty_like(q) for _ in range(2)]
+    gw.paged_attention(caches[0], held[0], q, 0.1)
+    torch.cuda.synchronize()
+    graphs, streams = [torch.cuda.CUDAGraph() for _ in range(2)], [torch.cuda.Stream() for _ in range(2)]
+    for i in range(2):
+        with torch.cuda.graph(graphs[i], stream=streams[i]):
+            gw.paged_attention(caches[i], held[i], q, 0.1, y=outs[i])
+    for step in (1, 2, 0, 1):
+        for i in range(2):
+            at = (step + i) % 3
+            for name, source in (("k_data", hosts[at][0][0]), ("v_data", hosts[at][1][0]), ("k_scales", hosts[at][0][1]), ("v_scales", hosts[at][1][1])):
+                getattr(caches[i], name).copy_(torch.from_numpy(np.ascontiguousarray(source)))
+            held[i].row_offsets.copy_(torch.from_numpy(batches[at].row_offsets))
+            held[i].context_lengths.copy_(torch.from_numpy(batches[at].lengths))
+            held[i].page_table.copy_(torch.from_numpy(batches[at].table))
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        assert gw.kernel_error() == 0
+        for i in range(2):
+            at = (step + i) % 3
+            assert_rows(outs[i], q, batches[at], hosts[at], 0.1, 0, what=f"step {step}")
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 4, 256), (8, 2, 512)])
+def test_a_layer_from_its_projections_to_its_output(gw, heads, kv_heads, dim):
+    """Q | K | V projection, append with norms and rotation, attention, output projection: three steps of two sequences, against
+    the same in 64 bits over what the cache holds."""
+    from gewell_b200 import _lib
+    hidden, page = 512, 16
+    g = torch.Generator().manual_seed(32)
+    w = (torch.randn(((heads + 2 * kv_heads) * dim, hidden), generator=g) * 0.05).bfloat16().cuda()
+    wo = (torch.randn((hidden, heads * dim), generator=g) * 0.02).bfloat16().cuda()
+    qw, kw = ((1 + 0.25 * torch.randn(dim, generator=g)).bfloat16().cuda() for _ in range(2))
+    f = torch.tensor([1e4 ** (-i / (dim // 2)) for i in range(dim // 2)], dtype=torch.float32).cuda()
+    parts = w.split([heads * dim, kv_heads * dim, kv_heads * dim])
+    query, key, value = (gw.make_projection(p, hidden, p.shape[0]) for p in parts)
+    projector = gw.QkvProjector(hidden, heads * dim, kv_heads * dim, 256, _lib.POLICY_ALWAYS)
+    table = torch.randperm(12, generator=g)[:10].reshape(2, 5).int().cuda()
+    cache = gw.KvCache(*(torch.full((12, kv_heads, page, dim), 127, dtype=torch.uint8).cuda() for _ in range(2)),
+                       *(torch.full((12, kv_heads), float("nan")).cuda() for _ in range(2)))
+    lengths = [0, 0]
+    for news in ([37, 20], [1, 1], [3, 0]):
+        lengths = [a + b for a, b in zip(lengths, news)]
+        rows = sum(news)
+        offsets = torch.tensor([0, news[0], rows], dtype=torch.int32).cuda()
+        batch = gw.SequenceBatch(offsets, torch.tensor(lengths, dtype=torch.int32).cuda(), table, rows, max(news))
+        x = torch.randn((rows, hidden), generator=g).bfloat16().cuda()
+        projector.prepare(rows)
+        q, k, v, joined_one = projector.run(query, key, value, x, _lib.PHASE_PREFILL)
+        assert joined_one
+        q, k, v = q.unflatten(1, (heads, dim)), k.unflatten(1, (kv_heads, dim)), v.unflatten(1, (kv_heads, dim))
+        turned = gw.kv_cache_append(cache, batch, k, v, key_weight=kw, frequencies=f, query=q, query_weight=qw)
+        seen = gw.paged_attention(cache, batch, turned, dim ** -0.5)
+        plan = gw.Bf16Plan(rows, heads * dim, hidden)
+        out = torch.empty((rows, hidden), dtype=torch.bfloat16).cuda()
+        plan.run(seen.flatten(1), wo, out, torch.empty(max(256, plan.scratch_bytes()), dtype=torch.uint8).cuda())
+        torch.cuda.synchronize()
+        assert gw.kernel_error() == 0
+        at = np.concatenate([np.arange(n - m, n) for n, m in zip(lengths, news)])
+        exact_q = oat.head_norm_rotary(f64(q), f64(qw), True, at, f.cpu().numpy())
+        assert (np.abs(f64(turned) - exact_q) <= 2.0 ** -8 * np.abs(exact_q) + 2.0 ** -19 * np.abs(exact_q).max(axis=-1, keepdims=True)).all()
+        held = Batch([(m, n) for n, m in zip(lengths, news)], page, 0)
+        held.table = table.cpu().numpy()
+        host = [(cache.k_data.cpu().numpy(), cache.k_scales.cpu().numpy()), (cache.v_data.cpu().numpy(), cache.v_scales.cpu().numpy())]
+        assert_rows(seen, turned, held, host, dim ** -0.5, 0)
+        exact = f64(seen.flatten(1)) @ f64(wo).T
+        assert (np.abs(f64(out) - exact) <= 2.0 ** -8 * np.abs(exact) + 2.0 ** -18 * (np.abs(f64(seen.flatten(1))) @ np.abs(f64(wo)).T)).all()
