@@ -1,12 +1,39 @@
 // Attention over a paged cache of E4M3 keys and values with a scale for every page and head.
 //
-//   o = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * q . k_j - m),   m the running maximum
+//   o = sum_j p_j v_j / sum_j p_j,   p_j = exp2(c_j k_j . q - m),   c_j = scale * log2(e) * kscale_j
 //
-// One warp per query row and head; a lane has D / 32 elements of q, of the sum and of every cached row.
+// One block takes tiles of kTokens cached tokens, N query columns (query rows times the query heads of one KV head) at a time,
+// with both products on the tensor cores and the cached codes as they are: nothing of the cache is converted or transposed.
+//   S^T [tokens, N]  = K [tokens, D] Q^T          A = K as it lies in its pages (a row of D codes), B = Q
+//   O^T [D, N]      += V^T [D, tokens] P^T        A = V as it lies in its pages, read along the tokens, B = P^T
+// Tokens lie on the tensor memory's lanes, so a lane needs one key scale and one value scale for all its columns, and
+// few query rows cost few columns: the same kernel serves single tokens and prompts.
+//
+// E4M3 holds four significant bits.  Queries and probabilities therefore enter as two parts, x = hi + lo with hi the nearest
+// code of x and lo that of the rest (eight bits, as BF16), two products over the same codes.  Block scaling (kind::mxf8f6f4, a power
+// of two for every 32 elements along the sum) gives every 32 elements of a query, and every 32 tokens of a column of P -- those
+// of one warp -- a range of their own, so that small probabilities are as exact as large ones, however far below the maximum.
+// That also takes the running maximum out of the loop: the reference m of a column only has to keep FP32 sums from
+// overflowing.  It is the maximum of the first tile, and is moved (with the sums rescaled) only when a probability exceeds 2^80.
+//
+//   warp 0      TMA: chunks of [128 tokens x 128 bytes] of K and V into a ring, page by page
+//   warp 1      tcgen05.mma: S of tile t + 1, then O += P V of tile t.  Rows of V that no query may see are zeroed here: a
+//               page's slots behind its last token may hold anything, NaN included, and 0 * NaN is NaN.
+//   warps 2..9  softmax: two warps for every 32 lanes, each half of the columns; queries into shared memory at the start of an item,
+//               results out at its end
+//
+// Work: attention_work.h.  An item that a cut between two blocks' ranges divides leaves FP32 partial sums in the scratch
+// memory, which a second kernel joins in the order of the blocks (the same bits on every run).
+// Every wait is bounded; a role that gives up reports it, all leave, and tensor memory is released.
+#include <algorithm>
 #include <string>
 
+#include "attention_work.h"
 #include "common.cuh"
+#include "gemm_tc.cuh"
 #include "paged.h"
+#include "pair.cuh"
+#include "ptx.cuh"
 
 using namespace gw;
 
@@ -14,65 +41,843 @@ namespace {
 
 __device__ uint32_t g_attention_error;       // first report since it was last taken
 
+constexpr int kSoftmaxWarps = 8;
+constexpr int kThreads = 32 * (2 + kSoftmaxWarps);
+constexpr int kChunkBytes = kTokens * 128;
+constexpr int kAtomBytes = 512;              // scale atom: 128 rows x 4 blocks of 32 elements
+constexpr uint32_t kMoveExponent = 127 + 80;      // a probability over its reference from which on the reference moves
+constexpr float kMost = 1.2089258196146292e24F;   // 2^80
+
 struct Attention {
   gw_kv_cache cache;
   gw_sequences batch;
   const bf16* query;
   bf16* output;
   uint64_t query_stride, output_stride;
-  uint32_t heads, group, window;
+  uint32_t heads, group, per_tile, window;
   float scale;
+  float* partial;             // [blocks][2][N][D], then [blocks][2][2][N] maxima and sums
+  int4* records;              // [blocks]: {first query row, columns, KV head, last block} of the item that its last piece begins, or last -1
 };
 
-template <int V>          // head width 128 * V / 4
-__global__ void __launch_bounds__(128) paged_attention_kernel(Attention a) {
-  constexpr int E = V;
-  griddep_enter();
-  const uint32_t lane = threadIdx.x % 32, width = 32 * E;
-  const uint32_t task = blockIdx.x * 4 + threadIdx.x / 32, row = task / a.heads, head = task % a.heads, kv = head / a.group;
-  if (row >= a.batch.rows) return;
-  uint32_t low = 0, high = a.batch.sequences;
-  while (low + 1 < high) {
-    const uint32_t middle = (low + high) / 2;
-    if (a.batch.row_offsets[middle] <= int(row)) low = middle; else high = middle;
+template <int D, int N>
+struct Layout {
+  static constexpr int kChunks = D / 128;
+  static constexpr int kQueryBytes = kChunks * N * 128;           // one part
+  static constexpr bool kOneBuffer = N <= 64;                     // both parts of P in the halves of 128-byte rows
+  static constexpr int kProbBytes = kOneBuffer ? kChunkBytes : 2 * kChunkBytes;
+  static constexpr int kLowOffset = kOneBuffer ? 64 : kChunkBytes;
+  static constexpr int kAtoms = 2 * kChunks + 2;                  // queries (both parts), ones, P
+  static constexpr int kSmall = kAtoms * kAtomBytes + 6 * N * 4 + 1024;      // and what is declared as Shared
+  static constexpr int kRoom = 227 * 1024 - 1024 - 2 * kQueryBytes - kProbBytes - kSmall;
+  static constexpr int kRing = kRoom / kChunkBytes > 16 ? 16 : kRoom / kChunkBytes;
+  static constexpr int kSmemBytes = 2 * kQueryBytes + kProbBytes + kRing * kChunkBytes + kSmall;      // 1024 bytes of it for the alignment
+  // tensor memory columns
+  static constexpr int kScores = kChunks * N;
+  static constexpr int kOnes = kScores + 2 * N;
+  static constexpr int kQueryScales = kOnes + 4;
+  static constexpr int kProbScales = kQueryScales + 8 * kChunks;
+  static constexpr int kColumns = 512;
+  static_assert(kProbScales + 4 <= kColumns, "tensor memory over-subscribed");
+  static_assert(kRing >= kChunks + 1, "a tile's chunks and one more");
+  static_assert(kSmemBytes + 1024 <= 227 * 1024 && kSmemBytes > 116 * 1024, "one block an SM");
+  static_assert(N % 16 == 0 && N <= 128 && D % 128 == 0, "");
+};
+
+struct Shared {
+  uint64_t full[16], empty[16], scores_full[2], scores_empty[2], probs_full, probs_empty, query_full, sums_full, drained;
+  uint32_t tensor_memory;
+  // units of all blocks, the block's range of them, and the item that has the first
+  int64_t units, from, to, item;
+  uint32_t sequence;
+  int head, tile;
+};
+
+// ---------------------------------------------------------------------------
+// walking over the block's pieces: every role has its own walk
+// ---------------------------------------------------------------------------
+struct Walk {
+  uint32_t sequence;
+  int head, tile;
+  int64_t item;
+  SequenceRows rows;
+  SequenceWork work;
+  // the piece
+  int begin, end, tiles;
+
+  __device__ __forceinline__ SequenceWork work_of(const Attention& a) const {
+    return SequenceWork{rows.context - rows.count, rows.count, int32_t(a.per_tile), int32_t(a.window)};
   }
-  const SequenceRows s = sequence_rows(a.batch, low);
-  if (s.bad && lane == 0) atomicCAS(&g_attention_error, 0u, 0xa2000000u | (low & 0xffffffu));
-  if (int(row) < s.first || int(row) >= s.first + s.count) return;
-  const int position = s.context - s.count + int(row) - s.first;
-  const int begin = a.window ? max(int64_t(0), int64_t(position) - a.window + 1) : 0;
-  float q[E], sum[E], total = 0.F, most = -INFINITY;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = __bfloat162float(a.query[size_t(row) * a.query_stride + head * width + lane * E + e]) * a.scale;
-    sum[e] = 0.F;
-  }
-  for (int token = begin; token <= position; ++token) {
-    const uint32_t ordinal = token / a.cache.page_tokens, slot = token % a.cache.page_tokens;
-    int page = -1;
-    if (ordinal < a.batch.page_table_stride) page = a.batch.page_table[size_t(low) * a.batch.page_table_stride + ordinal];
-    if (page < 0 || uint32_t(page) >= a.cache.pages) {
-      if (lane == 0) atomicCAS(&g_attention_error, 0u, 0xa1000000u | (low & 0xffffffu));
-      continue;
+  __device__ __forceinline__ void start(const Attention& a, const Shared& s) {
+    sequence = s.sequence;
+    head = s.head;
+    tile = s.tile;
+    item = s.item;
+    if (sequence < a.batch.sequences) {
+      rows = sequence_rows(a.batch, sequence);
+      work = work_of(a);
     }
-    const size_t at = size_t(page) * a.cache.kv_heads + kv;
-    const size_t place = (at * a.cache.page_tokens + slot) * width + lane * E;
-    float dot = 0.F;
-#pragma unroll
-    for (int e = 0; e < E; ++e) dot = fmaf(q[e], e4m3_to_float(static_cast<const uint8_t*>(a.cache.k_data)[place + e]), dot);
-#pragma unroll
-    for (int m = 16; m; m /= 2) dot += __shfl_xor_sync(0xffffffffu, dot, m);
-    dot *= a.cache.k_scales[at];
-    const float higher = fmaxf(most, dot), before = most == -INFINITY ? 0.F : expf(most - higher), p = expf(dot - higher);
-    total = total * before + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      sum[e] = sum[e] * before + p * a.cache.v_scales[at] * e4m3_to_float(static_cast<const uint8_t*>(a.cache.v_data)[place + e]);
-    most = higher;
   }
+  // The next piece; false: there is none.
+  __device__ __forceinline__ bool next(const Attention& a, const Shared& s) {
+    while (sequence < a.batch.sequences && item < s.to) {
+      if (tile < work.query_tiles()) {
+        tiles = work.token_tiles(tile);
+        const Piece p = piece_of(item, tiles, s.from, s.to);
+        if (p.here) {
+          begin = p.begin;
+          end = p.end;
+          return true;
+        }
+        advance();
+      } else {
+        tile = 0;
+        if (rows.count != 0 && uint32_t(++head) < a.cache.kv_heads) continue;
+        head = 0;
+        if (++sequence < a.batch.sequences) {
+          rows = sequence_rows(a.batch, sequence);
+          work = work_of(a);
+        }
+      }
+    }
+    return false;
+  }
+  __device__ __forceinline__ void advance() {
+    item += 1 + tiles;
+    ++tile;
+  }
+};
+
+// The block's range of units and the item that its first unit belongs to.
+__device__ __forceinline__ void find_start(const Attention& a, Shared& shared) {
+  constexpr int WARPS = kThreads / 32;
+  __shared__ int64_t sums[WARPS];
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  int64_t before = 0, total = 0, from = 0;
+  // first the total, then the sequence that has unit `from`
+  for (int pass = 0; pass < 2; ++pass) {
+    before = 0;
+    for (uint32_t base = 0; base < a.batch.sequences; base += kThreads) {
+      const uint32_t s = base + threadIdx.x;
+      int64_t mine = 0;
+      SequenceWork w{0, 0, 1, 0};
+      if (s < a.batch.sequences) {
+        const SequenceRows r = sequence_rows(a.batch, s);
+        if (r.bad && pass == 0 && blockIdx.x == 0) atomicCAS(&g_attention_error, 0u, 0xa2000000u | (s & 0xffffffu));
+        w = SequenceWork{r.context - r.count, r.count, int32_t(a.per_tile), int32_t(a.window)};
+        mine = w.units() * a.cache.kv_heads;
+      }
+      int64_t sum = mine;
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    a.output[size_t(row) * a.output_stride + head * width + lane * E + e] = __float2bfloat16_rn(total > 0.F ? sum[e] / total : 0.F);
+      for (int m = 1; m < 32; m *= 2) {
+        const int64_t other = __shfl_up_sync(0xffffffffu, sum, m);
+        if (lane >= uint32_t(m)) sum += other;
+      }
+      if (lane == 31) sums[warp] = sum;
+      __syncthreads();
+      int64_t low = before + sum - mine;
+#pragma unroll
+      for (int i = 0; i < WARPS; ++i) {
+        if (uint32_t(i) < warp) low += sums[i];
+        before += sums[i];
+      }
+      if (pass == 1 && low <= from && from < low + mine) {
+        const int64_t units = w.units(), at = from - low;
+        shared.sequence = s;
+        shared.head = int(at / units);
+        shared.tile = w.tile_with(at % units);
+        shared.item = low + shared.head * units + w.units_before(shared.tile);
+      }
+      __syncthreads();
+    }
+    if (pass == 0) {
+      total = before;
+      const int64_t parts = total < gridDim.x ? total : gridDim.x;
+      const bool idle = int64_t(blockIdx.x) >= parts;
+      from = idle ? total : range_start(total, blockIdx.x, parts);
+      if (threadIdx.x == 0) {
+        shared.units = total;
+        shared.from = from;
+        shared.to = idle ? total : range_start(total, blockIdx.x + 1, parts);
+        shared.item = total;
+        shared.sequence = a.batch.sequences;
+        shared.head = shared.tile = 0;
+      }
+      if (idle) break;
+    }
+  }
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------
+// small pieces
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ int page_at(const Attention& a, uint32_t sequence, int token) {
+  const uint32_t ordinal = uint32_t(token) / a.cache.page_tokens;
+  int page = -1;
+  if (ordinal < a.batch.page_table_stride) page = a.batch.page_table[size_t(sequence) * a.batch.page_table_stride + ordinal];
+  return page >= 0 && uint32_t(page) < a.cache.pages ? page : -1;
+}
+__device__ __forceinline__ uint32_t pack4(uint16_t low, uint16_t high) { return uint32_t(low) | uint32_t(high) << 16; }
+
+// hi and lo codes of two values of size below 448: hi the nearest codes, lo those of (x - hi) * low_scale
+__device__ __forceinline__ void two_parts(float a, float b, float low_scale, uint16_t& hi, uint16_t& lo) {
+  const __half2 x = __floats2half2_rn(a, b);
+  hi = __nv_cvt_halfraw2_to_fp8x2(__half2_raw(x), __NV_SATFINITE, __NV_E4M3);
+  const __half2 rest = __hmul2(__hsub2(x, __half2(__nv_cvt_fp8x2_to_halfraw2(hi, __NV_E4M3))), __float2half2_rn(low_scale));
+  lo = __nv_cvt_halfraw2_to_fp8x2(__half2_raw(rest), __NV_SATFINITE, __NV_E4M3);
+}
+
+// matrix descriptor of rows of 128 bytes, 128-byte swizzle, read across the rows: 8 rows of the sum are 1024 bytes apart
+__device__ __forceinline__ uint64_t across_desc(uint32_t address) { return ptx::smem_desc_sw128(address) | uint64_t(1024 >> 4) << 16; }
+
+// E4M3 x E4M3, UE8M0 scales of 32 elements, FP32 sums, M = 128
+__host__ __device__ constexpr uint32_t idesc_mx(uint32_t n, bool across) {
+  return (across ? 3u << 15 : 0u) | ((n >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void mma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(scale_a), "r"(scale_b)
+      : "memory");
+}
+
+template <int X>
+__device__ __forceinline__ void tmem_load(uint32_t address, uint32_t* r) {
+  if constexpr (X == 16) {
+    ptx::tmem_load16(address, r);
+  } else {
+    static_assert(X == 8);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(address) : "memory");
+  }
+}
+template <int X>
+__device__ __forceinline__ void tmem_store(uint32_t address, const uint32_t* r) {
+  if constexpr (X == 16) {
+    ptx::tmem_store16(address, r);
+  } else {
+    static_assert(X == 8);
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(address), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+  }
+}
+// C columns from `address` on, C a multiple of 8
+template <int C>
+__device__ __forceinline__ void tmem_load_columns(uint32_t address, uint32_t* r) {
+#pragma unroll
+  for (int j = 0; j + 16 <= C; j += 16) tmem_load<16>(address + j, r + j);
+  if constexpr (C % 16 != 0) tmem_load<8>(address + C - 8, r + C - 8);
+}
+template <int C>
+__device__ __forceinline__ void tmem_store_columns(uint32_t address, const uint32_t* r) {
+#pragma unroll
+  for (int j = 0; j + 16 <= C; j += 16) tmem_store<16>(address + j, r + j);
+  if constexpr (C % 16 != 0) tmem_store<8>(address + C - 8, r + C - 8);
+}
+
+__device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(32 * kSoftmaxWarps) : "memory"); }
+// whether the condition holds for any thread of the softmax warps
+__device__ __forceinline__ bool softmax_any(bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any) : "r"(uint32_t(mine)), "n"(32 * kSoftmaxWarps) : "memory");
+  return any != 0;
+}
+// order-preserving integer of a float that is no NaN
+__device__ __forceinline__ int ordered(float v) {
+  const int bits = __float_as_int(v);
+  return bits ^ ((bits >> 31) & 0x7fffffff);
+}
+
+// ---------------------------------------------------------------------------
+// the kernel
+// ---------------------------------------------------------------------------
+template <int D, int N>
+__global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
+                                                                      const __grid_constant__ CUtensorMap v_map,
+                                                                      const __grid_constant__ Attention a) {
+  using L = Layout<D, N>;
+  constexpr int CH = L::kChunks, RING = L::kRing, C = N / 2;
+  extern __shared__ uint8_t raw[];
+  uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* const query_hi = base;
+  uint8_t* const query_lo = query_hi + L::kQueryBytes;
+  uint8_t* const probs = query_lo + L::kQueryBytes;
+  uint8_t* const ring = probs + L::kProbBytes;
+  uint8_t* const atoms = ring + RING * kChunkBytes;              // [2 * CH] queries (hi, lo of a chunk), [1] ones, [1] P
+  uint8_t* const ones_atom = atoms + 2 * CH * kAtomBytes;
+  uint8_t* const probs_atom = ones_atom + kAtomBytes;
+  float* const reference = reinterpret_cast<float*>(probs_atom + kAtomBytes);     // [N] m of a column
+  float* const factor = reference + N;                                            // [N]
+  float* const by_warp = factor + N;                                              // [4][N]
+  __shared__ Shared s;
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < RING; ++i) {
+      ptx::mbar_init(&s.full[i], 1);
+      ptx::mbar_init(&s.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&s.scores_full[i], 1);
+      ptx::mbar_init(&s.scores_empty[i], kSoftmaxWarps);
+    }
+    ptx::mbar_init(&s.probs_full, kSoftmaxWarps);
+    ptx::mbar_init(&s.probs_empty, 1);
+    ptx::mbar_init(&s.query_full, kSoftmaxWarps);
+    ptx::mbar_init(&s.sums_full, 1);
+    ptx::mbar_init(&s.drained, 1);
+    ptx::fence_barrier_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(&s.tensor_memory, L::kColumns);
+    ptx::tmem_relinquish();
+  }
+  for (int i = threadIdx.x; i < kAtomBytes / 4; i += kThreads) {
+    reinterpret_cast<uint32_t*>(ones_atom)[i] = 0x7f7f7f7fu;      // 2^0
+    reinterpret_cast<uint32_t*>(probs_atom)[i] = 0x7f7f7f7fu;
+    for (int j = 0; j < 2 * CH; ++j) reinterpret_cast<uint32_t*>(atoms + j * kAtomBytes)[i] = 0x7f7f7f7fu;
+  }
+  ptx::fence_proxy_async_smem();
+  ptx::tc_fence_before_sync();
+  griddep_enter();
+  find_start(a, s);                                              // ends with __syncthreads()
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem = s.tensor_memory;
+  const auto failed = [](uint32_t code) {
+    atomicCAS(&g_attention_error, 0u, code | (blockIdx.x << 8));
+    return false;
+  };
+
+  if (warp == 0) {
+    // ----- producer: lane l brings the l-th page of a tile
+    const uint32_t page_tokens = a.cache.page_tokens, boxes = kTokens / page_tokens;
+    const int outside = int(a.cache.pages * a.cache.kv_heads * page_tokens);        // rows from here on read as zeros
+    int slot = 0, issued = 0;
+    uint32_t parity = 1;                                         // empty slots: the first pass does not wait
+    bool good = true;
+    Walk w;
+    w.start(a, s);
+    while (good && w.next(a, s)) {
+      const int first = w.work.first_token_tile(w.tile), low = w.work.low(w.tile), high = w.work.high(w.tile);
+      // row of the lane's page in the tensor maps
+      const auto row_of = [&](int t) {
+        const int64_t token = int64_t(first + t) * kTokens + lane * page_tokens;
+        if (lane >= boxes || token >= high || token + page_tokens <= low) return outside;
+        const int page = page_at(a, w.sequence, int(token));
+        if (page < 0) {
+          atomicCAS(&g_attention_error, 0u, 0xa1000000u | (w.sequence & 0xffffffu));
+          return outside;
+        }
+        return int((uint32_t(page) * a.cache.kv_heads + w.head) * page_tokens);
+      };
+      const auto bring = [&](const CUtensorMap* map, int row) {
+        for (int c = 0; c < CH; ++c) {
+          if (!ptx::mbar_wait_warp(&s.empty[slot], parity)) return failed(0xa3000000u | slot);
+          if (lane == 0) ptx::mbar_expect_tx(&s.full[slot], kChunkBytes);
+          __syncwarp();
+          if (lane < boxes) ptx::tma_load_2d(ring + slot * kChunkBytes + lane * page_tokens * 128, map, c * 128, row, &s.full[slot]);
+          ++issued;
+          if (++slot == RING) {
+            slot = 0;
+            parity ^= 1;
+          }
+        }
+        return true;
+      };
+      int row = row_of(w.begin), row_before = 0;
+      for (int t = w.begin; good && t < w.end; ++t) {
+        const int row_next = t + 1 < w.end ? row_of(t + 1) : 0;
+        good = bring(&k_map, row);
+        if (good && t > w.begin) good = bring(&v_map, row_before);
+        row_before = row;
+        row = row_next;
+      }
+      if (good && w.end > w.begin) good = bring(&v_map, row_before);
+      w.advance();
+    }
+    // the copies still in flight land before the block ends
+    for (int i = issued < RING ? issued : RING; i > 0; --i) {
+      if (slot == 0) {
+        slot = RING;
+        parity ^= 1;
+      }
+      --slot;
+      ptx::mbar_wait_warp(&s.full[slot], parity ^ 1, 0, 100000000ull);
+    }
+  } else if (warp == 1) {
+    // ----- both products
+    int slot = 0, item = 0, scored = 0, summed = 0;              // scored, summed: tiles over all items
+    uint32_t parity = 0;
+    bool good = true;
+    Walk w;
+    w.start(a, s);
+    if (ptx::elect_one()) ptx::tc_copy_sf_atom(tmem + L::kOnes, ptx::smem_desc_sf_atom(ptx::smem_u32(ones_atom)));
+    const auto wait_chunk = [&]() { return ptx::mbar_wait_warp(&s.full[slot], parity) || failed(0xa4000000u | slot); };
+    const auto next_chunk = [&]() {
+      if (++slot == RING) {
+        slot = 0;
+        parity ^= 1;
+      }
+    };
+    while (good && w.next(a, s)) {
+      if (w.end > w.begin) {
+        const int first = w.work.first_token_tile(w.tile), low = w.work.low(w.tile), high = w.work.high(w.tile);
+        good = ptx::mbar_wait_warp(&s.query_full, item & 1) || failed(0xa5000000u);
+        if (!good) break;
+        ptx::tc_fence_after_sync();
+        if (ptx::elect_one())
+#pragma unroll
+          for (int i = 0; i < 2 * CH; ++i)
+            ptx::tc_copy_sf_atom(tmem + L::kQueryScales + 4 * i, ptx::smem_desc_sf_atom(ptx::smem_u32(atoms + i * kAtomBytes)));
+        const auto score = [&]() {
+          const int buffer = scored & 1;
+          if (!ptx::mbar_wait_warp(&s.scores_empty[buffer], ((scored >> 1) & 1) ^ 1)) return failed(0xa6000000u | buffer);
+          ptx::tc_fence_after_sync();
+          for (int c = 0; c < CH; ++c) {
+            if (!wait_chunk()) return false;
+            ptx::tc_fence_after_sync();
+            if (ptx::elect_one()) {
+              const uint64_t keys = ptx::smem_desc_sw128(ptx::smem_u32(ring + slot * kChunkBytes));
+#pragma unroll
+              for (int part = 0; part < 2; ++part) {
+                const uint64_t queries = ptx::smem_desc_sw128(ptx::smem_u32((part ? query_lo : query_hi) + c * N * 128));
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  mma_mx(tmem + L::kScores + buffer * N, keys + 2 * k, queries + 2 * k, idesc_mx(N, false) | uint32_t(k) << 4, tmem + L::kOnes,
+                         tmem + L::kQueryScales + 4 * (2 * c + part), c | part | k);
+              }
+              ptx::tc_commit(&s.empty[slot]);
+              if (c == CH - 1) ptx::tc_commit(&s.scores_full[buffer]);
+            }
+            __syncwarp();
+            next_chunk();
+          }
+          ++scored;
+          return true;
+        };
+        const auto sum = [&](int t) {
+          if (!ptx::mbar_wait_warp(&s.probs_full, summed & 1)) return failed(0xa7000000u);
+          ptx::tc_fence_after_sync();
+          if (ptx::elect_one()) ptx::tc_copy_sf_atom(tmem + L::kProbScales, ptx::smem_desc_sf_atom(ptx::smem_u32(probs_atom)));
+          const int start = (first + t) * kTokens, clear_below = low - start, clear_from = high - start;
+          for (int c = 0; c < CH; ++c) {
+            if (!wait_chunk()) return false;
+            if (clear_below > 0 || clear_from < kTokens) {       // tokens that no query of the item sees
+              uint4* rows = reinterpret_cast<uint4*>(ring + slot * kChunkBytes);
+              for (int i = lane; i < clear_below * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
+              for (int i = clear_from * 8 + lane; i < kTokens * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
+              ptx::fence_proxy_async_smem();
+              __syncwarp();
+            }
+            ptx::tc_fence_after_sync();
+            if (ptx::elect_one()) {
+              const uint64_t values = across_desc(ptx::smem_u32(ring + slot * kChunkBytes));
+#pragma unroll
+              for (int part = 0; part < 2; ++part) {
+                const uint64_t p = across_desc(ptx::smem_u32(probs + part * L::kLowOffset));
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  mma_mx(tmem + c * N, values + 256 * k, p + 256 * k, idesc_mx(N, true) | uint32_t(k) << 4, tmem + L::kOnes,
+                         tmem + L::kProbScales, uint32_t(t > w.begin) | part | k);
+              }
+              ptx::tc_commit(&s.empty[slot]);
+              if (c == CH - 1) {
+                ptx::tc_commit(&s.probs_empty);
+                if (t == w.end - 1) ptx::tc_commit(&s.sums_full);
+              }
+            }
+            __syncwarp();
+            next_chunk();
+          }
+          ++summed;
+          return true;
+        };
+        good = score();
+        for (int t = w.begin; good && t < w.end; ++t) {
+          if (t + 1 < w.end) good = score();
+          if (good) good = sum(t);
+        }
+        ++item;
+      }
+      w.advance();
+    }
+    // products still in flight end before tensor memory is released
+    if (ptx::elect_one()) ptx::tc_commit(&s.drained);
+    __syncwarp();
+    ptx::mbar_wait_warp(&s.drained, 0, 0, 100000000ull);
+  } else {
+    // ----- softmax
+    const uint32_t quadrant = warp & 3, half = (warp - 2) / 4, column0 = half * C, member = threadIdx.x - 64;
+    const uint32_t lanes = tmem + (quadrant * 32 << 16);
+    const uint32_t row = quadrant * 32 + lane;                   // the lane's token in a tile
+    int item = 0, tile_count = 0;
+    if (member == 0) a.records[blockIdx.x] = make_int4(0, 0, 0, -1);
+    // A thread whose wait ran out waits no more, but goes on to the barriers that it shares with the others.
+    bool good = true;
+    const auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
+      if (good && !ptx::mbar_wait_bounded(bar, parity)) good = failed(code);
+    };
+    Walk w;
+    w.start(a, s);
+    while (w.next(a, s)) {
+      const int token_rows = min(int(a.per_tile), w.rows.count - w.tile * int(a.per_tile));
+      const int used = token_rows * int(a.group);                // columns of queries
+      const int first_row = w.rows.first + w.tile * int(a.per_tile), position0 = w.work.base + w.tile * int(a.per_tile);
+      const uint32_t head0 = w.head * a.group;
+      const auto output_of = [&](int column) {
+        return a.output + size_t(first_row + column / int(a.group)) * a.output_stride + size_t(head0 + column % int(a.group)) * D;
+      };
+      if (w.tiles == 0) {                                        // rows that see nothing
+        for (int column = warp - 2; column < used; column += kSoftmaxWarps)
+          for (int d = lane * 8; d < D; d += 256) *reinterpret_cast<uint4*>(output_of(column) + d) = make_uint4(0, 0, 0, 0);
+        w.advance();
+        continue;
+      }
+      // queries: a thread takes 32 elements at a time, which share a power of two
+      for (int block = member; block < N * (D / 32); block += 32 * kSoftmaxWarps) {
+        const int column = block / (D / 32), part = block % (D / 32), c = part / 4, k = part % 4;
+        uint4 bits[4];
+        if (column < used) {
+          const uint4* from = reinterpret_cast<const uint4*>(a.query + size_t(first_row + column / int(a.group)) * a.query_stride +
+                                                             size_t(head0 + column % int(a.group)) * D + part * 32);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) bits[i] = from[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) bits[i] = make_uint4(0, 0, 0, 0);
+        }
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(bits);
+        uint32_t largest = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) largest = max(largest, max(words[i] << 16 & 0x7fffffffu, words[i] & 0x7fff0000u));
+        const uint32_t exponent = largest >> 23;
+        // values times 2^(134 - exponent) lie below 2^8; blocks of less than 2^-114 count as zeros, infinities as NaN
+        const float up = exponent == 255 ? __uint_as_float(0x7fc00000u) : exponent < 13 ? 0.F : __uint_as_float((261 - exponent) << 23);
+        const uint32_t scale = exponent < 13 ? 127 : exponent - 7;
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint16_t h0, l0, h1, l1;
+          two_parts(__uint_as_float(words[2 * i] << 16) * up, __uint_as_float(words[2 * i] & 0xffff0000u) * up, 16.F, h0, l0);
+          two_parts(__uint_as_float(words[2 * i + 1] << 16) * up, __uint_as_float(words[2 * i + 1] & 0xffff0000u) * up, 16.F, h1, l1);
+          hi[i] = pack4(h0, h1);
+          lo[i] = pack4(l0, l1);
+        }
+        const uint32_t at = c * N * 128 + column * 128;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t place = at + (((2 * k + i) ^ (column & 7)) << 4);
+          *reinterpret_cast<uint4*>(query_hi + place) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+          *reinterpret_cast<uint4*>(query_lo + place) = make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+        }
+        const uint32_t scale_at = 2 * c * kAtomBytes + (column % 32) * 16 + column / 32 * 4 + k;
+        atoms[scale_at] = uint8_t(scale);
+        atoms[scale_at + kAtomBytes] = uint8_t(scale - 4);
+      }
+      if (member < N) reference[member] = int(member) < used ? -INFINITY : 0.F;      // scores without a query are 0
+      ptx::fence_proxy_async_smem();
+      ptx::tc_fence_before_sync();                               // the results of the item before were read
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&s.query_full);
+      softmax_sync();                                            // `reference`
+
+      float total[C];
+#pragma unroll
+      for (int j = 0; j < C; ++j) total[j] = 0.F;
+      const int first = w.work.first_token_tile(w.tile), low = w.work.low(w.tile), high = w.work.high(w.tile);
+      const auto page_of = [&](int t) {
+        const int64_t token = int64_t(first + t) * kTokens + row;
+        return t < w.end && token >= low && token < high ? page_at(a, w.sequence, int(token)) : -1;
+      };
+      const auto scales_of = [&](int page, float& key, float& value) {
+        key = value = 0.F;
+        if (page >= 0) {
+          const size_t at = size_t(page) * a.cache.kv_heads + w.head;
+          key = a.cache.k_scales[at];
+          value = a.cache.v_scales[at];
+        }
+      };
+      const float to_log2 = a.scale * 1.4426950408889634F;
+      int page = page_of(w.begin), page_next = page_of(w.begin + 1);
+      float key_scale, value_scale;
+      scales_of(page, key_scale, value_scale);
+
+      for (int t = w.begin; t < w.end; ++t) {
+        const int page_after = page_of(t + 2);
+        float key_scale_next, value_scale_next;
+        scales_of(page_next, key_scale_next, value_scale_next);
+        // the columns that see the lane's token: query row i where token <= position0 + i < token + window
+        const int64_t ahead = int64_t(first + t) * kTokens + row - position0;
+        int from = int(max(int64_t(0), min(ahead, int64_t(N)))) * int(a.group);
+        int to = a.window ? int(max(int64_t(0), min(ahead + a.window, int64_t(token_rows)))) * int(a.group) : used;
+        if (page < 0) to = 0;
+        const bool open = __all_sync(0xffffffffu, from == 0 && to == used);
+        const float scale = key_scale * to_log2;
+
+        const int buffer = tile_count & 1;
+        wait(&s.scores_full[buffer], (tile_count >> 1) & 1, 0xa8000000u);
+        ptx::tc_fence_after_sync();
+        const uint32_t scores = lanes + L::kScores + buffer * N + column0;
+        float p[C];
+        uint32_t exponents[C / 4];                               // of the largest p * value scale of the warp's 32 tokens, in bytes
+        // false: all of them fit
+        const auto probabilities = [&]() {
+          tmem_load_columns<C>(scores, reinterpret_cast<uint32_t*>(p));
+          ptx::tmem_load_wait();
+          float most = 0.F;
+          bool beyond = false;
+#pragma unroll
+          for (int j = 0; j < C; ++j) {
+            p[j] = exp2_approx(fmaf(p[j], scale, -reference[column0 + j]));
+            if (!open) p[j] = int(column0) + j >= from && int(column0) + j < to ? p[j] : 0.F;
+            most = fmaxf(most, p[j]);
+            const uint32_t exponent = __reduce_max_sync(0xffffffffu, __float_as_uint(p[j] * value_scale)) >> 23;
+            beyond |= exponent >= kMoveExponent;                 // NaN too
+            exponents[j / 4] = j % 4 == 0 ? exponent : exponents[j / 4] | exponent << (8 * (j % 4));
+          }
+          return beyond || most >= kMost;
+        };
+        if (t == w.begin || softmax_any(probabilities())) {
+          // the reference of a column moves to the largest score so far
+          tmem_load_columns<C>(scores, reinterpret_cast<uint32_t*>(p));
+          ptx::tmem_load_wait();
+#pragma unroll
+          for (int j = 0; j < C; ++j) {
+            const float score = p[j] * scale;
+            const bool seen = int(column0) + j >= from && int(column0) + j < to && score == score;
+            const int highest = __reduce_max_sync(0xffffffffu, ordered(seen ? score : -INFINITY));
+            if (lane == uint32_t(j % 32)) by_warp[quadrant * N + column0 + j] = __int_as_float(highest ^ ((highest >> 31) & 0x7fffffff));
+          }
+          softmax_sync();
+          if (member < N) {
+            const float before = reference[member];
+            const float now = fmaxf(before, fmaxf(fmaxf(by_warp[member], by_warp[N + member]), fmaxf(by_warp[2 * N + member], by_warp[3 * N + member])));
+            reference[member] = now;
+            factor[member] = before == -INFINITY ? 0.F : exp2_approx(before - now);
+          }
+          softmax_sync();
+          if (t > w.begin) {                                     // the sums so far, once the product before is done
+            wait(&s.probs_empty, (tile_count & 1) ^ 1, 0xa9000000u);
+            ptx::tc_fence_after_sync();
+#pragma unroll
+            for (int j = 0; j < C; ++j) total[j] *= factor[column0 + j];
+            for (int c = 0; c < CH; ++c) {
+              tmem_load_columns<C>(lanes + c * N + column0, reinterpret_cast<uint32_t*>(p));
+              ptx::tmem_load_wait();
+#pragma unroll
+              for (int j = 0; j < C; ++j) p[j] *= factor[column0 + j];
+              tmem_store_columns<C>(lanes + c * N + column0, reinterpret_cast<const uint32_t*>(p));
+            }
+            ptx::tmem_store_wait();
+          }
+          probabilities();
+        }
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&s.scores_empty[buffer]);
+        if (tile_count > 0) wait(&s.probs_empty, (tile_count & 1) ^ 1, 0xaa000000u);
+        // P: the warp's 32 tokens of a column share a power of two, 2^-7 of that of the largest
+        uint32_t mine[(C + 31) / 32];
+#pragma unroll
+        for (int j = 0; j < C; j += 8) {
+          uint32_t hi[2], lo[2];
+#pragma unroll
+          for (int i = 0; i < 8; i += 4) {
+            float scaled[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t exponent = exponents[(j + i) / 4] >> (8 * e) & 255u;
+              const float up = exponent < 8 ? 0.F : __uint_as_float((261 - exponent) << 23);
+              if (lane == uint32_t((j + i + e) % 32)) mine[(j + i + e) / 32] = exponent < 8 ? 127 : exponent - 7;
+              total[j + i + e] += p[j + i + e];
+              scaled[e] = p[j + i + e] * value_scale * up;
+            }
+            uint16_t h0, l0, h1, l1;
+            two_parts(scaled[0], scaled[1], 1.F, h0, l0);
+            two_parts(scaled[2], scaled[3], 1.F, h1, l1);
+            hi[i / 4] = pack4(h0, h1);
+            lo[i / 4] = pack4(l0, l1);
+          }
+          const uint32_t byte = column0 + j;
+          uint8_t* const to_hi = probs + row * 128 + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15);
+          *reinterpret_cast<uint2*>(to_hi) = make_uint2(hi[0], hi[1]);
+          uint8_t* const to_lo = L::kOneBuffer ? probs + row * 128 + ((((byte + 64) >> 4) ^ (row & 7)) << 4) + (byte & 15) : to_hi + L::kLowOffset;
+          *reinterpret_cast<uint2*>(to_lo) = make_uint2(lo[0], lo[1]);
+        }
+#pragma unroll
+        for (int i = 0; i < (C + 31) / 32; ++i) {
+          const uint32_t column = column0 + i * 32 + lane;
+          if (i * 32 + lane < uint32_t(C)) probs_atom[column % 32 * 16 + column / 32 * 4 + quadrant] = uint8_t(mine[i]);
+        }
+        ptx::fence_proxy_async_smem();
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&s.probs_full);
+        ++tile_count;
+        page = page_next;
+        page_next = page_after;
+        key_scale = key_scale_next;
+        value_scale = value_scale_next;
+      }
+      // sums of a column over the tokens
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        float v = total[j];
+#pragma unroll
+        for (int m = 16; m; m /= 2) v += __shfl_xor_sync(0xffffffffu, v, m);
+        if (lane == uint32_t(j % 32)) by_warp[quadrant * N + column0 + j] = v;
+      }
+      softmax_sync();
+      const bool whole = w.begin == 0 && w.end == w.tiles;
+      if (member < N) {
+        const float v = (by_warp[member] + by_warp[N + member]) + (by_warp[2 * N + member] + by_warp[3 * N + member]);
+        factor[member] = whole ? (v == 0.F ? 0.F : 1.F / v) : v;
+      }
+      softmax_sync();
+      wait(&s.sums_full, item & 1, 0xab000000u);
+      ptx::tc_fence_after_sync();
+      const uint32_t place = 2 * blockIdx.x + (w.begin == 0 ? 1 : 0);
+      float* const partial = a.partial + size_t(place) * N * D;
+      if (!whole && member < N) {
+        float* const totals = a.partial + size_t(gridDim.x) * 2 * N * D + size_t(place) * 2 * N;
+        totals[member] = reference[member];
+        totals[N + member] = factor[member];
+      }
+      if (!whole && w.begin == 0 && member == 0) {
+        const int64_t parts = min(s.units, int64_t(gridDim.x));
+        a.records[blockIdx.x] = make_int4(first_row, used, w.head, part_with(s.units, w.item + w.tiles, parts));
+      }
+      for (int c = 0; c < CH; ++c) {
+        float o[C];
+        tmem_load_columns<C>(lanes + c * N + column0, reinterpret_cast<uint32_t*>(o));
+        ptx::tmem_load_wait();
+        const uint32_t d = c * 128 + row;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+          const int column = column0 + j;
+          if (column < used) {
+            if (whole) output_of(column)[d] = __float2bfloat16_rn(o[j] * factor[column]);
+            else partial[size_t(column) * D + d] = o[j];
+          }
+        }
+      }
+      ++item;
+      w.advance();
+    }
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  if (warp == 1) ptx::tmem_dealloc(tmem, L::kColumns);
+}
+
+// Joins the pieces of the items that are divided between blocks: block x looks after the item that block x of the attention kernel
+// begins and does not end.  WPC warps share a column, each with every WPC-th piece.
+template <int D, int WPC>
+__global__ void __launch_bounds__(256) attention_join_kernel(const __grid_constant__ Attention a, uint32_t blocks, uint32_t columns) {
+  constexpr int E = D / 32;
+  __shared__ float shared[WPC > 1 ? 8 : 1][D + 1];
+  griddep_enter();
+  const int4 record = a.records[blockIdx.x];
+  if (record.w < 0) return;
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, share = warp % WPC, pieces = record.w - blockIdx.x + 1;
+  const float* const totals = a.partial + size_t(blocks) * 2 * columns * D;
+  const auto place = [&](uint32_t piece) { return 2 * (blockIdx.x + piece) + (piece == 0 ? 1 : 0); };
+  for (uint32_t column = blockIdx.y * (8 / WPC) + warp / WPC; column < uint32_t(record.y); column += gridDim.y * (8 / WPC)) {
+    float highest = -INFINITY;
+    for (uint32_t p = lane; p < pieces; p += 32) highest = fmaxf(highest, totals[size_t(place(p)) * 2 * columns + column]);
+#pragma unroll
+    for (int m = 16; m; m /= 2) highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, m));
+    float sum[E] = {}, total = 0.F;
+#pragma unroll 4
+    for (uint32_t p = share; p < pieces; p += WPC) {
+      const float* const at = totals + size_t(place(p)) * 2 * columns + column;
+      const float weight = at[0] == -INFINITY ? 0.F : exp2_approx(at[0] - highest);
+      total = fmaf(weight, at[columns], total);
+      const float4* const from = reinterpret_cast<const float4*>(a.partial + (size_t(place(p)) * columns + column) * D) + lane;
+#pragma unroll
+      for (int i = 0; i < E / 4; ++i) {
+        const float4 v = from[32 * i];
+        sum[4 * i] = fmaf(weight, v.x, sum[4 * i]);
+        sum[4 * i + 1] = fmaf(weight, v.y, sum[4 * i + 1]);
+        sum[4 * i + 2] = fmaf(weight, v.z, sum[4 * i + 2]);
+        sum[4 * i + 3] = fmaf(weight, v.w, sum[4 * i + 3]);
+      }
+    }
+    if constexpr (WPC > 1) {
+      static_assert(WPC == 8, "a column a block");
+#pragma unroll
+      for (int e = 0; e < E; ++e) shared[warp][128 * (e / 4) + lane * 4 + e % 4] = sum[e];
+      if (lane == 0) shared[warp][D] = total;
+      __syncthreads();
+      bf16* const to = a.output + size_t(record.x + column / a.group) * a.output_stride + size_t(record.z * a.group + column % a.group) * D;
+      total = 0.F;
+#pragma unroll
+      for (int i = 0; i < WPC; ++i) total += shared[i][D];
+      for (uint32_t d = threadIdx.x; d < uint32_t(D); d += 256) {
+        float v = 0.F;
+#pragma unroll
+        for (int i = 0; i < WPC; ++i) v += shared[i][d];
+        to[d] = __float2bfloat16_rn(total == 0.F ? 0.F : v / total);
+      }
+      __syncthreads();
+    } else {
+      bf16* const to = a.output + size_t(record.x + column / a.group) * a.output_stride + size_t(record.z * a.group + column % a.group) * D;
+      const float inverse = total == 0.F ? 0.F : 1.F / total;
+#pragma unroll
+      for (int i = 0; i < E / 4; ++i)
+        *reinterpret_cast<uint2*>(to + 128 * i + lane * 4) = make_uint2(pair::pack_bf16x2(sum[4 * i] * inverse, sum[4 * i + 1] * inverse),
+                                                                        pair::pack_bf16x2(sum[4 * i + 2] * inverse, sum[4 * i + 3] * inverse));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+// Columns of a block: 16 or 32 where all query rows of a sequence fit, else as many as tensor memory takes next to two tiles of
+// scores (512 columns: D / 128 * N sums, 2 N scores, up to 40 of scales).
+uint32_t columns_of(uint32_t head_dim, uint32_t group, uint32_t max_rows) {
+  const uint64_t needed = uint64_t(group) * max_rows;
+  return needed <= 16 ? 16 : needed <= 32 ? 32 : head_dim == 512 ? 64 : head_dim == 256 ? 96 : 128;
+}
+
+size_t partial_floats(uint32_t blocks, uint32_t columns, uint32_t head_dim) { return size_t(blocks) * 2 * columns * (head_dim + 2); }
+
+template <int D, int N>
+cudaError_t launch_attention(const Attention& a, const CUtensorMap& k_map, const CUtensorMap& v_map, uint32_t blocks, cudaStream_t stream) {
+  static bool known[kMaxDeviceSlots] = {};            // plain bools: two threads write the same
+  bool& ready = known[current_device_slot()];
+  if (!ready) {
+    const cudaError_t status = cudaFuncSetAttribute(paged_attention_kernel<D, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D, N>::kSmemBytes);
+    if (status != cudaSuccess) return status;
+    ready = true;
+  }
+  const cudaError_t status = launch_pdl_shared(paged_attention_kernel<D, N>, blocks, kThreads, Layout<D, N>::kSmemBytes, stream, k_map, v_map, a);
+  if (status != cudaSuccess) return status;
+  if constexpr (N <= 32) return launch_pdl(attention_join_kernel<D, 8>, dim3(blocks, N), 256, stream, a, blocks, uint32_t(N));
+  else return launch_pdl(attention_join_kernel<D, 1>, dim3(blocks, 4), 256, stream, a, blocks, uint32_t(N));
+}
+
+template <int D, int MOST>
+cudaError_t launch_columns(uint32_t columns, const Attention& a, const CUtensorMap& k_map, const CUtensorMap& v_map, uint32_t blocks, cudaStream_t stream) {
+  return columns == 16   ? launch_attention<D, 16>(a, k_map, v_map, blocks, stream)
+         : columns == 32 ? launch_attention<D, 32>(a, k_map, v_map, blocks, stream)
+                         : launch_attention<D, MOST>(a, k_map, v_map, blocks, stream);
 }
 
 }  // namespace
@@ -87,7 +892,11 @@ uint32_t gw::take_paged_attention_error() {
 
 extern "C" {
 
-size_t gw_paged_attention_scratch_bytes(const gw_kv_cache*, const gw_sequences*, uint32_t) { return 256; }
+size_t gw_paged_attention_scratch_bytes(const gw_kv_cache* cache, const gw_sequences* batch, uint32_t heads) {
+  if (!cache || !batch || cache->kv_heads == 0 || heads < cache->kv_heads) return 256;
+  const uint32_t blocks = sm_count(), columns = columns_of(cache->head_dim, heads / cache->kv_heads, std::max(1u, batch->max_rows));
+  return align_up(partial_floats(blocks, columns, cache->head_dim) * sizeof(float), 256) + align_up(blocks * sizeof(int4), 256);
+}
 
 gw_status gw_paged_attention_bf16(const gw_kv_cache* cache, const gw_sequences* batch, const void* query_bf16,
                                   uint64_t query_stride, uint32_t heads, float scale, uint32_t window, void* output_bf16,
@@ -106,13 +915,21 @@ gw_status gw_paged_attention_bf16(const gw_kv_cache* cache, const gw_sequences* 
   const size_t needed = gw_paged_attention_scratch_bytes(cache, batch, heads);
   if (!scratch || reinterpret_cast<uintptr_t>(scratch) % 256 != 0 || scratch_capacity < needed)
     return fail(GW_INVALID_ARGUMENT, "paged attention requires " + std::to_string(needed) + " bytes of 256-byte aligned scratch");
+  const uint32_t group = heads / cache->kv_heads, columns = columns_of(cache->head_dim, group, batch->max_rows), blocks = sm_count();
+  CUtensorMap k_map, v_map;
+  std::string error;
+  const uint64_t rows = uint64_t(cache->pages) * cache->kv_heads * cache->page_tokens;
+  if (!encode_tensor_map_2d(&k_map, cache->k_data, cache->head_dim, rows, cache->page_tokens, &error, 0) ||
+      !encode_tensor_map_2d(&v_map, cache->v_data, cache->head_dim, rows, cache->page_tokens, &error, 0))
+    return fail(GW_CUDA_ERROR, "paged attention: " + error);
+  const size_t floats = align_up(partial_floats(blocks, columns, cache->head_dim) * sizeof(float), 256);
   const Attention a{*cache, *batch, static_cast<const bf16*>(query_bf16), static_cast<bf16*>(output_bf16), query_stride, output_stride,
-                    heads, heads / cache->kv_heads, window, scale};
-  const uint64_t tasks = uint64_t(batch->rows) * heads;
-  GW_CUDA_CHECK(launch_pdl(cache->head_dim == 128   ? paged_attention_kernel<4>
-                           : cache->head_dim == 256 ? paged_attention_kernel<8>
-                                                    : paged_attention_kernel<16>,
-                           uint32_t((tasks + 3) / 4), 128, as_stream(stream), a),
+                    heads, group, columns / group, window > (1u << 30) ? 0 : window, scale,
+                    static_cast<float*>(scratch), reinterpret_cast<int4*>(static_cast<uint8_t*>(scratch) + floats)};
+  const cudaStream_t s = as_stream(stream);
+  GW_CUDA_CHECK((cache->head_dim == 128   ? launch_columns<128, 128>(columns, a, k_map, v_map, blocks, s)
+                 : cache->head_dim == 256 ? launch_columns<256, 96>(columns, a, k_map, v_map, blocks, s)
+                                          : launch_columns<512, 64>(columns, a, k_map, v_map, blocks, s)),
                 "paged attention");
   return GW_OK;
 }
