@@ -18,21 +18,23 @@ namespace gw {
 
 constexpr int kTokens = 128;      // cached tokens of a tile
 
-// sum of (a * i + b) / m over i < n, by the steps of Euclid's algorithm
-GW_HOST_DEVICE int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
-  int64_t sum = 0;
-  while (n > 0) {
-    sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
-    a %= m;
-    b %= m;
-    const int64_t last = a * n + b;
+// sum of (a * i + b) / kTokens over i < n, n up to 2^24 and a up to kTokens, by the steps of Euclid's algorithm.  After the first one
+// 32 bits hold everything but the sum, and 32-bit divisions take a fifth of the time that 64-bit ones take.
+GW_HOST_DEVICE int64_t floor_sum(int32_t count, int32_t slope, int64_t start) {
+  int64_t sum = int64_t(count) * (count - 1) / 2 * (slope / kTokens) + count * (start / kTokens);
+  uint32_t n = uint32_t(count), m = kTokens, a = uint32_t(slope % kTokens), b = uint32_t(start % kTokens);
+  while (true) {
+    const uint32_t last = a * n + b;              // a, b < m <= kTokens
+    if (last < m) return sum;
     n = last / m;
     b = last % m;
-    const int64_t t = m;
+    const uint32_t t = m;
     m = a;
     a = t;
+    sum += int64_t(n) * (n - 1) / 2 * (a / m) + int64_t(n) * (b / m);
+    a %= m;
+    b %= m;
   }
-  return sum;
 }
 
 // One sequence: `rows` query rows, the first at position `base` (below 0: no token), `per_tile` rows a query tile, and a window of
@@ -59,23 +61,14 @@ struct SequenceWork {
     int64_t units = tile;
     if (whole < tile) units += token_tiles(whole);
     const int64_t skip_high = base >= 0 ? 0 : -int64_t(base) / per_tile;      // tiles without any token
-    if (whole > skip_high) units += floor_sum(whole - skip_high, kTokens, per_tile, base + (skip_high + 1) * per_tile + kTokens - 1);
+    if (whole > skip_high) units += floor_sum(int32_t(whole - skip_high), per_tile, base + (skip_high + 1) * per_tile + kTokens - 1);
     if (window != 0) {
       const int64_t start = int64_t(base) - window + 1, skip_low = start >= 0 ? 0 : (-start + per_tile - 1) / per_tile;
-      if (whole > skip_low) units -= floor_sum(whole - skip_low, kTokens, per_tile, start + skip_low * per_tile);
+      if (whole > skip_low) units -= floor_sum(int32_t(whole - skip_low), per_tile, start + skip_low * per_tile);
     }
     return units;
   }
   GW_HOST_DEVICE int64_t units() const { return units_before(query_tiles()); }
-  // the query tile that has unit `at` of the sequence's units()
-  GW_HOST_DEVICE int32_t tile_with(int64_t at) const {
-    int32_t lowest = 0, highest = query_tiles();
-    while (lowest + 1 < highest) {
-      const int32_t middle = lowest + (highest - lowest) / 2;
-      if (units_before(middle) <= at) lowest = middle; else highest = middle;
-    }
-    return lowest;
-  }
 };
 
 // Range `part` of `parts` equal ones.

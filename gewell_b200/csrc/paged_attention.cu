@@ -14,13 +14,14 @@
 // of two for every 32 elements along the sum) gives every 32 elements of a query, and every 32 tokens of a column of P -- those
 // of one warp -- a range of their own, so that small probabilities are as exact as large ones, however far below the maximum.
 // That also takes the running maximum out of the loop: the reference m of a column only has to keep FP32 sums from
-// overflowing.  It is the maximum of the first tile, and is moved (with the sums rescaled) only when a probability exceeds 2^80.
+// overflowing.  It is the maximum of the first tile, and is moved (with the sums rescaled) only when a probability times its value scale
+// exceeds 2^40.  (Value scales below 2^-64 are taken for 2^-64 there, so no probability can pass 2^104 unseen.)
 //
 //   warp 0      TMA: chunks of [128 tokens x 128 bytes] of K and V into a ring, page by page
 //   warp 1      tcgen05.mma: S of tile t + 1, then O += P V of tile t.  Rows of V that no query may see are zeroed here: a
 //               page's slots behind its last token may hold anything, NaN included, and 0 * NaN is NaN.
-//   warps 2..9  softmax: two warps for every 32 lanes, each half of the columns; queries into shared memory at the start of an item,
-//               results out at its end
+//   the others  softmax: for every 32 lanes two warps (16 and 32 columns) or four, each with its share of the columns; queries into
+//               shared memory at the start of an item, results out at its end
 //
 // Work: attention_work.h.  An item that a cut between two blocks' ranges divides leaves FP32 partial sums in the scratch
 // memory, which a second kernel joins in the order of the blocks (the same bits on every run).
@@ -41,12 +42,10 @@ namespace {
 
 __device__ uint32_t g_attention_error;       // first report since it was last taken
 
-constexpr int kSoftmaxWarps = 8;
-constexpr int kThreads = 32 * (2 + kSoftmaxWarps);
+__host__ __device__ constexpr int softmax_warps(int columns) { return columns <= 32 ? 8 : 16; }
 constexpr int kChunkBytes = kTokens * 128;
 constexpr int kAtomBytes = 512;              // scale atom: 128 rows x 4 blocks of 32 elements
-constexpr uint32_t kMoveExponent = 127 + 80;      // a probability over its reference from which on the reference moves
-constexpr float kMost = 1.2089258196146292e24F;   // 2^80
+constexpr uint32_t kMoveBits = (127u + 40u) << 23;
 
 struct Attention {
   gw_kv_cache cache;
@@ -68,7 +67,7 @@ struct Layout {
   static constexpr int kProbBytes = kOneBuffer ? kChunkBytes : 2 * kChunkBytes;
   static constexpr int kLowOffset = kOneBuffer ? 64 : kChunkBytes;
   static constexpr int kAtoms = 2 * kChunks + 2;                  // queries (both parts), ones, P
-  static constexpr int kSmall = kAtoms * kAtomBytes + 6 * N * 4 + 1024;      // and what is declared as Shared
+  static constexpr int kSmall = kAtoms * kAtomBytes + 6 * N * 4 + 8 * N + 1024;      // and what is declared as Shared
   static constexpr int kRoom = 227 * 1024 - 1024 - 2 * kQueryBytes - kProbBytes - kSmall;
   static constexpr int kRing = kRoom / kChunkBytes > 16 ? 16 : kRoom / kChunkBytes;
   static constexpr int kSmemBytes = 2 * kQueryBytes + kProbBytes + kRing * kChunkBytes + kSmall;      // 1024 bytes of it for the alignment
@@ -81,7 +80,10 @@ struct Layout {
   static_assert(kProbScales + 4 <= kColumns, "tensor memory over-subscribed");
   static_assert(kRing >= kChunks + 1, "a tile's chunks and one more");
   static_assert(kSmemBytes + 1024 <= 227 * 1024 && kSmemBytes > 116 * 1024, "one block an SM");
-  static_assert(N % 16 == 0 && N <= 128 && D % 128 == 0, "");
+  static constexpr int kSoftmaxWarps = softmax_warps(N);
+  static constexpr int kThreads = 32 * (2 + kSoftmaxWarps);
+  static constexpr int kShare = N / (kSoftmaxWarps / 4);          // columns of a warp
+  static_assert(N % 16 == 0 && N <= 128 && D % 128 == 0 && kShare % 8 == 0 && kShare <= 32, "");
 };
 
 struct Shared {
@@ -89,6 +91,7 @@ struct Shared {
   uint32_t tensor_memory;
   // units of all blocks, the block's range of them, and the item that has the first
   int64_t units, from, to, item;
+  int64_t rest;                // units of that item's sequence and head in front of the range
   uint32_t sequence;
   int head, tile;
 };
@@ -148,62 +151,91 @@ struct Walk {
   }
 };
 
+__device__ __forceinline__ SequenceWork sequence_work(const Attention& a, uint32_t s, bool report) {
+  const SequenceRows r = sequence_rows(a.batch, s);
+  if (r.bad && report) atomicCAS(&g_attention_error, 0u, 0xa2000000u | (s & 0xffffffu));
+  return SequenceWork{r.context - r.count, r.count, int32_t(a.per_tile), int32_t(a.window)};
+}
+
 // The block's range of units and the item that its first unit belongs to.
+template <int THREADS>
 __device__ __forceinline__ void find_start(const Attention& a, Shared& shared) {
-  constexpr int WARPS = kThreads / 32;
+  constexpr int WARPS = THREADS / 32;
   __shared__ int64_t sums[WARPS];
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  int64_t before = 0, total = 0, from = 0;
-  // first the total, then the sequence that has unit `from`
-  for (int pass = 0; pass < 2; ++pass) {
-    before = 0;
-    for (uint32_t base = 0; base < a.batch.sequences; base += kThreads) {
-      const uint32_t s = base + threadIdx.x;
-      int64_t mine = 0;
-      SequenceWork w{0, 0, 1, 0};
-      if (s < a.batch.sequences) {
-        const SequenceRows r = sequence_rows(a.batch, s);
-        if (r.bad && pass == 0 && blockIdx.x == 0) atomicCAS(&g_attention_error, 0u, 0xa2000000u | (s & 0xffffffu));
-        w = SequenceWork{r.context - r.count, r.count, int32_t(a.per_tile), int32_t(a.window)};
-        mine = w.units() * a.cache.kv_heads;
-      }
-      int64_t sum = mine;
+  int64_t total = 0, from = 0, mine = 0, low = 0;
+  // units in front of sequence base + threadIdx.x, over `before` ones in front of sequence base; returns those behind the last one
+  const auto scan = [&](uint32_t base, int64_t before, bool report) {
+    const uint32_t s = base + threadIdx.x;
+    mine = s < a.batch.sequences ? sequence_work(a, s, report).units() * a.cache.kv_heads : 0;
+    int64_t sum = mine;
 #pragma unroll
-      for (int m = 1; m < 32; m *= 2) {
-        const int64_t other = __shfl_up_sync(0xffffffffu, sum, m);
-        if (lane >= uint32_t(m)) sum += other;
-      }
-      if (lane == 31) sums[warp] = sum;
-      __syncthreads();
-      int64_t low = before + sum - mine;
-#pragma unroll
-      for (int i = 0; i < WARPS; ++i) {
-        if (uint32_t(i) < warp) low += sums[i];
-        before += sums[i];
-      }
-      if (pass == 1 && low <= from && from < low + mine) {
-        const int64_t units = w.units(), at = from - low;
-        shared.sequence = s;
-        shared.head = int(at / units);
-        shared.tile = w.tile_with(at % units);
-        shared.item = low + shared.head * units + w.units_before(shared.tile);
-      }
-      __syncthreads();
+    for (int m = 1; m < 32; m *= 2) {
+      const int64_t other = __shfl_up_sync(0xffffffffu, sum, m);
+      if (lane >= uint32_t(m)) sum += other;
     }
-    if (pass == 0) {
-      total = before;
-      const int64_t parts = total < gridDim.x ? total : gridDim.x;
-      const bool idle = int64_t(blockIdx.x) >= parts;
-      from = idle ? total : range_start(total, blockIdx.x, parts);
-      if (threadIdx.x == 0) {
-        shared.units = total;
-        shared.from = from;
-        shared.to = idle ? total : range_start(total, blockIdx.x + 1, parts);
-        shared.item = total;
-        shared.sequence = a.batch.sequences;
-        shared.head = shared.tile = 0;
+    if (lane == 31) sums[warp] = sum;
+    __syncthreads();
+    low = before + sum - mine;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+      if (uint32_t(i) < warp) low += sums[i];
+      before += sums[i];
+    }
+    return before;
+  };
+  const auto found = [&](uint32_t base) {
+    if (low <= from && from < low + mine) {
+      const int64_t units = mine / a.cache.kv_heads, at = from - low;
+      shared.sequence = base + threadIdx.x;
+      shared.head = int(at / units);
+      shared.rest = at - shared.head * units;
+      shared.item = from - shared.rest;
+    }
+  };
+  const bool one = a.batch.sequences <= THREADS;
+  for (uint32_t base = 0; base < a.batch.sequences; base += THREADS) {
+    total = scan(base, total, blockIdx.x == 0);
+    if (!one) __syncthreads();
+  }
+  const int64_t parts = total < gridDim.x ? total : gridDim.x;
+  const bool idle = int64_t(blockIdx.x) >= parts;
+  from = idle ? total : range_start(total, blockIdx.x, parts);
+  if (threadIdx.x == 0) {
+    shared.units = total;
+    shared.from = from;
+    shared.to = idle ? total : range_start(total, blockIdx.x + 1, parts);
+    if (idle) shared.sequence = a.batch.sequences;
+    shared.tile = 0;
+  }
+  if (!idle) {
+    if (one) {
+      found(0);
+    } else {
+      int64_t before = 0;
+      for (uint32_t base = 0; base < a.batch.sequences && before <= from; base += THREADS) {
+        before = scan(base, before, false);
+        found(base);
+        __syncthreads();
       }
-      if (idle) break;
+    }
+  }
+  __syncthreads();
+  // the query tile, 32 candidates at a time
+  if (warp == 0 && !idle) {
+    const SequenceWork w = sequence_work(a, shared.sequence, false);
+    const int64_t rest = shared.rest;
+    int lowest = 0, highest = w.query_tiles();                 // units_before(lowest) <= rest < units_before(highest)
+    while (highest - lowest > 1) {
+      const int step = (highest - lowest + 31) / 32, candidate = min(lowest + int(lane) * step, highest);
+      const uint32_t below = __ballot_sync(0xffffffffu, candidate < highest && w.units_before(candidate) <= rest);
+      const int at = 31 - __clz(below);
+      highest = min(lowest + (at + 1) * step, highest);
+      lowest += at * step;
+    }
+    if (lane == 0) {
+      shared.tile = lowest;
+      shared.item += w.units_before(lowest);
     }
   }
   __syncthreads();
@@ -284,8 +316,10 @@ __device__ __forceinline__ void tmem_store_columns(uint32_t address, const uint3
   if constexpr (C % 16 != 0) tmem_store<8>(address + C - 8, r + C - 8);
 }
 
-__device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(32 * kSoftmaxWarps) : "memory"); }
+template <int THREADS>
+__device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(THREADS) : "memory"); }
 // whether the condition holds for any thread of the softmax warps
+template <int THREADS>
 __device__ __forceinline__ bool softmax_any(bool mine) {
   uint32_t any;
   asm volatile(
@@ -293,8 +327,31 @@ __device__ __forceinline__ bool softmax_any(bool mine) {
       "setp.ne.u32 p, %1, 0;\n\t"
       "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(any) : "r"(uint32_t(mine)), "n"(32 * kSoftmaxWarps) : "memory");
+      : "=r"(any) : "r"(uint32_t(mine)), "n"(THREADS) : "memory");
   return any != 0;
+}
+// v[j] summed over the lanes, for C columns (a power of two up to 32, or 24): lane j % 32 gets column j's (lanes beyond C: any)
+template <int C>
+__device__ __forceinline__ float lane_sums(float* v, uint32_t lane) {
+  if constexpr (C == 24) {
+    const float first = lane_sums<16>(v, lane), second = lane_sums<8>(v + 16, lane);
+    return lane < 16 ? first : second;
+  } else {
+#pragma unroll
+    for (int m = 16; m >= C; m /= 2)
+#pragma unroll
+      for (int j = 0; j < C; ++j) v[j] += __shfl_xor_sync(0xffffffffu, v[j], m);
+#pragma unroll
+    for (int m = C / 2; m; m /= 2) {
+      const bool upper = (lane & m) != 0;
+#pragma unroll
+      for (int j = 0; j < m; ++j) {
+        const float other = __shfl_xor_sync(0xffffffffu, upper ? v[j] : v[j + m], m);
+        v[j] = (upper ? v[j + m] : v[j]) + other;
+      }
+    }
+    return v[0];
+  }
 }
 // order-preserving integer of a float that is no NaN
 __device__ __forceinline__ int ordered(float v) {
@@ -306,11 +363,12 @@ __device__ __forceinline__ int ordered(float v) {
 // the kernel
 // ---------------------------------------------------------------------------
 template <int D, int N>
-__global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
+__global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_kernel(const __grid_constant__ CUtensorMap k_map,
                                                                       const __grid_constant__ CUtensorMap v_map,
                                                                       const __grid_constant__ Attention a) {
   using L = Layout<D, N>;
-  constexpr int CH = L::kChunks, RING = L::kRing, C = N / 2;
+  constexpr int CH = L::kChunks, RING = L::kRing, C = L::kShare, kSoftmaxWarps = L::kSoftmaxWarps, kSoftmaxThreads = 32 * kSoftmaxWarps,
+                kThreads = L::kThreads;
   extern __shared__ uint8_t raw[];
   uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t* const query_hi = base;
@@ -323,6 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
   float* const reference = reinterpret_cast<float*>(probs_atom + kAtomBytes);     // [N] m of a column
   float* const factor = reference + N;                                            // [N]
   float* const by_warp = factor + N;                                              // [4][N]
+  bf16** const output_at = reinterpret_cast<bf16**>(by_warp + 4 * N);             // [N]
   __shared__ Shared s;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
@@ -354,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
   ptx::fence_proxy_async_smem();
   ptx::tc_fence_before_sync();
   griddep_enter();
-  find_start(a, s);                                              // ends with __syncthreads()
+  find_start<kThreads>(a, s);                                    // ends with __syncthreads()
   ptx::tc_fence_after_sync();
   const uint32_t tmem = s.tensor_memory;
   const auto failed = [](uint32_t code) {
@@ -521,9 +580,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
     ptx::mbar_wait_warp(&s.drained, 0, 0, 100000000ull);
   } else {
     // ----- softmax
-    const uint32_t quadrant = warp & 3, half = (warp - 2) / 4, column0 = half * C, member = threadIdx.x - 64;
+    const uint32_t quadrant = warp & 3, column0 = (warp - 2) / 4 * C, member = threadIdx.x - 64;
     const uint32_t lanes = tmem + (quadrant * 32 << 16);
     const uint32_t row = quadrant * 32 + lane;                   // the lane's token in a tile
+    const uint32_t group = a.group;
     int item = 0, tile_count = 0;
     if (member == 0) a.records[blockIdx.x] = make_int4(0, 0, 0, -1);
     // A thread whose wait ran out waits no more, but goes on to the barriers that it shares with the others.
@@ -535,25 +595,30 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
     w.start(a, s);
     while (w.next(a, s)) {
       const int token_rows = min(int(a.per_tile), w.rows.count - w.tile * int(a.per_tile));
-      const int used = token_rows * int(a.group);                // columns of queries
+      const int used = token_rows * int(group);                  // columns of queries
       const int first_row = w.rows.first + w.tile * int(a.per_tile), position0 = w.work.base + w.tile * int(a.per_tile);
-      const uint32_t head0 = w.head * a.group;
-      const auto output_of = [&](int column) {
-        return a.output + size_t(first_row + column / int(a.group)) * a.output_stride + size_t(head0 + column % int(a.group)) * D;
-      };
+      const uint32_t head0 = w.head * group;
+      if (int(member) < N) {
+        const uint32_t at = member / group;
+        output_at[member] = a.output + size_t(first_row + at) * a.output_stride + size_t(head0 + member - at * group) * D;
+        reference[member] = int(member) < used ? -INFINITY : 0.F;        // scores without a query are 0
+      }
       if (w.tiles == 0) {                                        // rows that see nothing
+        softmax_sync<kSoftmaxThreads>();
         for (int column = warp - 2; column < used; column += kSoftmaxWarps)
-          for (int d = lane * 8; d < D; d += 256) *reinterpret_cast<uint4*>(output_of(column) + d) = make_uint4(0, 0, 0, 0);
+          for (int d = lane * 8; d < D; d += 256) *reinterpret_cast<uint4*>(output_at[column] + d) = make_uint4(0, 0, 0, 0);
+        softmax_sync<kSoftmaxThreads>();
         w.advance();
         continue;
       }
       // queries: a thread takes 32 elements at a time, which share a power of two
-      for (int block = member; block < N * (D / 32); block += 32 * kSoftmaxWarps) {
+      for (int block = member; block < N * (D / 32); block += kSoftmaxThreads) {
         const int column = block / (D / 32), part = block % (D / 32), c = part / 4, k = part % 4;
         uint4 bits[4];
         if (column < used) {
-          const uint4* from = reinterpret_cast<const uint4*>(a.query + size_t(first_row + column / int(a.group)) * a.query_stride +
-                                                             size_t(head0 + column % int(a.group)) * D + part * 32);
+          const uint32_t at = uint32_t(column) / group;
+          const uint4* from = reinterpret_cast<const uint4*>(a.query + size_t(first_row + at) * a.query_stride +
+                                                             size_t(head0 + column - at * group) * D + part * 32);
 #pragma unroll
           for (int i = 0; i < 4; ++i) bits[i] = from[i];
         } else {
@@ -588,12 +653,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
         atoms[scale_at] = uint8_t(scale);
         atoms[scale_at + kAtomBytes] = uint8_t(scale - 4);
       }
-      if (member < N) reference[member] = int(member) < used ? -INFINITY : 0.F;      // scores without a query are 0
       ptx::fence_proxy_async_smem();
       ptx::tc_fence_before_sync();                               // the results of the item before were read
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&s.query_full);
-      softmax_sync();                                            // `reference`
+      softmax_sync<kSoftmaxThreads>();                           // `reference`, `output_at`
 
       float total[C];
 #pragma unroll
@@ -622,54 +686,52 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
         scales_of(page_next, key_scale_next, value_scale_next);
         // the columns that see the lane's token: query row i where token <= position0 + i < token + window
         const int64_t ahead = int64_t(first + t) * kTokens + row - position0;
-        int from = int(max(int64_t(0), min(ahead, int64_t(N)))) * int(a.group);
-        int to = a.window ? int(max(int64_t(0), min(ahead + a.window, int64_t(token_rows)))) * int(a.group) : used;
+        const int from = int(max(int64_t(0), min(ahead, int64_t(N)))) * int(group);
+        int to = a.window ? int(max(int64_t(0), min(ahead + a.window, int64_t(token_rows)))) * int(group) : used;
         if (page < 0) to = 0;
         const bool open = __all_sync(0xffffffffu, from == 0 && to == used);
-        const float scale = key_scale * to_log2;
+        const uint32_t seen_from = from - column0, seen_span = to > from ? to - from : 0;       // column0 + j - from < span, unsigned
+        const float scale = key_scale * to_log2, bound_scale = fmaxf(value_scale, 5.42101086e-20F);       // 2^-64
 
         const int buffer = tile_count & 1;
         wait(&s.scores_full[buffer], (tile_count >> 1) & 1, 0xa8000000u);
         ptx::tc_fence_after_sync();
         const uint32_t scores = lanes + L::kScores + buffer * N + column0;
         float p[C];
-        uint32_t exponents[C / 4];                               // of the largest p * value scale of the warp's 32 tokens, in bytes
-        // false: all of them fit
-        const auto probabilities = [&]() {
+        uint32_t largest = 0;                                    // lane j: of column j, p * value scale over the warp's 32 tokens
+        // Once, or again after the reference moved, which it does at the first tile.
+        for (bool moved = false;; moved = true) {
           tmem_load_columns<C>(scores, reinterpret_cast<uint32_t*>(p));
           ptx::tmem_load_wait();
-          float most = 0.F;
-          bool beyond = false;
+          if (moved || t > w.begin) {
 #pragma unroll
-          for (int j = 0; j < C; ++j) {
-            p[j] = exp2_approx(fmaf(p[j], scale, -reference[column0 + j]));
-            if (!open) p[j] = int(column0) + j >= from && int(column0) + j < to ? p[j] : 0.F;
-            most = fmaxf(most, p[j]);
-            const uint32_t exponent = __reduce_max_sync(0xffffffffu, __float_as_uint(p[j] * value_scale)) >> 23;
-            beyond |= exponent >= kMoveExponent;                 // NaN too
-            exponents[j / 4] = j % 4 == 0 ? exponent : exponents[j / 4] | exponent << (8 * (j % 4));
+            for (int j = 0; j < C; ++j) {
+              p[j] = exp2_approx(fmaf(p[j], scale, -reference[column0 + j]));
+              if (!open) p[j] = uint32_t(j) - seen_from < seen_span ? p[j] : 0.F;
+              const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(p[j] * bound_scale));
+              if (lane == uint32_t(j)) largest = bits;
+            }
+            // NaN counts as beyond too
+            if (moved || !softmax_any<kSoftmaxThreads>(lane < uint32_t(C) && largest > kMoveBits)) break;
+            tmem_load_columns<C>(scores, reinterpret_cast<uint32_t*>(p));
+            ptx::tmem_load_wait();
           }
-          return beyond || most >= kMost;
-        };
-        if (t == w.begin || softmax_any(probabilities())) {
           // the reference of a column moves to the largest score so far
-          tmem_load_columns<C>(scores, reinterpret_cast<uint32_t*>(p));
-          ptx::tmem_load_wait();
 #pragma unroll
           for (int j = 0; j < C; ++j) {
             const float score = p[j] * scale;
-            const bool seen = int(column0) + j >= from && int(column0) + j < to && score == score;
+            const bool seen = uint32_t(j) - seen_from < seen_span && score == score;
             const int highest = __reduce_max_sync(0xffffffffu, ordered(seen ? score : -INFINITY));
-            if (lane == uint32_t(j % 32)) by_warp[quadrant * N + column0 + j] = __int_as_float(highest ^ ((highest >> 31) & 0x7fffffff));
+            if (lane == uint32_t(j)) by_warp[quadrant * N + column0 + j] = __int_as_float(highest ^ ((highest >> 31) & 0x7fffffff));
           }
-          softmax_sync();
+          softmax_sync<kSoftmaxThreads>();
           if (member < N) {
             const float before = reference[member];
             const float now = fmaxf(before, fmaxf(fmaxf(by_warp[member], by_warp[N + member]), fmaxf(by_warp[2 * N + member], by_warp[3 * N + member])));
             reference[member] = now;
             factor[member] = before == -INFINITY ? 0.F : exp2_approx(before - now);
           }
-          softmax_sync();
+          softmax_sync<kSoftmaxThreads>();
           if (t > w.begin) {                                     // the sums so far, once the product before is done
             wait(&s.probs_empty, (tile_count & 1) ^ 1, 0xa9000000u);
             ptx::tc_fence_after_sync();
@@ -684,44 +746,40 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
             }
             ptx::tmem_store_wait();
           }
-          probabilities();
         }
         ptx::tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&s.scores_empty[buffer]);
-        if (tile_count > 0) wait(&s.probs_empty, (tile_count & 1) ^ 1, 0xaa000000u);
         // P: the warp's 32 tokens of a column share a power of two, 2^-7 of that of the largest
-        uint32_t mine[(C + 31) / 32];
+        const uint32_t exponent = largest >> 23;
+        const float up = exponent < 8 ? 0.F : __uint_as_float((261 - exponent) << 23);
+        uint32_t hi[C / 4], lo[C / 4];
+#pragma unroll
+        for (int j = 0; j < C; j += 4) {
+          float scaled[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            total[j + e] += p[j + e];
+            scaled[e] = p[j + e] * (__shfl_sync(0xffffffffu, up, j + e) * value_scale);
+          }
+          uint16_t h0, l0, h1, l1;
+          two_parts(scaled[0], scaled[1], 1.F, h0, l0);
+          two_parts(scaled[2], scaled[3], 1.F, h1, l1);
+          hi[j / 4] = pack4(h0, h1);
+          lo[j / 4] = pack4(l0, l1);
+        }
+        if (tile_count > 0) wait(&s.probs_empty, (tile_count & 1) ^ 1, 0xaa000000u);
 #pragma unroll
         for (int j = 0; j < C; j += 8) {
-          uint32_t hi[2], lo[2];
-#pragma unroll
-          for (int i = 0; i < 8; i += 4) {
-            float scaled[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t exponent = exponents[(j + i) / 4] >> (8 * e) & 255u;
-              const float up = exponent < 8 ? 0.F : __uint_as_float((261 - exponent) << 23);
-              if (lane == uint32_t((j + i + e) % 32)) mine[(j + i + e) / 32] = exponent < 8 ? 127 : exponent - 7;
-              total[j + i + e] += p[j + i + e];
-              scaled[e] = p[j + i + e] * value_scale * up;
-            }
-            uint16_t h0, l0, h1, l1;
-            two_parts(scaled[0], scaled[1], 1.F, h0, l0);
-            two_parts(scaled[2], scaled[3], 1.F, h1, l1);
-            hi[i / 4] = pack4(h0, h1);
-            lo[i / 4] = pack4(l0, l1);
-          }
           const uint32_t byte = column0 + j;
           uint8_t* const to_hi = probs + row * 128 + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15);
-          *reinterpret_cast<uint2*>(to_hi) = make_uint2(hi[0], hi[1]);
+          *reinterpret_cast<uint2*>(to_hi) = make_uint2(hi[j / 4], hi[j / 4 + 1]);
           uint8_t* const to_lo = L::kOneBuffer ? probs + row * 128 + ((((byte + 64) >> 4) ^ (row & 7)) << 4) + (byte & 15) : to_hi + L::kLowOffset;
-          *reinterpret_cast<uint2*>(to_lo) = make_uint2(lo[0], lo[1]);
+          *reinterpret_cast<uint2*>(to_lo) = make_uint2(lo[j / 4], lo[j / 4 + 1]);
         }
-#pragma unroll
-        for (int i = 0; i < (C + 31) / 32; ++i) {
-          const uint32_t column = column0 + i * 32 + lane;
-          if (i * 32 + lane < uint32_t(C)) probs_atom[column % 32 * 16 + column / 32 * 4 + quadrant] = uint8_t(mine[i]);
+        if (lane < uint32_t(C)) {
+          const uint32_t column = column0 + lane;
+          probs_atom[column % 32 * 16 + column / 32 * 4 + quadrant] = uint8_t(exponent < 8 ? 127 : exponent - 7);
         }
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before_sync();
@@ -734,20 +792,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
         value_scale = value_scale_next;
       }
       // sums of a column over the tokens
-#pragma unroll
-      for (int j = 0; j < C; ++j) {
-        float v = total[j];
-#pragma unroll
-        for (int m = 16; m; m /= 2) v += __shfl_xor_sync(0xffffffffu, v, m);
-        if (lane == uint32_t(j % 32)) by_warp[quadrant * N + column0 + j] = v;
-      }
-      softmax_sync();
+      const float mine = lane_sums<C>(total, lane);
+      if (lane < uint32_t(C)) by_warp[quadrant * N + column0 + lane] = mine;
+      softmax_sync<kSoftmaxThreads>();
       const bool whole = w.begin == 0 && w.end == w.tiles;
       if (member < N) {
         const float v = (by_warp[member] + by_warp[N + member]) + (by_warp[2 * N + member] + by_warp[3 * N + member]);
         factor[member] = whole ? (v == 0.F ? 0.F : 1.F / v) : v;
       }
-      softmax_sync();
+      softmax_sync<kSoftmaxThreads>();
       wait(&s.sums_full, item & 1, 0xab000000u);
       ptx::tc_fence_after_sync();
       const uint32_t place = 2 * blockIdx.x + (w.begin == 0 ? 1 : 0);
@@ -766,17 +819,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
         tmem_load_columns<C>(lanes + c * N + column0, reinterpret_cast<uint32_t*>(o));
         ptx::tmem_load_wait();
         const uint32_t d = c * 128 + row;
+        if (whole) {
 #pragma unroll
-        for (int j = 0; j < C; ++j) {
-          const int column = column0 + j;
-          if (column < used) {
-            if (whole) output_of(column)[d] = __float2bfloat16_rn(o[j] * factor[column]);
-            else partial[size_t(column) * D + d] = o[j];
-          }
+          for (int j = 0; j < C; ++j)
+            if (int(column0) + j < used) output_at[column0 + j][d] = __float2bfloat16_rn(o[j] * factor[column0 + j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < C; ++j)
+            if (int(column0) + j < used) partial[size_t(column0 + j) * D + d] = o[j];
         }
       }
       ++item;
       w.advance();
+      softmax_sync<kSoftmaxThreads>();                           // `output_at`, `factor`, `reference` are free
     }
   }
   ptx::tc_fence_before_sync();
@@ -867,7 +922,7 @@ cudaError_t launch_attention(const Attention& a, const CUtensorMap& k_map, const
     if (status != cudaSuccess) return status;
     ready = true;
   }
-  const cudaError_t status = launch_pdl_shared(paged_attention_kernel<D, N>, blocks, kThreads, Layout<D, N>::kSmemBytes, stream, k_map, v_map, a);
+  const cudaError_t status = launch_pdl_shared(paged_attention_kernel<D, N>, blocks, Layout<D, N>::kThreads, Layout<D, N>::kSmemBytes, stream, k_map, v_map, a);
   if (status != cudaSuccess) return status;
   if constexpr (N <= 32) return launch_pdl(attention_join_kernel<D, 8>, dim3(blocks, N), 256, stream, a, blocks, uint32_t(N));
   else return launch_pdl(attention_join_kernel<D, 1>, dim3(blocks, 4), 256, stream, a, blocks, uint32_t(N));

@@ -17,10 +17,10 @@ static int draw(int low, int high) {
 
 int main() {
   for (int i = 0; i < 20000; ++i) {
-    const int n = draw(0, 40), m = draw(1, 200), a = draw(0, 300), b = draw(0, 5000);
+    const int n = draw(1, 300), a = draw(1, kTokens), b = draw(0, 5000);
     int64_t sum = 0;
-    for (int k = 0; k < n; ++k) sum += (int64_t(a) * k + b) / m;
-    REQUIRE(floor_sum(n, m, a, b) == sum);
+    for (int k = 0; k < n; ++k) sum += (int64_t(a) * k + b) / kTokens;
+    REQUIRE(floor_sum(n, a, b) == sum);
   }
   for (int round = 0; round < 3000; ++round) {
     const int sequences = draw(1, 9), heads = draw(1, 4), per_tile = draw(1, 128), window = draw(0, 2) ? 0 : draw(1, 700);
@@ -34,7 +34,6 @@ int main() {
       for (int t = 0; t < w.query_tiles(); ++t) {
         REQUIRE(w.units_before(t) == before);
         REQUIRE(w.token_tiles(t) >= 0 && w.low(t) <= w.high(t));
-        for (int64_t u = before; u < before + 1 + w.token_tiles(t); ++u) REQUIRE(w.tile_with(u) == t);
         before += 1 + w.token_tiles(t);
       }
       REQUIRE(w.units() == before);
