@@ -32,6 +32,8 @@ inline gw_status check_batch(const gw_sequences* b, const char* what) {
   return GW_OK;
 }
 
+constexpr int kMostTokens = 1 << 30;      // of a sequence
+
 #ifdef __CUDACC__
 // What a sequence brings to a step; count 0 where its offsets cannot be followed.
 struct SequenceRows {
@@ -40,8 +42,8 @@ struct SequenceRows {
 };
 __device__ __forceinline__ SequenceRows sequence_rows(const gw_sequences& b, uint32_t s) {
   const int low = b.row_offsets[s], high = b.row_offsets[s + 1], context = b.context_lengths[s];
-  const bool good = low >= 0 && high >= low && uint32_t(high) <= b.rows && uint32_t(high - low) <= b.max_rows;
-  return {low, good ? high - low : 0, context, !good};
+  const bool good = low >= 0 && high >= low && uint32_t(high) <= b.rows && uint32_t(high - low) <= b.max_rows && context <= kMostTokens;
+  return {low, good ? high - low : 0, good && context > 0 ? context : 0, !good};
 }
 #endif
 

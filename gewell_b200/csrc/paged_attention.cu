@@ -13,15 +13,16 @@
 // code of x and lo that of the rest (eight bits, as BF16), two products over the same codes.  Block scaling (kind::mxf8f6f4, a power
 // of two for every 32 elements along the sum) gives every 32 elements of a query, and every 32 tokens of a column of P -- those
 // of one warp -- a range of their own, so that small probabilities are as exact as large ones, however far below the maximum.
-// That also takes the running maximum out of the loop: the reference m of a column only has to keep FP32 sums from
-// overflowing.  It is the maximum of the first tile, and is moved (with the sums rescaled) only when a probability times its value scale
-// exceeds 2^40.  (Value scales below 2^-64 are taken for 2^-64 there, so no probability can pass 2^104 unseen.)
+// That also takes the running maximum out of the loop.  The reference m of a column only has to keep FP32 sums in range: it is 0
+// at first, and moves to the maximum so far (with the sums rescaled) only when a probability times its value scale exceeds 2^40, or
+// when a column's first tokens all lie below 2^-40.  (Value scales below 2^-64 are taken for 2^-64 there, so that no probability
+// passes 2^104 unseen.)
 //
-//   warp 0      TMA: chunks of [128 tokens x 128 bytes] of K and V into a ring, page by page
+//   warp 0      TMA: chunks of [128 tokens x 128 bytes] of K and V into a ring, page by page; the pages' scales
 //   warp 1      tcgen05.mma: S of tile t + 1, then O += P V of tile t.  Rows of V that no query may see are zeroed here: a
 //               page's slots behind its last token may hold anything, NaN included, and 0 * NaN is NaN.
-//   the others  softmax: for every 32 lanes two warps (16 and 32 columns) or four, each with its share of the columns; queries into
-//               shared memory at the start of an item, results out at its end
+//   the others  softmax: for every 32 lanes two warps (three for 96 columns), each with its share of the columns; queries into shared
+//               memory at the start of an item, results out at its end
 //
 // Work: attention_work.h.  An item that a cut between two blocks' ranges divides leaves FP32 partial sums in the scratch
 // memory, which a second kernel joins in the order of the blocks (the same bits on every run).
@@ -42,10 +43,11 @@ namespace {
 
 __device__ uint32_t g_attention_error;       // first report since it was last taken
 
-__host__ __device__ constexpr int softmax_warps(int columns) { return columns <= 32 ? 8 : 16; }
+__host__ __device__ constexpr int softmax_warps(int columns) { return columns <= 64 ? 8 : 12; }
 constexpr int kChunkBytes = kTokens * 128;
 constexpr int kAtomBytes = 512;              // scale atom: 128 rows x 4 blocks of 32 elements
-constexpr uint32_t kMoveBits = (127u + 40u) << 23;
+constexpr uint32_t kHighBits = (127u + 40u) << 23, kLowBits = (127u - 40u) << 23;
+constexpr int kScaleTiles = 16;              // tiles whose scales are kept: more than the ring and the score buffers can hold
 
 struct Attention {
   gw_kv_cache cache;
@@ -53,24 +55,50 @@ struct Attention {
   const bf16* query;
   bf16* output;
   uint64_t query_stride, output_stride;
-  uint32_t heads, group, per_tile, window;
+  uint32_t heads, group, per_tile, window, page_shift;       // page_tokens = 1 << page_shift
   float scale;
   float* partial;             // [blocks][2][N][D], then [blocks][2][2][N] maxima and sums
   int4* records;              // [blocks]: {first query row, columns, KV head, last block} of the item that its last piece begins, or last -1
 };
 
+// What the softmax warps of a block share about the item at hand.
+struct Item {
+  int begin, end, tiles, first_token;          // token tiles of the piece, of the item; position of tile 0's first token
+  int used, token_rows, first_row, position0;  // columns with a query, query rows, the first one, its position
+  int head, whole, last_block;                 // last_block: -1, or the last block of an item that this one begins and does not end
+};
+
+struct Shared {
+  uint64_t full[16], empty[16], scales_full[kScaleTiles], scores_full[2], scores_empty[2], probs_full, probs_empty, checked, query_full, sums_full,
+      softmax, drained;
+  float2 scales[kScaleTiles][8];               // {key, value} of a tile's pages; a value scale below 0: no page
+  int move[4];                                 // of the last tiles: some warp asks for the reference to be moved
+  uint32_t tensor_memory;
+  // units of all blocks, the block's range of them, and the item that has the first
+  int64_t units, from, to, item;
+  int64_t rest;                // units of that item's sequence and head in front of the range
+  uint32_t sequence;
+  int head, tile;
+};
+
 template <int D, int N>
 struct Layout {
+  static constexpr int kSoftmaxWarps = softmax_warps(N);
+  static constexpr int kThreads = 32 * (2 + kSoftmaxWarps);
+  static constexpr int kShare = N / (kSoftmaxWarps / 4);          // columns of a warp
   static constexpr int kChunks = D / 128;
   static constexpr int kQueryBytes = kChunks * N * 128;           // one part
   static constexpr bool kOneBuffer = N <= 64;                     // both parts of P in the halves of 128-byte rows
   static constexpr int kProbBytes = kOneBuffer ? kChunkBytes : 2 * kChunkBytes;
   static constexpr int kLowOffset = kOneBuffer ? 64 : kChunkBytes;
   static constexpr int kAtoms = 2 * kChunks + 2;                  // queries (both parts), ones, P
-  static constexpr int kSmall = kAtoms * kAtomBytes + 6 * N * 4 + 8 * N + 1024;      // and what is declared as Shared
-  static constexpr int kRoom = 227 * 1024 - 1024 - 2 * kQueryBytes - kProbBytes - kSmall;
+  static constexpr int kFloats = 7 * N + 32 * kSoftmaxWarps;      // reference, factor, settled, by_warp; factors of a warp
+  static constexpr int kSmall = kAtoms * kAtomBytes + kFloats * 4 + 8 * N;
+  static constexpr int kAlignment = 1024;
+  static constexpr int kStatic = 3072;                            // at least what is declared in the kernel
+  static constexpr int kRoom = 227 * 1024 - kStatic - kAlignment - 2 * kQueryBytes - kProbBytes - kSmall;
   static constexpr int kRing = kRoom / kChunkBytes > 16 ? 16 : kRoom / kChunkBytes;
-  static constexpr int kSmemBytes = 2 * kQueryBytes + kProbBytes + kRing * kChunkBytes + kSmall;      // 1024 bytes of it for the alignment
+  static constexpr int kSmemBytes = kAlignment + 2 * kQueryBytes + kProbBytes + kRing * kChunkBytes + kSmall;
   // tensor memory columns
   static constexpr int kScores = kChunks * N;
   static constexpr int kOnes = kScores + 2 * N;
@@ -79,21 +107,10 @@ struct Layout {
   static constexpr int kColumns = 512;
   static_assert(kProbScales + 4 <= kColumns, "tensor memory over-subscribed");
   static_assert(kRing >= kChunks + 1, "a tile's chunks and one more");
-  static_assert(kSmemBytes + 1024 <= 227 * 1024 && kSmemBytes > 116 * 1024, "one block an SM");
-  static constexpr int kSoftmaxWarps = softmax_warps(N);
-  static constexpr int kThreads = 32 * (2 + kSoftmaxWarps);
-  static constexpr int kShare = N / (kSoftmaxWarps / 4);          // columns of a warp
+  static_assert(kRing / (2 * kChunks) + 4 < kScaleTiles, "scales of a tile are read before those of a later one take their place");
+  static_assert(kSmemBytes > 116 * 1024, "one block an SM");
+  static_assert(sizeof(Shared) + sizeof(Item) + 512 <= kStatic, "");
   static_assert(N % 16 == 0 && N <= 128 && D % 128 == 0 && kShare % 8 == 0 && kShare <= 32, "");
-};
-
-struct Shared {
-  uint64_t full[16], empty[16], scores_full[2], scores_empty[2], probs_full, probs_empty, query_full, sums_full, drained;
-  uint32_t tensor_memory;
-  // units of all blocks, the block's range of them, and the item that has the first
-  int64_t units, from, to, item;
-  int64_t rest;                // units of that item's sequence and head in front of the range
-  uint32_t sequence;
-  int head, tile;
 };
 
 // ---------------------------------------------------------------------------
@@ -249,11 +266,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ int page_at(const Attention& a, uint32_t sequence, int token) {
-  const uint32_t ordinal = uint32_t(token) / a.cache.page_tokens;
-  int page = -1;
-  if (ordinal < a.batch.page_table_stride) page = a.batch.page_table[size_t(sequence) * a.batch.page_table_stride + ordinal];
-  return page >= 0 && uint32_t(page) < a.cache.pages ? page : -1;
+// Entry of the page table as it is (-1 behind its end).  Nothing is asked of the value here: a warp that looks at it waits for it.
+__device__ __forceinline__ int page_entry(const Attention& a, uint32_t sequence, int token) {
+  const uint32_t ordinal = uint32_t(token) >> a.page_shift;
+  return ordinal < a.batch.page_table_stride ? a.batch.page_table[size_t(sequence) * a.batch.page_table_stride + ordinal] : -1;
 }
 __device__ __forceinline__ uint32_t pack4(uint16_t low, uint16_t high) { return uint32_t(low) | uint32_t(high) << 16; }
 
@@ -292,15 +308,9 @@ __device__ __forceinline__ void tmem_load(uint32_t address, uint32_t* r) {
                  : "r"(address) : "memory");
   }
 }
-template <int X>
-__device__ __forceinline__ void tmem_store(uint32_t address, const uint32_t* r) {
-  if constexpr (X == 16) {
-    ptx::tmem_store16(address, r);
-  } else {
-    static_assert(X == 8);
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                 ::"r"(address), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
-  }
+__device__ __forceinline__ void tmem_store8(uint32_t address, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(address), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 // C columns from `address` on, C a multiple of 8
 template <int C>
@@ -309,49 +319,47 @@ __device__ __forceinline__ void tmem_load_columns(uint32_t address, uint32_t* r)
   for (int j = 0; j + 16 <= C; j += 16) tmem_load<16>(address + j, r + j);
   if constexpr (C % 16 != 0) tmem_load<8>(address + C - 8, r + C - 8);
 }
-template <int C>
-__device__ __forceinline__ void tmem_store_columns(uint32_t address, const uint32_t* r) {
-#pragma unroll
-  for (int j = 0; j + 16 <= C; j += 16) tmem_store<16>(address + j, r + j);
-  if constexpr (C % 16 != 0) tmem_store<8>(address + C - 8, r + C - 8);
-}
 
-template <int THREADS>
-__device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(THREADS) : "memory"); }
-// whether the condition holds for any thread of the softmax warps
-template <int THREADS>
-__device__ __forceinline__ bool softmax_any(bool mine) {
-  uint32_t any;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(any) : "r"(uint32_t(mine)), "n"(THREADS) : "memory");
-  return any != 0;
-}
-// v[j] summed over the lanes, for C columns (a power of two up to 32, or 24): lane j % 32 gets column j's (lanes beyond C: any)
+// v[lane] for lanes below C (a multiple of 8 up to 32), by the bits of the lane's number
 template <int C>
-__device__ __forceinline__ float lane_sums(float* v, uint32_t lane) {
-  if constexpr (C == 24) {
-    const float first = lane_sums<16>(v, lane), second = lane_sums<8>(v + 16, lane);
-    return lane < 16 ? first : second;
-  } else {
+__device__ __forceinline__ uint32_t pick(const uint32_t* v, uint32_t lane) {
+  uint32_t r[C / 8];
+  const bool b0 = lane & 1, b1 = lane & 2, b2 = lane & 4;
 #pragma unroll
-    for (int m = 16; m >= C; m /= 2)
-#pragma unroll
-      for (int j = 0; j < C; ++j) v[j] += __shfl_xor_sync(0xffffffffu, v[j], m);
-#pragma unroll
-    for (int m = C / 2; m; m /= 2) {
-      const bool upper = (lane & m) != 0;
-#pragma unroll
-      for (int j = 0; j < m; ++j) {
-        const float other = __shfl_xor_sync(0xffffffffu, upper ? v[j] : v[j + m], m);
-        v[j] = (upper ? v[j + m] : v[j]) + other;
-      }
-    }
-    return v[0];
+  for (int i = 0; i < C / 8; ++i) {
+    const uint32_t* u = v + 8 * i;
+    const uint32_t a0 = b0 ? u[1] : u[0], a1 = b0 ? u[3] : u[2], a2 = b0 ? u[5] : u[4], a3 = b0 ? u[7] : u[6];
+    const uint32_t c0 = b1 ? a1 : a0, c1 = b1 ? a3 : a2;
+    r[i] = b2 ? c1 : c0;
   }
+  uint32_t result = r[0];
+#pragma unroll
+  for (int i = 1; i < C / 8; ++i) result = lane >= uint32_t(8 * i) ? r[i] : result;
+  return result;
+}
+// v[j] summed over the lanes, for C columns (a multiple of 8 up to 32): lane j gets column j's
+template <int C>
+__device__ __forceinline__ float lane_sums(const float (&v)[C], uint32_t lane) {
+  const bool b0 = lane & 1, b1 = lane & 2, b2 = lane & 4;
+  float result = 0.F;
+#pragma unroll
+  for (int i = 0; i < C / 8; ++i) {
+    float u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      u[j] = v[8 * i + j];
+      u[j] += __shfl_xor_sync(0xffffffffu, u[j], 16);
+      u[j] += __shfl_xor_sync(0xffffffffu, u[j], 8);
+    }
+    float x[4], y[2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = (b2 ? u[j + 4] : u[j]) + __shfl_xor_sync(0xffffffffu, b2 ? u[j] : u[j + 4], 4);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) y[j] = (b1 ? x[j + 2] : x[j]) + __shfl_xor_sync(0xffffffffu, b1 ? x[j] : x[j + 2], 2);
+    const float sum = (b0 ? y[1] : y[0]) + __shfl_xor_sync(0xffffffffu, b0 ? y[0] : y[1], 1);
+    if (lane / 8 == uint32_t(i)) result = sum;
+  }
+  return result;
 }
 // order-preserving integer of a float that is no NaN
 __device__ __forceinline__ int ordered(float v) {
@@ -380,9 +388,12 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
   uint8_t* const probs_atom = ones_atom + kAtomBytes;
   float* const reference = reinterpret_cast<float*>(probs_atom + kAtomBytes);     // [N] m of a column
   float* const factor = reference + N;                                            // [N]
-  float* const by_warp = factor + N;                                              // [4][N]
-  bf16** const output_at = reinterpret_cast<bf16**>(by_warp + 4 * N);             // [N]
+  int* const settled = reinterpret_cast<int*>(factor + N);                        // [N] the reference holds: some token lies above 2^-40
+  float* const by_warp = factor + 2 * N;                                          // [4][N]
+  float* const spread = by_warp + 4 * N;                                          // [softmax warps][32]
+  bf16** const output_at = reinterpret_cast<bf16**>(spread + 32 * kSoftmaxWarps); // [N]
   __shared__ Shared s;
+  __shared__ Item shared_item;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
@@ -396,7 +407,11 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     }
     ptx::mbar_init(&s.probs_full, kSoftmaxWarps);
     ptx::mbar_init(&s.probs_empty, 1);
+    ptx::mbar_init(&s.checked, kSoftmaxWarps);
+    ptx::mbar_init(&s.softmax, kSoftmaxWarps);
     ptx::mbar_init(&s.query_full, kSoftmaxWarps);
+    for (int i = 0; i < kScaleTiles; ++i) ptx::mbar_init(&s.scales_full[i], 1);
+    for (int i = 0; i < 4; ++i) s.move[i] = 0;
     ptx::mbar_init(&s.sums_full, 1);
     ptx::mbar_init(&s.drained, 1);
     ptx::fence_barrier_init();
@@ -425,23 +440,31 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     // ----- producer: lane l brings the l-th page of a tile
     const uint32_t page_tokens = a.cache.page_tokens, boxes = kTokens / page_tokens;
     const int outside = int(a.cache.pages * a.cache.kv_heads * page_tokens);        // rows from here on read as zeros
-    int slot = 0, issued = 0;
+    int slot = 0, issued = 0, tile_count = 0;
     uint32_t parity = 1;                                         // empty slots: the first pass does not wait
     bool good = true;
     Walk w;
     w.start(a, s);
     while (good && w.next(a, s)) {
-      const int first = w.work.first_token_tile(w.tile), low = w.work.low(w.tile), high = w.work.high(w.tile);
-      // row of the lane's page in the tensor maps
-      const auto row_of = [&](int t) {
-        const int64_t token = int64_t(first + t) * kTokens + lane * page_tokens;
-        if (lane >= boxes || token >= high || token + page_tokens <= low) return outside;
-        const int page = page_at(a, w.sequence, int(token));
-        if (page < 0) {
-          atomicCAS(&g_attention_error, 0u, 0xa1000000u | (w.sequence & 0xffffffu));
-          return outside;
+      const int first_token = w.work.first_token_tile(w.tile) * kTokens + lane * page_tokens, low = w.work.low(w.tile), high = w.work.high(w.tile);
+      // entry of the page table, or -2 for a page that is not needed
+      const auto entry_of = [&](int t) {
+        const int token = first_token + t * kTokens;
+        return lane < boxes && t < w.end && token < high && token + int(page_tokens) > low ? page_entry(a, w.sequence, token) : -2;
+      };
+      const auto scales_of = [&](int entry) {
+        float2 v = make_float2(0.F, -1.F);
+        if (uint32_t(entry) < a.cache.pages) {
+          const size_t at = size_t(entry) * a.cache.kv_heads + w.head;
+          v = make_float2(a.cache.k_scales[at], a.cache.v_scales[at]);
         }
-        return int((uint32_t(page) * a.cache.kv_heads + w.head) * page_tokens);
+        return v;
+      };
+      // row of the page in the tensor maps
+      const auto row_of = [&](int entry) {
+        if (uint32_t(entry) < a.cache.pages) return int((uint32_t(entry) * a.cache.kv_heads + w.head) * page_tokens);
+        if (entry != -2) atomicCAS(&g_attention_error, 0u, 0xa1000000u | (w.sequence & 0xffffffu));
+        return outside;
       };
       const auto bring = [&](const CUtensorMap* map, int row) {
         for (int c = 0; c < CH; ++c) {
@@ -457,13 +480,20 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         }
         return true;
       };
-      int row = row_of(w.begin), row_before = 0;
+      int entry = entry_of(w.begin), entry_next = entry_of(w.begin + 1), row_before = 0;
+      float2 scales = scales_of(entry);
       for (int t = w.begin; good && t < w.end; ++t) {
-        const int row_next = t + 1 < w.end ? row_of(t + 1) : 0;
+        const int entry_after = entry_of(t + 2), row = row_of(entry);
         good = bring(&k_map, row);
+        if (lane < boxes) s.scales[tile_count % kScaleTiles][lane] = scales;
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&s.scales_full[tile_count % kScaleTiles]);
+        ++tile_count;
+        scales = scales_of(entry_next);
         if (good && t > w.begin) good = bring(&v_map, row_before);
         row_before = row;
-        row = row_next;
+        entry = entry_next;
+        entry_next = entry_after;
       }
       if (good && w.end > w.begin) good = bring(&v_map, row_before);
       w.advance();
@@ -579,46 +609,78 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     __syncwarp();
     ptx::mbar_wait_warp(&s.drained, 0, 0, 100000000ull);
   } else {
-    // ----- softmax
+    // ----- softmax.  Code that runs once an item is kept in short loops: what is not in the instruction cache costs more to
+    // fetch than to execute (the reference's move, unrolled, took 16000 cycles).
     const uint32_t quadrant = warp & 3, column0 = (warp - 2) / 4 * C, member = threadIdx.x - 64;
     const uint32_t lanes = tmem + (quadrant * 32 << 16);
     const uint32_t row = quadrant * 32 + lane;                   // the lane's token in a tile
     const uint32_t group = a.group;
+    float* const my_spread = spread + 32 * (warp - 2);
     int item = 0, tile_count = 0;
     if (member == 0) a.records[blockIdx.x] = make_int4(0, 0, 0, -1);
-    // A thread whose wait ran out waits no more, but goes on to the barriers that it shares with the others.
+    // A thread whose wait ran out waits no more, but goes on to the end.
     bool good = true;
     const auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
       if (good && !ptx::mbar_wait_bounded(bar, parity)) good = failed(code);
     };
-    Walk w;
-    w.start(a, s);
-    while (w.next(a, s)) {
-      const int token_rows = min(int(a.per_tile), w.rows.count - w.tile * int(a.per_tile));
-      const int used = token_rows * int(group);                  // columns of queries
-      const int first_row = w.rows.first + w.tile * int(a.per_tile), position0 = w.work.base + w.tile * int(a.per_tile);
-      const uint32_t head0 = w.head * group;
+    // a barrier of the softmax warps, bounded as all waits are
+    uint32_t meetings = 0;
+    const auto together = [&]() {
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&s.softmax);
+      wait(&s.softmax, meetings & 1, 0xae000000u);
+      __syncwarp();
+      ++meetings;
+    };
+    Walk w;                                                      // of the first thread
+    if (member == 0) w.start(a, s);
+    while (true) {
+      if (member == 0) {
+        Item m;
+        if (w.next(a, s)) {
+          const int64_t parts = min(s.units, int64_t(gridDim.x));
+          m.begin = w.begin;
+          m.end = w.end;
+          m.tiles = w.tiles;
+          m.first_token = w.work.first_token_tile(w.tile) * kTokens;
+          m.token_rows = min(int(a.per_tile), w.rows.count - w.tile * int(a.per_tile));
+          m.used = m.token_rows * int(group);
+          m.first_row = w.rows.first + w.tile * int(a.per_tile);
+          m.position0 = w.work.base + w.tile * int(a.per_tile);
+          m.head = w.head;
+          m.whole = w.begin == 0 && w.end == w.tiles;
+          m.last_block = w.begin == 0 && w.end < w.tiles ? part_with(s.units, w.item + w.tiles, parts) : -1;
+          w.advance();
+        } else {
+          m.tiles = -1;
+        }
+        shared_item = m;
+      }
+      together();
+      const Item& m = shared_item;
+      if (m.tiles < 0) break;
       if (int(member) < N) {
         const uint32_t at = member / group;
-        output_at[member] = a.output + size_t(first_row + at) * a.output_stride + size_t(head0 + member - at * group) * D;
-        reference[member] = int(member) < used ? -INFINITY : 0.F;        // scores without a query are 0
+        output_at[member] = a.output + size_t(m.first_row + at) * a.output_stride + size_t(m.head * group + member - at * group) * D;
+        reference[member] = 0.F;
+        settled[member] = int(member) >= m.used;
       }
-      if (w.tiles == 0) {                                        // rows that see nothing
-        softmax_sync<kSoftmaxThreads>();
-        for (int column = warp - 2; column < used; column += kSoftmaxWarps)
+      if (m.tiles == 0) {                                        // rows that see nothing
+        together();
+        for (int column = warp - 2; column < m.used; column += kSoftmaxWarps)
           for (int d = lane * 8; d < D; d += 256) *reinterpret_cast<uint4*>(output_at[column] + d) = make_uint4(0, 0, 0, 0);
-        softmax_sync<kSoftmaxThreads>();
-        w.advance();
+        together();
         continue;
       }
       // queries: a thread takes 32 elements at a time, which share a power of two
+#pragma unroll 1
       for (int block = member; block < N * (D / 32); block += kSoftmaxThreads) {
         const int column = block / (D / 32), part = block % (D / 32), c = part / 4, k = part % 4;
         uint4 bits[4];
-        if (column < used) {
+        if (column < m.used) {
           const uint32_t at = uint32_t(column) / group;
-          const uint4* from = reinterpret_cast<const uint4*>(a.query + size_t(first_row + at) * a.query_stride +
-                                                             size_t(head0 + column - at * group) * D + part * 32);
+          const uint4* from = reinterpret_cast<const uint4*>(a.query + size_t(m.first_row + at) * a.query_stride +
+                                                             size_t(m.head * group + column - at * group) * D + part * 32);
 #pragma unroll
           for (int i = 0; i < 4; ++i) bits[i] = from[i];
         } else {
@@ -657,92 +719,125 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       ptx::tc_fence_before_sync();                               // the results of the item before were read
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&s.query_full);
-      softmax_sync<kSoftmaxThreads>();                           // `reference`, `output_at`
+      together();                           // `reference`, `settled`, `output_at`
 
       float total[C];
 #pragma unroll
       for (int j = 0; j < C; ++j) total[j] = 0.F;
-      const int first = w.work.first_token_tile(w.tile), low = w.work.low(w.tile), high = w.work.high(w.tile);
-      const auto page_of = [&](int t) {
-        const int64_t token = int64_t(first + t) * kTokens + row;
-        return t < w.end && token >= low && token < high ? page_at(a, w.sequence, int(token)) : -1;
-      };
-      const auto scales_of = [&](int page, float& key, float& value) {
-        key = value = 0.F;
-        if (page >= 0) {
-          const size_t at = size_t(page) * a.cache.kv_heads + w.head;
-          key = a.cache.k_scales[at];
-          value = a.cache.v_scales[at];
-        }
-      };
+      const int used = m.used, end = m.end, token_rows = m.token_rows;
       const float to_log2 = a.scale * 1.4426950408889634F;
-      int page = page_of(w.begin), page_next = page_of(w.begin + 1);
-      float key_scale, value_scale;
-      scales_of(page, key_scale, value_scale);
+      int ahead = m.first_token + m.begin * kTokens + int(row) - m.position0;      // of the lane's token, to the first query
 
-      for (int t = w.begin; t < w.end; ++t) {
-        const int page_after = page_of(t + 2);
-        float key_scale_next, value_scale_next;
-        scales_of(page_next, key_scale_next, value_scale_next);
-        // the columns that see the lane's token: query row i where token <= position0 + i < token + window
-        const int64_t ahead = int64_t(first + t) * kTokens + row - position0;
-        const int from = int(max(int64_t(0), min(ahead, int64_t(N)))) * int(group);
-        int to = a.window ? int(max(int64_t(0), min(ahead + a.window, int64_t(token_rows)))) * int(group) : used;
-        if (page < 0) to = 0;
+#pragma unroll 1
+      for (int t = m.begin; t < end; ++t, ahead += kTokens) {
+        const int entry = tile_count % kScaleTiles;
+        wait(&s.scales_full[entry], tile_count / kScaleTiles & 1, 0xac000000u);
+        const float2 scales = s.scales[entry][row >> a.page_shift];
+        // the columns that see the lane's token: query row i where ahead <= i < ahead + window
+        const int from = max(0, min(ahead, N)) * int(group);
+        int to = a.window ? max(0, min(ahead + int(a.window), token_rows)) * int(group) : used;
+        if (scales.y < 0.F) to = 0;
         const bool open = __all_sync(0xffffffffu, from == 0 && to == used);
         const uint32_t seen_from = from - column0, seen_span = to > from ? to - from : 0;       // column0 + j - from < span, unsigned
-        const float scale = key_scale * to_log2, bound_scale = fmaxf(value_scale, 5.42101086e-20F);       // 2^-64
+        const float scale = scales.x * to_log2, value_scale = scales.y < 0.F ? 0.F : scales.y, bound_scale = fmaxf(value_scale, 5.42101086e-20F);
+        // lane j: whether any of the warp's tokens may be seen from column j
+        const int seen_low = __reduce_min_sync(0xffffffffu, from), seen_high = __reduce_max_sync(0xffffffffu, to);
+        const bool sees = seen_low <= int(column0 + lane) && int(column0 + lane) < seen_high;
 
         const int buffer = tile_count & 1;
         wait(&s.scores_full[buffer], (tile_count >> 1) & 1, 0xa8000000u);
         ptx::tc_fence_after_sync();
         const uint32_t scores = lanes + L::kScores + buffer * N + column0;
         float p[C];
-        uint32_t largest = 0;                                    // lane j: of column j, p * value scale over the warp's 32 tokens
-        // Once, or again after the reference moved, which it does at the first tile.
+        uint32_t hi[C / 4], lo[C / 4], exponent;
+        // Once, or again after the reference moved.
+#pragma unroll 1
         for (bool moved = false;; moved = true) {
           tmem_load_columns<C>(scores, reinterpret_cast<uint32_t*>(p));
           ptx::tmem_load_wait();
-          if (moved || t > w.begin) {
-#pragma unroll
-            for (int j = 0; j < C; ++j) {
-              p[j] = exp2_approx(fmaf(p[j], scale, -reference[column0 + j]));
-              if (!open) p[j] = uint32_t(j) - seen_from < seen_span ? p[j] : 0.F;
-              const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(p[j] * bound_scale));
-              if (lane == uint32_t(j)) largest = bits;
-            }
-            // NaN counts as beyond too
-            if (moved || !softmax_any<kSoftmaxThreads>(lane < uint32_t(C) && largest > kMoveBits)) break;
-            tmem_load_columns<C>(scores, reinterpret_cast<uint32_t*>(p));
-            ptx::tmem_load_wait();
-          }
-          // the reference of a column moves to the largest score so far
+          uint32_t bits[C];
 #pragma unroll
           for (int j = 0; j < C; ++j) {
-            const float score = p[j] * scale;
-            const bool seen = uint32_t(j) - seen_from < seen_span && score == score;
-            const int highest = __reduce_max_sync(0xffffffffu, ordered(seen ? score : -INFINITY));
-            if (lane == uint32_t(j)) by_warp[quadrant * N + column0 + j] = __int_as_float(highest ^ ((highest >> 31) & 0x7fffffff));
+            p[j] = exp2_approx(fmaf(p[j], scale, -reference[column0 + j]));
+            if (!open) p[j] = uint32_t(j) - seen_from < seen_span ? p[j] : 0.F;
+            // over the warp's tokens; not below 2^-119, where the factor below would not be finite
+            bits[j] = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaf(p[j], bound_scale, 1.5046327691e-36F)));
           }
-          softmax_sync<kSoftmaxThreads>();
+          const uint32_t largest = pick<C>(bits, lane);          // lane j: of column j
+          exponent = largest >> 23;
+          if (!moved) {
+            bool ask = false;
+            if (lane < uint32_t(C)) {
+              // NaN counts as too high
+              ask = largest > kHighBits;
+              if (!settled[column0 + lane] && sees) {
+                if (largest < kLowBits) ask = true;
+                else settled[column0 + lane] = 1;
+              }
+              if (ask) s.move[tile_count & 3] = 1;
+            }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&s.checked);
+          }
+          // P: the warp's 32 tokens of a column share a power of two, 2^-7 of that of the largest
+          __syncwarp();
+          my_spread[lane] = __uint_as_float((261 - exponent) << 23);
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < C; j += 4) {
+            const float4 up = *reinterpret_cast<const float4*>(my_spread + j);
+            uint16_t h0, l0, h1, l1;
+            // in this order: the factor of a column that sees none of these tokens is 2^126, and 0 stays 0
+            two_parts(p[j] * value_scale * up.x, p[j + 1] * value_scale * up.y, 1.F, h0, l0);
+            two_parts(p[j + 2] * value_scale * up.z, p[j + 3] * value_scale * up.w, 1.F, h1, l1);
+            hi[j / 4] = pack4(h0, h1);
+            lo[j / 4] = pack4(l0, l1);
+          }
+          if (moved) break;
+          wait(&s.checked, tile_count & 1, 0xad000000u);
+          if (member == 0) s.move[(tile_count + 2) & 3] = 0;
+          if (*reinterpret_cast<volatile int*>(&s.move[tile_count & 3]) == 0) break;
+          // the reference of a column moves to the largest score so far
+#pragma unroll 1
+          for (int j = 0; j < C; j += 8) {
+            float score[8];
+            tmem_load<8>(scores + j, reinterpret_cast<uint32_t*>(score));
+            ptx::tmem_load_wait();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float v = score[e] * scale;
+              const bool seen = uint32_t(j + e) - seen_from < seen_span && v == v;
+              const int highest = __reduce_max_sync(0xffffffffu, ordered(seen ? v : -INFINITY));
+              if (lane == uint32_t(e)) by_warp[quadrant * N + column0 + j + e] = __int_as_float(highest ^ ((highest >> 31) & 0x7fffffff));
+            }
+          }
+          together();
           if (member < N) {
+            const float highest = fmaxf(fmaxf(by_warp[member], by_warp[N + member]), fmaxf(by_warp[2 * N + member], by_warp[3 * N + member]));
             const float before = reference[member];
-            const float now = fmaxf(before, fmaxf(fmaxf(by_warp[member], by_warp[N + member]), fmaxf(by_warp[2 * N + member], by_warp[3 * N + member])));
+            // A column that has not settled has had no token before this tile, and one that sees none here keeps its reference.
+            const bool had = settled[member] != 0, has = highest != -INFINITY;
+            const float now = !has ? before : had ? fmaxf(before, highest) : highest;
             reference[member] = now;
-            factor[member] = before == -INFINITY ? 0.F : exp2_approx(before - now);
+            factor[member] = had ? exp2_approx(before - now) : 0.F;
+            settled[member] = had || has;
           }
-          softmax_sync<kSoftmaxThreads>();
-          if (t > w.begin) {                                     // the sums so far, once the product before is done
+          together();
+          if (t > m.begin) {                                     // the sums so far, once the product before is done
             wait(&s.probs_empty, (tile_count & 1) ^ 1, 0xa9000000u);
             ptx::tc_fence_after_sync();
 #pragma unroll
             for (int j = 0; j < C; ++j) total[j] *= factor[column0 + j];
-            for (int c = 0; c < CH; ++c) {
-              tmem_load_columns<C>(lanes + c * N + column0, reinterpret_cast<uint32_t*>(p));
+#pragma unroll 1
+            for (int i = 0; i < CH * (C / 8); ++i) {
+              const int j = i % (C / 8) * 8;
+              const uint32_t at = lanes + i / (C / 8) * N + column0 + j;
+              float sum[8];
+              tmem_load<8>(at, reinterpret_cast<uint32_t*>(sum));
               ptx::tmem_load_wait();
 #pragma unroll
-              for (int j = 0; j < C; ++j) p[j] *= factor[column0 + j];
-              tmem_store_columns<C>(lanes + c * N + column0, reinterpret_cast<const uint32_t*>(p));
+              for (int e = 0; e < 8; ++e) sum[e] *= factor[column0 + j + e];
+              tmem_store8(at, reinterpret_cast<const uint32_t*>(sum));
             }
             ptx::tmem_store_wait();
           }
@@ -750,24 +845,8 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         ptx::tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&s.scores_empty[buffer]);
-        // P: the warp's 32 tokens of a column share a power of two, 2^-7 of that of the largest
-        const uint32_t exponent = largest >> 23;
-        const float up = exponent < 8 ? 0.F : __uint_as_float((261 - exponent) << 23);
-        uint32_t hi[C / 4], lo[C / 4];
 #pragma unroll
-        for (int j = 0; j < C; j += 4) {
-          float scaled[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            total[j + e] += p[j + e];
-            scaled[e] = p[j + e] * (__shfl_sync(0xffffffffu, up, j + e) * value_scale);
-          }
-          uint16_t h0, l0, h1, l1;
-          two_parts(scaled[0], scaled[1], 1.F, h0, l0);
-          two_parts(scaled[2], scaled[3], 1.F, h1, l1);
-          hi[j / 4] = pack4(h0, h1);
-          lo[j / 4] = pack4(l0, l1);
-        }
+        for (int j = 0; j < C; ++j) total[j] += p[j];
         if (tile_count > 0) wait(&s.probs_empty, (tile_count & 1) ^ 1, 0xaa000000u);
 #pragma unroll
         for (int j = 0; j < C; j += 8) {
@@ -779,59 +858,54 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         }
         if (lane < uint32_t(C)) {
           const uint32_t column = column0 + lane;
-          probs_atom[column % 32 * 16 + column / 32 * 4 + quadrant] = uint8_t(exponent < 8 ? 127 : exponent - 7);
+          probs_atom[column % 32 * 16 + column / 32 * 4 + quadrant] = uint8_t(exponent - 7);
         }
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&s.probs_full);
         ++tile_count;
-        page = page_next;
-        page_next = page_after;
-        key_scale = key_scale_next;
-        value_scale = value_scale_next;
       }
       // sums of a column over the tokens
-      const float mine = lane_sums<C>(total, lane);
+      const float mine = lane_sums(total, lane);
       if (lane < uint32_t(C)) by_warp[quadrant * N + column0 + lane] = mine;
-      softmax_sync<kSoftmaxThreads>();
-      const bool whole = w.begin == 0 && w.end == w.tiles;
+      together();
+      const bool whole = m.whole;
+      const uint32_t place = 2 * blockIdx.x + (m.begin == 0 ? 1 : 0);
       if (member < N) {
         const float v = (by_warp[member] + by_warp[N + member]) + (by_warp[2 * N + member] + by_warp[3 * N + member]);
-        factor[member] = whole ? (v == 0.F ? 0.F : 1.F / v) : v;
+        factor[member] = v == 0.F ? 0.F : 1.F / v;
+        if (!whole) {
+          float* const totals = a.partial + size_t(gridDim.x) * 2 * N * D + size_t(place) * 2 * N;
+          totals[member] = reference[member];
+          totals[N + member] = v;
+        }
       }
-      softmax_sync<kSoftmaxThreads>();
+      if (member == 0 && m.last_block >= 0) a.records[blockIdx.x] = make_int4(m.first_row, used, m.head, m.last_block);
+      together();
       wait(&s.sums_full, item & 1, 0xab000000u);
       ptx::tc_fence_after_sync();
-      const uint32_t place = 2 * blockIdx.x + (w.begin == 0 ? 1 : 0);
-      float* const partial = a.partial + size_t(place) * N * D;
-      if (!whole && member < N) {
-        float* const totals = a.partial + size_t(gridDim.x) * 2 * N * D + size_t(place) * 2 * N;
-        totals[member] = reference[member];
-        totals[N + member] = factor[member];
-      }
-      if (!whole && w.begin == 0 && member == 0) {
-        const int64_t parts = min(s.units, int64_t(gridDim.x));
-        a.records[blockIdx.x] = make_int4(first_row, used, w.head, part_with(s.units, w.item + w.tiles, parts));
-      }
-      for (int c = 0; c < CH; ++c) {
-        float o[C];
-        tmem_load_columns<C>(lanes + c * N + column0, reinterpret_cast<uint32_t*>(o));
-        ptx::tmem_load_wait();
-        const uint32_t d = c * 128 + row;
-        if (whole) {
+      float* const partial = a.partial + (size_t(place) * N + column0) * D + row;
+#pragma unroll 1
+      for (int j = 0; j < C; j += 8) {
+        if (int(column0) + j >= used) break;
+#pragma unroll 1
+        for (int c = 0; c < CH; ++c) {
+          float o[8];
+          tmem_load<8>(lanes + c * N + column0 + j, reinterpret_cast<uint32_t*>(o));
+          ptx::tmem_load_wait();
 #pragma unroll
-          for (int j = 0; j < C; ++j)
-            if (int(column0) + j < used) output_at[column0 + j][d] = __float2bfloat16_rn(o[j] * factor[column0 + j]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < C; ++j)
-            if (int(column0) + j < used) partial[size_t(column0 + j) * D + d] = o[j];
+          for (int e = 0; e < 8; ++e) {
+            const int column = column0 + j + e;
+            if (column < used) {
+              if (whole) output_at[column][c * 128 + row] = __float2bfloat16_rn(o[e] * factor[column]);
+              else partial[(j + e) * D + c * 128] = o[e];
+            }
+          }
         }
       }
       ++item;
-      w.advance();
-      softmax_sync<kSoftmaxThreads>();                           // `output_at`, `factor`, `reference` are free
+      together();                           // what the item had in shared memory is free
     }
   }
   ptx::tc_fence_before_sync();
@@ -908,7 +982,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_consta
 // scores (512 columns: D / 128 * N sums, 2 N scores, up to 40 of scales).
 uint32_t columns_of(uint32_t head_dim, uint32_t group, uint32_t max_rows) {
   const uint64_t needed = uint64_t(group) * max_rows;
-  return needed <= 16 ? 16 : needed <= 32 ? 32 : head_dim == 512 ? 64 : head_dim == 256 ? 96 : 128;
+  return needed <= 16 ? 16 : needed <= 32 ? 32 : head_dim == 512 ? 64 : 96;
 }
 
 size_t partial_floats(uint32_t blocks, uint32_t columns, uint32_t head_dim) { return size_t(blocks) * 2 * columns * (head_dim + 2); }
@@ -979,10 +1053,10 @@ gw_status gw_paged_attention_bf16(const gw_kv_cache* cache, const gw_sequences* 
     return fail(GW_CUDA_ERROR, "paged attention: " + error);
   const size_t floats = align_up(partial_floats(blocks, columns, cache->head_dim) * sizeof(float), 256);
   const Attention a{*cache, *batch, static_cast<const bf16*>(query_bf16), static_cast<bf16*>(output_bf16), query_stride, output_stride,
-                    heads, group, columns / group, window > (1u << 30) ? 0 : window, scale,
+                    heads, group, columns / group, window > (1u << 30) ? 0 : window, uint32_t(__builtin_ctz(cache->page_tokens)), scale,
                     static_cast<float*>(scratch), reinterpret_cast<int4*>(static_cast<uint8_t*>(scratch) + floats)};
   const cudaStream_t s = as_stream(stream);
-  GW_CUDA_CHECK((cache->head_dim == 128   ? launch_columns<128, 128>(columns, a, k_map, v_map, blocks, s)
+  GW_CUDA_CHECK((cache->head_dim == 128   ? launch_columns<128, 96>(columns, a, k_map, v_map, blocks, s)
                  : cache->head_dim == 256 ? launch_columns<256, 96>(columns, a, k_map, v_map, blocks, s)
                                           : launch_columns<512, 64>(columns, a, k_map, v_map, blocks, s)),
                 "paged attention");

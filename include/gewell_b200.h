@@ -387,8 +387,8 @@ typedef struct gw_kv_cache {
  * page page_table[s * page_table_stride + position / page_tokens].  Only entries of pages that the call needs are read.
  * rows: token rows that the step's arrays have (rows behind the last sequence are left as they are); max_rows: at least the rows
  * of the sequence with the most.  A position below 0 (a context shorter than its rows, as batches are padded) is no token: nothing
- * is appended for it, and it sees nothing.  Offsets outside 0 .. rows, sequences of more than max_rows rows, positions behind the
- * page table and page numbers outside the cache are not followed: those tokens are left out and gw_debug_kernel_error() reports
+ * is appended for it, and it sees nothing.  Offsets outside 0 .. rows, sequences of more than max_rows rows or 2^30 tokens, positions
+ * behind the page table and page numbers outside the cache are not followed: those tokens are left out and gw_debug_kernel_error() reports
  * 0xa....... . */
 typedef struct gw_sequences {
   const int32_t* row_offsets;     /* [sequences + 1] */
