@@ -19,9 +19,10 @@
 // passes 2^104 unseen.)
 //
 //   warp 0      TMA: chunks of [128 tokens x 128 bytes] of K and V into a ring, page by page; the pages' scales
-//   warp 1      tcgen05.mma: S of tile t + 1, then O += P V of tile t.  Rows of V that no query may see are zeroed here: a
-//               page's slots behind its last token may hold anything, NaN included, and 0 * NaN is NaN.
-//   the others  softmax: for every 32 lanes two warps (three for 96 columns), each with its share of the columns; queries into shared
+//   warp 1      one thread issues tcgen05.mma: S of tile t + 1, then O += P V of tile t
+//   warp 2      zeroes rows of V that no query may see: a page's slots behind its last token may hold anything, NaN included, and
+//               0 * NaN is NaN
+//   warps 4..   softmax: for every 32 lanes two warps (three for 96 columns), each with its share of the columns; queries into shared
 //               memory at the start of an item, results out at its end
 //
 // Work: attention_work.h.  An item that a cut between two blocks' ranges divides leaves FP32 partial sums in the scratch
@@ -44,6 +45,7 @@ namespace {
 __device__ uint32_t g_attention_error;       // first report since it was last taken
 
 __host__ __device__ constexpr int softmax_warps(int columns) { return columns <= 64 ? 8 : 12; }
+constexpr int kFirstSoftmaxWarp = 4;
 constexpr int kChunkBytes = kTokens * 128;
 constexpr int kAtomBytes = 512;              // scale atom: 128 rows x 4 blocks of 32 elements
 constexpr uint32_t kHighBits = (127u + 40u) << 23, kLowBits = (127u - 40u) << 23;
@@ -69,7 +71,7 @@ struct Item {
 };
 
 struct Shared {
-  uint64_t full[16], empty[16], scales_full[kScaleTiles], scores_full[2], scores_empty[2], probs_full, probs_empty, checked, query_full, sums_full,
+  uint64_t full[16], empty[16], cleared[16], scales_full[kScaleTiles], scores_full[2], scores_empty[2], probs_full, probs_empty, checked, query_full, sums_full,
       softmax, drained;
   float2 scales[kScaleTiles][8];               // {key, value} of a tile's pages; a value scale below 0: no page
   int move[4];                                 // of the last tiles: some warp asks for the reference to be moved
@@ -84,7 +86,7 @@ struct Shared {
 template <int D, int N>
 struct Layout {
   static constexpr int kSoftmaxWarps = softmax_warps(N);
-  static constexpr int kThreads = 32 * (2 + kSoftmaxWarps);
+  static constexpr int kThreads = 32 * (kFirstSoftmaxWarp + kSoftmaxWarps);
   static constexpr int kShare = N / (kSoftmaxWarps / 4);          // columns of a warp
   static constexpr int kChunks = D / 128;
   static constexpr int kQueryBytes = kChunks * N * 128;           // one part
@@ -281,6 +283,12 @@ __device__ __forceinline__ void two_parts(float a, float b, float low_scale, uin
   lo = __nv_cvt_halfraw2_to_fp8x2(__half2_raw(rest), __NV_SATFINITE, __NV_E4M3);
 }
 
+// whether a token tile has tokens outside [low, high)
+__device__ __forceinline__ bool needs_clearing(int token_tile, int low, int high) {
+  const int start = token_tile * kTokens;
+  return low > start || high < start + kTokens;
+}
+
 // matrix descriptor of rows of 128 bytes, 128-byte swizzle, read across the rows: 8 rows of the sum are 1024 bytes apart
 __device__ __forceinline__ uint64_t across_desc(uint32_t address) { return ptx::smem_desc_sw128(address) | uint64_t(1024 >> 4) << 16; }
 
@@ -399,7 +407,8 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
   if (threadIdx.x == 0) {
     for (int i = 0; i < RING; ++i) {
       ptx::mbar_init(&s.full[i], 1);
-      ptx::mbar_init(&s.empty[i], 1);
+      ptx::mbar_init(&s.cleared[i], 1);
+      ptx::mbar_init(&s.empty[i], 2);                            // both products' thread and the warp that zeroes
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&s.scores_full[i], 1);
@@ -508,114 +517,150 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       ptx::mbar_wait_warp(&s.full[slot], parity ^ 1, 0, 100000000ull);
     }
   } else if (warp == 1) {
-    // ----- both products
-    int slot = 0, item = 0, scored = 0, summed = 0;              // scored, summed: tiles over all items
-    uint32_t parity = 0;
-    bool good = true;
-    Walk w;
-    w.start(a, s);
-    if (ptx::elect_one()) ptx::tc_copy_sf_atom(tmem + L::kOnes, ptx::smem_desc_sf_atom(ptx::smem_u32(ones_atom)));
-    const auto wait_chunk = [&]() { return ptx::mbar_wait_warp(&s.full[slot], parity) || failed(0xa4000000u | slot); };
-    const auto next_chunk = [&]() {
-      if (++slot == RING) {
-        slot = 0;
-        parity ^= 1;
-      }
-    };
-    while (good && w.next(a, s)) {
-      if (w.end > w.begin) {
-        const int first = w.work.first_token_tile(w.tile), low = w.work.low(w.tile), high = w.work.high(w.tile);
-        good = ptx::mbar_wait_warp(&s.query_full, item & 1) || failed(0xa5000000u);
-        if (!good) break;
-        ptx::tc_fence_after_sync();
-        if (ptx::elect_one())
-#pragma unroll
-          for (int i = 0; i < 2 * CH; ++i)
-            ptx::tc_copy_sf_atom(tmem + L::kQueryScales + 4 * i, ptx::smem_desc_sf_atom(ptx::smem_u32(atoms + i * kAtomBytes)));
-        const auto score = [&]() {
-          const int buffer = scored & 1;
-          if (!ptx::mbar_wait_warp(&s.scores_empty[buffer], ((scored >> 1) & 1) ^ 1)) return failed(0xa6000000u | buffer);
+    // ----- both products, by one thread: the compiler keeps its descriptors in uniform registers only where it knows that one thread
+    // runs the code (72 to 110 cycles an instruction otherwise, whatever N)
+    if (ptx::elect_one()) {
+      int slot = 0, item = 0, scored = 0, summed = 0;                    // scored, summed: tiles over all items
+      uint32_t parity = 0;
+      bool good = true;
+      const auto wait = [&](uint64_t* bar, uint32_t phase, uint32_t code) {
+        good = good && (ptx::mbar_wait_bounded(bar, phase) || failed(code));
+      };
+      const uint64_t ring_rows = ptx::smem_desc_sw128(ptx::smem_u32(ring)), ring_across = across_desc(ptx::smem_u32(ring));
+      const uint64_t hi_rows = ptx::smem_desc_sw128(ptx::smem_u32(query_hi)), lo_rows = ptx::smem_desc_sw128(ptx::smem_u32(query_lo));
+      const uint64_t probs_across = across_desc(ptx::smem_u32(probs));
+      const uint64_t atom = ptx::smem_desc_sf_atom(ptx::smem_u32(atoms));
+      Walk w;
+      w.start(a, s);
+      ptx::tc_copy_sf_atom(tmem + L::kOnes, ptx::smem_desc_sf_atom(ptx::smem_u32(ones_atom)));
+      const auto next_chunk = [&]() {
+        if (++slot == RING) {
+          slot = 0;
+          parity ^= 1;
+        }
+      };
+      while (good && w.next(a, s)) {
+        if (w.end > w.begin) {
+          const int first = w.work.first_token_tile(w.tile), low = w.work.low(w.tile), high = w.work.high(w.tile);
+          wait(&s.query_full, item & 1, 0xa5000000u);
+          if (!good) break;
           ptx::tc_fence_after_sync();
-          for (int c = 0; c < CH; ++c) {
-            if (!wait_chunk()) return false;
-            ptx::tc_fence_after_sync();
-            if (ptx::elect_one()) {
-              const uint64_t keys = ptx::smem_desc_sw128(ptx::smem_u32(ring + slot * kChunkBytes));
 #pragma unroll
-              for (int part = 0; part < 2; ++part) {
-                const uint64_t queries = ptx::smem_desc_sw128(ptx::smem_u32((part ? query_lo : query_hi) + c * N * 128));
+          for (int i = 0; i < 2 * CH; ++i) ptx::tc_copy_sf_atom(tmem + L::kQueryScales + 4 * i, atom + uint64_t(i * (kAtomBytes >> 4)));
+          const auto score = [&]() {
+            const int buffer = scored & 1;
+            wait(&s.scores_empty[buffer], ((scored >> 1) & 1) ^ 1, 0xa6000000u | buffer);
+            const uint32_t d = tmem + L::kScores + buffer * N;
+#pragma unroll 1
+            for (int c = 0; good && c < CH; ++c) {
+              wait(&s.full[slot], parity, 0xa4000000u | slot);
+              if (!good) return;
+              ptx::tc_fence_after_sync();
+              const uint64_t keys = ring_rows + uint64_t(slot * (kChunkBytes >> 4)), offset = uint64_t(c * (N * 128 >> 4));
+              const uint32_t scales = tmem + L::kQueryScales + 8 * c;
+#pragma unroll
+              for (int part = 0; part < 2; ++part)
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  mma_mx(tmem + L::kScores + buffer * N, keys + 2 * k, queries + 2 * k, idesc_mx(N, false) | uint32_t(k) << 4, tmem + L::kOnes,
-                         tmem + L::kQueryScales + 4 * (2 * c + part), c | part | k);
-              }
+                  mma_mx(d, keys + 2 * k, (part ? lo_rows : hi_rows) + offset + 2 * k, idesc_mx(N, false) | uint32_t(k) << 4, tmem + L::kOnes,
+                         scales + 4 * part, c | part | k);
               ptx::tc_commit(&s.empty[slot]);
               if (c == CH - 1) ptx::tc_commit(&s.scores_full[buffer]);
+              next_chunk();
             }
-            __syncwarp();
-            next_chunk();
-          }
-          ++scored;
-          return true;
-        };
-        const auto sum = [&](int t) {
-          if (!ptx::mbar_wait_warp(&s.probs_full, summed & 1)) return failed(0xa7000000u);
-          ptx::tc_fence_after_sync();
-          if (ptx::elect_one()) ptx::tc_copy_sf_atom(tmem + L::kProbScales, ptx::smem_desc_sf_atom(ptx::smem_u32(probs_atom)));
-          const int start = (first + t) * kTokens, clear_below = low - start, clear_from = high - start;
-          for (int c = 0; c < CH; ++c) {
-            if (!wait_chunk()) return false;
-            if (clear_below > 0 || clear_from < kTokens) {       // tokens that no query of the item sees
-              uint4* rows = reinterpret_cast<uint4*>(ring + slot * kChunkBytes);
-              for (int i = lane; i < clear_below * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
-              for (int i = clear_from * 8 + lane; i < kTokens * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
-              ptx::fence_proxy_async_smem();
-              __syncwarp();
-            }
+            ++scored;
+          };
+          const auto sum = [&](int t) {
+            wait(&s.probs_full, summed & 1, 0xa7000000u);
+            if (!good) return;
             ptx::tc_fence_after_sync();
-            if (ptx::elect_one()) {
-              const uint64_t values = across_desc(ptx::smem_u32(ring + slot * kChunkBytes));
+            ptx::tc_copy_sf_atom(tmem + L::kProbScales, ptx::smem_desc_sf_atom(ptx::smem_u32(probs_atom)));
+            const bool clear = needs_clearing(first + t, low, high);
+#pragma unroll 1
+            for (int c = 0; c < CH; ++c) {
+              wait(&s.full[slot], parity, 0xa4000000u | slot);
+              if (clear) wait(&s.cleared[slot], parity, 0xaf000000u | slot);
+              if (!good) return;
+              ptx::tc_fence_after_sync();
+              const uint64_t values = ring_across + uint64_t(slot * (kChunkBytes >> 4));
 #pragma unroll
-              for (int part = 0; part < 2; ++part) {
-                const uint64_t p = across_desc(ptx::smem_u32(probs + part * L::kLowOffset));
+              for (int part = 0; part < 2; ++part)
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  mma_mx(tmem + c * N, values + 256 * k, p + 256 * k, idesc_mx(N, true) | uint32_t(k) << 4, tmem + L::kOnes,
-                         tmem + L::kProbScales, uint32_t(t > w.begin) | part | k);
-              }
+                  mma_mx(tmem + c * N, values + 256 * k, probs_across + uint64_t(part * (L::kLowOffset >> 4)) + 256 * k,
+                         idesc_mx(N, true) | uint32_t(k) << 4, tmem + L::kOnes, tmem + L::kProbScales, uint32_t(t > w.begin) | part | k);
               ptx::tc_commit(&s.empty[slot]);
               if (c == CH - 1) {
                 ptx::tc_commit(&s.probs_empty);
                 if (t == w.end - 1) ptx::tc_commit(&s.sums_full);
               }
+              next_chunk();
             }
-            __syncwarp();
-            next_chunk();
+            ++summed;
+          };
+          score();
+#pragma unroll 1
+          for (int t = w.begin; good && t < w.end; ++t) {
+            if (t + 1 < w.end) score();
+            if (good) sum(t);
           }
-          ++summed;
-          return true;
-        };
-        good = score();
-        for (int t = w.begin; good && t < w.end; ++t) {
-          if (t + 1 < w.end) good = score();
-          if (good) good = sum(t);
+          ++item;
         }
-        ++item;
+        w.advance();
+      }
+      // products still in flight end before tensor memory is released
+      ptx::tc_commit(&s.drained);
+      ptx::mbar_wait_bounded(&s.drained, 0, 100000000ull);
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    // ----- rows of V that no query of an item sees; every chunk is waited for, in the order in which the products take them, so that
+    // this warp is never a lap of the ring away
+    int slot = 0;
+    uint32_t parity = 0;
+    bool good = true;
+    Walk w;
+    w.start(a, s);
+    const auto chunk = [&](bool clear, int clear_below, int clear_from) {
+      for (int c = 0; good && c < CH; ++c) {
+        good = ptx::mbar_wait_warp(&s.full[slot], parity, 20) || failed(0xa9000000u | slot);
+        if (!good) return;
+        if (clear) {
+          uint4* rows = reinterpret_cast<uint4*>(ring + slot * kChunkBytes);
+          for (int i = lane; i < clear_below * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
+          for (int i = clear_from * 8 + lane; i < kTokens * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) {
+          ptx::mbar_arrive(&s.cleared[slot]);
+          ptx::mbar_arrive(&s.empty[slot]);
+        }
+        if (++slot == RING) {
+          slot = 0;
+          parity ^= 1;
+        }
+      }
+    };
+    while (good && w.next(a, s)) {
+      const int first = w.work.first_token_tile(w.tile), low = w.work.low(w.tile), high = w.work.high(w.tile);
+      if (w.end > w.begin) chunk(false, 0, 0);
+      for (int t = w.begin; good && t < w.end; ++t) {
+        if (t + 1 < w.end) chunk(false, 0, 0);
+        const int start = (first + t) * kTokens;
+        chunk(needs_clearing(first + t, low, high), low - start, high - start);
       }
       w.advance();
     }
-    // products still in flight end before tensor memory is released
-    if (ptx::elect_one()) ptx::tc_commit(&s.drained);
-    __syncwarp();
-    ptx::mbar_wait_warp(&s.drained, 0, 0, 100000000ull);
-  } else {
+  } else if (warp >= kFirstSoftmaxWarp) {
     // ----- softmax.  Code that runs once an item is kept in short loops: what is not in the instruction cache costs more to
     // fetch than to execute (the reference's move, unrolled, took 16000 cycles).
-    const uint32_t quadrant = warp & 3, column0 = (warp - 2) / 4 * C, member = threadIdx.x - 64;
+    const uint32_t quadrant = warp & 3, column0 = (warp - kFirstSoftmaxWarp) / 4 * C,
+                   member = threadIdx.x - 32 * kFirstSoftmaxWarp;
     const uint32_t lanes = tmem + (quadrant * 32 << 16);
     const uint32_t row = quadrant * 32 + lane;                   // the lane's token in a tile
     const uint32_t group = a.group;
-    float* const my_spread = spread + 32 * (warp - 2);
+    float* const my_spread = spread + 32 * (warp - kFirstSoftmaxWarp);
     int item = 0, tile_count = 0;
     if (member == 0) a.records[blockIdx.x] = make_int4(0, 0, 0, -1);
     // A thread whose wait ran out waits no more, but goes on to the end.
@@ -667,7 +712,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       }
       if (m.tiles == 0) {                                        // rows that see nothing
         together();
-        for (int column = warp - 2; column < m.used; column += kSoftmaxWarps)
+        for (int column = warp - kFirstSoftmaxWarp; column < m.used; column += kSoftmaxWarps)
           for (int d = lane * 8; d < D; d += 256) *reinterpret_cast<uint4*>(output_at[column] + d) = make_uint4(0, 0, 0, 0);
         together();
         continue;
@@ -824,7 +869,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
           }
           together();
           if (t > m.begin) {                                     // the sums so far, once the product before is done
-            wait(&s.probs_empty, (tile_count & 1) ^ 1, 0xa9000000u);
+            wait(&s.probs_empty, (tile_count & 1) ^ 1, 0xaa000000u);
             ptx::tc_fence_after_sync();
 #pragma unroll
             for (int j = 0; j < C; ++j) total[j] *= factor[column0 + j];
