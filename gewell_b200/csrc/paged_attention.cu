@@ -22,8 +22,10 @@
 //   warp 1      one thread issues tcgen05.mma: S of tile t + 1, then O += P V of tile t
 //   warp 2      zeroes rows of V that no query may see: a page's slots behind its last token may hold anything, NaN included, and
 //               0 * NaN is NaN
-//   warps 4..   softmax: for every 32 lanes two warps (three for 96 columns), each with its share of the columns; queries into shared
-//               memory at the start of an item, results out at its end
+//   warp 3      walks over the items for the softmax warps
+//   warps 4..   softmax: for every 32 lanes two warps (three for 96 columns), each with its share of the columns.  After an item's last
+//               tile they bring the next item's queries to shared memory, so that its first scores are computed while they write the
+//               results of the one before.
 //
 // Work: attention_work.h.  An item that a cut between two blocks' ranges divides leaves FP32 partial sums in the scratch
 // memory, which a second kernel joins in the order of the blocks (the same bits on every run).
@@ -49,6 +51,7 @@ constexpr int kFirstSoftmaxWarp = 4;
 constexpr int kChunkBytes = kTokens * 128;
 constexpr int kAtomBytes = 512;              // scale atom: 128 rows x 4 blocks of 32 elements
 constexpr uint32_t kHighBits = (127u + 40u) << 23, kLowBits = (127u - 40u) << 23;
+constexpr int kItems = 4;                    // items that the walk is ahead at most
 constexpr int kScaleTiles = 16;              // tiles whose scales are kept: more than the ring and the score buffers can hold
 
 struct Attention {
@@ -63,7 +66,7 @@ struct Attention {
   int4* records;              // [blocks]: {first query row, columns, KV head, last block} of the item that its last piece begins, or last -1
 };
 
-// What the softmax warps of a block share about the item at hand.
+// An item as the softmax warps see it.
 struct Item {
   int begin, end, tiles, first_token;          // token tiles of the piece, of the item; position of tile 0's first token
   int used, token_rows, first_row, position0;  // columns with a query, query rows, the first one, its position
@@ -72,8 +75,9 @@ struct Item {
 
 struct Shared {
   uint64_t full[16], empty[16], cleared[16], scales_full[kScaleTiles], scores_full[2], scores_empty[2], probs_full, probs_empty, checked, query_full, sums_full,
-      softmax, drained;
+      softmax, items_full[kItems], items_empty[kItems], drained;
   float2 scales[kScaleTiles][8];               // {key, value} of a tile's pages; a value scale below 0: no page
+  Item items[kItems];
   int move[4];                                 // of the last tiles: some warp asks for the reference to be moved
   uint32_t tensor_memory;
   // units of all blocks, the block's range of them, and the item that has the first
@@ -111,7 +115,7 @@ struct Layout {
   static_assert(kRing >= kChunks + 1, "a tile's chunks and one more");
   static_assert(kRing / (2 * kChunks) + 4 < kScaleTiles, "scales of a tile are read before those of a later one take their place");
   static_assert(kSmemBytes > 116 * 1024, "one block an SM");
-  static_assert(sizeof(Shared) + sizeof(Item) + 512 <= kStatic, "");
+  static_assert(sizeof(Shared) + 512 <= kStatic, "");
   static_assert(N % 16 == 0 && N <= 128 && D % 128 == 0 && kShare % 8 == 0 && kShare <= 32, "");
 };
 
@@ -401,7 +405,6 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
   float* const spread = by_warp + 4 * N;                                          // [softmax warps][32]
   bf16** const output_at = reinterpret_cast<bf16**>(spread + 32 * kSoftmaxWarps); // [N]
   __shared__ Shared s;
-  __shared__ Item shared_item;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
@@ -421,6 +424,10 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     ptx::mbar_init(&s.query_full, kSoftmaxWarps);
     for (int i = 0; i < kScaleTiles; ++i) ptx::mbar_init(&s.scales_full[i], 1);
     for (int i = 0; i < 4; ++i) s.move[i] = 0;
+    for (int i = 0; i < kItems; ++i) {
+      ptx::mbar_init(&s.items_full[i], 1);
+      ptx::mbar_init(&s.items_empty[i], kSoftmaxWarps);
+    }
     ptx::mbar_init(&s.sums_full, 1);
     ptx::mbar_init(&s.drained, 1);
     ptx::fence_barrier_init();
@@ -652,6 +659,39 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       }
       w.advance();
     }
+  } else if (warp == 3) {
+    // ----- the items for the softmax warps; tiles of -1 end them
+    if (lane == 0) {
+      a.records[blockIdx.x] = make_int4(0, 0, 0, -1);
+      const int64_t parts = min(s.units, int64_t(gridDim.x));
+      bool good = true, more = true;
+      Walk w;
+      w.start(a, s);
+      for (int n = 0; good && more; ++n) {
+        more = w.next(a, s);
+        good = ptx::mbar_wait_bounded(&s.items_empty[n % kItems], (n / kItems & 1) ^ 1) || failed(0xb0000000u);
+        if (!good) break;
+        Item& m = s.items[n % kItems];
+        m.tiles = -1;
+        if (more) {
+          m.begin = w.begin;
+          m.end = w.end;
+          m.tiles = w.tiles;
+          m.first_token = w.work.first_token_tile(w.tile) * kTokens;
+          m.token_rows = min(int(a.per_tile), w.rows.count - w.tile * int(a.per_tile));
+          m.used = m.token_rows * int(a.group);
+          m.first_row = w.rows.first + w.tile * int(a.per_tile);
+          m.position0 = w.work.base + w.tile * int(a.per_tile);
+          m.head = w.head;
+          m.whole = w.begin == 0 && w.end == w.tiles;
+          m.last_block = w.begin == 0 && w.end < w.tiles ? part_with(s.units, w.item + w.tiles, parts) : -1;
+          if (m.last_block >= 0) a.records[blockIdx.x] = make_int4(m.first_row, m.used, m.head, m.last_block);
+          w.advance();
+        }
+        ptx::mbar_arrive(&s.items_full[n % kItems]);
+      }
+    }
+    __syncwarp();
   } else if (warp >= kFirstSoftmaxWarp) {
     // ----- softmax.  Code that runs once an item is kept in short loops: what is not in the instruction cache costs more to
     // fetch than to execute (the reference's move, unrolled, took 16000 cycles).
@@ -661,8 +701,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     const uint32_t row = quadrant * 32 + lane;                   // the lane's token in a tile
     const uint32_t group = a.group;
     float* const my_spread = spread + 32 * (warp - kFirstSoftmaxWarp);
-    int item = 0, tile_count = 0;
-    if (member == 0) a.records[blockIdx.x] = make_int4(0, 0, 0, -1);
+    int scored_items = 0, tile_count = 0;
     // A thread whose wait ran out waits no more, but goes on to the end.
     bool good = true;
     const auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
@@ -677,47 +716,8 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       __syncwarp();
       ++meetings;
     };
-    Walk w;                                                      // of the first thread
-    if (member == 0) w.start(a, s);
-    while (true) {
-      if (member == 0) {
-        Item m;
-        if (w.next(a, s)) {
-          const int64_t parts = min(s.units, int64_t(gridDim.x));
-          m.begin = w.begin;
-          m.end = w.end;
-          m.tiles = w.tiles;
-          m.first_token = w.work.first_token_tile(w.tile) * kTokens;
-          m.token_rows = min(int(a.per_tile), w.rows.count - w.tile * int(a.per_tile));
-          m.used = m.token_rows * int(group);
-          m.first_row = w.rows.first + w.tile * int(a.per_tile);
-          m.position0 = w.work.base + w.tile * int(a.per_tile);
-          m.head = w.head;
-          m.whole = w.begin == 0 && w.end == w.tiles;
-          m.last_block = w.begin == 0 && w.end < w.tiles ? part_with(s.units, w.item + w.tiles, parts) : -1;
-          w.advance();
-        } else {
-          m.tiles = -1;
-        }
-        shared_item = m;
-      }
-      together();
-      const Item& m = shared_item;
-      if (m.tiles < 0) break;
-      if (int(member) < N) {
-        const uint32_t at = member / group;
-        output_at[member] = a.output + size_t(m.first_row + at) * a.output_stride + size_t(m.head * group + member - at * group) * D;
-        reference[member] = 0.F;
-        settled[member] = int(member) >= m.used;
-      }
-      if (m.tiles == 0) {                                        // rows that see nothing
-        together();
-        for (int column = warp - kFirstSoftmaxWarp; column < m.used; column += kSoftmaxWarps)
-          for (int d = lane * 8; d < D; d += 256) *reinterpret_cast<uint4*>(output_at[column] + d) = make_uint4(0, 0, 0, 0);
-        together();
-        continue;
-      }
-      // queries: a thread takes 32 elements at a time, which share a power of two
+    // Queries of an item: a thread takes 32 elements at a time, which share a power of two.
+    const auto bring_queries = [&](const Item& m) {
 #pragma unroll 1
       for (int block = member; block < N * (D / 32); block += kSoftmaxThreads) {
         const int column = block / (D / 32), part = block % (D / 32), c = part / 4, k = part % 4;
@@ -761,11 +761,38 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         atoms[scale_at + kAtomBytes] = uint8_t(scale - 4);
       }
       ptx::fence_proxy_async_smem();
-      ptx::tc_fence_before_sync();                               // the results of the item before were read
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&s.query_full);
-      together();                           // `reference`, `settled`, `output_at`
-
+    };
+    // From item n on, what the warps need of it before its first tile; false: there is none.
+    const auto next_item = [&](int n) {
+      wait(&s.items_full[n % kItems], n / kItems & 1, 0xb1000000u);
+      good = __all_sync(0xffffffffu, good);                      // a warp goes on or leaves as one
+      const Item& m = s.items[n % kItems];
+      if (!good || m.tiles < 0) return false;
+      if (m.tiles > 0) bring_queries(m);
+      return true;
+    };
+    bool more = next_item(0);
+#pragma unroll 1
+    for (int n = 0; more; ++n) {
+      const Item& m = s.items[n % kItems];
+      if (int(member) < N) {
+        const uint32_t at = member / group;
+        output_at[member] = a.output + size_t(m.first_row + at) * a.output_stride + size_t(m.head * group + member - at * group) * D;
+        reference[member] = 0.F;
+        settled[member] = int(member) >= m.used;
+      }
+      together();
+      if (m.tiles == 0) {                                        // rows that see nothing
+#pragma unroll 1
+        for (int column = warp - kFirstSoftmaxWarp; column < m.used; column += kSoftmaxWarps)
+          for (int d = lane * 8; d < D; d += 256) *reinterpret_cast<uint4*>(output_at[column] + d) = make_uint4(0, 0, 0, 0);
+        more = next_item(n + 1);
+        together();
+        if (lane == 0) ptx::mbar_arrive(&s.items_empty[n % kItems]);
+        continue;
+      }
       float total[C];
 #pragma unroll
       for (int j = 0; j < C; ++j) total[j] = 0.F;
@@ -911,6 +938,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         if (lane == 0) ptx::mbar_arrive(&s.probs_full);
         ++tile_count;
       }
+      more = next_item(n + 1);                                   // its queries, while the last product runs
       // sums of a column over the tokens
       const float mine = lane_sums(total, lane);
       if (lane < uint32_t(C)) by_warp[quadrant * N + column0 + lane] = mine;
@@ -926,9 +954,8 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
           totals[N + member] = v;
         }
       }
-      if (member == 0 && m.last_block >= 0) a.records[blockIdx.x] = make_int4(m.first_row, used, m.head, m.last_block);
       together();
-      wait(&s.sums_full, item & 1, 0xab000000u);
+      wait(&s.sums_full, scored_items & 1, 0xab000000u);
       ptx::tc_fence_after_sync();
       float* const partial = a.partial + (size_t(place) * N + column0) * D + row;
 #pragma unroll 1
@@ -949,8 +976,12 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
           }
         }
       }
-      ++item;
-      together();                           // what the item had in shared memory is free
+      ++scored_items;
+      // The sums were read: the next item's first product may overwrite them once it has the probabilities that this thread
+      // publishes later.  What the item had in shared memory is free.
+      ptx::tc_fence_before_sync();
+      together();
+      if (lane == 0) ptx::mbar_arrive(&s.items_empty[n % kItems]);
     }
   }
   ptx::tc_fence_before_sync();
