@@ -18,11 +18,12 @@
 // when a column's first tokens all lie below 2^-40.  (Value scales below 2^-64 are taken for 2^-64 there, so that no probability
 // passes 2^104 unseen.)
 //
-//   warp 0      TMA: chunks of [128 tokens x 128 bytes] of K and V into a ring, page by page; the pages' scales
-//   warp 1      one thread issues tcgen05.mma: S of tile t + 1, then O += P V of tile t
+//   warp 0      TMA: chunks of [128 tokens x 128 bytes] of K and V into a ring, page by page; the pages' scales, and what the softmax
+//               warps need to know of an item
+//   warps 1, 3  one thread each issues tcgen05.mma: S of the tiles, as far ahead as there is room, and O += P V.  One thread for
+//               both spent half of its time in barriers, with nothing left in the tensor pipe's queue.
 //   warp 2      zeroes rows of V that no query may see: a page's slots behind its last token may hold anything, NaN included, and
 //               0 * NaN is NaN
-//   warp 3      walks over the items for the softmax warps
 //   warps 4..   softmax: for every 32 lanes two warps (three for 96 columns), each with its share of the columns.  After an item's last
 //               tile they bring the next item's queries to shared memory, so that its first scores are computed while they write the
 //               results of the one before.
@@ -60,7 +61,8 @@ struct Attention {
   const bf16* query;
   bf16* output;
   uint64_t query_stride, output_stride;
-  uint32_t heads, group, per_tile, window, page_shift;       // page_tokens = 1 << page_shift
+  uint32_t heads, group, group_inverse, per_tile, window;    // group_inverse: x / group is x * group_inverse >> 16 for columns x
+  uint32_t page_shift;                                       // page_tokens = 1 << page_shift
   float scale;
   float* partial;             // [blocks][2][N][D], then [blocks][2][2][N] maxima and sums
   int4* records;              // [blocks]: {first query row, columns, KV head, last block} of the item that its last piece begins, or last -1
@@ -70,12 +72,12 @@ struct Attention {
 struct Item {
   int begin, end, tiles, first_token;          // token tiles of the piece, of the item; position of tile 0's first token
   int used, token_rows, first_row, position0;  // columns with a query, query rows, the first one, its position
-  int head, whole, last_block;                 // last_block: -1, or the last block of an item that this one begins and does not end
+  int head, whole;
 };
 
 struct Shared {
   uint64_t full[16], empty[16], cleared[16], scales_full[kScaleTiles], scores_full[2], scores_empty[2], probs_full, probs_empty, checked, query_full, sums_full,
-      softmax, items_full[kItems], items_empty[kItems], drained;
+      softmax, items_full[kItems], items_empty[kItems], drained, drained_sums;
   float2 scales[kScaleTiles][8];               // {key, value} of a tile's pages; a value scale below 0: no page
   Item items[kItems];
   int move[4];                                 // of the last tiles: some warp asks for the reference to be moved
@@ -430,6 +432,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     }
     ptx::mbar_init(&s.sums_full, 1);
     ptx::mbar_init(&s.drained, 1);
+    ptx::mbar_init(&s.drained_sums, 1);
     ptx::fence_barrier_init();
   }
   if (warp == 1) {
@@ -459,9 +462,35 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     int slot = 0, issued = 0, tile_count = 0;
     uint32_t parity = 1;                                         // empty slots: the first pass does not wait
     bool good = true;
+    const int64_t parts = min(s.units, int64_t(gridDim.x));
+    if (lane == 0) a.records[blockIdx.x] = make_int4(0, 0, 0, -1);
     Walk w;
     w.start(a, s);
-    while (good && w.next(a, s)) {
+    for (int n = 0; good; ++n) {
+      const bool more = w.next(a, s);
+      good = ptx::mbar_wait_warp(&s.items_empty[n % kItems], (n / kItems & 1) ^ 1) || failed(0xb0000000u);
+      if (!good) break;
+      if (lane == 0) {
+        Item& m = s.items[n % kItems];
+        m.tiles = -1;                                            // the end
+        if (more) {
+          m.begin = w.begin;
+          m.end = w.end;
+          m.tiles = w.tiles;
+          m.first_token = w.work.first_token_tile(w.tile) * kTokens;
+          m.token_rows = min(int(a.per_tile), w.rows.count - w.tile * int(a.per_tile));
+          m.used = m.token_rows * int(a.group);
+          m.first_row = w.rows.first + w.tile * int(a.per_tile);
+          m.position0 = w.work.base + w.tile * int(a.per_tile);
+          m.head = w.head;
+          m.whole = w.begin == 0 && w.end == w.tiles;
+          if (w.begin == 0 && w.end < w.tiles)
+            a.records[blockIdx.x] = make_int4(m.first_row, m.used, w.head, part_with(s.units, w.item + w.tiles, parts));
+        }
+        ptx::mbar_arrive(&s.items_full[n % kItems]);
+      }
+      __syncwarp();
+      if (!more) break;
       const int first_token = w.work.first_token_tile(w.tile) * kTokens + lane * page_tokens, low = w.work.low(w.tile), high = w.work.high(w.tile);
       // entry of the page table, or -2 for a page that is not needed
       const auto entry_of = [&](int t) {
@@ -524,45 +553,45 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       ptx::mbar_wait_warp(&s.full[slot], parity ^ 1, 0, 100000000ull);
     }
   } else if (warp == 1) {
-    // ----- both products, by one thread: the compiler keeps its descriptors in uniform registers only where it knows that one thread
-    // runs the code (72 to 110 cycles an instruction otherwise, whatever N)
+    // ----- S, by one thread: the compiler keeps its descriptors in uniform registers only where it knows that one thread runs the code
+    // (72 to 110 cycles an instruction otherwise, whatever N; 36 at N = 16, 44 at 64, 51 at 96 here)
     if (ptx::elect_one()) {
-      int slot = 0, item = 0, scored = 0, summed = 0;                    // scored, summed: tiles over all items
+      int slot = 0, item = 0, scored = 0;
       uint32_t parity = 0;
       bool good = true;
       const auto wait = [&](uint64_t* bar, uint32_t phase, uint32_t code) {
         good = good && (ptx::mbar_wait_bounded(bar, phase) || failed(code));
       };
-      const uint64_t ring_rows = ptx::smem_desc_sw128(ptx::smem_u32(ring)), ring_across = across_desc(ptx::smem_u32(ring));
-      const uint64_t hi_rows = ptx::smem_desc_sw128(ptx::smem_u32(query_hi)), lo_rows = ptx::smem_desc_sw128(ptx::smem_u32(query_lo));
-      const uint64_t probs_across = across_desc(ptx::smem_u32(probs));
-      const uint64_t atom = ptx::smem_desc_sf_atom(ptx::smem_u32(atoms));
-      Walk w;
-      w.start(a, s);
-      ptx::tc_copy_sf_atom(tmem + L::kOnes, ptx::smem_desc_sf_atom(ptx::smem_u32(ones_atom)));
-      const auto next_chunk = [&]() {
-        if (++slot == RING) {
-          slot = 0;
+      const auto skip = [&](int chunks) {
+        slot += chunks;
+        if (slot >= RING) {
+          slot -= RING;
           parity ^= 1;
         }
       };
+      const uint64_t ring_rows = ptx::smem_desc_sw128(ptx::smem_u32(ring));
+      const uint64_t hi_rows = ptx::smem_desc_sw128(ptx::smem_u32(query_hi)), lo_rows = ptx::smem_desc_sw128(ptx::smem_u32(query_lo));
+      const uint64_t atom = ptx::smem_desc_sf_atom(ptx::smem_u32(atoms));
+      ptx::tc_copy_sf_atom(tmem + L::kOnes, ptx::smem_desc_sf_atom(ptx::smem_u32(ones_atom)));
+      Walk w;
+      w.start(a, s);
       while (good && w.next(a, s)) {
         if (w.end > w.begin) {
-          const int first = w.work.first_token_tile(w.tile), low = w.work.low(w.tile), high = w.work.high(w.tile);
           wait(&s.query_full, item & 1, 0xa5000000u);
           if (!good) break;
           ptx::tc_fence_after_sync();
 #pragma unroll
           for (int i = 0; i < 2 * CH; ++i) ptx::tc_copy_sf_atom(tmem + L::kQueryScales + 4 * i, atom + uint64_t(i * (kAtomBytes >> 4)));
-          const auto score = [&]() {
+#pragma unroll 1
+          for (int t = w.begin; good && t < w.end; ++t) {
             const int buffer = scored & 1;
             wait(&s.scores_empty[buffer], ((scored >> 1) & 1) ^ 1, 0xa6000000u | buffer);
             const uint32_t d = tmem + L::kScores + buffer * N;
+            wait(&s.full[slot], parity, 0xa4000000u | slot);
 #pragma unroll 1
             for (int c = 0; good && c < CH; ++c) {
-              wait(&s.full[slot], parity, 0xa4000000u | slot);
-              if (!good) return;
               ptx::tc_fence_after_sync();
+              const int this_slot = slot;
               const uint64_t keys = ring_rows + uint64_t(slot * (kChunkBytes >> 4)), offset = uint64_t(c * (N * 128 >> 4));
               const uint32_t scales = tmem + L::kQueryScales + 8 * c;
 #pragma unroll
@@ -571,46 +600,16 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
                 for (int k = 0; k < 4; ++k)
                   mma_mx(d, keys + 2 * k, (part ? lo_rows : hi_rows) + offset + 2 * k, idesc_mx(N, false) | uint32_t(k) << 4, tmem + L::kOnes,
                          scales + 4 * part, c | part | k);
-              ptx::tc_commit(&s.empty[slot]);
-              if (c == CH - 1) ptx::tc_commit(&s.scores_full[buffer]);
-              next_chunk();
+              skip(1);
+              // before the commit, which comes back once its products have left the queue
+              if (c + 1 < CH) wait(&s.full[slot], parity, 0xa4000000u | slot);
+              ptx::tc_commit(&s.empty[this_slot]);
             }
+            ptx::tc_commit(&s.scores_full[buffer]);
             ++scored;
-          };
-          const auto sum = [&](int t) {
-            wait(&s.probs_full, summed & 1, 0xa7000000u);
-            if (!good) return;
-            ptx::tc_fence_after_sync();
-            ptx::tc_copy_sf_atom(tmem + L::kProbScales, ptx::smem_desc_sf_atom(ptx::smem_u32(probs_atom)));
-            const bool clear = needs_clearing(first + t, low, high);
-#pragma unroll 1
-            for (int c = 0; c < CH; ++c) {
-              wait(&s.full[slot], parity, 0xa4000000u | slot);
-              if (clear) wait(&s.cleared[slot], parity, 0xaf000000u | slot);
-              if (!good) return;
-              ptx::tc_fence_after_sync();
-              const uint64_t values = ring_across + uint64_t(slot * (kChunkBytes >> 4));
-#pragma unroll
-              for (int part = 0; part < 2; ++part)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  mma_mx(tmem + c * N, values + 256 * k, probs_across + uint64_t(part * (L::kLowOffset >> 4)) + 256 * k,
-                         idesc_mx(N, true) | uint32_t(k) << 4, tmem + L::kOnes, tmem + L::kProbScales, uint32_t(t > w.begin) | part | k);
-              ptx::tc_commit(&s.empty[slot]);
-              if (c == CH - 1) {
-                ptx::tc_commit(&s.probs_empty);
-                if (t == w.end - 1) ptx::tc_commit(&s.sums_full);
-              }
-              next_chunk();
-            }
-            ++summed;
-          };
-          score();
-#pragma unroll 1
-          for (int t = w.begin; good && t < w.end; ++t) {
-            if (t + 1 < w.end) score();
-            if (good) sum(t);
+            if (t > w.begin) skip(CH);                           // V of the tile before
           }
+          skip(CH);
           ++item;
         }
         w.advance();
@@ -618,6 +617,63 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       // products still in flight end before tensor memory is released
       ptx::tc_commit(&s.drained);
       ptx::mbar_wait_bounded(&s.drained, 0, 100000000ull);
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    // ----- O += P V, by one thread
+    if (ptx::elect_one()) {
+      int slot = 0, summed = 0;
+      uint32_t parity = 0;
+      bool good = true;
+      const auto wait = [&](uint64_t* bar, uint32_t phase, uint32_t code) {
+        good = good && (ptx::mbar_wait_bounded(bar, phase) || failed(code));
+      };
+      const auto skip = [&](int chunks) {
+        slot += chunks;
+        if (slot >= RING) {
+          slot -= RING;
+          parity ^= 1;
+        }
+      };
+      const uint64_t ring_across = across_desc(ptx::smem_u32(ring)), probs_across = across_desc(ptx::smem_u32(probs));
+      Walk w;
+      w.start(a, s);
+      while (good && w.next(a, s)) {
+        const int first = w.work.first_token_tile(w.tile), low = w.work.low(w.tile), high = w.work.high(w.tile);
+        if (w.end > w.begin) skip(CH);                           // K of the first tile
+#pragma unroll 1
+        for (int t = w.begin; good && t < w.end; ++t) {
+          if (t + 1 < w.end) skip(CH);                           // K of the next one
+          const bool clear = needs_clearing(first + t, low, high);
+          uint64_t* const ready = clear ? s.cleared : s.full;
+          wait(&s.probs_full, summed & 1, 0xa7000000u);
+          wait(&ready[slot], parity, 0xaf000000u | slot);
+          if (!good) break;
+          ptx::tc_fence_after_sync();
+          ptx::tc_copy_sf_atom(tmem + L::kProbScales, ptx::smem_desc_sf_atom(ptx::smem_u32(probs_atom)));
+#pragma unroll 1
+          for (int c = 0; good && c < CH; ++c) {
+            ptx::tc_fence_after_sync();
+            const int this_slot = slot;
+            const uint64_t values = ring_across + uint64_t(slot * (kChunkBytes >> 4));
+#pragma unroll
+            for (int part = 0; part < 2; ++part)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_mx(tmem + c * N, values + 256 * k, probs_across + uint64_t(part * (L::kLowOffset >> 4)) + 256 * k,
+                       idesc_mx(N, true) | uint32_t(k) << 4, tmem + L::kOnes, tmem + L::kProbScales, uint32_t(t > w.begin) | part | k);
+            skip(1);
+            if (c + 1 < CH) wait(&ready[slot], parity, 0xaf000000u | slot);
+            ptx::tc_commit(&s.empty[this_slot]);
+          }
+          ptx::tc_commit(&s.probs_empty);
+          if (t == w.end - 1) ptx::tc_commit(&s.sums_full);
+          ++summed;
+        }
+        w.advance();
+      }
+      ptx::tc_commit(&s.drained_sums);
+      ptx::mbar_wait_bounded(&s.drained_sums, 0, 100000000ull);
     }
     __syncwarp();
   } else if (warp == 2) {
@@ -659,39 +715,6 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       }
       w.advance();
     }
-  } else if (warp == 3) {
-    // ----- the items for the softmax warps; tiles of -1 end them
-    if (lane == 0) {
-      a.records[blockIdx.x] = make_int4(0, 0, 0, -1);
-      const int64_t parts = min(s.units, int64_t(gridDim.x));
-      bool good = true, more = true;
-      Walk w;
-      w.start(a, s);
-      for (int n = 0; good && more; ++n) {
-        more = w.next(a, s);
-        good = ptx::mbar_wait_bounded(&s.items_empty[n % kItems], (n / kItems & 1) ^ 1) || failed(0xb0000000u);
-        if (!good) break;
-        Item& m = s.items[n % kItems];
-        m.tiles = -1;
-        if (more) {
-          m.begin = w.begin;
-          m.end = w.end;
-          m.tiles = w.tiles;
-          m.first_token = w.work.first_token_tile(w.tile) * kTokens;
-          m.token_rows = min(int(a.per_tile), w.rows.count - w.tile * int(a.per_tile));
-          m.used = m.token_rows * int(a.group);
-          m.first_row = w.rows.first + w.tile * int(a.per_tile);
-          m.position0 = w.work.base + w.tile * int(a.per_tile);
-          m.head = w.head;
-          m.whole = w.begin == 0 && w.end == w.tiles;
-          m.last_block = w.begin == 0 && w.end < w.tiles ? part_with(s.units, w.item + w.tiles, parts) : -1;
-          if (m.last_block >= 0) a.records[blockIdx.x] = make_int4(m.first_row, m.used, m.head, m.last_block);
-          w.advance();
-        }
-        ptx::mbar_arrive(&s.items_full[n % kItems]);
-      }
-    }
-    __syncwarp();
   } else if (warp >= kFirstSoftmaxWarp) {
     // ----- softmax.  Code that runs once an item is kept in short loops: what is not in the instruction cache costs more to
     // fetch than to execute (the reference's move, unrolled, took 16000 cycles).
@@ -716,49 +739,44 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       __syncwarp();
       ++meetings;
     };
-    // Queries of an item: a thread takes 32 elements at a time, which share a power of two.
+    // Queries of an item: a thread takes 8 elements at a time; the 32 of four neighbouring threads share a power of two.
     const auto bring_queries = [&](const Item& m) {
+      const int used = m.used, first_row = m.first_row, head0 = m.head * int(group);
+      const auto load = [&](int unit) {
+        const uint32_t column = unit / (D / 8), e = unit % (D / 8), at = column * a.group_inverse >> 16;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (unit < N * (D / 8) && int(column) < used)
+          v = *reinterpret_cast<const uint4*>(a.query + size_t(first_row + at) * a.query_stride + size_t(head0 + column - at * group) * D + e * 8);
+        return v;
+      };
+      uint4 next = load(member);
 #pragma unroll 1
-      for (int block = member; block < N * (D / 32); block += kSoftmaxThreads) {
-        const int column = block / (D / 32), part = block % (D / 32), c = part / 4, k = part % 4;
-        uint4 bits[4];
-        if (column < m.used) {
-          const uint32_t at = uint32_t(column) / group;
-          const uint4* from = reinterpret_cast<const uint4*>(a.query + size_t(m.first_row + at) * a.query_stride +
-                                                             size_t(m.head * group + column - at * group) * D + part * 32);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) bits[i] = from[i];
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) bits[i] = make_uint4(0, 0, 0, 0);
-        }
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(bits);
+      for (int unit = member; unit < N * (D / 8); unit += kSoftmaxThreads) {
+        const uint4 bits = next;
+        next = load(unit + kSoftmaxThreads);
+        const uint32_t words[4] = {bits.x, bits.y, bits.z, bits.w};
         uint32_t largest = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) largest = max(largest, max(words[i] << 16 & 0x7fffffffu, words[i] & 0x7fff0000u));
+        for (int i = 0; i < 4; ++i) largest = max(largest, max(words[i] << 16 & 0x7fffffffu, words[i] & 0x7fff0000u));
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
         const uint32_t exponent = largest >> 23;
         // values times 2^(134 - exponent) lie below 2^8; blocks of less than 2^-114 count as zeros, infinities as NaN
         const float up = exponent == 255 ? __uint_as_float(0x7fc00000u) : exponent < 13 ? 0.F : __uint_as_float((261 - exponent) << 23);
         const uint32_t scale = exponent < 13 ? 127 : exponent - 7;
-        uint32_t hi[8], lo[8];
+        uint16_t h[4], l[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint16_t h0, l0, h1, l1;
-          two_parts(__uint_as_float(words[2 * i] << 16) * up, __uint_as_float(words[2 * i] & 0xffff0000u) * up, 16.F, h0, l0);
-          two_parts(__uint_as_float(words[2 * i + 1] << 16) * up, __uint_as_float(words[2 * i + 1] & 0xffff0000u) * up, 16.F, h1, l1);
-          hi[i] = pack4(h0, h1);
-          lo[i] = pack4(l0, l1);
+        for (int i = 0; i < 4; ++i)
+          two_parts(__uint_as_float(words[i] << 16) * up, __uint_as_float(words[i] & 0xffff0000u) * up, 16.F, h[i], l[i]);
+        const uint32_t column = unit / (D / 8), e = unit % (D / 8), c = e / 16, byte = e % 16 * 8;
+        const uint32_t place = c * N * 128 + column * 128 + (((byte >> 4) ^ (column & 7)) << 4) + (byte & 15);
+        *reinterpret_cast<uint2*>(query_hi + place) = make_uint2(pack4(h[0], h[1]), pack4(h[2], h[3]));
+        *reinterpret_cast<uint2*>(query_lo + place) = make_uint2(pack4(l[0], l[1]), pack4(l[2], l[3]));
+        if (e % 4 == 0) {
+          const uint32_t scale_at = 2 * c * kAtomBytes + (column % 32) * 16 + column / 32 * 4 + e / 4 % 4;
+          atoms[scale_at] = uint8_t(scale);
+          atoms[scale_at + kAtomBytes] = uint8_t(scale - 4);
         }
-        const uint32_t at = c * N * 128 + column * 128;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t place = at + (((2 * k + i) ^ (column & 7)) << 4);
-          *reinterpret_cast<uint4*>(query_hi + place) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-          *reinterpret_cast<uint4*>(query_lo + place) = make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
-        }
-        const uint32_t scale_at = 2 * c * kAtomBytes + (column % 32) * 16 + column / 32 * 4 + k;
-        atoms[scale_at] = uint8_t(scale);
-        atoms[scale_at + kAtomBytes] = uint8_t(scale - 4);
       }
       ptx::fence_proxy_async_smem();
       __syncwarp();
@@ -778,7 +796,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     for (int n = 0; more; ++n) {
       const Item& m = s.items[n % kItems];
       if (int(member) < N) {
-        const uint32_t at = member / group;
+        const uint32_t at = member * a.group_inverse >> 16;
         output_at[member] = a.output + size_t(m.first_row + at) * a.output_stride + size_t(m.head * group + member - at * group) * D;
         reference[member] = 0.F;
         settled[member] = int(member) >= m.used;
@@ -947,7 +965,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       const uint32_t place = 2 * blockIdx.x + (m.begin == 0 ? 1 : 0);
       if (member < N) {
         const float v = (by_warp[member] + by_warp[N + member]) + (by_warp[2 * N + member] + by_warp[3 * N + member]);
-        factor[member] = v == 0.F ? 0.F : 1.F / v;
+        factor[member] = v == 0.F ? 0.F : rcp_approx_ftz(v);
         if (!whole) {
           float* const totals = a.partial + size_t(gridDim.x) * 2 * N * D + size_t(place) * 2 * N;
           totals[member] = reference[member];
@@ -957,22 +975,31 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       together();
       wait(&s.sums_full, scored_items & 1, 0xab000000u);
       ptx::tc_fence_after_sync();
+      // eight columns at a time, to the output or to the block's partial sums
       float* const partial = a.partial + (size_t(place) * N + column0) * D + row;
 #pragma unroll 1
-      for (int j = 0; j < C; j += 8) {
-        if (int(column0) + j >= used) break;
+      for (int j = 0; j < C && int(column0) + j < used; j += 8) {
+        float by[8];
+        bf16* to[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          by[e] = factor[column0 + j + e];
+          to[e] = output_at[column0 + j + e] + row;
+        }
+        const int left = used - int(column0) - j;
 #pragma unroll 1
         for (int c = 0; c < CH; ++c) {
           float o[8];
           tmem_load<8>(lanes + c * N + column0 + j, reinterpret_cast<uint32_t*>(o));
           ptx::tmem_load_wait();
+          if (whole) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int column = column0 + j + e;
-            if (column < used) {
-              if (whole) output_at[column][c * 128 + row] = __float2bfloat16_rn(o[e] * factor[column]);
-              else partial[(j + e) * D + c * 128] = o[e];
-            }
+            for (int e = 0; e < 8; ++e)
+              if (e < left) to[e][c * 128] = __float2bfloat16_rn(o[e] * by[e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (e < left) partial[(j + e) * D + c * 128] = o[e];
           }
         }
       }
@@ -1129,7 +1156,7 @@ gw_status gw_paged_attention_bf16(const gw_kv_cache* cache, const gw_sequences* 
     return fail(GW_CUDA_ERROR, "paged attention: " + error);
   const size_t floats = align_up(partial_floats(blocks, columns, cache->head_dim) * sizeof(float), 256);
   const Attention a{*cache, *batch, static_cast<const bf16*>(query_bf16), static_cast<bf16*>(output_bf16), query_stride, output_stride,
-                    heads, group, columns / group, window > (1u << 30) ? 0 : window, uint32_t(__builtin_ctz(cache->page_tokens)), scale,
+                    heads, group, (65536 + group - 1) / group, columns / group, window > (1u << 30) ? 0 : window, uint32_t(__builtin_ctz(cache->page_tokens)), scale,
                     static_cast<float*>(scratch), reinterpret_cast<int4*>(static_cast<uint8_t*>(scratch) + floats)};
   const cudaStream_t s = as_stream(stream);
   GW_CUDA_CHECK((cache->head_dim == 128   ? launch_columns<128, 96>(columns, a, k_map, v_map, blocks, s)
