@@ -10,19 +10,21 @@
 
 #ifdef __CUDACC__
 #define GW_HOST_DEVICE __host__ __device__ __forceinline__
+#define GW_HOST_DEVICE_CALL __host__ __device__ __noinline__      // long code that runs once, in several places
 #else
 #define GW_HOST_DEVICE inline
+#define GW_HOST_DEVICE_CALL inline
 #endif
 
 namespace gw {
 
 constexpr int kTokens = 128;      // cached tokens of a tile
 
-// sum of (a * i + b) / kTokens over i < n, n up to 2^24 and a up to kTokens, by the steps of Euclid's algorithm.  After the first one
-// 32 bits hold everything but the sum, and 32-bit divisions take a fifth of the time that 64-bit ones take.
-GW_HOST_DEVICE int64_t floor_sum(int32_t count, int32_t slope, int64_t start) {
-  int64_t sum = int64_t(count) * (count - 1) / 2 * (slope / kTokens) + count * (start / kTokens);
-  uint32_t n = uint32_t(count), m = kTokens, a = uint32_t(slope % kTokens), b = uint32_t(start % kTokens);
+// sum of (slope * i + start) / kTokens over i < count, count up to 2^24, slope up to kTokens and the sum below 2^31, by the steps of
+// Euclid's algorithm.  In 32 bits: a 64-bit division is 120 instructions.
+GW_HOST_DEVICE uint32_t floor_sum(uint32_t count, uint32_t slope, uint32_t start) {
+  uint32_t sum = uint32_t(uint64_t(count) * (count - 1) / 2 * (slope / kTokens)) + count * (start / kTokens);
+  uint32_t n = count, m = kTokens, a = slope % kTokens, b = start % kTokens;
   while (true) {
     const uint32_t last = a * n + b;              // a, b < m <= kTokens
     if (last < m) return sum;
@@ -31,64 +33,68 @@ GW_HOST_DEVICE int64_t floor_sum(int32_t count, int32_t slope, int64_t start) {
     const uint32_t t = m;
     m = a;
     a = t;
-    sum += int64_t(n) * (n - 1) / 2 * (a / m) + int64_t(n) * (b / m);
+    sum += uint32_t(uint64_t(n) * (n - 1) / 2) * (a / m) + n * (b / m);
     a %= m;
     b %= m;
   }
 }
 
-// One sequence: `rows` query rows, the first at position `base` (below 0: no token), `per_tile` rows a query tile, and a window of
-// `window` tokens (0: none).
+// One sequence: `rows` query rows (up to 2^24), the first at position `base` (below 0: no token; up to 2^30), `per_tile` rows a
+// query tile, and a window of `window` tokens (0: none; up to 2^30).
 struct SequenceWork {
   int32_t base, rows, per_tile, window;
 
   GW_HOST_DEVICE int32_t query_tiles() const { return (rows + per_tile - 1) / per_tile; }
   // the tokens that a query tile reads: [low, high)
   GW_HOST_DEVICE int32_t low(int32_t tile) const {
-    const int64_t at = int64_t(base) + int64_t(tile) * per_tile - window + 1;
-    return window == 0 || at < 0 ? 0 : int32_t(at);
+    const int32_t at = base + tile * per_tile - window + 1;
+    return window == 0 || at < 0 ? 0 : at;
   }
   GW_HOST_DEVICE int32_t high(int32_t tile) const {
-    const int64_t end = int64_t(tile + 1) * per_tile, at = int64_t(base) + (end < rows ? end : rows);
-    return at < 0 ? 0 : int32_t(at);
+    const int32_t end = (tile + 1) * per_tile, at = base + (end < rows ? end : rows);
+    return at < 0 ? 0 : at;
   }
   GW_HOST_DEVICE int32_t first_token_tile(int32_t tile) const { return low(tile) / kTokens; }
-  GW_HOST_DEVICE int32_t token_tiles(int32_t tile) const { return int32_t((int64_t(high(tile)) + kTokens - 1) / kTokens) - first_token_tile(tile); }
+  GW_HOST_DEVICE int32_t token_tiles(int32_t tile) const { return (high(tile) + kTokens - 1) / kTokens - first_token_tile(tile); }
   // units of the query tiles in front of `tile`
-  GW_HOST_DEVICE int64_t units_before(int32_t tile) const {
+  GW_HOST_DEVICE_CALL uint32_t units_before(int32_t tile) const {
     if (tile <= 0) return 0;
     const int32_t whole = tile < query_tiles() ? tile : tile - 1;       // the last one may have fewer rows
-    int64_t units = tile;
+    uint32_t units = tile;
     if (whole < tile) units += token_tiles(whole);
-    const int64_t skip_high = base >= 0 ? 0 : -int64_t(base) / per_tile;      // tiles without any token
-    if (whole > skip_high) units += floor_sum(int32_t(whole - skip_high), per_tile, base + (skip_high + 1) * per_tile + kTokens - 1);
+    const int32_t skip_high = base >= 0 ? 0 : -base / per_tile;         // tiles without any token
+    if (whole > skip_high) units += floor_sum(whole - skip_high, per_tile, uint32_t(base + (skip_high + 1) * per_tile + kTokens - 1));
     if (window != 0) {
-      const int64_t start = int64_t(base) - window + 1, skip_low = start >= 0 ? 0 : (-start + per_tile - 1) / per_tile;
-      if (whole > skip_low) units -= floor_sum(int32_t(whole - skip_low), per_tile, start + skip_low * per_tile);
+      const int32_t start = base - window + 1, skip_low = start >= 0 ? 0 : (-start + per_tile - 1) / per_tile;
+      if (whole > skip_low) units -= floor_sum(whole - skip_low, per_tile, uint32_t(start + skip_low * per_tile));
     }
     return units;
   }
-  GW_HOST_DEVICE int64_t units() const { return units_before(query_tiles()); }
+  GW_HOST_DEVICE uint32_t units() const { return rows <= 0 ? 0 : rows <= per_tile ? 1 + token_tiles(0) : units_before(query_tiles()); }
 };
 
-// Range `part` of `parts` equal ones.
-GW_HOST_DEVICE int64_t range_start(int64_t units, int64_t part, int64_t parts) { return units * part / parts; }
-// The part that has unit `at`.
-GW_HOST_DEVICE int32_t part_with(int64_t units, int64_t at, int64_t parts) {
-  int64_t part = at * parts / units;
-  while (part + 1 < parts && range_start(units, part + 1, parts) <= at) ++part;
-  while (part > 0 && range_start(units, part, parts) > at) --part;
-  return int32_t(part);
-}
+// `units` in `parts` equal ranges (parts <= units < 2^31, parts up to 2^15).
+struct Ranges {
+  uint32_t whole, rest, parts;      // units / parts, units % parts
+  GW_HOST_DEVICE Ranges(uint32_t units, uint32_t parts) : whole(units / parts), rest(units - units / parts * parts), parts(parts) {}
+  GW_HOST_DEVICE uint32_t start(uint32_t part) const { return whole * part + rest * part / parts; }
+  // the range that has unit `at`
+  GW_HOST_DEVICE uint32_t with(uint32_t at) const {
+    uint32_t part = at / whole < parts ? at / whole : parts - 1;
+    while (start(part) > at) --part;
+    return part;
+  }
+};
 
 // What the range [from, to) has of an item whose units start at `item`: token tiles [begin, end) of its `tiles`.
 struct Piece {
   int32_t begin, end;
   bool here;          // false: nothing of it is computed in this range
 };
-GW_HOST_DEVICE Piece piece_of(int64_t item, int32_t tiles, int64_t from, int64_t to) {
-  const int64_t begin = from - item - 1 > 0 ? from - item - 1 : 0, end = to - item - 1 < tiles ? to - item - 1 : tiles;
-  return {int32_t(begin < tiles ? begin : tiles), int32_t(end > 0 ? end : 0), tiles == 0 ? from <= item && item < to : begin < end};
+GW_HOST_DEVICE Piece piece_of(uint32_t item, int32_t tiles, uint32_t from, uint32_t to) {
+  const int32_t begin = int32_t(from - item) - 1, end = int32_t(to - item) - 1;
+  const int32_t first = begin > 0 ? begin : 0, last = end < tiles ? end : tiles;
+  return {first, last, tiles == 0 ? from <= item && item < to : first < last};
 }
 
 }  // namespace gw

@@ -15,8 +15,8 @@
 // of one warp -- a range of their own, so that small probabilities are as exact as large ones, however far below the maximum.
 // That also takes the running maximum out of the loop.  The reference m of a column only has to keep FP32 sums in range: it is 0
 // at first, and moves to the maximum so far (with the sums rescaled) only when a probability times its value scale exceeds 2^40, or
-// when a column's first tokens all lie below 2^-40.  (Value scales below 2^-64 are taken for 2^-64 there, so that no probability
-// passes 2^104 unseen.)
+// when a column's first tokens all lie below 2^-40.  (Value scales below 2^-64 are taken for 2^-64, so that no probability passes
+// 2^104 unseen.)
 //
 //   warp 0      TMA: chunks of [128 tokens x 128 bytes] of K and V into a ring, page by page; the pages' scales, and what the softmax
 //               warps need to know of an item
@@ -24,9 +24,12 @@
 //               both spent half of its time in barriers, with nothing left in the tensor pipe's queue.
 //   warp 2      zeroes rows of V that no query may see: a page's slots behind its last token may hold anything, NaN included, and
 //               0 * NaN is NaN
-//   warps 4..   softmax: for every 32 lanes two warps (three for 96 columns), each with its share of the columns.  After an item's last
+//   warps 4..   softmax: for every 32 lanes two warps (four at 64 columns), each with its share of the columns.  After an item's last
 //               tile they bring the next item's queries to shared memory, so that its first scores are computed while they write the
 //               results of the one before.
+// Two groups of softmax warps with a tile each at a time were slower (16 query rows of drafts 75 -> 84 us, a windowed prompt 128 ->
+// 171 us): the warps waited for instructions.  For the same reason only the producer walks over the items, and what runs once
+// an item is in short loops.
 //
 // Work: attention_work.h.  An item that a cut between two blocks' ranges divides leaves FP32 partial sums in the scratch
 // memory, which a second kernel joins in the order of the blocks (the same bits on every run).
@@ -47,7 +50,7 @@ namespace {
 
 __device__ uint32_t g_attention_error;       // first report since it was last taken
 
-__host__ __device__ constexpr int softmax_warps(int columns) { return columns <= 64 ? 8 : 12; }
+__host__ __device__ constexpr int softmax_warps(int columns) { return columns <= 32 ? 8 : 16; }
 constexpr int kFirstSoftmaxWarp = 4;
 constexpr int kChunkBytes = kTokens * 128;
 constexpr int kAtomBytes = 512;              // scale atom: 128 rows x 4 blocks of 32 elements
@@ -68,23 +71,24 @@ struct Attention {
   int4* records;              // [blocks]: {first query row, columns, KV head, last block} of the item that its last piece begins, or last -1
 };
 
-// An item as the softmax warps see it.
+// A piece of an item, as the producer tells the other warps; tiles of -1 end them.
 struct Item {
-  int begin, end, tiles, first_token;          // token tiles of the piece, of the item; position of tile 0's first token
+  int begin, end, tiles, first_tile;           // token tiles of the piece, of the item; where the item's begin in the sequence
+  int low, high;                               // the tokens that it reads
   int used, token_rows, first_row, position0;  // columns with a query, query rows, the first one, its position
   int head, whole;
 };
 
 struct Shared {
-  uint64_t full[16], empty[16], cleared[16], scales_full[kScaleTiles], scores_full[2], scores_empty[2], probs_full, probs_empty, checked, query_full, sums_full,
-      softmax, items_full[kItems], items_empty[kItems], drained, drained_sums;
+  uint64_t full[16], empty[16], cleared[16], scales_full[kScaleTiles], items_full[kItems], items_empty[kItems];
+  uint64_t scores_full[2], scores_empty[2], probs_full[2], probs_empty[2], checked, query_full, sums_full, softmax, drained, drained_sums;
   float2 scales[kScaleTiles][8];               // {key, value} of a tile's pages; a value scale below 0: no page
   Item items[kItems];
   int move[4];                                 // of the last tiles: some warp asks for the reference to be moved
   uint32_t tensor_memory;
   // units of all blocks, the block's range of them, and the item that has the first
-  int64_t units, from, to, item;
-  int64_t rest;                // units of that item's sequence and head in front of the range
+  uint32_t units, from, to, item;
+  uint32_t rest;               // units of that item's sequence and head in front of the range
   uint32_t sequence;
   int head, tile;
 };
@@ -96,11 +100,10 @@ struct Layout {
   static constexpr int kShare = N / (kSoftmaxWarps / 4);          // columns of a warp
   static constexpr int kChunks = D / 128;
   static constexpr int kQueryBytes = kChunks * N * 128;           // one part
-  static constexpr bool kOneBuffer = N <= 64;                     // both parts of P in the halves of 128-byte rows
-  static constexpr int kProbBytes = kOneBuffer ? kChunkBytes : 2 * kChunkBytes;
-  static constexpr int kLowOffset = kOneBuffer ? 64 : kChunkBytes;
-  static constexpr int kAtoms = 2 * kChunks + 2;                  // queries (both parts), ones, P
-  static constexpr int kFloats = 7 * N + 32 * kSoftmaxWarps;      // reference, factor, settled, by_warp; factors of a warp
+  static constexpr int kProbBytes = 2 * kChunkBytes;              // rows of 128 bytes: the first part in one half, the second in the other
+  static constexpr int kLowOffset = 64;
+  static constexpr int kAtoms = 2 * kChunks + 3;        // queries (both parts), ones, P
+  static constexpr int kFloats = 7 * N + 32 * kSoftmaxWarps;      // as laid out in the kernel
   static constexpr int kSmall = kAtoms * kAtomBytes + kFloats * 4 + 8 * N;
   static constexpr int kAlignment = 1024;
   static constexpr int kStatic = 3072;                            // at least what is declared in the kernel
@@ -113,21 +116,21 @@ struct Layout {
   static constexpr int kQueryScales = kOnes + 4;
   static constexpr int kProbScales = kQueryScales + 8 * kChunks;
   static constexpr int kColumns = 512;
-  static_assert(kProbScales + 4 <= kColumns, "tensor memory over-subscribed");
+  static_assert(kProbScales + 8 <= kColumns, "tensor memory over-subscribed");
   static_assert(kRing >= kChunks + 1, "a tile's chunks and one more");
   static_assert(kRing / (2 * kChunks) + 4 < kScaleTiles, "scales of a tile are read before those of a later one take their place");
   static_assert(kSmemBytes > 116 * 1024, "one block an SM");
   static_assert(sizeof(Shared) + 512 <= kStatic, "");
-  static_assert(N % 16 == 0 && N <= 128 && D % 128 == 0 && kShare % 8 == 0 && kShare <= 32, "");
+  static_assert(N % 16 == 0 && N <= 64 && D % 128 == 0 && kShare % 8 == 0, "");
 };
 
 // ---------------------------------------------------------------------------
-// walking over the block's pieces: every role has its own walk
+// walking over the block's pieces
 // ---------------------------------------------------------------------------
 struct Walk {
   uint32_t sequence;
   int head, tile;
-  int64_t item;
+  uint32_t item;
   SequenceRows rows;
   SequenceWork work;
   // the piece
@@ -186,81 +189,86 @@ __device__ __forceinline__ SequenceWork sequence_work(const Attention& a, uint32
 template <int THREADS>
 __device__ __forceinline__ void find_start(const Attention& a, Shared& shared) {
   constexpr int WARPS = THREADS / 32;
-  __shared__ int64_t sums[WARPS];
+  __shared__ uint32_t sums[WARPS];
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  int64_t total = 0, from = 0, mine = 0, low = 0;
-  // units in front of sequence base + threadIdx.x, over `before` ones in front of sequence base; returns those behind the last one
-  const auto scan = [&](uint32_t base, int64_t before, bool report) {
+  uint32_t before = 0, from = 0;
+  bool idle = false;
+  // First the units of all sequences, then the sequence that has the block's first one; one round does both where there is a thread for
+  // every sequence.
+  const bool one = a.batch.sequences <= THREADS;
+#pragma unroll 1
+  for (uint32_t base = 0, round = 0; round < 2; ) {
     const uint32_t s = base + threadIdx.x;
-    mine = s < a.batch.sequences ? sequence_work(a, s, report).units() * a.cache.kv_heads : 0;
-    int64_t sum = mine;
+    const uint32_t each = s < a.batch.sequences ? sequence_work(a, s, round == 0 && blockIdx.x == 0).units() : 0, mine = each * a.cache.kv_heads;
+    uint32_t sum = mine;
 #pragma unroll
     for (int m = 1; m < 32; m *= 2) {
-      const int64_t other = __shfl_up_sync(0xffffffffu, sum, m);
+      const uint32_t other = __shfl_up_sync(0xffffffffu, sum, m);
       if (lane >= uint32_t(m)) sum += other;
     }
     if (lane == 31) sums[warp] = sum;
     __syncthreads();
-    low = before + sum - mine;
-#pragma unroll
+    uint32_t low = before + sum - mine;
+#pragma unroll 1
     for (int i = 0; i < WARPS; ++i) {
       if (uint32_t(i) < warp) low += sums[i];
       before += sums[i];
     }
-    return before;
-  };
-  const auto found = [&](uint32_t base) {
-    if (low <= from && from < low + mine) {
-      const int64_t units = mine / a.cache.kv_heads, at = from - low;
-      shared.sequence = base + threadIdx.x;
-      shared.head = int(at / units);
-      shared.rest = at - shared.head * units;
+    __syncthreads();
+    base += THREADS;
+    const bool end = base >= a.batch.sequences;
+    if (round == 0 && end) {
+      const uint32_t parts = min(before, gridDim.x);
+      idle = blockIdx.x >= parts;
+      uint32_t to = from = before;
+      if (!idle) {
+        const Ranges ranges(before, parts);
+        from = ranges.start(blockIdx.x);
+        to = ranges.start(blockIdx.x + 1);
+      }
+      if (threadIdx.x == 0) {
+        shared.units = before;
+        shared.from = from;
+        shared.to = to;
+        shared.tile = 0;
+        if (idle) shared.sequence = a.batch.sequences;
+      }
+      if (idle) break;
+    }
+    if ((round == 1 || (one && end)) && low <= from && from - low < mine) {
+      shared.sequence = s;
+      shared.head = int((from - low) / each);
+      shared.rest = (from - low) - shared.head * each;
       shared.item = from - shared.rest;
     }
-  };
-  const bool one = a.batch.sequences <= THREADS;
-  for (uint32_t base = 0; base < a.batch.sequences; base += THREADS) {
-    total = scan(base, total, blockIdx.x == 0);
-    if (!one) __syncthreads();
-  }
-  const int64_t parts = total < gridDim.x ? total : gridDim.x;
-  const bool idle = int64_t(blockIdx.x) >= parts;
-  from = idle ? total : range_start(total, blockIdx.x, parts);
-  if (threadIdx.x == 0) {
-    shared.units = total;
-    shared.from = from;
-    shared.to = idle ? total : range_start(total, blockIdx.x + 1, parts);
-    if (idle) shared.sequence = a.batch.sequences;
-    shared.tile = 0;
-  }
-  if (!idle) {
-    if (one) {
-      found(0);
-    } else {
-      int64_t before = 0;
-      for (uint32_t base = 0; base < a.batch.sequences && before <= from; base += THREADS) {
-        before = scan(base, before, false);
-        found(base);
-        __syncthreads();
-      }
+    if (end) {
+      if (one) break;
+      base = before = 0;
+      ++round;
+    } else if (round == 1 && before > from) {
+      break;
     }
   }
   __syncthreads();
   // the query tile, 32 candidates at a time
   if (warp == 0 && !idle) {
     const SequenceWork w = sequence_work(a, shared.sequence, false);
-    const int64_t rest = shared.rest;
+    const uint32_t rest = shared.rest;
     int lowest = 0, highest = w.query_tiles();                 // units_before(lowest) <= rest < units_before(highest)
+    uint32_t at_lowest = 0;
+#pragma unroll 1
     while (highest - lowest > 1) {
       const int step = (highest - lowest + 31) / 32, candidate = min(lowest + int(lane) * step, highest);
-      const uint32_t below = __ballot_sync(0xffffffffu, candidate < highest && w.units_before(candidate) <= rest);
+      const uint32_t units = w.units_before(candidate);
+      const uint32_t below = __ballot_sync(0xffffffffu, candidate < highest && units <= rest);
       const int at = 31 - __clz(below);
+      at_lowest = __shfl_sync(0xffffffffu, units, at);
       highest = min(lowest + (at + 1) * step, highest);
       lowest += at * step;
     }
     if (lane == 0) {
       shared.tile = lowest;
-      shared.item += w.units_before(lowest);
+      shared.item += at_lowest;
     }
   }
   __syncthreads();
@@ -281,11 +289,13 @@ __device__ __forceinline__ int page_entry(const Attention& a, uint32_t sequence,
 }
 __device__ __forceinline__ uint32_t pack4(uint16_t low, uint16_t high) { return uint32_t(low) | uint32_t(high) << 16; }
 
-// hi and lo codes of two values of size below 448: hi the nearest codes, lo those of (x - hi) * low_scale
-__device__ __forceinline__ void two_parts(float a, float b, float low_scale, uint16_t& hi, uint16_t& lo) {
+// hi and lo codes of two values of size below 448: hi the nearest codes, lo those of (x - hi) * SCALE
+template <int SCALE>
+__device__ __forceinline__ void two_parts(float a, float b, uint16_t& hi, uint16_t& lo) {
   const __half2 x = __floats2half2_rn(a, b);
   hi = __nv_cvt_halfraw2_to_fp8x2(__half2_raw(x), __NV_SATFINITE, __NV_E4M3);
-  const __half2 rest = __hmul2(__hsub2(x, __half2(__nv_cvt_fp8x2_to_halfraw2(hi, __NV_E4M3))), __float2half2_rn(low_scale));
+  __half2 rest = __hsub2(x, __half2(__nv_cvt_fp8x2_to_halfraw2(hi, __NV_E4M3)));
+  if constexpr (SCALE != 1) rest = __hmul2(rest, __float2half2_rn(float(SCALE)));
   lo = __nv_cvt_halfraw2_to_fp8x2(__half2_raw(rest), __NV_SATFINITE, __NV_E4M3);
 }
 
@@ -389,22 +399,21 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
                                                                       const __grid_constant__ CUtensorMap v_map,
                                                                       const __grid_constant__ Attention a) {
   using L = Layout<D, N>;
-  constexpr int CH = L::kChunks, RING = L::kRing, C = L::kShare, kSoftmaxWarps = L::kSoftmaxWarps, kSoftmaxThreads = 32 * kSoftmaxWarps,
-                kThreads = L::kThreads;
+  constexpr int CH = L::kChunks, RING = L::kRing, C = L::kShare, kSoftmaxWarps = L::kSoftmaxWarps, kSoftmaxThreads = 32 * kSoftmaxWarps, kThreads = L::kThreads;
   extern __shared__ uint8_t raw[];
   uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t* const query_hi = base;
   uint8_t* const query_lo = query_hi + L::kQueryBytes;
   uint8_t* const probs = query_lo + L::kQueryBytes;
   uint8_t* const ring = probs + L::kProbBytes;
-  uint8_t* const atoms = ring + RING * kChunkBytes;              // [2 * CH] queries (hi, lo of a chunk), [1] ones, [1] P
+  uint8_t* const atoms = ring + RING * kChunkBytes;              // [2 * CH] queries (hi, lo of a chunk), [1] ones, [2] P
   uint8_t* const ones_atom = atoms + 2 * CH * kAtomBytes;
   uint8_t* const probs_atom = ones_atom + kAtomBytes;
-  float* const reference = reinterpret_cast<float*>(probs_atom + kAtomBytes);     // [N] m of a column
+  float* const reference = reinterpret_cast<float*>(probs_atom + 2 * kAtomBytes); // [N] m of a column
   float* const factor = reference + N;                                            // [N]
   int* const settled = reinterpret_cast<int*>(factor + N);                        // [N] the reference holds: some token lies above 2^-40
   float* const by_warp = factor + 2 * N;                                          // [4][N]
-  float* const spread = by_warp + 4 * N;                                          // [softmax warps][32]
+  float* const spread = by_warp + 4 * N;                                        // [softmax warps][32]
   bf16** const output_at = reinterpret_cast<bf16**>(spread + 32 * kSoftmaxWarps); // [N]
   __shared__ Shared s;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -418,17 +427,17 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&s.scores_full[i], 1);
       ptx::mbar_init(&s.scores_empty[i], kSoftmaxWarps);
+      ptx::mbar_init(&s.probs_full[i], kSoftmaxWarps);
+      ptx::mbar_init(&s.probs_empty[i], 1);
     }
-    ptx::mbar_init(&s.probs_full, kSoftmaxWarps);
-    ptx::mbar_init(&s.probs_empty, 1);
     ptx::mbar_init(&s.checked, kSoftmaxWarps);
+    for (int i = 0; i < 4; ++i) s.move[i] = 0;
     ptx::mbar_init(&s.softmax, kSoftmaxWarps);
     ptx::mbar_init(&s.query_full, kSoftmaxWarps);
     for (int i = 0; i < kScaleTiles; ++i) ptx::mbar_init(&s.scales_full[i], 1);
-    for (int i = 0; i < 4; ++i) s.move[i] = 0;
     for (int i = 0; i < kItems; ++i) {
       ptx::mbar_init(&s.items_full[i], 1);
-      ptx::mbar_init(&s.items_empty[i], kSoftmaxWarps);
+      ptx::mbar_init(&s.items_empty[i], kSoftmaxWarps + 3);      // and both products' threads and the warp that zeroes
     }
     ptx::mbar_init(&s.sums_full, 1);
     ptx::mbar_init(&s.drained, 1);
@@ -439,10 +448,8 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     ptx::tmem_alloc(&s.tensor_memory, L::kColumns);
     ptx::tmem_relinquish();
   }
-  for (int i = threadIdx.x; i < kAtomBytes / 4; i += kThreads) {
-    reinterpret_cast<uint32_t*>(ones_atom)[i] = 0x7f7f7f7fu;      // 2^0
-    reinterpret_cast<uint32_t*>(probs_atom)[i] = 0x7f7f7f7fu;
-    for (int j = 0; j < 2 * CH; ++j) reinterpret_cast<uint32_t*>(atoms + j * kAtomBytes)[i] = 0x7f7f7f7fu;
+  for (int i = threadIdx.x; i < kAtomBytes / 4; i += kThreads) {        // 2^0
+    for (int j = 0; j < L::kAtoms; ++j) reinterpret_cast<uint32_t*>(atoms + j * kAtomBytes)[i] = 0x7f7f7f7fu;
   }
   ptx::fence_proxy_async_smem();
   ptx::tc_fence_before_sync();
@@ -450,9 +457,12 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
   find_start<kThreads>(a, s);                                    // ends with __syncthreads()
   ptx::tc_fence_after_sync();
   const uint32_t tmem = s.tensor_memory;
-  const auto failed = [](uint32_t code) {
-    atomicCAS(&g_attention_error, 0u, code | (blockIdx.x << 8));
-    return false;
+  // What a role gave up on, reported at the end.  A thread whose wait ran out waits no more, but goes on to the end; the roles of one
+  // warp or thread leave at once.
+  uint32_t error = 0;
+  const auto wait = [&error](uint64_t* bar, uint32_t phase, uint32_t code) {
+    if (error == 0 && !ptx::mbar_wait_bounded(bar, phase)) error = code;
+    return error == 0;
   };
 
   if (warp == 0) {
@@ -461,15 +471,15 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     const int outside = int(a.cache.pages * a.cache.kv_heads * page_tokens);        // rows from here on read as zeros
     int slot = 0, issued = 0, tile_count = 0;
     uint32_t parity = 1;                                         // empty slots: the first pass does not wait
-    bool good = true;
-    const int64_t parts = min(s.units, int64_t(gridDim.x));
     if (lane == 0) a.records[blockIdx.x] = make_int4(0, 0, 0, -1);
     Walk w;
     w.start(a, s);
-    for (int n = 0; good; ++n) {
+#pragma unroll 1
+    for (int n = 0;; ++n) {
       const bool more = w.next(a, s);
-      good = ptx::mbar_wait_warp(&s.items_empty[n % kItems], (n / kItems & 1) ^ 1) || failed(0xb0000000u);
-      if (!good) break;
+      wait(&s.items_empty[n % kItems], (n / kItems & 1) ^ 1, 0xb0000000u);
+      error = __reduce_max_sync(0xffffffffu, error);             // the warp leaves as one
+      if (error) break;
       if (lane == 0) {
         Item& m = s.items[n % kItems];
         m.tiles = -1;                                            // the end
@@ -477,7 +487,9 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
           m.begin = w.begin;
           m.end = w.end;
           m.tiles = w.tiles;
-          m.first_token = w.work.first_token_tile(w.tile) * kTokens;
+          m.first_tile = w.work.first_token_tile(w.tile);
+          m.low = w.work.low(w.tile);
+          m.high = w.work.high(w.tile);
           m.token_rows = min(int(a.per_tile), w.rows.count - w.tile * int(a.per_tile));
           m.used = m.token_rows * int(a.group);
           m.first_row = w.rows.first + w.tile * int(a.per_tile);
@@ -485,7 +497,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
           m.head = w.head;
           m.whole = w.begin == 0 && w.end == w.tiles;
           if (w.begin == 0 && w.end < w.tiles)
-            a.records[blockIdx.x] = make_int4(m.first_row, m.used, w.head, part_with(s.units, w.item + w.tiles, parts));
+            a.records[blockIdx.x] = make_int4(m.first_row, m.used, w.head, Ranges(s.units, min(s.units, gridDim.x)).with(w.item + w.tiles));
         }
         ptx::mbar_arrive(&s.items_full[n % kItems]);
       }
@@ -505,15 +517,12 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         }
         return v;
       };
-      // row of the page in the tensor maps
-      const auto row_of = [&](int entry) {
-        if (uint32_t(entry) < a.cache.pages) return int((uint32_t(entry) * a.cache.kv_heads + w.head) * page_tokens);
-        if (entry != -2) atomicCAS(&g_attention_error, 0u, 0xa1000000u | (w.sequence & 0xffffffu));
-        return outside;
-      };
       const auto bring = [&](const CUtensorMap* map, int row) {
+#pragma unroll 1
         for (int c = 0; c < CH; ++c) {
-          if (!ptx::mbar_wait_warp(&s.empty[slot], parity)) return failed(0xa3000000u | slot);
+          wait(&s.empty[slot], parity, 0xa3000000u | slot);
+          error = __reduce_max_sync(0xffffffffu, error);
+          if (error) return;
           if (lane == 0) ptx::mbar_expect_tx(&s.full[slot], kChunkBytes);
           __syncwarp();
           if (lane < boxes) ptx::tma_load_2d(ring + slot * kChunkBytes + lane * page_tokens * 128, map, c * 128, row, &s.full[slot]);
@@ -523,45 +532,48 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
             parity ^= 1;
           }
         }
-        return true;
       };
+      // K of a tile, then V of the one before; the pages two tiles ahead and the scales one ahead are asked for meanwhile
       int entry = entry_of(w.begin), entry_next = entry_of(w.begin + 1), row_before = 0;
       float2 scales = scales_of(entry);
-      for (int t = w.begin; good && t < w.end; ++t) {
-        const int entry_after = entry_of(t + 2), row = row_of(entry);
-        good = bring(&k_map, row);
-        if (lane < boxes) s.scales[tile_count % kScaleTiles][lane] = scales;
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&s.scales_full[tile_count % kScaleTiles]);
-        ++tile_count;
-        scales = scales_of(entry_next);
-        if (good && t > w.begin) good = bring(&v_map, row_before);
+#pragma unroll 1
+      for (int t = w.begin; error == 0 && w.begin < w.end && t <= w.end; ++t) {
+        const int entry_after = entry_of(t + 2);
+        int row = outside;
+        if (t < w.end) {
+          if (uint32_t(entry) < a.cache.pages) row = int((uint32_t(entry) * a.cache.kv_heads + w.head) * page_tokens);
+          else if (entry != -2) atomicCAS(&g_attention_error, 0u, 0xa1000000u | (w.sequence & 0xffffffu));
+          bring(&k_map, row);
+          if (lane < boxes) s.scales[tile_count % kScaleTiles][lane] = scales;
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(&s.scales_full[tile_count % kScaleTiles]);
+          ++tile_count;
+          scales = scales_of(entry_next);
+        }
+        if (error == 0 && t > w.begin) bring(&v_map, row_before);
         row_before = row;
         entry = entry_next;
         entry_next = entry_after;
       }
-      if (good && w.end > w.begin) good = bring(&v_map, row_before);
+      if (error) break;
       w.advance();
     }
     // the copies still in flight land before the block ends
+#pragma unroll 1
     for (int i = issued < RING ? issued : RING; i > 0; --i) {
       if (slot == 0) {
         slot = RING;
         parity ^= 1;
       }
       --slot;
-      ptx::mbar_wait_warp(&s.full[slot], parity ^ 1, 0, 100000000ull);
+      ptx::mbar_wait_bounded(&s.full[slot], parity ^ 1, 100000000ull);
     }
   } else if (warp == 1) {
     // ----- S, by one thread: the compiler keeps its descriptors in uniform registers only where it knows that one thread runs the code
-    // (72 to 110 cycles an instruction otherwise, whatever N; 36 at N = 16, 44 at 64, 51 at 96 here)
+    // (72 to 110 cycles an instruction otherwise, whatever N; 36 at N = 16, 44 at 64 here)
     if (ptx::elect_one()) {
       int slot = 0, item = 0, scored = 0;
       uint32_t parity = 0;
-      bool good = true;
-      const auto wait = [&](uint64_t* bar, uint32_t phase, uint32_t code) {
-        good = good && (ptx::mbar_wait_bounded(bar, phase) || failed(code));
-      };
       const auto skip = [&](int chunks) {
         slot += chunks;
         if (slot >= RING) {
@@ -573,46 +585,47 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       const uint64_t hi_rows = ptx::smem_desc_sw128(ptx::smem_u32(query_hi)), lo_rows = ptx::smem_desc_sw128(ptx::smem_u32(query_lo));
       const uint64_t atom = ptx::smem_desc_sf_atom(ptx::smem_u32(atoms));
       ptx::tc_copy_sf_atom(tmem + L::kOnes, ptx::smem_desc_sf_atom(ptx::smem_u32(ones_atom)));
-      Walk w;
-      w.start(a, s);
-      while (good && w.next(a, s)) {
-        if (w.end > w.begin) {
-          wait(&s.query_full, item & 1, 0xa5000000u);
-          if (!good) break;
-          ptx::tc_fence_after_sync();
-#pragma unroll
-          for (int i = 0; i < 2 * CH; ++i) ptx::tc_copy_sf_atom(tmem + L::kQueryScales + 4 * i, atom + uint64_t(i * (kAtomBytes >> 4)));
 #pragma unroll 1
-          for (int t = w.begin; good && t < w.end; ++t) {
-            const int buffer = scored & 1;
-            wait(&s.scores_empty[buffer], ((scored >> 1) & 1) ^ 1, 0xa6000000u | buffer);
-            const uint32_t d = tmem + L::kScores + buffer * N;
-            wait(&s.full[slot], parity, 0xa4000000u | slot);
+      for (int n = 0; wait(&s.items_full[n % kItems], n / kItems & 1, 0xb1000000u); ++n) {
+        const Item& m = s.items[n % kItems];
+        const int begin = m.begin, end = m.end, tiles = m.tiles;
+        ptx::mbar_arrive(&s.items_empty[n % kItems]);
+        if (tiles < 0) break;
+        if (tiles == 0) continue;
+        if (!wait(&s.query_full, item++ & 1, 0xa5000000u)) break;
+        ptx::tc_fence_after_sync();
 #pragma unroll 1
-            for (int c = 0; good && c < CH; ++c) {
-              ptx::tc_fence_after_sync();
-              const int this_slot = slot;
-              const uint64_t keys = ring_rows + uint64_t(slot * (kChunkBytes >> 4)), offset = uint64_t(c * (N * 128 >> 4));
-              const uint32_t scales = tmem + L::kQueryScales + 8 * c;
+        for (int i = 0; i < 2 * CH; ++i) ptx::tc_copy_sf_atom(tmem + L::kQueryScales + 4 * i, atom + uint64_t(i * (kAtomBytes >> 4)));
+#pragma unroll 1
+        for (int t = begin; t < end; ++t) {
+          const int buffer = scored & 1;
+          wait(&s.scores_empty[buffer], ((scored >> 1) & 1) ^ 1, 0xa6000000u | buffer);
+          const uint32_t d = tmem + L::kScores + buffer * N;
+          if (!wait(&s.full[slot], parity, 0xa4000000u | slot)) break;
+#pragma unroll 1
+          for (int c = 0; c < CH; ++c) {
+            ptx::tc_fence_after_sync();
+            const int this_slot = slot;
+            const uint64_t keys = ring_rows + uint64_t(slot * (kChunkBytes >> 4)), offset = uint64_t(c * (N * 128 >> 4));
+            const uint32_t scales = tmem + L::kQueryScales + 8 * c;
 #pragma unroll
-              for (int part = 0; part < 2; ++part)
+            for (int part = 0; part < 2; ++part)
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  mma_mx(d, keys + 2 * k, (part ? lo_rows : hi_rows) + offset + 2 * k, idesc_mx(N, false) | uint32_t(k) << 4, tmem + L::kOnes,
-                         scales + 4 * part, c | part | k);
-              skip(1);
-              // before the commit, which comes back once its products have left the queue
-              if (c + 1 < CH) wait(&s.full[slot], parity, 0xa4000000u | slot);
-              ptx::tc_commit(&s.empty[this_slot]);
-            }
-            ptx::tc_commit(&s.scores_full[buffer]);
-            ++scored;
-            if (t > w.begin) skip(CH);                           // V of the tile before
+              for (int k = 0; k < 4; ++k)
+                mma_mx(d, keys + 2 * k, (part ? lo_rows : hi_rows) + offset + 2 * k, idesc_mx(N, false) | uint32_t(k) << 4, tmem + L::kOnes,
+                       scales + 4 * part, c | part | k);
+            skip(1);
+            // before the commit, which comes back once its products have left the queue
+            if (c + 1 < CH && !wait(&s.full[slot], parity, 0xa4000000u | slot)) break;
+            ptx::tc_commit(&s.empty[this_slot]);
           }
-          skip(CH);
-          ++item;
+          if (error) break;
+          ptx::tc_commit(&s.scores_full[buffer]);
+          ++scored;
+          if (t > begin) skip(CH);                               // V of the tile before
         }
-        w.advance();
+        if (error) break;
+        skip(CH);
       }
       // products still in flight end before tensor memory is released
       ptx::tc_commit(&s.drained);
@@ -624,10 +637,6 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     if (ptx::elect_one()) {
       int slot = 0, summed = 0;
       uint32_t parity = 0;
-      bool good = true;
-      const auto wait = [&](uint64_t* bar, uint32_t phase, uint32_t code) {
-        good = good && (ptx::mbar_wait_bounded(bar, phase) || failed(code));
-      };
       const auto skip = [&](int chunks) {
         slot += chunks;
         if (slot >= RING) {
@@ -636,23 +645,28 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         }
       };
       const uint64_t ring_across = across_desc(ptx::smem_u32(ring)), probs_across = across_desc(ptx::smem_u32(probs));
-      Walk w;
-      w.start(a, s);
-      while (good && w.next(a, s)) {
-        const int first = w.work.first_token_tile(w.tile), low = w.work.low(w.tile), high = w.work.high(w.tile);
-        if (w.end > w.begin) skip(CH);                           // K of the first tile
+      const uint64_t atom = ptx::smem_desc_sf_atom(ptx::smem_u32(probs_atom));
 #pragma unroll 1
-        for (int t = w.begin; good && t < w.end; ++t) {
-          if (t + 1 < w.end) skip(CH);                           // K of the next one
-          const bool clear = needs_clearing(first + t, low, high);
-          uint64_t* const ready = clear ? s.cleared : s.full;
-          wait(&s.probs_full, summed & 1, 0xa7000000u);
-          wait(&ready[slot], parity, 0xaf000000u | slot);
-          if (!good) break;
+      for (int n = 0; wait(&s.items_full[n % kItems], n / kItems & 1, 0xb2000000u); ++n) {
+        const Item& m = s.items[n % kItems];
+        const int begin = m.begin, end = m.end, tiles = m.tiles, first_tile = m.first_tile, low = m.low, high = m.high;
+        ptx::mbar_arrive(&s.items_empty[n % kItems]);
+        if (tiles < 0) break;
+        if (tiles == 0) continue;
+        skip(CH);                                                // K of the first tile
+#pragma unroll 1
+        for (int t = begin; t < end; ++t) {
+          if (t + 1 < end) skip(CH);                             // K of the next one
+          uint64_t* const ready = needs_clearing(first_tile + t, low, high) ? s.cleared : s.full;
+          const int buffer = summed & 1;
+          wait(&s.probs_full[buffer], (summed >> 1) & 1, 0xa7000000u);
+          if (!wait(&ready[slot], parity, 0xaf000000u | slot)) break;
           ptx::tc_fence_after_sync();
-          ptx::tc_copy_sf_atom(tmem + L::kProbScales, ptx::smem_desc_sf_atom(ptx::smem_u32(probs_atom)));
+          const uint32_t scales = tmem + L::kProbScales + 4 * buffer;
+          const uint64_t p = probs_across + uint64_t(buffer * (kChunkBytes >> 4));
+          ptx::tc_copy_sf_atom(scales, atom + uint64_t(buffer * (kAtomBytes >> 4)));
 #pragma unroll 1
-          for (int c = 0; good && c < CH; ++c) {
+          for (int c = 0; c < CH; ++c) {
             ptx::tc_fence_after_sync();
             const int this_slot = slot;
             const uint64_t values = ring_across + uint64_t(slot * (kChunkBytes >> 4));
@@ -660,17 +674,18 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
             for (int part = 0; part < 2; ++part)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                mma_mx(tmem + c * N, values + 256 * k, probs_across + uint64_t(part * (L::kLowOffset >> 4)) + 256 * k,
-                       idesc_mx(N, true) | uint32_t(k) << 4, tmem + L::kOnes, tmem + L::kProbScales, uint32_t(t > w.begin) | part | k);
+                mma_mx(tmem + c * N, values + 256 * k, p + uint64_t(part * (L::kLowOffset >> 4)) + 256 * k, idesc_mx(N, true) | uint32_t(k) << 4,
+                       tmem + L::kOnes, scales, uint32_t(t > begin) | part | k);
             skip(1);
-            if (c + 1 < CH) wait(&ready[slot], parity, 0xaf000000u | slot);
+            if (c + 1 < CH && !wait(&ready[slot], parity, 0xaf000000u | slot)) break;
             ptx::tc_commit(&s.empty[this_slot]);
           }
-          ptx::tc_commit(&s.probs_empty);
-          if (t == w.end - 1) ptx::tc_commit(&s.sums_full);
+          if (error) break;
+          ptx::tc_commit(&s.probs_empty[buffer]);
+          if (t == end - 1) ptx::tc_commit(&s.sums_full);
           ++summed;
         }
-        w.advance();
+        if (error) break;
       }
       ptx::tc_commit(&s.drained_sums);
       ptx::mbar_wait_bounded(&s.drained_sums, 0, 100000000ull);
@@ -681,17 +696,28 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     // this warp is never a lap of the ring away
     int slot = 0;
     uint32_t parity = 0;
-    bool good = true;
-    Walk w;
-    w.start(a, s);
-    const auto chunk = [&](bool clear, int clear_below, int clear_from) {
-      for (int c = 0; good && c < CH; ++c) {
-        good = ptx::mbar_wait_warp(&s.full[slot], parity, 20) || failed(0xa9000000u | slot);
-        if (!good) return;
-        if (clear) {
+#pragma unroll 1
+    for (int n = 0;; ++n) {
+      wait(&s.items_full[n % kItems], n / kItems & 1, 0xb3000000u);
+      error = __reduce_max_sync(0xffffffffu, error);
+      if (error) break;
+      const Item& m = s.items[n % kItems];
+      const int begin = m.begin, steps = 2 * (m.end - m.begin), tiles = m.tiles, first_tile = m.first_tile, low = m.low, high = m.high;
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&s.items_empty[n % kItems]);
+      if (tiles < 0) break;
+      // in the ring's order: K of the first tile, then K of the next one and V of each
+#pragma unroll 1
+      for (int i = 0; error == 0 && i < CH * steps; ++i) {
+        const int step = i / CH, t = begin + (step == steps - 1 ? steps / 2 - 1 : (step - 1) / 2), start = (first_tile + t) * kTokens;
+        wait(&s.full[slot], parity, 0xa9000000u | slot);
+        error = __reduce_max_sync(0xffffffffu, error);
+        if (error) break;
+        if ((step == steps - 1 || (step >= 2 && step % 2 == 0)) && needs_clearing(first_tile + t, low, high)) {
           uint4* rows = reinterpret_cast<uint4*>(ring + slot * kChunkBytes);
-          for (int i = lane; i < clear_below * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
-          for (int i = clear_from * 8 + lane; i < kTokens * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+          for (int k = lane; k < kTokens * 8; k += 32)
+            if (start + k / 8 < low || start + k / 8 >= high) rows[k] = make_uint4(0, 0, 0, 0);
           ptx::fence_proxy_async_smem();
           __syncwarp();
         }
@@ -704,32 +730,17 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
           parity ^= 1;
         }
       }
-    };
-    while (good && w.next(a, s)) {
-      const int first = w.work.first_token_tile(w.tile), low = w.work.low(w.tile), high = w.work.high(w.tile);
-      if (w.end > w.begin) chunk(false, 0, 0);
-      for (int t = w.begin; good && t < w.end; ++t) {
-        if (t + 1 < w.end) chunk(false, 0, 0);
-        const int start = (first + t) * kTokens;
-        chunk(needs_clearing(first + t, low, high), low - start, high - start);
-      }
-      w.advance();
+      if (error) break;
     }
-  } else if (warp >= kFirstSoftmaxWarp) {
+  } else {
     // ----- softmax.  Code that runs once an item is kept in short loops: what is not in the instruction cache costs more to
     // fetch than to execute (the reference's move, unrolled, took 16000 cycles).
-    const uint32_t quadrant = warp & 3, column0 = (warp - kFirstSoftmaxWarp) / 4 * C,
-                   member = threadIdx.x - 32 * kFirstSoftmaxWarp;
+    const uint32_t quadrant = warp & 3, column0 = (warp - kFirstSoftmaxWarp) / 4 * C, member = threadIdx.x - 32 * kFirstSoftmaxWarp;
     const uint32_t lanes = tmem + (quadrant * 32 << 16);
     const uint32_t row = quadrant * 32 + lane;                   // the lane's token in a tile
     const uint32_t group = a.group;
     float* const my_spread = spread + 32 * (warp - kFirstSoftmaxWarp);
     int scored_items = 0, tile_count = 0;
-    // A thread whose wait ran out waits no more, but goes on to the end.
-    bool good = true;
-    const auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
-      if (good && !ptx::mbar_wait_bounded(bar, parity)) good = failed(code);
-    };
     // a barrier of the softmax warps, bounded as all waits are
     uint32_t meetings = 0;
     const auto together = [&]() {
@@ -767,7 +778,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         uint16_t h[4], l[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          two_parts(__uint_as_float(words[i] << 16) * up, __uint_as_float(words[i] & 0xffff0000u) * up, 16.F, h[i], l[i]);
+          two_parts<16>(__uint_as_float(words[i] << 16) * up, __uint_as_float(words[i] & 0xffff0000u) * up, h[i], l[i]);
         const uint32_t column = unit / (D / 8), e = unit % (D / 8), c = e / 16, byte = e % 16 * 8;
         const uint32_t place = c * N * 128 + column * 128 + (((byte >> 4) ^ (column & 7)) << 4) + (byte & 15);
         *reinterpret_cast<uint2*>(query_hi + place) = make_uint2(pack4(h[0], h[1]), pack4(h[2], h[3]));
@@ -782,18 +793,74 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&s.query_full);
     };
-    // From item n on, what the warps need of it before its first tile; false: there is none.
-    const auto next_item = [&](int n) {
-      wait(&s.items_full[n % kItems], n / kItems & 1, 0xb1000000u);
-      good = __all_sync(0xffffffffu, good);                      // a warp goes on or leaves as one
-      const Item& m = s.items[n % kItems];
-      if (!good || m.tiles < 0) return false;
-      if (m.tiles > 0) bring_queries(m);
-      return true;
-    };
-    bool more = next_item(0);
+    float total[C];
 #pragma unroll 1
-    for (int n = 0; more; ++n) {
+    for (int n = -1;;) {
+      // the next item's queries, while the last product of the one before runs: its scores are all computed
+      wait(&s.items_full[(n + 1) % kItems], (n + 1) / kItems & 1, 0xb4000000u);
+      error = __reduce_max_sync(0xffffffffu, error);             // a warp goes on or leaves as one
+      const bool more = error == 0 && s.items[(n + 1) % kItems].tiles >= 0;
+      if (more && s.items[(n + 1) % kItems].tiles > 0) bring_queries(s.items[(n + 1) % kItems]);
+      if (n >= 0) {
+        const Item& m = s.items[n % kItems];
+        if (m.tiles > 0) {
+          const int used = m.used;
+          // sums of a column over the tokens
+          const float sum = lane_sums(total, lane);
+          if (lane < uint32_t(C)) by_warp[quadrant * N + column0 + lane] = sum;
+          together();
+          const bool whole = m.whole;
+          const uint32_t place = 2 * blockIdx.x + (m.begin == 0 ? 1 : 0);
+          if (member < N) {
+            const float v = (by_warp[member] + by_warp[N + member]) + (by_warp[2 * N + member] + by_warp[3 * N + member]);
+            factor[member] = v == 0.F ? 0.F : rcp_approx_ftz(v);
+            if (!whole) {
+              float* const totals = a.partial + size_t(gridDim.x) * 2 * N * D + size_t(place) * 2 * N;
+              totals[member] = reference[member];
+              totals[N + member] = v;
+            }
+          }
+          together();
+          wait(&s.sums_full, scored_items & 1, 0xab000000u);
+          ptx::tc_fence_after_sync();
+          // eight columns at a time, to the output or to the block's partial sums
+          float* const partial = a.partial + size_t(place) * N * D + row;
+#pragma unroll 1
+          for (int j = (warp - kFirstSoftmaxWarp) / 4 * 8; j < used; j += kSoftmaxWarps / 4 * 8) {
+            float by[8];
+            bf16* to[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              by[e] = factor[j + e];
+              to[e] = output_at[j + e] + row;
+            }
+            const int left = used - j;
+#pragma unroll 1
+            for (int c = 0; c < CH; ++c) {
+              float o[8];
+              tmem_load<8>(lanes + c * N + j, reinterpret_cast<uint32_t*>(o));
+              ptx::tmem_load_wait();
+              if (whole) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  if (e < left) to[e][c * 128] = __float2bfloat16_rn(o[e] * by[e]);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  if (e < left) partial[(j + e) * D + c * 128] = o[e];
+              }
+            }
+          }
+          ++scored_items;
+        }
+        // The sums were read: the next item's first product may overwrite them once it has the probabilities that this thread
+        // publishes later.  What the item had in shared memory is free.
+        ptx::tc_fence_before_sync();
+        together();
+        if (lane == 0) ptx::mbar_arrive(&s.items_empty[n % kItems]);
+      }
+      if (!more) break;
+      ++n;
       const Item& m = s.items[n % kItems];
       if (int(member) < N) {
         const uint32_t at = member * a.group_inverse >> 16;
@@ -806,43 +873,48 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
 #pragma unroll 1
         for (int column = warp - kFirstSoftmaxWarp; column < m.used; column += kSoftmaxWarps)
           for (int d = lane * 8; d < D; d += 256) *reinterpret_cast<uint4*>(output_at[column] + d) = make_uint4(0, 0, 0, 0);
-        more = next_item(n + 1);
-        together();
-        if (lane == 0) ptx::mbar_arrive(&s.items_empty[n % kItems]);
         continue;
       }
-      float total[C];
 #pragma unroll
       for (int j = 0; j < C; ++j) total[j] = 0.F;
-      const int used = m.used, end = m.end, token_rows = m.token_rows;
+      const int used = m.used, begin = m.begin, end = m.end, token_rows = m.token_rows;
       const float to_log2 = a.scale * 1.4426950408889634F;
-      int ahead = m.first_token + m.begin * kTokens + int(row) - m.position0;      // of the lane's token, to the first query
 
 #pragma unroll 1
-      for (int t = m.begin; t < end; ++t, ahead += kTokens) {
-        const int entry = tile_count % kScaleTiles;
+      for (int t = begin; t < end; ++t, ++tile_count) {
+        const int entry = tile_count % kScaleTiles, buffer = tile_count & 1, round = tile_count >> 1 & 1;
+        const int ahead = (m.first_tile + t) * kTokens + int(row) - m.position0;       // of the lane's token, to the first query
         wait(&s.scales_full[entry], tile_count / kScaleTiles & 1, 0xac000000u);
         const float2 scales = s.scales[entry][row >> a.page_shift];
-        // the columns that see the lane's token: query row i where ahead <= i < ahead + window
-        const int from = max(0, min(ahead, N)) * int(group);
-        int to = a.window ? max(0, min(ahead + int(a.window), token_rows)) * int(group) : used;
-        if (scales.y < 0.F) to = 0;
-        const bool open = __all_sync(0xffffffffu, from == 0 && to == used);
-        const uint32_t seen_from = from - column0, seen_span = to > from ? to - from : 0;       // column0 + j - from < span, unsigned
-        const float scale = scales.x * to_log2, value_scale = scales.y < 0.F ? 0.F : scales.y, bound_scale = fmaxf(value_scale, 5.42101086e-20F);
-        // lane j: whether any of the warp's tokens may be seen from column j
-        const int seen_low = __reduce_min_sync(0xffffffffu, from), seen_high = __reduce_max_sync(0xffffffffu, to);
-        const bool sees = seen_low <= int(column0 + lane) && int(column0 + lane) < seen_high;
+        // The columns that see the lane's token: query row i where ahead <= i < ahead + window.  Most tiles are open: seen from every column.
+        const int tile_ahead = ahead - int(row);
+        const bool open = __all_sync(0xffffffffu, scales.y >= 0.F) && used == N && tile_ahead + kTokens <= 1 &&
+                          (a.window == 0 || tile_ahead + int(a.window) >= token_rows);
+        uint32_t seen_from = 0, seen_span = N;                   // column0 + j - from < span, unsigned
+        int seen_low = 0, seen_high = N;                         // columns that may see any of the warp's tokens
+        if (!open) {
+          const int from = max(0, min(ahead, N)) * int(group);
+          int to = a.window ? max(0, min(ahead + int(a.window), token_rows)) * int(group) : used;
+          if (!(scales.y >= 0.F)) to = 0;
+          seen_from = from - column0;
+          seen_span = to > from ? to - from : 0;
+          seen_low = __reduce_min_sync(0xffffffffu, from);
+          seen_high = __reduce_max_sync(0xffffffffu, to);
+        }
+        const float scale = scales.x * to_log2, value_scale = fmaxf(scales.y, 5.42101086e-20F);         // 2^-64
 
-        const int buffer = tile_count & 1;
-        wait(&s.scores_full[buffer], (tile_count >> 1) & 1, 0xa8000000u);
+        wait(&s.scores_full[buffer], round, 0xa8000000u);
+        if (tile_count >= 2) wait(&s.probs_empty[buffer], round ^ 1, 0xaa000000u);
         ptx::tc_fence_after_sync();
         const uint32_t scores = lanes + L::kScores + buffer * N + column0;
-        float p[C];
-        uint32_t hi[C / 4], lo[C / 4], exponent;
-        // Once, or again after the reference moved.
+        uint8_t* const my_probs = probs + buffer * kChunkBytes + row * 128;
+        uint8_t* const my_atom = probs_atom + buffer * kAtomBytes;
+        bool added = false;
+        // Once, or again after the reference moved.  What a warp that asks for a move has is not added to the sums; what the others added
+        // stays: a move scales what is in the sums.
 #pragma unroll 1
         for (bool moved = false;; moved = true) {
+          float p[C];
           tmem_load_columns<C>(scores, reinterpret_cast<uint32_t*>(p));
           ptx::tmem_load_wait();
           uint32_t bits[C];
@@ -850,38 +922,50 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
           for (int j = 0; j < C; ++j) {
             p[j] = exp2_approx(fmaf(p[j], scale, -reference[column0 + j]));
             if (!open) p[j] = uint32_t(j) - seen_from < seen_span ? p[j] : 0.F;
-            // over the warp's tokens; not below 2^-119, where the factor below would not be finite
-            bits[j] = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaf(p[j], bound_scale, 1.5046327691e-36F)));
+            bits[j] = __reduce_max_sync(0xffffffffu, __float_as_uint(p[j] * value_scale));          // over the warp's tokens
           }
           const uint32_t largest = pick<C>(bits, lane);          // lane j: of column j
-          exponent = largest >> 23;
-          if (!moved) {
-            bool ask = false;
-            if (lane < uint32_t(C)) {
-              // NaN counts as too high
-              ask = largest > kHighBits;
-              if (!settled[column0 + lane] && sees) {
-                if (largest < kLowBits) ask = true;
-                else settled[column0 + lane] = 1;
-              }
-              if (ask) s.move[tile_count & 3] = 1;
+          const uint32_t exponent = max(largest >> 23, 8u);      // below, the factor would not be finite
+          bool ask = false;
+          if (!moved && lane < uint32_t(C)) {
+            const uint32_t column = column0 + lane;
+            ask = largest > kHighBits;                           // NaN too
+            if (!settled[column] && seen_low <= int(column) && int(column) < seen_high) {
+              if (largest < kLowBits) ask = true;
+              else settled[column] = 1;
             }
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&s.checked);
+            if (ask) s.move[tile_count & 3] = 1;
           }
+          ask = __any_sync(0xffffffffu, ask);
+          if (!moved && lane == 0) ptx::mbar_arrive(&s.checked);
           // P: the warp's 32 tokens of a column share a power of two, 2^-7 of that of the largest
-          __syncwarp();
           my_spread[lane] = __uint_as_float((261 - exponent) << 23);
+          if (lane < uint32_t(C)) {
+            const uint32_t column = column0 + lane;
+            my_atom[column % 32 * 16 + column / 32 * 4 + quadrant] = uint8_t(exponent - 7);
+          }
           __syncwarp();
 #pragma unroll
-          for (int j = 0; j < C; j += 4) {
-            const float4 up = *reinterpret_cast<const float4*>(my_spread + j);
-            uint16_t h0, l0, h1, l1;
-            // in this order: the factor of a column that sees none of these tokens is 2^126, and 0 stays 0
-            two_parts(p[j] * value_scale * up.x, p[j + 1] * value_scale * up.y, 1.F, h0, l0);
-            two_parts(p[j + 2] * value_scale * up.z, p[j + 3] * value_scale * up.w, 1.F, h1, l1);
-            hi[j / 4] = pack4(h0, h1);
-            lo[j / 4] = pack4(l0, l1);
+          for (int j = 0; j < C; j += 8) {
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+              const float4 up = *reinterpret_cast<const float4*>(my_spread + j + i);
+              uint16_t h0, l0, h1, l1;
+              // in this order: the factor of a column that sees none of these tokens is 2^126, and 0 stays 0
+              two_parts<1>(p[j + i] * value_scale * up.x, p[j + i + 1] * value_scale * up.y, h0, l0);
+              two_parts<1>(p[j + i + 2] * value_scale * up.z, p[j + i + 3] * value_scale * up.w, h1, l1);
+              hi[i / 4] = pack4(h0, h1);
+              lo[i / 4] = pack4(l0, l1);
+            }
+            const uint32_t byte = column0 + j;
+            *reinterpret_cast<uint2*>(my_probs + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15)) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2*>(my_probs + ((((byte >> 4) + 4) ^ (row & 7)) << 4) + (byte & 15)) = make_uint2(lo[0], lo[1]);
+          }
+          if (!added && !ask) {
+            added = true;
+#pragma unroll
+            for (int j = 0; j < C; ++j) total[j] += p[j];
           }
           if (moved) break;
           wait(&s.checked, tile_count & 1, 0xad000000u);
@@ -909,15 +993,15 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
             const bool had = settled[member] != 0, has = highest != -INFINITY;
             const float now = !has ? before : had ? fmaxf(before, highest) : highest;
             reference[member] = now;
-            factor[member] = had ? exp2_approx(before - now) : 0.F;
+            factor[member] = !has ? 1.F : had ? exp2_approx(before - now) : 0.F;
             settled[member] = had || has;
           }
           together();
-          if (t > m.begin) {                                     // the sums so far, once the product before is done
-            wait(&s.probs_empty, (tile_count & 1) ^ 1, 0xaa000000u);
-            ptx::tc_fence_after_sync();
 #pragma unroll
-            for (int j = 0; j < C; ++j) total[j] *= factor[column0 + j];
+          for (int j = 0; j < C; ++j) total[j] *= factor[column0 + j];
+          if (t > begin) {                                       // the sums so far, once the product before is done
+            wait(&s.probs_empty[buffer ^ 1], (tile_count - 1) >> 1 & 1, 0xab100000u);
+            ptx::tc_fence_after_sync();
 #pragma unroll 1
             for (int i = 0; i < CH * (C / 8); ++i) {
               const int j = i % (C / 8) * 8;
@@ -932,85 +1016,17 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
             ptx::tmem_store_wait();
           }
         }
-        ptx::tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&s.scores_empty[buffer]);
-#pragma unroll
-        for (int j = 0; j < C; ++j) total[j] += p[j];
-        if (tile_count > 0) wait(&s.probs_empty, (tile_count & 1) ^ 1, 0xaa000000u);
-#pragma unroll
-        for (int j = 0; j < C; j += 8) {
-          const uint32_t byte = column0 + j;
-          uint8_t* const to_hi = probs + row * 128 + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15);
-          *reinterpret_cast<uint2*>(to_hi) = make_uint2(hi[j / 4], hi[j / 4 + 1]);
-          uint8_t* const to_lo = L::kOneBuffer ? probs + row * 128 + ((((byte + 64) >> 4) ^ (row & 7)) << 4) + (byte & 15) : to_hi + L::kLowOffset;
-          *reinterpret_cast<uint2*>(to_lo) = make_uint2(lo[j / 4], lo[j / 4 + 1]);
-        }
-        if (lane < uint32_t(C)) {
-          const uint32_t column = column0 + lane;
-          probs_atom[column % 32 * 16 + column / 32 * 4 + quadrant] = uint8_t(exponent - 7);
-        }
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&s.probs_full);
-        ++tile_count;
-      }
-      more = next_item(n + 1);                                   // its queries, while the last product runs
-      // sums of a column over the tokens
-      const float mine = lane_sums(total, lane);
-      if (lane < uint32_t(C)) by_warp[quadrant * N + column0 + lane] = mine;
-      together();
-      const bool whole = m.whole;
-      const uint32_t place = 2 * blockIdx.x + (m.begin == 0 ? 1 : 0);
-      if (member < N) {
-        const float v = (by_warp[member] + by_warp[N + member]) + (by_warp[2 * N + member] + by_warp[3 * N + member]);
-        factor[member] = v == 0.F ? 0.F : rcp_approx_ftz(v);
-        if (!whole) {
-          float* const totals = a.partial + size_t(gridDim.x) * 2 * N * D + size_t(place) * 2 * N;
-          totals[member] = reference[member];
-          totals[N + member] = v;
+        if (lane == 0) {
+          ptx::mbar_arrive(&s.probs_full[buffer]);
+          ptx::mbar_arrive(&s.scores_empty[buffer]);
         }
       }
-      together();
-      wait(&s.sums_full, scored_items & 1, 0xab000000u);
-      ptx::tc_fence_after_sync();
-      // eight columns at a time, to the output or to the block's partial sums
-      float* const partial = a.partial + (size_t(place) * N + column0) * D + row;
-#pragma unroll 1
-      for (int j = 0; j < C && int(column0) + j < used; j += 8) {
-        float by[8];
-        bf16* to[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          by[e] = factor[column0 + j + e];
-          to[e] = output_at[column0 + j + e] + row;
-        }
-        const int left = used - int(column0) - j;
-#pragma unroll 1
-        for (int c = 0; c < CH; ++c) {
-          float o[8];
-          tmem_load<8>(lanes + c * N + column0 + j, reinterpret_cast<uint32_t*>(o));
-          ptx::tmem_load_wait();
-          if (whole) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (e < left) to[e][c * 128] = __float2bfloat16_rn(o[e] * by[e]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (e < left) partial[(j + e) * D + c * 128] = o[e];
-          }
-        }
-      }
-      ++scored_items;
-      // The sums were read: the next item's first product may overwrite them once it has the probabilities that this thread
-      // publishes later.  What the item had in shared memory is free.
-      ptx::tc_fence_before_sync();
-      together();
-      if (lane == 0) ptx::mbar_arrive(&s.items_empty[n % kItems]);
     }
   }
+  if (error != 0) atomicCAS(&g_attention_error, 0u, error | (blockIdx.x << 8));
   ptx::tc_fence_before_sync();
   __syncthreads();
   ptx::tc_fence_after_sync();
@@ -1082,10 +1098,10 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_consta
 // host
 // ---------------------------------------------------------------------------
 // Columns of a block: 16 or 32 where all query rows of a sequence fit, else as many as tensor memory takes next to two tiles of
-// scores (512 columns: D / 128 * N sums, 2 N scores, up to 40 of scales).
-uint32_t columns_of(uint32_t head_dim, uint32_t group, uint32_t max_rows) {
+// scores at D = 512 (512 columns: D / 128 * N sums, 2 N scores, up to 44 of scales).
+uint32_t columns_of(uint32_t group, uint32_t max_rows) {
   const uint64_t needed = uint64_t(group) * max_rows;
-  return needed <= 16 ? 16 : needed <= 32 ? 32 : head_dim == 512 ? 64 : 96;
+  return needed <= 16 ? 16 : needed <= 32 ? 32 : 64;
 }
 
 size_t partial_floats(uint32_t blocks, uint32_t columns, uint32_t head_dim) { return size_t(blocks) * 2 * columns * (head_dim + 2); }
@@ -1105,11 +1121,11 @@ cudaError_t launch_attention(const Attention& a, const CUtensorMap& k_map, const
   else return launch_pdl(attention_join_kernel<D, 1>, dim3(blocks, 4), 256, stream, a, blocks, uint32_t(N));
 }
 
-template <int D, int MOST>
+template <int D>
 cudaError_t launch_columns(uint32_t columns, const Attention& a, const CUtensorMap& k_map, const CUtensorMap& v_map, uint32_t blocks, cudaStream_t stream) {
   return columns == 16   ? launch_attention<D, 16>(a, k_map, v_map, blocks, stream)
          : columns == 32 ? launch_attention<D, 32>(a, k_map, v_map, blocks, stream)
-                         : launch_attention<D, MOST>(a, k_map, v_map, blocks, stream);
+                         : launch_attention<D, 64>(a, k_map, v_map, blocks, stream);
 }
 
 }  // namespace
@@ -1126,7 +1142,7 @@ extern "C" {
 
 size_t gw_paged_attention_scratch_bytes(const gw_kv_cache* cache, const gw_sequences* batch, uint32_t heads) {
   if (!cache || !batch || cache->kv_heads == 0 || heads < cache->kv_heads) return 256;
-  const uint32_t blocks = sm_count(), columns = columns_of(cache->head_dim, heads / cache->kv_heads, std::max(1u, batch->max_rows));
+  const uint32_t blocks = sm_count(), columns = columns_of(heads / cache->kv_heads, std::max(1u, batch->max_rows));
   return align_up(partial_floats(blocks, columns, cache->head_dim) * sizeof(float), 256) + align_up(blocks * sizeof(int4), 256);
 }
 
@@ -1147,7 +1163,7 @@ gw_status gw_paged_attention_bf16(const gw_kv_cache* cache, const gw_sequences* 
   const size_t needed = gw_paged_attention_scratch_bytes(cache, batch, heads);
   if (!scratch || reinterpret_cast<uintptr_t>(scratch) % 256 != 0 || scratch_capacity < needed)
     return fail(GW_INVALID_ARGUMENT, "paged attention requires " + std::to_string(needed) + " bytes of 256-byte aligned scratch");
-  const uint32_t group = heads / cache->kv_heads, columns = columns_of(cache->head_dim, group, batch->max_rows), blocks = sm_count();
+  const uint32_t group = heads / cache->kv_heads, columns = columns_of(group, batch->max_rows), blocks = sm_count();
   CUtensorMap k_map, v_map;
   std::string error;
   const uint64_t rows = uint64_t(cache->pages) * cache->kv_heads * cache->page_tokens;
@@ -1159,9 +1175,9 @@ gw_status gw_paged_attention_bf16(const gw_kv_cache* cache, const gw_sequences* 
                     heads, group, (65536 + group - 1) / group, columns / group, window > (1u << 30) ? 0 : window, uint32_t(__builtin_ctz(cache->page_tokens)), scale,
                     static_cast<float*>(scratch), reinterpret_cast<int4*>(static_cast<uint8_t*>(scratch) + floats)};
   const cudaStream_t s = as_stream(stream);
-  GW_CUDA_CHECK((cache->head_dim == 128   ? launch_columns<128, 96>(columns, a, k_map, v_map, blocks, s)
-                 : cache->head_dim == 256 ? launch_columns<256, 96>(columns, a, k_map, v_map, blocks, s)
-                                          : launch_columns<512, 64>(columns, a, k_map, v_map, blocks, s)),
+  GW_CUDA_CHECK((cache->head_dim == 128   ? launch_columns<128>(columns, a, k_map, v_map, blocks, s)
+                 : cache->head_dim == 256 ? launch_columns<256>(columns, a, k_map, v_map, blocks, s)
+                                          : launch_columns<512>(columns, a, k_map, v_map, blocks, s)),
                 "paged attention");
   return GW_OK;
 }

@@ -18,19 +18,19 @@ static int draw(int low, int high) {
 int main() {
   for (int i = 0; i < 20000; ++i) {
     const int n = draw(1, 300), a = draw(1, kTokens), b = draw(0, 5000);
-    int64_t sum = 0;
-    for (int k = 0; k < n; ++k) sum += (int64_t(a) * k + b) / kTokens;
+    uint32_t sum = 0;
+    for (int k = 0; k < n; ++k) sum += uint32_t(a * k + b) / kTokens;
     REQUIRE(floor_sum(n, a, b) == sum);
   }
   for (int round = 0; round < 3000; ++round) {
     const int sequences = draw(1, 9), heads = draw(1, 4), per_tile = draw(1, 128), window = draw(0, 2) ? 0 : draw(1, 700);
     std::vector<SequenceWork> all;
-    int64_t units = 0;
+    uint32_t units = 0;
     for (int s = 0; s < sequences; ++s) {
       const int rows = draw(0, 3) ? draw(0, 6) : draw(0, 900), context = draw(0, 4) ? rows + draw(0, 3000) : draw(0, rows);
       all.push_back({context - rows, rows, per_tile, window});
       const SequenceWork& w = all.back();
-      int64_t before = 0;
+      uint32_t before = 0;
       for (int t = 0; t < w.query_tiles(); ++t) {
         REQUIRE(w.units_before(t) == before);
         REQUIRE(w.token_tiles(t) >= 0 && w.low(t) <= w.high(t));
@@ -41,12 +41,14 @@ int main() {
     }
     if (units == 0) continue;
     const int parts = int(units < 148 ? draw(1, int(units)) : draw(1, 148));
+    const Ranges ranges(units, parts);
+    REQUIRE(ranges.start(0) == 0 && ranges.start(parts) == units);
     std::vector<std::vector<int>> taken;       // by item: how often each token tile
     std::vector<int> owners, zeros;
     for (int part = 0; part < parts; ++part) {
-      const int64_t from = range_start(units, part, parts), to = range_start(units, part + 1, parts);
-      REQUIRE(from < to && part_with(units, from, parts) == part && part_with(units, to - 1, parts) == part);
-      int64_t item = 0;
+      const uint32_t from = ranges.start(part), to = ranges.start(part + 1);
+      REQUIRE(from < to && ranges.with(from) == uint32_t(part) && ranges.with(to - 1) == uint32_t(part));
+      uint32_t item = 0;
       size_t number = 0;
       int first_pieces = 0, later_pieces = 0;
       for (const SequenceWork& w : all)
@@ -63,10 +65,10 @@ int main() {
                 ++first_pieces;
                 ++owners[number];
                 // the blocks of the other pieces are the ones up to that of the last unit
-                const int last = part_with(units, item + tiles, parts);
+                const int last = int(ranges.with(item + tiles));
                 REQUIRE(last > part);
                 for (int other = part + 1; other <= last; ++other) {
-                  const Piece q = piece_of(item, tiles, range_start(units, other, parts), range_start(units, other + 1, parts));
+                  const Piece q = piece_of(item, tiles, ranges.start(other), ranges.start(other + 1));
                   REQUIRE(q.here && q.begin > 0 && (other == last) == (q.end == tiles));
                 }
               }
@@ -80,8 +82,13 @@ int main() {
       REQUIRE(owners[i] <= 1 && zeros[i] == (taken[i].empty() ? 1 : 0));
     }
   }
-  const SequenceWork huge{1 << 30, 1 << 24, 1, 1 << 20};
-  REQUIRE(huge.units() > 0 && huge.units() == int64_t(huge.rows) + huge.units_before(huge.rows) - huge.rows);
+  const SequenceWork far{(1 << 30) - 4096, 4096, 64, 0}, wide{0, 1 << 24, 128, 1 << 20};
+  uint32_t units = 0;
+  for (int t = 0; t < far.query_tiles(); ++t) units += 1 + far.token_tiles(t);
+  REQUIRE(far.units() == units);
+  units = 0;
+  for (int t = 0; t < wide.query_tiles(); ++t) units += 1 + wide.token_tiles(t);
+  REQUIRE(wide.units() == units);
   std::puts("PASS");
   return 0;
 }
