@@ -18,7 +18,7 @@
 // when a column's first tokens all lie below 2^-40.  (Value scales below 2^-64 are taken for 2^-64, so that no probability passes
 // 2^104 unseen.)
 //
-//   warp 0      TMA: chunks of [128 tokens x 128 bytes] of K and V into a ring, page by page; the pages' scales, and what the softmax
+//   warp 0      TMA: chunks of [128 tokens x 128 bytes] into a ring for K and one for V, page by page; the pages' scales, and what the softmax
 //               warps need to know of an item
 //   warps 1, 3  one thread each issues tcgen05.mma: S of the tiles, as far ahead as there is room, and O += P V.  One thread for
 //               both spent half of its time in barriers, with nothing left in the tensor pipe's queue.
@@ -33,6 +33,8 @@
 //
 // Work: attention_work.h.  An item that a cut between two blocks' ranges divides leaves FP32 partial sums in the scratch
 // memory, which a second kernel joins in the order of the blocks (the same bits on every run).
+// A thread waits on a barrier for every phase of it, or for none: with one ring for K and V the thread of S could ask for a phase
+// while the one before, of V, was still open, and a parity cannot tell that from the phase being complete.
 // Every wait is bounded; a role that gives up reports it, all leave, and tensor memory is released.
 #include <algorithm>
 #include <string>
@@ -80,7 +82,7 @@ struct Item {
 };
 
 struct Shared {
-  uint64_t full[16], empty[16], cleared[16], scales_full[kScaleTiles], items_full[kItems], items_empty[kItems];
+  uint64_t k_full[8], k_empty[8], v_full[8], v_empty[8], v_cleared[8], scales_full[kScaleTiles], items_full[kItems], items_empty[kItems];
   uint64_t scores_full[2], scores_empty[2], probs_full[2], probs_empty[2], checked, query_full, sums_full, softmax, drained, drained_sums;
   float2 scales[kScaleTiles][8];               // {key, value} of a tile's pages; a value scale below 0: no page
   Item items[kItems];
@@ -108,8 +110,9 @@ struct Layout {
   static constexpr int kAlignment = 1024;
   static constexpr int kStatic = 3072;                            // at least what is declared in the kernel
   static constexpr int kRoom = 227 * 1024 - kStatic - kAlignment - 2 * kQueryBytes - kProbBytes - kSmall;
-  static constexpr int kRing = kRoom / kChunkBytes > 16 ? 16 : kRoom / kChunkBytes;
-  static constexpr int kSmemBytes = kAlignment + 2 * kQueryBytes + kProbBytes + kRing * kChunkBytes + kSmall;
+  static constexpr int kRings = kRoom / kChunkBytes > 16 ? 16 : kRoom / kChunkBytes;          // chunks
+  static constexpr int kKeyRing = (kRings + 1) / 2, kValueRing = kRings / 2;
+  static constexpr int kSmemBytes = kAlignment + 2 * kQueryBytes + kProbBytes + kRings * kChunkBytes + kSmall;
   // tensor memory columns
   static constexpr int kScores = kChunks * N;
   static constexpr int kOnes = kScores + 2 * N;
@@ -117,8 +120,8 @@ struct Layout {
   static constexpr int kProbScales = kQueryScales + 8 * kChunks;
   static constexpr int kColumns = 512;
   static_assert(kProbScales + 8 <= kColumns, "tensor memory over-subscribed");
-  static_assert(kRing >= kChunks + 1, "a tile's chunks and one more");
-  static_assert(kRing / (2 * kChunks) + 4 < kScaleTiles, "scales of a tile are read before those of a later one take their place");
+  static_assert(kValueRing >= 2, "a chunk and the next");
+  static_assert(kKeyRing / kChunks + 4 < kScaleTiles, "scales of a tile are read before those of a later one take their place");
   static_assert(kSmemBytes > 116 * 1024, "one block an SM");
   static_assert(sizeof(Shared) + 512 <= kStatic, "");
   static_assert(N % 16 == 0 && N <= 64 && D % 128 == 0 && kShare % 8 == 0, "");
@@ -399,14 +402,15 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
                                                                       const __grid_constant__ CUtensorMap v_map,
                                                                       const __grid_constant__ Attention a) {
   using L = Layout<D, N>;
-  constexpr int CH = L::kChunks, RING = L::kRing, C = L::kShare, kSoftmaxWarps = L::kSoftmaxWarps, kSoftmaxThreads = 32 * kSoftmaxWarps, kThreads = L::kThreads;
+  constexpr int CH = L::kChunks, KEYS = L::kKeyRing, VALUES = L::kValueRing, C = L::kShare, kSoftmaxWarps = L::kSoftmaxWarps, kSoftmaxThreads = 32 * kSoftmaxWarps, kThreads = L::kThreads;
   extern __shared__ uint8_t raw[];
   uint8_t* const base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t* const query_hi = base;
   uint8_t* const query_lo = query_hi + L::kQueryBytes;
   uint8_t* const probs = query_lo + L::kQueryBytes;
-  uint8_t* const ring = probs + L::kProbBytes;
-  uint8_t* const atoms = ring + RING * kChunkBytes;              // [2 * CH] queries (hi, lo of a chunk), [1] ones, [2] P
+  uint8_t* const k_ring = probs + L::kProbBytes;
+  uint8_t* const v_ring = k_ring + KEYS * kChunkBytes;
+  uint8_t* const atoms = v_ring + VALUES * kChunkBytes;              // [2 * CH] queries (hi, lo of a chunk), [1] ones, [2] P
   uint8_t* const ones_atom = atoms + 2 * CH * kAtomBytes;
   uint8_t* const probs_atom = ones_atom + kAtomBytes;
   float* const reference = reinterpret_cast<float*>(probs_atom + 2 * kAtomBytes); // [N] m of a column
@@ -419,10 +423,12 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < RING; ++i) {
-      ptx::mbar_init(&s.full[i], 1);
-      ptx::mbar_init(&s.cleared[i], 1);
-      ptx::mbar_init(&s.empty[i], 2);                            // both products' thread and the warp that zeroes
+    for (int i = 0; i < 8; ++i) {
+      ptx::mbar_init(&s.k_full[i], 1);
+      ptx::mbar_init(&s.k_empty[i], 1);
+      ptx::mbar_init(&s.v_full[i], 1);
+      ptx::mbar_init(&s.v_cleared[i], 1);
+      ptx::mbar_init(&s.v_empty[i], 2);                          // the product's thread and the warp that zeroes
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&s.scores_full[i], 1);
@@ -469,8 +475,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     // ----- producer: lane l brings the l-th page of a tile
     const uint32_t page_tokens = a.cache.page_tokens, boxes = kTokens / page_tokens;
     const int outside = int(a.cache.pages * a.cache.kv_heads * page_tokens);        // rows from here on read as zeros
-    int slot = 0, issued = 0, tile_count = 0;
-    uint32_t parity = 1;                                         // empty slots: the first pass does not wait
+    int issued[2] = {0, 0}, tile_count = 0;                      // chunks of K and of V so far
     if (lane == 0) a.records[blockIdx.x] = make_int4(0, 0, 0, -1);
     Walk w;
     w.start(a, s);
@@ -517,20 +522,16 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         }
         return v;
       };
-      const auto bring = [&](const CUtensorMap* map, int row) {
+      const auto bring = [&](const CUtensorMap* map, int row, int& count, uint32_t chunks, uint64_t* full, uint64_t* empty, uint8_t* ring) {
 #pragma unroll 1
-        for (int c = 0; c < CH; ++c) {
-          wait(&s.empty[slot], parity, 0xa3000000u | slot);
+        for (int c = 0; c < CH; ++c, ++count) {
+          const uint32_t lap = uint32_t(count) / chunks, slot = uint32_t(count) - lap * chunks;
+          wait(&empty[slot], (lap & 1) ^ 1, 0xa3000000u | slot);               // empty slots: the first lap does not wait
           error = __reduce_max_sync(0xffffffffu, error);
           if (error) return;
-          if (lane == 0) ptx::mbar_expect_tx(&s.full[slot], kChunkBytes);
+          if (lane == 0) ptx::mbar_expect_tx(&full[slot], kChunkBytes);
           __syncwarp();
-          if (lane < boxes) ptx::tma_load_2d(ring + slot * kChunkBytes + lane * page_tokens * 128, map, c * 128, row, &s.full[slot]);
-          ++issued;
-          if (++slot == RING) {
-            slot = 0;
-            parity ^= 1;
-          }
+          if (lane < boxes) ptx::tma_load_2d(ring + slot * kChunkBytes + lane * page_tokens * 128, map, c * 128, row, &full[slot]);
         }
       };
       // K of a tile, then V of the one before; the pages two tiles ahead and the scales one ahead are asked for meanwhile
@@ -543,14 +544,14 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         if (t < w.end) {
           if (uint32_t(entry) < a.cache.pages) row = int((uint32_t(entry) * a.cache.kv_heads + w.head) * page_tokens);
           else if (entry != -2) atomicCAS(&g_attention_error, 0u, 0xa1000000u | (w.sequence & 0xffffffu));
-          bring(&k_map, row);
+          bring(&k_map, row, issued[0], KEYS, s.k_full, s.k_empty, k_ring);
           if (lane < boxes) s.scales[tile_count % kScaleTiles][lane] = scales;
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive(&s.scales_full[tile_count % kScaleTiles]);
           ++tile_count;
           scales = scales_of(entry_next);
         }
-        if (error == 0 && t > w.begin) bring(&v_map, row_before);
+        if (error == 0 && t > w.begin) bring(&v_map, row_before, issued[1], VALUES, s.v_full, s.v_empty, v_ring);
         row_before = row;
         entry = entry_next;
         entry_next = entry_after;
@@ -560,13 +561,10 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     }
     // the copies still in flight land before the block ends
 #pragma unroll 1
-    for (int i = issued < RING ? issued : RING; i > 0; --i) {
-      if (slot == 0) {
-        slot = RING;
-        parity ^= 1;
-      }
-      --slot;
-      ptx::mbar_wait_bounded(&s.full[slot], parity ^ 1, 100000000ull);
+    for (int back = 1; back <= KEYS; ++back) {
+      const int keys = issued[0] - back, values = issued[1] - back;
+      if (keys >= 0) ptx::mbar_wait_bounded(&s.k_full[keys % KEYS], keys / KEYS & 1, 100000000ull);
+      if (values >= 0 && back <= VALUES) ptx::mbar_wait_bounded(&s.v_full[values % VALUES], values / VALUES & 1, 100000000ull);
     }
   } else if (warp == 1) {
     // ----- S, by one thread: the compiler keeps its descriptors in uniform registers only where it knows that one thread runs the code
@@ -574,14 +572,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     if (ptx::elect_one()) {
       int slot = 0, item = 0, scored = 0;
       uint32_t parity = 0;
-      const auto skip = [&](int chunks) {
-        slot += chunks;
-        if (slot >= RING) {
-          slot -= RING;
-          parity ^= 1;
-        }
-      };
-      const uint64_t ring_rows = ptx::smem_desc_sw128(ptx::smem_u32(ring));
+      const uint64_t ring_rows = ptx::smem_desc_sw128(ptx::smem_u32(k_ring));
       const uint64_t hi_rows = ptx::smem_desc_sw128(ptx::smem_u32(query_hi)), lo_rows = ptx::smem_desc_sw128(ptx::smem_u32(query_lo));
       const uint64_t atom = ptx::smem_desc_sf_atom(ptx::smem_u32(atoms));
       ptx::tc_copy_sf_atom(tmem + L::kOnes, ptx::smem_desc_sf_atom(ptx::smem_u32(ones_atom)));
@@ -601,7 +592,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
           const int buffer = scored & 1;
           wait(&s.scores_empty[buffer], ((scored >> 1) & 1) ^ 1, 0xa6000000u | buffer);
           const uint32_t d = tmem + L::kScores + buffer * N;
-          if (!wait(&s.full[slot], parity, 0xa4000000u | slot)) break;
+          if (!wait(&s.k_full[slot], parity, 0xa4000000u | slot)) break;
 #pragma unroll 1
           for (int c = 0; c < CH; ++c) {
             ptx::tc_fence_after_sync();
@@ -614,18 +605,19 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
               for (int k = 0; k < 4; ++k)
                 mma_mx(d, keys + 2 * k, (part ? lo_rows : hi_rows) + offset + 2 * k, idesc_mx(N, false) | uint32_t(k) << 4, tmem + L::kOnes,
                        scales + 4 * part, c | part | k);
-            skip(1);
+            if (++slot == KEYS) {
+              slot = 0;
+              parity ^= 1;
+            }
             // before the commit, which comes back once its products have left the queue
-            if (c + 1 < CH && !wait(&s.full[slot], parity, 0xa4000000u | slot)) break;
-            ptx::tc_commit(&s.empty[this_slot]);
+            if (c + 1 < CH && !wait(&s.k_full[slot], parity, 0xa4000000u | slot)) break;
+            ptx::tc_commit(&s.k_empty[this_slot]);
           }
           if (error) break;
           ptx::tc_commit(&s.scores_full[buffer]);
           ++scored;
-          if (t > begin) skip(CH);                               // V of the tile before
         }
         if (error) break;
-        skip(CH);
       }
       // products still in flight end before tensor memory is released
       ptx::tc_commit(&s.drained);
@@ -637,14 +629,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     if (ptx::elect_one()) {
       int slot = 0, summed = 0;
       uint32_t parity = 0;
-      const auto skip = [&](int chunks) {
-        slot += chunks;
-        if (slot >= RING) {
-          slot -= RING;
-          parity ^= 1;
-        }
-      };
-      const uint64_t ring_across = across_desc(ptx::smem_u32(ring)), probs_across = across_desc(ptx::smem_u32(probs));
+      const uint64_t ring_across = across_desc(ptx::smem_u32(v_ring)), probs_across = across_desc(ptx::smem_u32(probs));
       const uint64_t atom = ptx::smem_desc_sf_atom(ptx::smem_u32(probs_atom));
 #pragma unroll 1
       for (int n = 0; wait(&s.items_full[n % kItems], n / kItems & 1, 0xb2000000u); ++n) {
@@ -653,14 +638,17 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         ptx::mbar_arrive(&s.items_empty[n % kItems]);
         if (tiles < 0) break;
         if (tiles == 0) continue;
-        skip(CH);                                                // K of the first tile
 #pragma unroll 1
         for (int t = begin; t < end; ++t) {
-          if (t + 1 < end) skip(CH);                             // K of the next one
-          uint64_t* const ready = needs_clearing(first_tile + t, low, high) ? s.cleared : s.full;
+          // once the chunk is there, the warp that zeroes has finished with what was in its place before
+          const bool clear = needs_clearing(first_tile + t, low, high);
+          const auto ready = [&]() {
+            wait(&s.v_full[slot], parity, 0xa5100000u | slot);
+            return clear ? wait(&s.v_cleared[slot], parity, 0xaf000000u | slot) : error == 0;
+          };
           const int buffer = summed & 1;
           wait(&s.probs_full[buffer], (summed >> 1) & 1, 0xa7000000u);
-          if (!wait(&ready[slot], parity, 0xaf000000u | slot)) break;
+          if (!ready()) break;
           ptx::tc_fence_after_sync();
           const uint32_t scales = tmem + L::kProbScales + 4 * buffer;
           const uint64_t p = probs_across + uint64_t(buffer * (kChunkBytes >> 4));
@@ -676,9 +664,12 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
               for (int k = 0; k < 4; ++k)
                 mma_mx(tmem + c * N, values + 256 * k, p + uint64_t(part * (L::kLowOffset >> 4)) + 256 * k, idesc_mx(N, true) | uint32_t(k) << 4,
                        tmem + L::kOnes, scales, uint32_t(t > begin) | part | k);
-            skip(1);
-            if (c + 1 < CH && !wait(&ready[slot], parity, 0xaf000000u | slot)) break;
-            ptx::tc_commit(&s.empty[this_slot]);
+            if (++slot == VALUES) {
+              slot = 0;
+              parity ^= 1;
+            }
+            if (c + 1 < CH && !ready()) break;
+            ptx::tc_commit(&s.v_empty[this_slot]);
           }
           if (error) break;
           ptx::tc_commit(&s.probs_empty[buffer]);
@@ -692,8 +683,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     }
     __syncwarp();
   } else if (warp == 2) {
-    // ----- rows of V that no query of an item sees; every chunk is waited for, in the order in which the products take them, so that
-    // this warp is never a lap of the ring away
+    // ----- rows of V that no query of an item sees; every chunk is waited for, so that this warp is never a lap of the ring away
     int slot = 0;
     uint32_t parity = 0;
 #pragma unroll 1
@@ -702,19 +692,18 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       error = __reduce_max_sync(0xffffffffu, error);
       if (error) break;
       const Item& m = s.items[n % kItems];
-      const int begin = m.begin, steps = 2 * (m.end - m.begin), tiles = m.tiles, first_tile = m.first_tile, low = m.low, high = m.high;
+      const int begin = m.begin, end = m.end, tiles = m.tiles, first_tile = m.first_tile, low = m.low, high = m.high;
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&s.items_empty[n % kItems]);
       if (tiles < 0) break;
-      // in the ring's order: K of the first tile, then K of the next one and V of each
 #pragma unroll 1
-      for (int i = 0; error == 0 && i < CH * steps; ++i) {
-        const int step = i / CH, t = begin + (step == steps - 1 ? steps / 2 - 1 : (step - 1) / 2), start = (first_tile + t) * kTokens;
-        wait(&s.full[slot], parity, 0xa9000000u | slot);
+      for (int i = 0; i < CH * (end - begin); ++i) {
+        const int tile = first_tile + begin + i / CH, start = tile * kTokens;
+        wait(&s.v_full[slot], parity, 0xa9000000u | slot);
         error = __reduce_max_sync(0xffffffffu, error);
         if (error) break;
-        if ((step == steps - 1 || (step >= 2 && step % 2 == 0)) && needs_clearing(first_tile + t, low, high)) {
-          uint4* rows = reinterpret_cast<uint4*>(ring + slot * kChunkBytes);
+        if (needs_clearing(tile, low, high)) {
+          uint4* rows = reinterpret_cast<uint4*>(v_ring + slot * kChunkBytes);
 #pragma unroll 1
           for (int k = lane; k < kTokens * 8; k += 32)
             if (start + k / 8 < low || start + k / 8 >= high) rows[k] = make_uint4(0, 0, 0, 0);
@@ -722,10 +711,10 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
           __syncwarp();
         }
         if (lane == 0) {
-          ptx::mbar_arrive(&s.cleared[slot]);
-          ptx::mbar_arrive(&s.empty[slot]);
+          ptx::mbar_arrive(&s.v_cleared[slot]);
+          ptx::mbar_arrive(&s.v_empty[slot]);
         }
-        if (++slot == RING) {
+        if (++slot == VALUES) {
           slot = 0;
           parity ^= 1;
         }

@@ -174,6 +174,25 @@ def test_strided_rows_and_the_same_inputs_twice(gw):
     assert torch.equal(again, got)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,page,rows", [(32, 4, 512, 128, 1), (32, 16, 256, 64, 1), (32, 8, 128, 16, 3), (16, 2, 512, 64, 300)])
+def test_many_passes_give_the_same_bits(gw, heads, kv_heads, dim, page, rows):
+    """Long sequences that wait for memory, pass behind pass: what the warps of a block hand each other must not depend on who is late."""
+    count = 12 if rows < 16 else 2
+    batch = Batch([(rows, 9000 + 700 * s) for s in range(count)], page, 40)
+    g = torch.Generator(device="cuda").manual_seed(41)
+    shape = (batch.pages, kv_heads, page, dim)
+    data = [torch.randn(shape, generator=g, device="cuda").clamp_(-4, 4).mul_(64).to(torch.float8_e4m3fn) for _ in range(2)]
+    cache = gw.KvCache(*data, *(torch.full(shape[:2], 1 / 64, device="cuda") for _ in range(2)))
+    held, q = batch.device(gw), queries(batch.rows, heads, dim, 42)
+    first = gw.paged_attention(cache, held, q, dim ** -0.5)
+    for _ in range(60):
+        again = gw.paged_attention(cache, held, q, dim ** -0.5)
+        assert torch.equal(again, first)
+    assert gw.kernel_error() == 0
+    host = [(d.view(torch.uint8).cpu().numpy(), np.full(shape[:2], 1 / 64, dtype=np.float32)) for d in data]
+    assert_rows(first, q, batch, host, dim ** -0.5, 0, rows_of=[0])
+
+
 def test_bad_pages_are_left_out(gw):
     """A page number outside the cache, and a context that reaches behind the page table: those tokens do not count, and it is reported."""
     batch = Batch([(1, 100), (20, 90)], 16, 26)
