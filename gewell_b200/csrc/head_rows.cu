@@ -8,14 +8,16 @@
 //
 //   y_i = n_i cos a - n_j sin a,  y_j = n_j cos a + n_i sin a,  a = position * f,  n = x * rsqrt(mean(x^2) + eps) * w
 //
-// The angle in turns, position * (f / 2 pi), is formed and reduced to [-1/2, 1/2] in 64 bits: in 32 bits position 250000 at
-// f = 1 would be off by 0.01 rad.  What is left goes to the hardware's sine and cosine (absolute error 2^-21, against BF16's
-// 2^-9 and E4M3's 2^-4 at the end); everything else is FP32 and is rounded once.
+// The angle in turns, position * (f / 2 pi), is formed as the sum of two FP32 numbers, exact to 2^-28 up to position 2^24 (in 64
+// bits beyond), and reduced to [-1/2, 1/2]: in 32 bits position 250000 at f = 1 would be off by 0.01 rad.  What is left goes to the
+// hardware's sine and cosine (absolute error 2^-21, against BF16's 2^-9 and E4M3's 2^-4 at the end); everything else is FP32 and is
+// rounded once.
 #include <algorithm>
 #include <string>
 
 #include "common.cuh"
 #include "paged.h"
+#include "pair.cuh"
 
 using namespace gw;
 
@@ -71,31 +73,42 @@ struct Raw {
   }
 };
 
-// A lane's share of the rotation: turns per position of its pairs.
+// A lane's share of the rotation: the frequencies of its pairs.
 template <int V>
-struct Turns {
-  static constexpr int E = 4 * V;
-  double per_position[E];
-  __device__ __forceinline__ void load(const Rotary& r, uint32_t lane_at, uint32_t half, bool active) {
+__device__ __forceinline__ void load_frequencies(const Rotary& r, uint32_t lane_at, uint32_t half, bool active, float* f) {
+  constexpr int E = 4 * V;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      // kWhole: pair (at + e, at + e + half).  kNeighbours: E / 2 pairs of the first half, then E / 2 of the second.
-      const uint32_t pair = r.kind == kWhole ? lane_at + e : e < E / 2 ? lane_at / 2 + e : (half + lane_at) / 2 + (e - E / 2);
-      const bool used = active && r.kind != kNone && r.kind != kPart && 2 * pair < r.width;
-      per_position[e] = used ? double(r.frequencies[pair]) * 0.15915494309189535 : 0.0;     // 1 / 2 pi
-    }
+  for (int e = 0; e < E; ++e) {
+    // kWhole: pair (at + e, at + e + half).  kNeighbours: E / 2 pairs of the first half, then E / 2 of the second.
+    const uint32_t pair = r.kind == kWhole ? lane_at + e : e < E / 2 ? lane_at / 2 + e : (half + lane_at) / 2 + (e - E / 2);
+    const bool used = active && r.kind != kNone && r.kind != kPart && 2 * pair < r.width;
+    f[e] = used ? r.frequencies[pair] : 0.F;
   }
-};
+}
 
-__device__ __forceinline__ void sine_cosine(double turns, float& s, float& c) {
-  const float angle = float(turns - rint(turns)) * 6.283185307179586F;
-  __sincosf(angle, &s, &c);
+constexpr double kTurn = 0.15915494309189535;       // 1 / 2 pi
+
+__device__ __noinline__ float far_turns(float frequency, int position) {
+  const double turns = double(frequency) * kTurn * double(position);
+  return float(turns - rint(turns));
+}
+__device__ __forceinline__ void sine_cosine(float frequency, int position, float& s, float& c) {
+  float turns;
+  if (uint32_t(position + (1 << 24)) <= 2u << 24) {
+    constexpr float high = float(kTurn), low = float(kTurn - double(high));
+    const float f = frequency * high, f_rest = fmaf(frequency, high, -f) + frequency * low;        // turns per position
+    const float p = float(position), whole = p * f;
+    turns = (whole - rintf(whole)) + fmaf(p, f_rest, fmaf(p, f, -whole));
+  } else {
+    turns = far_turns(frequency, position);
+  }
+  __sincosf(turns * 6.283185307179586F, &s, &c);
 }
 
 template <int V>
-__device__ __forceinline__ void angles(const Turns<V>& t, int position, float* s, float* c) {
+__device__ __forceinline__ void angles(const float* frequencies, int position, float* s, float* c) {
 #pragma unroll
-  for (int e = 0; e < 4 * V; ++e) sine_cosine(t.per_position[e] * double(position), s[e], c[e]);
+  for (int e = 0; e < 4 * V; ++e) sine_cosine(frequencies[e], position, s[e], c[e]);
 }
 
 __device__ __forceinline__ void turn(float& a, float& b, float s, float c) {
@@ -140,7 +153,7 @@ __device__ __forceinline__ void rotate(const Rotary& r, float* lo, float* hi, co
         const uint32_t pair = first ? i : i - pairs;
         const float other = stage[first ? i + pairs : pair];
         float sine, cosine;
-        sine_cosine(double(r.frequencies[pair]) * 0.15915494309189535 * double(position), sine, cosine);
+        sine_cosine(r.frequencies[pair], position, sine, cosine);
         mine = first ? fmaf(-other, sine, mine * cosine) : fmaf(other, sine, mine * cosine);
       }
     }
@@ -162,8 +175,7 @@ __device__ __forceinline__ float inverse_rms(const float* lo, const float* hi, f
 // ---------------------------------------------------------------------------
 struct NormRotary {
   Heads query, key;                    // key.heads == 0: none
-  uint32_t rows, width, per_task;      // heads that a task takes
-  uint32_t query_tasks, tasks;         // of a row
+  uint32_t rows, width, per_task, tasks;       // heads of a row that a task takes, tasks of a row
   const int32_t* positions;            // or NULL: those of the batch
   gw_sequences batch;
   Rotary rotary;
@@ -184,58 +196,69 @@ __device__ __forceinline__ bool position_in_batch(const gw_sequences& b, uint32_
 
 constexpr int kNormWarps = 4;
 
+// A warp takes heads of one row, queries and keys in one line, the next head's values on their way meanwhile; the row's angles are
+// computed once.
 template <int LPH, int V>
-__global__ void __launch_bounds__(32 * kNormWarps) qk_norm_rotary_kernel(NormRotary a) {
+__global__ void __launch_bounds__(32 * kNormWarps, V == 1 ? 8 : 6) qk_norm_rotary_kernel(NormRotary a) {
   constexpr int E = 4 * V, kSide = 32 / LPH;
   __shared__ float stage[kNormWarps][kSide * LPH * 2 * E];
   griddep_enter();
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, group = lane / LPH, at = lane % LPH * E, half = a.width / 2;
   const uint32_t task = blockIdx.x * kNormWarps + warp;
-  const uint32_t row = task / a.tasks, part = task % a.tasks;
+  const uint32_t row = task / a.tasks, first = task % a.tasks * a.per_task, last = min(first + a.per_task, a.query.heads + a.key.heads);
   if (row >= a.rows) return;
-  const bool is_key = part >= a.query_tasks;
-  const Heads& h = is_key ? a.key : a.query;
-  const uint32_t first = (is_key ? part - a.query_tasks : part) * a.per_task, last = min(first + a.per_task, h.heads);
+  const bool inside = at < half;
+  const auto load = [&](uint32_t head, Raw<V>& lo, Raw<V>& hi) {
+    lo.clear();
+    hi.clear();
+    if (inside && head < last) {
+      const bool is_key = head >= a.query.heads;
+      const bf16* from = is_key ? a.key.input + size_t(row) * a.key.input_stride : a.query.input + size_t(row) * a.query.input_stride;
+      from += size_t(is_key ? head - a.query.heads : head) * a.width + at;
+      lo.load(from);
+      hi.load(from + half);
+    }
+  };
+  Raw<V> next_lo, next_hi;
+  load(first + group, next_lo, next_hi);
   int position = 0;
   if (a.positions != nullptr) position = a.positions[row];
   else if (a.batch.sequences && !position_in_batch(a.batch, row, position)) return;
-  const bool inside = at < half;
-  float s[E], c[E], weight_lo[E], weight_hi[E];
+  float s[E], c[E];
   {
-    Turns<V> turns;
-    turns.load(a.rotary, at, half, inside);
-    angles(turns, position, s, c);
-  }
-  const bool weighted = h.weight != nullptr;
-#pragma unroll
-  for (int e = 0; e < E; ++e) weight_lo[e] = weight_hi[e] = 1.F;
-  if (weighted && inside) {
-    Raw<V> raw;
-    raw.load(h.weight + at);
-    raw.unpack(weight_lo);
-    raw.load(h.weight + half + at);
-    raw.unpack(weight_hi);
+    float frequencies[E];
+    load_frequencies<V>(a.rotary, at, half, inside, frequencies);
+    angles<V>(frequencies, position, s, c);
   }
   const float inverse_width = 1.F / float(a.width);
-  for (uint32_t head = first; head < last; head += kSide) {
-    const bool active = inside && head + group < last;
-    const size_t place = size_t(head + group) * a.width + at;
+#pragma unroll 1
+  for (uint32_t at_head = first; at_head < last; at_head += kSide) {
+    const uint32_t head = at_head + group;
+    const bool active = inside && head < last, is_key = head >= a.query.heads;
     float lo[E], hi[E];
-    Raw<V> raw_lo, raw_hi;
-    raw_lo.clear();
-    raw_hi.clear();
-    if (active) {
-      const bf16* from = h.input + size_t(row) * h.input_stride + place;
-      raw_lo.load(from);
-      raw_hi.load(from + half);
-    }
-    raw_lo.unpack(lo);
-    raw_hi.unpack(hi);
-    const float inverse = h.normalize ? inverse_rms<LPH, E>(lo, hi, inverse_width, a.epsilon) : 1.F;
+    next_lo.unpack(lo);
+    next_hi.unpack(hi);
+    load(head + kSide, next_lo, next_hi);
+    const float rms = inverse_rms<LPH, E>(lo, hi, inverse_width, a.epsilon);
+    const float inverse = (is_key ? a.key.normalize : a.query.normalize) ? rms : 1.F;
+    const bf16* weight = is_key ? a.key.weight : a.query.weight;
+    if (weight != nullptr && inside) {
+      Raw<V> raw;
+      float w[E];
+      raw.load(weight + at);
+      raw.unpack(w);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      lo[e] = lo[e] * inverse * weight_lo[e];
-      hi[e] = hi[e] * inverse * weight_hi[e];
+      for (int e = 0; e < E; ++e) lo[e] = lo[e] * inverse * w[e];
+      raw.load(weight + half + at);
+      raw.unpack(w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) hi[e] = hi[e] * inverse * w[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        lo[e] *= inverse;
+        hi[e] *= inverse;
+      }
     }
     rotate<V>(a.rotary, lo, hi, s, c, position, at, half, active, stage[warp] + group * LPH * 2 * E);
     if (active) {
@@ -246,7 +269,8 @@ __global__ void __launch_bounds__(32 * kNormWarps) qk_norm_rotary_kernel(NormRot
         out_lo[e] = *reinterpret_cast<const uint32_t*>(&l);
         out_hi[e] = *reinterpret_cast<const uint32_t*>(&u);
       }
-      bf16* to = h.output + size_t(row) * h.output_stride + place;
+      bf16* to = is_key ? a.key.output + size_t(row) * a.key.output_stride : a.query.output + size_t(row) * a.query.output_stride;
+      to += size_t(is_key ? head - a.query.heads : head) * a.width + at;
       if constexpr (V == 1) {
         *reinterpret_cast<uint2*>(to) = make_uint2(out_lo[0], out_lo[1]);
         *reinterpret_cast<uint2*>(to + half) = make_uint2(out_hi[0], out_hi[1]);
@@ -268,6 +292,7 @@ struct Append {
   const int32_t* positions;
   Rotary rotary;
   float epsilon;
+  uint32_t heads_each;                 // KV heads of a block
 };
 
 // What the call brings to one page of one sequence.
@@ -295,13 +320,13 @@ __device__ __forceinline__ Segment segment_at(const Append& a, uint32_t sequence
   return g;
 }
 
-// The block's segment: number blockIdx.x over all sequences, found by a scan over their counts.
+// Segment `wanted` of all sequences, found by a scan over their counts.
 template <int THREADS>
-__device__ __forceinline__ Segment find_segment(const Append& a) {
+__device__ __forceinline__ Segment find_segment(const Append& a, uint32_t wanted) {
   constexpr int WARPS = THREADS / 32;
   __shared__ uint32_t totals[WARPS];
   __shared__ Segment found;
-  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, wanted = blockIdx.x;
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) found.page = -1;
   uint32_t before = 0;
   for (uint32_t base = 0; base < a.batch.sequences; base += THREADS) {
@@ -362,18 +387,23 @@ __device__ __forceinline__ uint32_t softer(uint32_t codes, float ratio) {
   return out;
 }
 
-// One block: the call's tokens of one page, one KV head, keys or values.  W warps take tokens in T rounds; a token's raw values
-// stay in registers between the search for the loudest element and the rounding, which norms and rotates again (T > 1).
-template <int LPH, int V, int W, int T>
-__global__ void __launch_bounds__(32 * W) kv_append_kernel(Append a) {
-  constexpr int E = 4 * V, kSide = 32 / LPH;
+// A cluster of one to eight blocks takes the call's tokens of one page, a token at a time for LPH lanes, for a few KV heads one
+// after the other, keys or values: the angles are computed once, the next head's values are on their way while a head is rounded,
+// and of every head the blocks tell one another their loudest element.
+template <int LPH, int V, int W>
+__global__ void __launch_bounds__(32 * W, (V == 1 || W == 16 ? 32 : 20) / W) kv_append_kernel(Append a) {
+  constexpr int E = 4 * V, kSide = 32 / LPH, kMostBlocks = 8;
+  constexpr uint32_t width = LPH * 2 * E, half = width / 2;
   __shared__ float stage[W][kSide * LPH * 2 * E];
-  __shared__ float loudest_of[W];
+  __shared__ float loudest_of[2][kMostBlocks][W];
+  const uint32_t blocks = W == 16 ? pair::cluster_size() : 1, rank = W == 16 ? pair::cluster_rank() : 0;
+  if (W == 16 && blocks > 1) pair::cluster_arrive();               // the others run before their shared memory is written
   griddep_enter();
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, group = lane / LPH, at = lane % LPH * E;
-  const uint32_t width = LPH * 2 * E, half = width / 2;
-  const uint32_t head = blockIdx.y % a.cache.kv_heads;
-  const bool is_key = blockIdx.y < a.cache.kv_heads;
+  const uint32_t parts = gridDim.y / 2;
+  const bool is_key = blockIdx.y < parts;
+  const uint32_t first_head = (is_key ? blockIdx.y : blockIdx.y - parts) * a.heads_each;
+  const uint32_t last_head = min(first_head + a.heads_each, a.cache.kv_heads);
   Segment g;
   if constexpr (W == 1) {                                  // one row a sequence
     const SequenceRows s = sequence_rows(a.batch, blockIdx.x);
@@ -381,112 +411,128 @@ __global__ void __launch_bounds__(32 * W) kv_append_kernel(Append a) {
     if (segments_of(s, a.cache.page_tokens) == 0) return;
     g = segment_at(a, blockIdx.x, s, 0);
   } else {
-    g = find_segment<32 * W>(a);
+    g = find_segment<32 * W>(a, blockIdx.x / blocks);
   }
-  if (g.page < 0) return;
+  __syncwarp();
+  if (W == 16 && blocks > 1) pair::cluster_wait();
+  if (g.page < 0) return;                                  // all blocks of a cluster alike
   const Heads& h = is_key ? a.key : a.value;
   Rotary rotary = a.rotary;
   if (!is_key) rotary.kind = kNone;
 
-  Raw<V> raw_lo[T], raw_hi[T];
-  int position[T];
-#pragma unroll
-  for (int t = 0; t < T; ++t) {
-    const int token = (t * W + warp) * kSide + group;
-    position[t] = 0;
-    raw_lo[t].clear();
-    raw_hi[t].clear();
-    if (token < g.count) {
-      const bf16* from = h.input + size_t(g.row + token) * h.input_stride + size_t(head) * width + at;
-      raw_lo[t].load(from);
-      raw_hi[t].load(from + half);
-      position[t] = a.positions != nullptr ? a.positions[g.row + token] : g.position + token;
-    }
-  }
-  float weight_lo[E], weight_hi[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) weight_lo[e] = weight_hi[e] = 1.F;
-  if (h.weight != nullptr) {
-    Raw<V> raw;
-    raw.load(h.weight + at);
-    raw.unpack(weight_lo);
-    raw.load(h.weight + half + at);
-    raw.unpack(weight_hi);
-  }
-  Turns<V> turns;
-  turns.load(rotary, at, half, true);
-
-  const auto finished = [&](int t, float* lo, float* hi) {
-    raw_lo[t].unpack(lo);
-    raw_hi[t].unpack(hi);
-    const float inverse = h.normalize ? inverse_rms<LPH, E>(lo, hi, 1.F / float(width), a.epsilon) : 1.F;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      lo[e] = lo[e] * inverse * weight_lo[e];
-      hi[e] = hi[e] * inverse * weight_hi[e];
-    }
-    if (rotary.kind != kNone) {
-      float s[E], c[E];
-      if (rotary.kind != kPart) angles(turns, position[t], s, c);
-      rotate<V>(rotary, lo, hi, s, c, position[t], at, half, true, stage[warp] + group * LPH * 2 * E);
+  const uint32_t token = (rank * W + warp) * kSide + group;
+  const bool active = token < uint32_t(g.count);
+  const bf16* const from = h.input + size_t(g.row + token) * h.input_stride + at;
+  Raw<V> next_lo, next_hi;
+  const auto load = [&](uint32_t head) {
+    next_lo.clear();
+    next_hi.clear();
+    if (active && head < last_head) {
+      next_lo.load(from + size_t(head) * width);
+      next_hi.load(from + size_t(head) * width + half);
     }
   };
+  load(first_head);
+  const int position = !active ? 0 : a.positions != nullptr ? a.positions[g.row + token] : g.position + int(token);
+  float s[E], c[E];
+  if (rotary.kind != kNone) {
+    float frequencies[E];
+    load_frequencies<V>(rotary, at, half, true, frequencies);
+    angles<V>(frequencies, position, s, c);
+  }
+  Raw<V> weight_lo, weight_hi;
+  weight_lo.clear();
+  weight_hi.clear();
+  if (h.weight != nullptr) {
+    weight_lo.load(h.weight + at);
+    weight_hi.load(h.weight + half + at);
+  }
 
-  float loudest = 0.F, lo[E], hi[E];
+#pragma unroll 1
+  for (uint32_t head = first_head; head < last_head; ++head) {
+    float lo[E], hi[E];
+    next_lo.unpack(lo);
+    next_hi.unpack(hi);
+    load(head + 1);
+    float* const scale_at = (is_key ? a.cache.k_scales : a.cache.v_scales) + size_t(g.page) * a.cache.kv_heads + head;
+    float old = g.slot > 0 ? *scale_at : 0.F;
+    if (!(old > 0.F && old <= 3.4028234e38F)) old = 0.F;
+    const float inverse = h.normalize ? inverse_rms<LPH, E>(lo, hi, 1.F / float(width), a.epsilon) : 1.F;
+    if (h.weight != nullptr) {
+      float w[E];
+      weight_lo.unpack(w);
 #pragma unroll
-  for (int t = 0; t < T; ++t) {
-    if ((t * W + warp) * kSide >= uint32_t(g.count)) break;          // the same for the whole warp
-    finished(t, lo, hi);
-    if ((t * W + warp) * kSide + group < uint32_t(g.count))
+      for (int e = 0; e < E; ++e) lo[e] = lo[e] * inverse * w[e];
+      weight_hi.unpack(w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) hi[e] = hi[e] * inverse * w[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        lo[e] *= inverse;
+        hi[e] *= inverse;
+      }
+    }
+    rotate<V>(rotary, lo, hi, s, c, position, at, half, true, stage[warp] + group * LPH * 2 * E);
+
+    float loudest = 0.F;                                   // of what is no NaN
+#pragma unroll
+    for (int e = 0; e < E; ++e) loudest = fmaxf(loudest, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
+    if (!(loudest <= 3.4028234e38F)) {
+      loudest = 0.F;
 #pragma unroll
       for (int e = 0; e < E; ++e) loudest = fmaxf(loudest, fmaxf(finite_size(lo[e]), finite_size(hi[e])));
-  }
-#pragma unroll
-  for (int m = 16; m; m /= 2) loudest = fmaxf(loudest, __shfl_xor_sync(0xffffffffu, loudest, m));
-  float* scale_at = (is_key ? a.cache.k_scales : a.cache.v_scales) + size_t(g.page) * a.cache.kv_heads + head;
-  float old = g.slot > 0 ? *scale_at : 0.F;
-  if (!(old > 0.F && old <= 3.4028234e38F)) old = 0.F;
-  if constexpr (W > 1) {
-    if (lane == 0) loudest_of[warp] = loudest;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < W; ++w) loudest = fmaxf(loudest, loudest_of[w]);
-  } else {
-    __syncwarp();
-  }
-  const float scale = fmaxf(old, page_scale(loudest)), inverse_scale = __frcp_rn(scale);
-  if (threadIdx.x == 0) *scale_at = scale;
-
-  uint8_t* page = static_cast<uint8_t*>(is_key ? a.cache.k_data : a.cache.v_data) +
-                  (size_t(g.page) * a.cache.kv_heads + head) * a.cache.page_tokens * width;
-  if (g.slot > 0 && scale > old) {                         // a louder token than the page had
-    const float ratio = old * inverse_scale;
-    uint4* codes = reinterpret_cast<uint4*>(page);
-#pragma unroll 4
-    for (uint32_t i = threadIdx.x; i < uint32_t(g.slot) * width / 16; i += 32 * W) {
-      uint4 v = codes[i];
-      v = make_uint4(softer(v.x, ratio), softer(v.y, ratio), softer(v.z, ratio), softer(v.w, ratio));
-      codes[i] = v;
     }
-  }
+    if (!active) loudest = 0.F;
 #pragma unroll
-  for (int t = 0; t < T; ++t) {
-    if ((t * W + warp) * kSide >= uint32_t(g.count)) break;
-    if (T > 1) finished(t, lo, hi);
-    const uint32_t token = (t * W + warp) * kSide + group;
-    if (token >= uint32_t(g.count)) continue;
-    uint8_t* to = page + size_t(g.slot + token) * width + at;
+    for (int m = 16; m; m /= 2) loudest = fmaxf(loudest, __shfl_xor_sync(0xffffffffu, loudest, m));
+    if constexpr (W > 1) {
+      float (&loudest_here)[kMostBlocks][W] = loudest_of[(head - first_head) & 1];
+      if (W == 16 && blocks > 1) {
+        if (lane < blocks) pair::store_cluster(pair::cluster_address(&loudest_here[rank][warp], lane), loudest);
+        __syncwarp();
+        pair::cluster_arrive();
+        pair::cluster_wait();
+      } else {
+        if (lane == 0) loudest_here[0][warp] = loudest;
+        __syncthreads();
+      }
+      loudest = 0.F;
+      for (uint32_t i = lane; i < blocks * W; i += 32) loudest = fmaxf(loudest, loudest_here[i / W][i % W]);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      lo[e] *= inverse_scale;
-      hi[e] *= inverse_scale;
-    }
-    if constexpr (V == 1) {
-      *reinterpret_cast<uint32_t*>(to) = e4m3x4(lo[0], lo[1], lo[2], lo[3]);
-      *reinterpret_cast<uint32_t*>(to + half) = e4m3x4(hi[0], hi[1], hi[2], hi[3]);
+      for (int m = 16; m; m /= 2) loudest = fmaxf(loudest, __shfl_xor_sync(0xffffffffu, loudest, m));
     } else {
-      *reinterpret_cast<uint2*>(to) = make_uint2(e4m3x4(lo[0], lo[1], lo[2], lo[3]), e4m3x4(lo[4], lo[5], lo[6], lo[7]));
-      *reinterpret_cast<uint2*>(to + half) = make_uint2(e4m3x4(hi[0], hi[1], hi[2], hi[3]), e4m3x4(hi[4], hi[5], hi[6], hi[7]));
+      __syncwarp();
+    }
+    const float scale = fmaxf(old, page_scale(loudest)), inverse_scale = __frcp_rn(scale);
+    if (rank == 0 && threadIdx.x == 0) *scale_at = scale;
+
+    uint8_t* const page = static_cast<uint8_t*>(is_key ? a.cache.k_data : a.cache.v_data) +
+                          (size_t(g.page) * a.cache.kv_heads + head) * a.cache.page_tokens * width;
+    if (g.slot > 0 && scale > old) {                       // a louder token than the page had
+      const float ratio = old * inverse_scale;
+      uint4* codes = reinterpret_cast<uint4*>(page);
+#pragma unroll 4
+      for (uint32_t i = rank * 32 * W + threadIdx.x; i < uint32_t(g.slot) * width / 16; i += blocks * 32 * W) {
+        uint4 v = codes[i];
+        v = make_uint4(softer(v.x, ratio), softer(v.y, ratio), softer(v.z, ratio), softer(v.w, ratio));
+        codes[i] = v;
+      }
+    }
+    if (active) {
+      uint8_t* to = page + size_t(g.slot + token) * width + at;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        lo[e] *= inverse_scale;
+        hi[e] *= inverse_scale;
+      }
+      if constexpr (V == 1) {
+        *reinterpret_cast<uint32_t*>(to) = e4m3x4(lo[0], lo[1], lo[2], lo[3]);
+        *reinterpret_cast<uint32_t*>(to + half) = e4m3x4(hi[0], hi[1], hi[2], hi[3]);
+      } else {
+        *reinterpret_cast<uint2*>(to) = make_uint2(e4m3x4(lo[0], lo[1], lo[2], lo[3]), e4m3x4(lo[4], lo[5], lo[6], lo[7]));
+        *reinterpret_cast<uint2*>(to + half) = make_uint2(e4m3x4(hi[0], hi[1], hi[2], hi[3]), e4m3x4(hi[4], hi[5], hi[6], hi[7]));
+      }
     }
   }
 }
@@ -519,11 +565,16 @@ Heads heads_of(const gw_head_rows& h) {
                static_cast<const bf16*>(h.weight), h.heads, h.normalize};
 }
 
+// Parts of `count` heads such that `units` times the parts are at least `wanted`, if the heads allow it; heads of a part.
+uint32_t heads_each(uint32_t count, uint64_t units, uint64_t wanted) {
+  const uint64_t parts = std::min<uint64_t>(count, std::max<uint64_t>(1, (wanted + units - 1) / units));
+  return uint32_t((count + parts - 1) / parts);
+}
+
 cudaError_t launch_norm_rotary(NormRotary a, cudaStream_t stream) {
-  const int lanes = a.width <= 64 ? 8 : a.width <= 128 ? 16 : 32;
-  a.per_task = 32 / lanes;
-  a.query_tasks = (a.query.heads + a.per_task - 1) / a.per_task;
-  a.tasks = a.query_tasks + (a.key.heads + a.per_task - 1) / a.per_task;
+  const uint32_t lanes = a.width <= 64 ? 8 : a.width <= 128 ? 16 : 32, side = 32 / lanes, heads = a.query.heads + a.key.heads;
+  a.per_task = side * heads_each((heads + side - 1) / side, a.rows, 148 * 48);
+  a.tasks = (heads + a.per_task - 1) / a.per_task;
   const uint64_t tasks = uint64_t(a.rows) * a.tasks;
   if (tasks > 0xffffffffull - 64) return cudaErrorInvalidValue;
   const auto kernel = a.width <= 64    ? qk_norm_rotary_kernel<8, 1>
@@ -534,20 +585,36 @@ cudaError_t launch_norm_rotary(NormRotary a, cudaStream_t stream) {
 }
 
 template <int LPH, int V>
-cudaError_t launch_append(const Append& a, cudaStream_t stream) {
-  const uint32_t page = a.cache.page_tokens, most = std::min(page, a.batch.max_rows), sequences = a.batch.sequences;
+cudaError_t launch_append(Append a, cudaStream_t stream) {
+  const uint32_t page = a.cache.page_tokens, most = std::min(page, a.batch.max_rows), sequences = a.batch.sequences, heads = a.cache.kv_heads;
   constexpr uint32_t kSide = 32 / LPH;
-  const dim3 heads(1, 2 * a.cache.kv_heads);
-  if (a.batch.max_rows == 1) return launch_pdl(kv_append_kernel<LPH, V, 1, 1>, dim3(sequences, heads.y), 32, stream, a);
+  a.heads_each = 1;
+  if (a.batch.max_rows == 1) return launch_pdl(kv_append_kernel<LPH, V, 1>, dim3(sequences, 2 * heads), 32, stream, a);
   // a sequence of n rows touches at most 1 + (n + page - 2) / page pages
   const uint64_t bound = std::min(uint64_t(sequences) * (1 + (a.batch.max_rows + page - 2) / page),
                                   sequences + (uint64_t(a.batch.rows) + uint64_t(sequences) * (page - 2)) / page);
-  const dim3 grid(uint32_t(bound), heads.y);
-  if (most <= 4 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 4, 1>, grid, 128, stream, a);
-  if (most <= 16 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 16, 1>, grid, 512, stream, a);
-  if (most <= 32 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 16, 2>, grid, 512, stream, a);
-  if (most <= 64 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 16, 4>, grid, 512, stream, a);
-  return launch_pdl(kv_append_kernel<LPH, V, 16, 8>, grid, 512, stream, a);
+  uint32_t blocks = 1;
+  if (most > 8 * kSide)
+    while (16 * kSide * blocks < most) blocks *= 2;
+  a.heads_each = heads_each(heads, 2 * bound * blocks, 148 * 4);
+  const dim3 grid(uint32_t(bound) * blocks, 2 * ((heads + a.heads_each - 1) / a.heads_each));
+  if (most <= 4 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 4>, grid, 128, stream, a);
+  if (most <= 8 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 8>, grid, 256, stream, a);
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(512);
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2]{};
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = blocks;
+  attributes[0].val.clusterDim.y = 1;
+  attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attributes;
+  config.numAttrs = 2;
+  note_launch();
+  return cudaLaunchKernelEx(&config, kv_append_kernel<LPH, V, 16>, a);
 }
 
 }  // namespace

@@ -16,9 +16,16 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
 // address of the same shared-memory location in the pair's leader (cluster rank 0)
 __device__ __forceinline__ uint32_t leader_address(const void* local) {
@@ -34,6 +41,9 @@ __device__ __forceinline__ uint32_t cluster_address(const void* local, uint32_t 
 }
 __device__ __forceinline__ void store_cluster(uint32_t cluster_address, const uint32_t* v) {
   asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+__device__ __forceinline__ void store_cluster(uint32_t cluster_address, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_address), "f"(v) : "memory");
 }
 // Plain (CTA-scope release) form on purpose: measured on B200, the .release.cluster form of this arrive
 // cost the scale-loader warps about 1000 cycles per stage.  What the arrival publishes is tensor memory

@@ -18,9 +18,15 @@ TRANSFORM_IDENTITY = _lib.TRANSFORM_IDENTITY
 TRANSFORM_GELU_TANH_MULTIPLY = _lib.TRANSFORM_GELU_TANH_MULTIPLY
 
 
+_loaded = None
+
+
 def _library():
-    from . import lib
-    return lib
+    global _loaded
+    if _loaded is None:
+        from . import lib
+        _loaded = lib
+    return _loaded
 
 
 def _ptr(t) -> int:
@@ -720,11 +726,21 @@ class FfnBlock:
 
 # --------------------------------------------------------------------------- attention between the projections
 
-def _on_current(device):
+# The host's share of a call on a few rows is several times the kernel's, so what these calls look up, they look up once: a tensor's
+# device as a number, the library, the current device and its stream without objects around them.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_BF16, _I32 = torch.bfloat16, torch.int32
+
+
+def _on_current(device: int) -> int:
     """The launches go to the current device, so the tensors have to lie there."""
-    if device.type != "cuda" or device.index != torch.cuda.current_device():
-        raise _lib.GewellInvalidArgument(f"tensors on {device}: the current CUDA device's are wanted")
+    if device < 0 or device != _current_device():
+        raise _lib.GewellInvalidArgument("tensors of the current CUDA device are wanted")
     return device
+
+
+def _stream_on(device: int, stream) -> int:
+    return _raw_stream(device) if stream is None and _raw_stream is not None else _stream(stream)
 
 
 class KvCache:
@@ -741,7 +757,7 @@ class KvCache:
                 raise _lib.GewellInvalidArgument("keys and values have one shape and lie on one device")
         self.k_data, self.v_data, self.k_scales, self.v_scales = k_data, v_data, k_scales, v_scales
         self.pages, self.kv_heads, self.page_tokens, self.head_dim = k_data.shape
-        self.device = k_data.device
+        self.device_index = k_data.get_device()
         self._struct = _lib.KvCache(_ptr(k_data), _ptr(v_data), _ptr(k_scales), _ptr(v_scales), *k_data.shape)
         self._ref = ctypes.byref(self._struct)
 
@@ -758,58 +774,73 @@ class SequenceBatch:
         if row_offsets.shape[0] != count + 1 or page_table.shape[0] != count or page_table.stride(0) < page_table.shape[1]:
             raise _lib.GewellInvalidArgument("row_offsets has one entry more than there are sequences, page_table a row for each")
         self.row_offsets, self.context_lengths, self.page_table = row_offsets, context_lengths, page_table
-        self.rows, self.max_rows, self.device = rows, max_rows, row_offsets.device
+        self.rows, self.max_rows, self.device_index = rows, max_rows, row_offsets.get_device()
         stride = page_table.stride(0) if count > 1 else max(1, page_table.shape[1])
         self._struct = _lib.Sequences(_ptr(row_offsets), _ptr(context_lengths), _ptr(page_table), stride, count, rows, max_rows)
         self._ref = ctypes.byref(self._struct)
 
 
-def _head_rows(x: torch.Tensor, weight, normalize: bool, y=None, rows=None):
-    """gw_head_rows of x [rows, heads, head_dim]."""
-    for t in (x,) if y is None else (x, y):
-        if t.dim() != 3 or t.dtype != torch.bfloat16 or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
-            raise _lib.GewellInvalidArgument("heads are BF16 [rows, heads, head_dim], a row's heads side by side")
-    if y is not None and (y.shape != x.shape or y.device != x.device):
-        raise _lib.GewellInvalidArgument("the output has its input's shape and device")
-    if rows is not None and x.shape[0] < rows:
-        raise _lib.GewellInvalidArgument(f"{x.shape[0]} rows of heads for {rows} token rows")
-    if weight is not None and (weight.dtype != torch.bfloat16 or weight.shape != x.shape[2:] or not weight.is_contiguous() or weight.device != x.device):
+def _layout(x: torch.Tensor, device: int):
+    """(rows, heads, head_dim, elements from row to row) of BF16 [rows, heads, head_dim] with a row's heads side by side."""
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3 or x.dtype is not _BF16 or stride[2] != 1 or (stride[1] != shape[2] and shape[1] > 1) or x.get_device() != device:
+        raise _lib.GewellInvalidArgument("heads are BF16 [rows, heads, head_dim] on the other tensors' device, a row's heads side by side")
+    rows, heads, dim = shape
+    return rows, heads, dim, stride[0] if rows > 1 else heads * dim
+
+
+def _output(x: torch.Tensor, rows: int, heads: int, dim: int, y, device: int):
+    """(y, its row stride); a new tensor for None."""
+    if y is None:
+        return torch.empty_like(x, memory_format=torch.contiguous_format), heads * dim
+    at = _layout(y, device)
+    if at[:3] != (rows, heads, dim):
+        raise _lib.GewellInvalidArgument("the output has its input's shape")
+    return y, at[3]
+
+
+def _head_weight(weight, dim: int, device: int) -> int:
+    if weight is None:
+        return 0
+    if weight.dtype is not _BF16 or weight.shape != (dim,) or weight.stride(0) != 1 or weight.get_device() != device:
         raise _lib.GewellInvalidArgument("a head norm's weight is BF16 [head_dim]")
-    single = x.shape[0] <= 1
-    return _lib.HeadRows(x.data_ptr(), x.shape[1] * x.shape[2] if single else x.stride(0), _ptr(y),
-                         0 if y is None else y.shape[1] * y.shape[2] if single else y.stride(0), _ptr(weight), x.shape[1], int(normalize))
+    return weight.data_ptr()
 
 
-def _rotary(frequencies, interleaved: bool, device):
+def _rotary(frequencies, interleaved: bool, device: int):
     if frequencies is None:
         return None
-    if frequencies.dtype != torch.float32 or frequencies.dim() != 1 or not frequencies.is_contiguous() or frequencies.device != device:
+    if frequencies.dtype is not torch.float32 or frequencies.dim() != 1 or frequencies.stride(0) != 1 or frequencies.get_device() != device:
         raise _lib.GewellInvalidArgument("inverse frequencies are FP32 [width / 2]")
-    return ctypes.byref(_lib.Rotary(frequencies.data_ptr(), 2 * frequencies.shape[0], int(interleaved)))
+    return ctypes.byref(_lib.Rotary(frequencies.data_ptr(), 2 * frequencies.shape[0], interleaved))
 
 
-def _check_positions(positions, rows: int, device):
-    if positions.dtype != torch.int32 or positions.dim() != 1 or positions.shape[0] < rows or not positions.is_contiguous() or positions.device != device:
+def _positions(positions, rows: int, device: int) -> int:
+    if positions is None:
+        return 0
+    if positions.dtype is not _I32 or positions.dim() != 1 or positions.shape[0] < rows or positions.stride(0) != 1 or positions.get_device() != device:
         raise _lib.GewellInvalidArgument("positions are int32 [rows]")
+    return positions.data_ptr()
 
 
-def qk_norm_rotary(query: torch.Tensor, key, query_weight, key_weight, positions: torch.Tensor, frequencies, epsilon: float = 1e-6,
+def qk_norm_rotary(query: torch.Tensor, key, query_weight, key_weight, positions, frequencies, epsilon: float = 1e-6,
                    interleaved: bool = False, query_out=None, key_out=None, stream=None):
     """RMS norm of every head of query [rows, heads, head_dim] and key [rows, kv_heads, head_dim] (or None; rows of a joined
-    projection will do) and rotation by position, in one launch; returns (query_out, key_out)."""
-    _on_current(query.device)
-    rows = query.shape[0]
-    query_out = torch.empty(query.shape, dtype=torch.bfloat16, device=query.device) if query_out is None else query_out
-    q = _head_rows(query, query_weight, True, query_out)
+    projection will do) and rotation by position, in one launch; returns (query_out, key_out).  positions int32 [rows] (or None
+    where nothing is rotated)."""
+    device = _on_current(query.get_device())
+    rows, heads, dim, stride = _layout(query, device)
+    query_out, out_stride = _output(query, rows, heads, dim, query_out, device)
+    q = _lib.HeadRows(query.data_ptr(), stride, query_out.data_ptr(), out_stride, _head_weight(query_weight, dim, device), heads, 1)
     k = None
     if key is not None:
-        if key.shape[0] != rows or key.shape[2] != query.shape[2] or key.device != query.device:
+        key_rows, kv_heads, key_dim, stride = _layout(key, device)
+        if key_rows != rows or key_dim != dim:
             raise _lib.GewellInvalidArgument("queries and keys have the same rows and head width")
-        key_out = torch.empty(key.shape, dtype=torch.bfloat16, device=key.device) if key_out is None else key_out
-        k = ctypes.byref(_head_rows(key, key_weight, True, key_out))
-    _check_positions(positions, rows, query.device)
-    _check(_library().gw_qk_norm_rotary_bf16(ctypes.byref(q), k, rows, query.shape[2], positions.data_ptr(),
-                                             _rotary(frequencies, interleaved, query.device), epsilon, _stream(stream)))
+        key_out, out_stride = _output(key, rows, kv_heads, dim, key_out, device)
+        k = ctypes.byref(_lib.HeadRows(key.data_ptr(), stride, key_out.data_ptr(), out_stride, _head_weight(key_weight, dim, device), kv_heads, 1))
+    _check(_library().gw_qk_norm_rotary_bf16(ctypes.byref(q), k, rows, dim, _positions(positions, rows, device),
+                                             _rotary(frequencies, interleaved, device), epsilon, _stream_on(device, stream)))
     return query_out, key_out
 
 
@@ -818,39 +849,44 @@ def kv_cache_append(cache: KvCache, batch: SequenceBatch, key: torch.Tensor, val
                     positions=None, query=None, query_weight=None, query_out=None, epsilon: float = 1e-6, stream=None):
     """Keys and values [rows, kv_heads, head_dim] of a step into their pages: norms, rotation of the keys, quantisation.  With
     `query` [rows, heads, head_dim] its heads are normed and rotated in the same call; returns query_out then, else None."""
-    device = _on_current(cache.device)
-    for x in (key, value, query):
-        if x is not None and (x.device != device or x.shape[-1] != cache.head_dim):
-            raise _lib.GewellInvalidArgument("heads have the cache's width and lie on its device")
-    if batch.device != device:
+    device, dim, rows = _on_current(cache.device_index), cache.head_dim, batch.rows
+    if batch.device_index != device:
         raise _lib.GewellInvalidArgument("the batch lies on the cache's device")
-    k = _head_rows(key, key_weight, normalize_key, None, batch.rows)
-    v = _head_rows(value, None, normalize_value, None, batch.rows)
+    made = []
+    for x, weight, normalize in ((key, key_weight, normalize_key), (value, None, normalize_value)):
+        x_rows, heads, x_dim, stride = _layout(x, device)
+        if x_dim != dim or x_rows < rows:
+            raise _lib.GewellInvalidArgument("keys and values have the cache's head width and the batch's rows")
+        made.append(ctypes.byref(_lib.HeadRows(x.data_ptr(), stride, 0, 0, _head_weight(weight, dim, device), heads, normalize)))
     q = None
     if query is not None:
-        query_out = torch.empty(query.shape, dtype=torch.bfloat16, device=device) if query_out is None else query_out
-        q = ctypes.byref(_head_rows(query, query_weight, True, query_out, batch.rows))
-    if positions is not None:
-        _check_positions(positions, batch.rows, device)
-    _check(_library().gw_kv_cache_append(cache._ref, batch._ref, ctypes.byref(k), ctypes.byref(v), q, _ptr(positions),
-                                         _rotary(frequencies, interleaved, device), epsilon, _stream(stream)))
+        q_rows, heads, q_dim, stride = _layout(query, device)
+        if q_dim != dim or q_rows < rows:
+            raise _lib.GewellInvalidArgument("queries have the cache's head width and the batch's rows")
+        query_out, out_stride = _output(query, q_rows, heads, dim, query_out, device)
+        q = ctypes.byref(_lib.HeadRows(query.data_ptr(), stride, query_out.data_ptr(), out_stride, _head_weight(query_weight, dim, device), heads, 1))
+    _check(_library().gw_kv_cache_append(cache._ref, batch._ref, made[0], made[1], q, _positions(positions, rows, device),
+                                         _rotary(frequencies, interleaved, device), epsilon, _stream_on(device, stream)))
     return query_out if query is not None else None
 
 
 def paged_attention(cache: KvCache, batch: SequenceBatch, query: torch.Tensor, scale: float, window: int = 0, y=None, scratch=None,
                     stream=None):
     """Attention of query [rows, heads, head_dim] over the cache, which holds the step's own tokens already; BF16 [rows, heads,
-    head_dim] (rows behind the last sequence are not written).  `scratch`: uint8 that later calls on the same stream may share (allocated for the call if None)."""
-    device = _on_current(cache.device)
-    y = torch.empty(query.shape, dtype=torch.bfloat16, device=device) if y is None else y
-    q = _head_rows(query, None, False, y, batch.rows)
-    if query.device != device or batch.device != device or query.shape[2] != cache.head_dim:
-        raise _lib.GewellInvalidArgument("queries have the cache's head width; queries, batch and cache lie on one device")
+    head_dim] (rows behind the last sequence are not written).  `scratch`: uint8 that later calls on the same stream may share
+    (allocated for the call if None)."""
+    device = _on_current(cache.device_index)
+    rows, heads, dim, stride = _layout(query, device)
+    if batch.device_index != device or dim != cache.head_dim or rows < batch.rows:
+        raise _lib.GewellInvalidArgument("queries have the cache's head width and the batch's rows; all lie on one device")
+    y, out_stride = _output(query, rows, heads, dim, y, device)
     lib = _library()
     if scratch is None:
-        scratch = torch.empty(max(256, lib.gw_paged_attention_scratch_bytes(cache._ref, batch._ref, q.heads)), dtype=torch.uint8, device=device)
-    _check(lib.gw_paged_attention_bf16(cache._ref, batch._ref, q.input, q.input_stride, q.heads, scale, window, q.output, q.output_stride,
-                                       scratch.data_ptr(), scratch.numel(), _stream(stream)))
+        scratch = torch.empty(lib.gw_paged_attention_scratch_bytes(cache._ref, batch._ref, heads), dtype=torch.uint8, device=query.device)
+    elif scratch.dtype is not torch.uint8 or scratch.get_device() != device or not scratch.is_contiguous():
+        raise _lib.GewellInvalidArgument("scratch is contiguous uint8 on the cache's device")
+    _check(lib.gw_paged_attention_bf16(cache._ref, batch._ref, query.data_ptr(), stride, heads, scale, window, y.data_ptr(), out_stride,
+                                       scratch.data_ptr(), scratch.numel(), _stream_on(device, stream)))
     return y
 
 
