@@ -74,41 +74,45 @@ struct Raw {
 };
 
 // A lane's share of the rotation: the frequencies of its pairs.
-template <int V>
+template <int V, bool WHOLE>
 __device__ __forceinline__ void load_frequencies(const Rotary& r, uint32_t lane_at, uint32_t half, bool active, float* f) {
   constexpr int E = 4 * V;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     // kWhole: pair (at + e, at + e + half).  kNeighbours: E / 2 pairs of the first half, then E / 2 of the second.
-    const uint32_t pair = r.kind == kWhole ? lane_at + e : e < E / 2 ? lane_at / 2 + e : (half + lane_at) / 2 + (e - E / 2);
-    const bool used = active && r.kind != kNone && r.kind != kPart && 2 * pair < r.width;
+    const uint32_t pair = WHOLE ? lane_at + e : e < E / 2 ? lane_at / 2 + e : (half + lane_at) / 2 + (e - E / 2);
+    const bool used = active && (WHOLE || (r.kind == kNeighbours && 2 * pair < r.width));
     f[e] = used ? r.frequencies[pair] : 0.F;
   }
 }
 
 constexpr double kTurn = 0.15915494309189535;       // 1 / 2 pi
+constexpr int kNear = 1 << 24;
 
-__device__ __noinline__ float far_turns(float frequency, int position) {
+__device__ __forceinline__ bool is_near(int position) { return uint32_t(position + kNear) <= 2u * kNear; }
+__device__ __forceinline__ float near_turns(float frequency, float position) {
+  constexpr float high = float(kTurn), low = float(kTurn - double(high));
+  const float f = frequency * high, f_rest = fmaf(frequency, low, fmaf(frequency, high, -f));        // turns per position
+  const float whole = position * f;
+  return (whole - rintf(whole)) + fmaf(position, f_rest, fmaf(position, f, -whole));
+}
+__device__ __forceinline__ float far_turns(float frequency, int position) {
   const double turns = double(frequency) * kTurn * double(position);
   return float(turns - rint(turns));
 }
-__device__ __forceinline__ void sine_cosine(float frequency, int position, float& s, float& c) {
-  float turns;
-  if (uint32_t(position + (1 << 24)) <= 2u << 24) {
-    constexpr float high = float(kTurn), low = float(kTurn - double(high));
-    const float f = frequency * high, f_rest = fmaf(frequency, high, -f) + frequency * low;        // turns per position
-    const float p = float(position), whole = p * f;
-    turns = (whole - rintf(whole)) + fmaf(p, f_rest, fmaf(p, f, -whole));
-  } else {
-    turns = far_turns(frequency, position);
-  }
-  __sincosf(turns * 6.283185307179586F, &s, &c);
-}
+__device__ __forceinline__ void sine_cosine(float turns, float& s, float& c) { __sincosf(turns * 6.283185307179586F, &s, &c); }
 
 template <int V>
 __device__ __forceinline__ void angles(const float* frequencies, int position, float* s, float* c) {
+  constexpr int E = 4 * V;
 #pragma unroll
-  for (int e = 0; e < 4 * V; ++e) sine_cosine(frequencies[e], position, s[e], c[e]);
+  for (int e = 0; e < E; ++e) s[e] = near_turns(frequencies[e], float(position));
+  if (!is_near(position)) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[e] = far_turns(frequencies[e], position);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) sine_cosine(s[e], s[e], c[e]);
 }
 
 __device__ __forceinline__ void turn(float& a, float& b, float s, float c) {
@@ -119,11 +123,11 @@ __device__ __forceinline__ void turn(float& a, float& b, float s, float c) {
 
 // lo / hi: a lane's values of the head's halves, in place.  `stage`: half-split rotation of a part goes through 2 * half
 // floats of shared memory that belong to these LPH lanes.
-template <int V>
+template <int LPH, int V, bool WHOLE>
 __device__ __forceinline__ void rotate(const Rotary& r, float* lo, float* hi, const float* s, const float* c, int position, uint32_t at,
                                        uint32_t half, bool active, float* stage) {
   constexpr int E = 4 * V;
-  if (r.kind == kWhole) {
+  if (WHOLE) {
 #pragma unroll
     for (int e = 0; e < E; ++e) turn(lo[e], hi[e], s[e], c[e]);
   } else if (r.kind == kNeighbours) {
@@ -142,19 +146,20 @@ __device__ __forceinline__ void rotate(const Rotary& r, float* lo, float* hi, co
       }
     }
     __syncwarp();
+    const uint32_t pairs = r.width / 2;
+#pragma unroll 1                                           // kept short: the other kinds' registers count
+    for (uint32_t pair = at / E; pair < pairs; pair += LPH) {
+      float sine, cosine;
+      const float f = r.frequencies[pair];
+      sine_cosine(is_near(position) ? near_turns(f, float(position)) : far_turns(f, position), sine, cosine);
+      turn(stage[pair], stage[pairs + pair], sine, cosine);
+    }
+    __syncwarp();
     if (active) {
-      const uint32_t pairs = r.width / 2;
 #pragma unroll
-      for (int e = 0; e < 2 * E; ++e) {
-        const uint32_t i = e < E ? at + e : half + at + (e - E);
-        if (i >= r.width) continue;
-        float& mine = e < E ? lo[e] : hi[e - E];
-        const bool first = i < pairs;
-        const uint32_t pair = first ? i : i - pairs;
-        const float other = stage[first ? i + pairs : pair];
-        float sine, cosine;
-        sine_cosine(r.frequencies[pair], position, sine, cosine);
-        mine = first ? fmaf(-other, sine, mine * cosine) : fmaf(other, sine, mine * cosine);
+      for (int e = 0; e < E; ++e) {
+        lo[e] = stage[at + e];
+        hi[e] = stage[half + at + e];
       }
     }
   }
@@ -198,7 +203,7 @@ constexpr int kNormWarps = 4;
 
 // A warp takes heads of one row, queries and keys in one line, the next head's values on their way meanwhile; the row's angles are
 // computed once.
-template <int LPH, int V>
+template <int LPH, int V, bool WHOLE>
 __global__ void __launch_bounds__(32 * kNormWarps, V == 1 ? 8 : 6) qk_norm_rotary_kernel(NormRotary a) {
   constexpr int E = 4 * V, kSide = 32 / LPH;
   __shared__ float stage[kNormWarps][kSide * LPH * 2 * E];
@@ -227,7 +232,7 @@ __global__ void __launch_bounds__(32 * kNormWarps, V == 1 ? 8 : 6) qk_norm_rotar
   float s[E], c[E];
   {
     float frequencies[E];
-    load_frequencies<V>(a.rotary, at, half, inside, frequencies);
+    load_frequencies<V, WHOLE>(a.rotary, at, half, inside, frequencies);
     angles<V>(frequencies, position, s, c);
   }
   const float inverse_width = 1.F / float(a.width);
@@ -260,7 +265,7 @@ __global__ void __launch_bounds__(32 * kNormWarps, V == 1 ? 8 : 6) qk_norm_rotar
         hi[e] *= inverse;
       }
     }
-    rotate<V>(a.rotary, lo, hi, s, c, position, at, half, active, stage[warp] + group * LPH * 2 * E);
+    rotate<LPH, V, WHOLE>(a.rotary, lo, hi, s, c, position, at, half, active, stage[warp] + group * LPH * 2 * E);
     if (active) {
       uint32_t out_lo[2 * V], out_hi[2 * V];
 #pragma unroll
@@ -292,7 +297,7 @@ struct Append {
   const int32_t* positions;
   Rotary rotary;
   float epsilon;
-  uint32_t heads_each;                 // KV heads of a block
+  uint32_t each;                       // items of a block: the KV heads' keys are the first items, their values the others
 };
 
 // What the call brings to one page of one sequence.
@@ -387,23 +392,52 @@ __device__ __forceinline__ uint32_t softer(uint32_t codes, float ratio) {
   return out;
 }
 
+// a word of another block's shared memory
+__device__ __forceinline__ void store_word(uint32_t at, uint32_t value) {
+  asm volatile("st.relaxed.cluster.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(value) : "memory");
+}
+// The largest of `count` words (up to 32), each waited for until it is no longer 0.
+__device__ __forceinline__ uint32_t largest_of(const uint32_t* words, uint32_t count, uint32_t lane) {
+  uint32_t word = 0;
+  if (lane < count) {
+    for (uint32_t spins = 0; (word = *const_cast<const volatile uint32_t*>(words + lane)) == 0; ++spins) {
+      if (spins == 1u << 26) {                             // seconds
+        report(0xa3000000u);
+        break;
+      }
+    }
+  }
+  return __reduce_max_sync(0xffffffffu, word);
+}
+
+constexpr int kMostItems = 16;         // of a block
+
 // A cluster of one to eight blocks takes the call's tokens of one page, a token at a time for LPH lanes, for a few KV heads one
-// after the other, keys or values: the angles are computed once, the next head's values are on their way while a head is rounded,
-// and of every head the blocks tell one another their loudest element.
-template <int LPH, int V, int W>
+// after the other: the angles are computed once, the next head's values are on their way while a head is rounded.  Of every head
+// each warp sends all blocks the scale that its tokens and the page's codes want; the largest is the page's.
+template <int LPH, int V, int W, bool WHOLE>
 __global__ void __launch_bounds__(32 * W, (V == 1 || W == 16 ? 32 : 20) / W) kv_append_kernel(Append a) {
-  constexpr int E = 4 * V, kSide = 32 / LPH, kMostBlocks = 8;
+  constexpr int E = 4 * V, kSide = 32 / LPH;
   constexpr uint32_t width = LPH * 2 * E, half = width / 2;
-  __shared__ float stage[W][kSide * LPH * 2 * E];
-  __shared__ float loudest_of[2][kMostBlocks][W];
+  __shared__ __align__(16) float stage[W][kSide * LPH * 2 * E];
+  constexpr int kMostBlocks = W == 16 ? 8 : 1;
+  __shared__ uint32_t of_block[kMostItems], arrived[kMostItems];   // the scale that the block's warps want so far, and how many they are
+  __shared__ uint32_t wanted[kMostItems][kMostBlocks];             // the scale that a block of the cluster wants, 0 before
   const uint32_t blocks = W == 16 ? pair::cluster_size() : 1, rank = W == 16 ? pair::cluster_rank() : 0;
-  if (W == 16 && blocks > 1) pair::cluster_arrive();               // the others run before their shared memory is written
+  if constexpr (W > 1) {
+    if (threadIdx.x < kMostItems) {
+      of_block[threadIdx.x] = arrived[threadIdx.x] = 0;
+      for (int i = 0; i < kMostBlocks; ++i) wanted[threadIdx.x][i] = 0;
+    }
+    __syncthreads();
+    if (W == 16) pair::cluster_arrive();                   // the others run, and are ready, before anything is sent to them
+  }
   griddep_enter();
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, group = lane / LPH, at = lane % LPH * E;
-  const uint32_t parts = gridDim.y / 2;
-  const bool is_key = blockIdx.y < parts;
-  const uint32_t first_head = (is_key ? blockIdx.y : blockIdx.y - parts) * a.heads_each;
-  const uint32_t last_head = min(first_head + a.heads_each, a.cache.kv_heads);
+  const uint32_t kv_heads = a.cache.kv_heads, first = blockIdx.y * a.each, last = min(first + a.each, 2 * kv_heads);
+  const bool kept_used = first < kv_heads && (WHOLE || a.rotary.kind == kNeighbours);
+  float s[E], c[E];
+  if (kept_used) load_frequencies<V, WHOLE>(a.rotary, at, half, true, c);
   Segment g;
   if constexpr (W == 1) {                                  // one row a sequence
     const SequenceRows s = sequence_rows(a.batch, blockIdx.x);
@@ -414,126 +448,161 @@ __global__ void __launch_bounds__(32 * W, (V == 1 || W == 16 ? 32 : 20) / W) kv_
     g = find_segment<32 * W>(a, blockIdx.x / blocks);
   }
   __syncwarp();
-  if (W == 16 && blocks > 1) pair::cluster_wait();
+  if constexpr (W == 16) pair::cluster_wait();
   if (g.page < 0) return;                                  // all blocks of a cluster alike
-  const Heads& h = is_key ? a.key : a.value;
-  Rotary rotary = a.rotary;
-  if (!is_key) rotary.kind = kNone;
-
   const uint32_t token = (rank * W + warp) * kSide + group;
   const bool active = token < uint32_t(g.count);
-  const bf16* const from = h.input + size_t(g.row + token) * h.input_stride + at;
   Raw<V> next_lo, next_hi;
-  const auto load = [&](uint32_t head) {
+  const auto load = [&](uint32_t item) {
     next_lo.clear();
     next_hi.clear();
-    if (active && head < last_head) {
-      next_lo.load(from + size_t(head) * width);
-      next_hi.load(from + size_t(head) * width + half);
+    if (active && item < last) {
+      const bool is_key = item < kv_heads;
+      const bf16* from = is_key ? a.key.input + size_t(g.row + token) * a.key.input_stride : a.value.input + size_t(g.row + token) * a.value.input_stride;
+      from += (is_key ? item : item - kv_heads) * width + at;
+      next_lo.load(from);
+      next_hi.load(from + half);
     }
   };
-  load(first_head);
+  load(first);
   const int position = !active ? 0 : a.positions != nullptr ? a.positions[g.row + token] : g.position + int(token);
-  float s[E], c[E];
-  if (rotary.kind != kNone) {
-    float frequencies[E];
-    load_frequencies<V>(rotary, at, half, true, frequencies);
-    angles<V>(frequencies, position, s, c);
-  }
-  Raw<V> weight_lo, weight_hi;
-  weight_lo.clear();
-  weight_hi.clear();
-  if (h.weight != nullptr) {
-    weight_lo.load(h.weight + at);
-    weight_hi.load(h.weight + half + at);
+  // A lane's sines and cosines wait in shared memory: 64 registers a thread are all there are.
+  float4* const kept = reinterpret_cast<float4*>(stage[warp]) + lane;
+  if (kept_used) {
+    angles<V>(c, position, s, c);
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      kept[e * 8] = make_float4(s[e], s[e + 1], s[e + 2], s[e + 3]);
+      kept[(E + e) * 8] = make_float4(c[e], c[e + 1], c[e + 2], c[e + 3]);
+    }
   }
 
+  // Between an item's scales and its codes lies the next item: what the warps send one another is on its way meanwhile.
+  float done_lo[E], done_hi[E], old_scale = 0.F, asked = 0.F;
 #pragma unroll 1
-  for (uint32_t head = first_head; head < last_head; ++head) {
-    float lo[E], hi[E];
-    next_lo.unpack(lo);
-    next_hi.unpack(hi);
-    load(head + 1);
-    float* const scale_at = (is_key ? a.cache.k_scales : a.cache.v_scales) + size_t(g.page) * a.cache.kv_heads + head;
-    float old = g.slot > 0 ? *scale_at : 0.F;
-    if (!(old > 0.F && old <= 3.4028234e38F)) old = 0.F;
-    const float inverse = h.normalize ? inverse_rms<LPH, E>(lo, hi, 1.F / float(width), a.epsilon) : 1.F;
-    if (h.weight != nullptr) {
-      float w[E];
-      weight_lo.unpack(w);
+  for (uint32_t item = first; item <= last; ++item) {
+    float lo[E], hi[E], old = 0.F, scale = 0.F;
+    if (item < last) {
+      const bool is_key = item < kv_heads;
+      const uint32_t head = is_key ? item : item - kv_heads;
+      const Heads& h = is_key ? a.key : a.value;
+      next_lo.unpack(lo);
+      next_hi.unpack(hi);
+      load(item + 1);
+      if (g.slot > 0) old = (is_key ? a.cache.k_scales : a.cache.v_scales)[size_t(g.page) * kv_heads + head];
+      if (!(old > 0.F && old <= 3.4028234e38F)) old = 0.F;
+      const float inverse = h.normalize ? inverse_rms<LPH, E>(lo, hi, 1.F / float(width), a.epsilon) : 1.F;
+      if (h.weight != nullptr) {
+        Raw<V> raw;
+        float w[E];
+        raw.load(h.weight + at);
+        raw.unpack(w);
 #pragma unroll
-      for (int e = 0; e < E; ++e) lo[e] = lo[e] * inverse * w[e];
-      weight_hi.unpack(w);
+        for (int e = 0; e < E; ++e) lo[e] = lo[e] * inverse * w[e];
+        raw.load(h.weight + half + at);
+        raw.unpack(w);
 #pragma unroll
-      for (int e = 0; e < E; ++e) hi[e] = hi[e] * inverse * w[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        lo[e] *= inverse;
-        hi[e] *= inverse;
-      }
-    }
-    rotate<V>(rotary, lo, hi, s, c, position, at, half, true, stage[warp] + group * LPH * 2 * E);
-
-    float loudest = 0.F;                                   // of what is no NaN
-#pragma unroll
-    for (int e = 0; e < E; ++e) loudest = fmaxf(loudest, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
-    if (!(loudest <= 3.4028234e38F)) {
-      loudest = 0.F;
-#pragma unroll
-      for (int e = 0; e < E; ++e) loudest = fmaxf(loudest, fmaxf(finite_size(lo[e]), finite_size(hi[e])));
-    }
-    if (!active) loudest = 0.F;
-#pragma unroll
-    for (int m = 16; m; m /= 2) loudest = fmaxf(loudest, __shfl_xor_sync(0xffffffffu, loudest, m));
-    if constexpr (W > 1) {
-      float (&loudest_here)[kMostBlocks][W] = loudest_of[(head - first_head) & 1];
-      if (W == 16 && blocks > 1) {
-        if (lane < blocks) pair::store_cluster(pair::cluster_address(&loudest_here[rank][warp], lane), loudest);
-        __syncwarp();
-        pair::cluster_arrive();
-        pair::cluster_wait();
+        for (int e = 0; e < E; ++e) hi[e] = hi[e] * inverse * w[e];
       } else {
-        if (lane == 0) loudest_here[0][warp] = loudest;
-        __syncthreads();
-      }
-      loudest = 0.F;
-      for (uint32_t i = lane; i < blocks * W; i += 32) loudest = fmaxf(loudest, loudest_here[i / W][i % W]);
 #pragma unroll
-      for (int m = 16; m; m /= 2) loudest = fmaxf(loudest, __shfl_xor_sync(0xffffffffu, loudest, m));
-    } else {
-      __syncwarp();
-    }
-    const float scale = fmaxf(old, page_scale(loudest)), inverse_scale = __frcp_rn(scale);
-    if (rank == 0 && threadIdx.x == 0) *scale_at = scale;
+        for (int e = 0; e < E; ++e) {
+          lo[e] *= inverse;
+          hi[e] *= inverse;
+        }
+      }
+      if (is_key) {
+        float s[E], c[E];
+        if (kept_used) {
+#pragma unroll
+          for (int e = 0; e < E; e += 4) {
+            const float4 x = kept[e * 8], y = kept[(E + e) * 8];
+            s[e] = x.x, s[e + 1] = x.y, s[e + 2] = x.z, s[e + 3] = x.w;
+            c[e] = y.x, c[e + 1] = y.y, c[e + 2] = y.z, c[e + 3] = y.w;
+          }
+        }
+        rotate<LPH, V, WHOLE>(a.rotary, lo, hi, s, c, position, at, half, true, stage[warp] + group * LPH * 2 * E);
+      }
 
-    uint8_t* const page = static_cast<uint8_t*>(is_key ? a.cache.k_data : a.cache.v_data) +
-                          (size_t(g.page) * a.cache.kv_heads + head) * a.cache.page_tokens * width;
-    if (g.slot > 0 && scale > old) {                       // a louder token than the page had
-      const float ratio = old * inverse_scale;
-      uint4* codes = reinterpret_cast<uint4*>(page);
-#pragma unroll 4
-      for (uint32_t i = rank * 32 * W + threadIdx.x; i < uint32_t(g.slot) * width / 16; i += blocks * 32 * W) {
-        uint4 v = codes[i];
-        v = make_uint4(softer(v.x, ratio), softer(v.y, ratio), softer(v.z, ratio), softer(v.w, ratio));
-        codes[i] = v;
-      }
-    }
-    if (active) {
-      uint8_t* to = page + size_t(g.slot + token) * width + at;
+      float loudest = 0.F;                                   // of what is no NaN
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        lo[e] *= inverse_scale;
-        hi[e] *= inverse_scale;
+      for (int e = 0; e < E; ++e) loudest = fmaxf(loudest, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
+      if (!(loudest <= 3.4028234e38F)) {
+        loudest = 0.F;
+#pragma unroll
+        for (int e = 0; e < E; ++e) loudest = fmaxf(loudest, fmaxf(finite_size(lo[e]), finite_size(hi[e])));
       }
-      if constexpr (V == 1) {
-        *reinterpret_cast<uint32_t*>(to) = e4m3x4(lo[0], lo[1], lo[2], lo[3]);
-        *reinterpret_cast<uint32_t*>(to + half) = e4m3x4(hi[0], hi[1], hi[2], hi[3]);
-      } else {
-        *reinterpret_cast<uint2*>(to) = make_uint2(e4m3x4(lo[0], lo[1], lo[2], lo[3]), e4m3x4(lo[4], lo[5], lo[6], lo[7]));
-        *reinterpret_cast<uint2*>(to + half) = make_uint2(e4m3x4(hi[0], hi[1], hi[2], hi[3]), e4m3x4(hi[4], hi[5], hi[6], hi[7]));
+      if (!active) loudest = 0.F;
+      // once all warps' scales are known, all have read the old one
+      scale = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(old, page_scale(loudest)))));
+      if constexpr (W > 1) {
+        // The last warp of the block sends what all want.  A word is its own flag: no scale is 0.
+        const uint32_t i = item - first;
+        uint32_t last_one = 0, most = 0;
+        if (lane == 0) {
+          atomicMax_block(&of_block[i], __float_as_uint(scale));
+          __threadfence_block();
+          if (atomicAdd_block(&arrived[i], 1) == W - 1) {
+            last_one = 1;
+            __threadfence_block();
+            most = *const_cast<volatile uint32_t*>(&of_block[i]);
+            if (blocks == 1) *const_cast<volatile uint32_t*>(&wanted[i][0]) = most;
+          }
+        }
+        if (W == 16 && blocks > 1 && __shfl_sync(0xffffffffu, last_one, 0)) {
+          most = __shfl_sync(0xffffffffu, most, 0);
+          if (lane < blocks) store_word(pair::cluster_address(&wanted[i][rank], lane), most);
+        }
       }
     }
+    if (item > first) {
+      const uint32_t before = item - 1, head = before < kv_heads ? before : before - kv_heads;
+      const bool is_key = before < kv_heads;
+      float final_scale = asked;
+      if constexpr (W > 1)
+        final_scale = __uint_as_float(largest_of(wanted[before - first], blocks, lane));
+      const float inverse_scale = __frcp_rn(final_scale);
+      if (rank == 0 && threadIdx.x == 0) (is_key ? a.cache.k_scales : a.cache.v_scales)[size_t(g.page) * kv_heads + head] = final_scale;
+
+      uint8_t* const page = static_cast<uint8_t*>(is_key ? a.cache.k_data : a.cache.v_data) +
+                            (size_t(g.page) * kv_heads + head) * a.cache.page_tokens * width;
+      if (g.slot > 0 && final_scale > old_scale) {         // a louder token than the page had
+        const float ratio = old_scale * inverse_scale;
+        uint4* codes = reinterpret_cast<uint4*>(page);
+#pragma unroll(W == 16 ? 1 : 4)                           // registers
+        for (uint32_t i = rank * 32 * W + threadIdx.x; i < uint32_t(g.slot) * width / 16; i += blocks * 32 * W) {
+          uint4 v = codes[i];
+          v = make_uint4(softer(v.x, ratio), softer(v.y, ratio), softer(v.z, ratio), softer(v.w, ratio));
+          codes[i] = v;
+        }
+      }
+      if (active) {
+        uint8_t* to = page + size_t(g.slot + token) * width + at;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          done_lo[e] *= inverse_scale;
+          done_hi[e] *= inverse_scale;
+        }
+        if constexpr (V == 1) {
+          *reinterpret_cast<uint32_t*>(to) = e4m3x4(done_lo[0], done_lo[1], done_lo[2], done_lo[3]);
+          *reinterpret_cast<uint32_t*>(to + half) = e4m3x4(done_hi[0], done_hi[1], done_hi[2], done_hi[3]);
+        } else {
+          *reinterpret_cast<uint2*>(to) = make_uint2(e4m3x4(done_lo[0], done_lo[1], done_lo[2], done_lo[3]), e4m3x4(done_lo[4], done_lo[5], done_lo[6], done_lo[7]));
+          *reinterpret_cast<uint2*>(to + half) = make_uint2(e4m3x4(done_hi[0], done_hi[1], done_hi[2], done_hi[3]), e4m3x4(done_hi[4], done_hi[5], done_hi[6], done_hi[7]));
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      done_lo[e] = lo[e];
+      done_hi[e] = hi[e];
+    }
+    old_scale = old;
+    asked = scale;
+    __syncwarp();
+  }
+  if constexpr (W == 16) {                                 // nobody leaves while somebody may still send to it
+    pair::cluster_arrive_relaxed();
+    pair::cluster_wait();
   }
 }
 
@@ -577,29 +646,33 @@ cudaError_t launch_norm_rotary(NormRotary a, cudaStream_t stream) {
   a.tasks = (heads + a.per_task - 1) / a.per_task;
   const uint64_t tasks = uint64_t(a.rows) * a.tasks;
   if (tasks > 0xffffffffull - 64) return cudaErrorInvalidValue;
-  const auto kernel = a.width <= 64    ? qk_norm_rotary_kernel<8, 1>
-                      : a.width <= 128 ? qk_norm_rotary_kernel<16, 1>
-                      : a.width <= 256 ? qk_norm_rotary_kernel<32, 1>
-                                       : qk_norm_rotary_kernel<32, 2>;
+  const bool whole = a.rotary.kind == kWhole;
+  const auto kernel = a.width <= 64    ? (whole ? qk_norm_rotary_kernel<8, 1, true> : qk_norm_rotary_kernel<8, 1, false>)
+                      : a.width <= 128 ? (whole ? qk_norm_rotary_kernel<16, 1, true> : qk_norm_rotary_kernel<16, 1, false>)
+                      : a.width <= 256 ? (whole ? qk_norm_rotary_kernel<32, 1, true> : qk_norm_rotary_kernel<32, 1, false>)
+                                       : (whole ? qk_norm_rotary_kernel<32, 2, true> : qk_norm_rotary_kernel<32, 2, false>);
   return launch_pdl(kernel, uint32_t((tasks + kNormWarps - 1) / kNormWarps), 32 * kNormWarps, stream, a);
 }
 
-template <int LPH, int V>
+template <int LPH, int V, bool WHOLE>
 cudaError_t launch_append(Append a, cudaStream_t stream) {
   const uint32_t page = a.cache.page_tokens, most = std::min(page, a.batch.max_rows), sequences = a.batch.sequences, heads = a.cache.kv_heads;
   constexpr uint32_t kSide = 32 / LPH;
-  a.heads_each = 1;
-  if (a.batch.max_rows == 1) return launch_pdl(kv_append_kernel<LPH, V, 1>, dim3(sequences, 2 * heads), 32, stream, a);
+  a.each = 1;
+  if (a.batch.max_rows == 1) return launch_pdl(kv_append_kernel<LPH, V, 1, WHOLE>, dim3(sequences, 2 * heads), 32, stream, a);
   // a sequence of n rows touches at most 1 + (n + page - 2) / page pages
   const uint64_t bound = std::min(uint64_t(sequences) * (1 + (a.batch.max_rows + page - 2) / page),
                                   sequences + (uint64_t(a.batch.rows) + uint64_t(sequences) * (page - 2)) / page);
   uint32_t blocks = 1;
   if (most > 8 * kSide)
     while (16 * kSide * blocks < most) blocks *= 2;
-  a.heads_each = heads_each(heads, 2 * bound * blocks, 148 * 4);
-  const dim3 grid(uint32_t(bound) * blocks, 2 * ((heads + a.heads_each - 1) / a.heads_each));
-  if (most <= 4 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 4>, grid, 128, stream, a);
-  if (most <= 8 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 8>, grid, 256, stream, a);
+  // Few parts of the heads: what a block does before its first item takes 5 us.  4096 rows of 4 heads of 512 in pages of 128, 264 blocks of
+  // 512 threads for each part: 26 / 30 / 41 us with one / two / four parts; 9 sequences of up to 700 rows, 8 heads of 128 in pages of 16,
+  // 204 blocks of 256: 15 / 14 / 11 / 12 with one / two / three / six.
+  a.each = std::min<uint32_t>(kMostItems, heads_each(2 * heads, bound * blocks, most > 8 * kSide ? 148 : 148 * 4));
+  const dim3 grid(uint32_t(bound) * blocks, (2 * heads + a.each - 1) / a.each);
+  if (most <= 4 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 4, WHOLE>, grid, 128, stream, a);
+  if (most <= 8 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 8, WHOLE>, grid, 256, stream, a);
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
   config.blockDim = dim3(512);
@@ -614,7 +687,7 @@ cudaError_t launch_append(Append a, cudaStream_t stream) {
   config.attrs = attributes;
   config.numAttrs = 2;
   note_launch();
-  return cudaLaunchKernelEx(&config, kv_append_kernel<LPH, V, 16>, a);
+  return cudaLaunchKernelEx(&config, kv_append_kernel<LPH, V, 16, WHOLE>, a);
 }
 
 }  // namespace
@@ -689,7 +762,10 @@ gw_status gw_kv_cache_append(const gw_kv_cache* cache, const gw_sequences* batch
   a.epsilon = epsilon;
   const cudaStream_t s = as_stream(stream);
   if (query) GW_CUDA_CHECK(launch_norm_rotary(q, s), "cache append (queries)");
-  const auto launch = width == 128 ? &launch_append<16, 1> : width == 256 ? &launch_append<32, 1> : &launch_append<32, 2>;
+  const bool whole = a.rotary.kind == kWhole;
+  const auto launch = width == 128   ? (whole ? &launch_append<16, 1, true> : &launch_append<16, 1, false>)
+                      : width == 256 ? (whole ? &launch_append<32, 1, true> : &launch_append<32, 1, false>)
+                                     : (whole ? &launch_append<32, 2, true> : &launch_append<32, 2, false>);
   GW_CUDA_CHECK(launch(a, s), what);
   return GW_OK;
 }
