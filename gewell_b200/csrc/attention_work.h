@@ -6,6 +6,7 @@
 // ranges, one for each block; an item that a cut divides is computed in pieces and joined afterwards.
 #pragma once
 
+#include <cmath>
 #include <cstdint>
 
 #ifdef __CUDACC__
@@ -69,6 +70,12 @@ struct SequenceWork {
       if (whole > skip_low) units -= floor_sum(whole - skip_low, per_tile, uint32_t(start + skip_low * per_tile));
     }
     return units;
+  }
+  // perhaps 2^31 units or more, which the sums here cannot hold
+  GW_HOST_DEVICE bool too_many() const {
+    const float tokens = fmaxf(0.F, float(base) + float(rows)), span = float(window) + float(per_tile);
+    const float tiles = float(query_tiles()), with_tokens = fminf(tiles, tokens / float(per_tile) + 1.F);
+    return tiles + with_tokens * ((window != 0 ? fminf(span, tokens) : tokens) * (1.F / kTokens) + 3.F) >= 2147483648.F;
   }
   GW_HOST_DEVICE uint32_t units() const { return rows <= 0 ? 0 : rows <= per_tile ? 1 + token_tiles(0) : units_before(query_tiles()); }
 };

@@ -188,6 +188,8 @@ __device__ __forceinline__ SequenceWork sequence_work(const Attention& a, uint32
   return SequenceWork{r.context - r.count, r.count, int32_t(a.per_tile), int32_t(a.window)};
 }
 
+__device__ __forceinline__ uint32_t add_up(uint32_t a, uint32_t b) { return a + b < a ? UINT32_MAX : a + b; }
+
 // The block's range of units and the item that its first unit belongs to.
 template <int THREADS>
 __device__ __forceinline__ void find_start(const Attention& a, Shared& shared) {
@@ -202,12 +204,17 @@ __device__ __forceinline__ void find_start(const Attention& a, Shared& shared) {
 #pragma unroll 1
   for (uint32_t base = 0, round = 0; round < 2; ) {
     const uint32_t s = base + threadIdx.x;
-    const uint32_t each = s < a.batch.sequences ? sequence_work(a, s, round == 0 && blockIdx.x == 0).units() : 0, mine = each * a.cache.kv_heads;
+    uint32_t each = 0, mine = 0;                               // 2^32 - 1: that many or more, here and in sums
+    if (s < a.batch.sequences) {
+      const SequenceWork w = sequence_work(a, s, round == 0 && blockIdx.x == 0);
+      each = w.too_many() ? UINT32_MAX : w.units();
+      mine = __umulhi(each, a.cache.kv_heads) != 0 ? UINT32_MAX : each * a.cache.kv_heads;
+    }
     uint32_t sum = mine;
 #pragma unroll
     for (int m = 1; m < 32; m *= 2) {
       const uint32_t other = __shfl_up_sync(0xffffffffu, sum, m);
-      if (lane >= uint32_t(m)) sum += other;
+      if (lane >= uint32_t(m)) sum = add_up(sum, other);
     }
     if (lane == 31) sums[warp] = sum;
     __syncthreads();
@@ -215,12 +222,16 @@ __device__ __forceinline__ void find_start(const Attention& a, Shared& shared) {
 #pragma unroll 1
     for (int i = 0; i < WARPS; ++i) {
       if (uint32_t(i) < warp) low += sums[i];
-      before += sums[i];
+      before = add_up(before, sums[i]);
     }
     __syncthreads();
     base += THREADS;
     const bool end = base >= a.batch.sequences;
     if (round == 0 && end) {
+      if (before > uint32_t(INT32_MAX)) {                      // nothing is computed
+        if (blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(&g_attention_error, 0u, 0xa2ffffffu);
+        before = 0;
+      }
       const uint32_t parts = min(before, gridDim.x);
       idle = blockIdx.x >= parts;
       uint32_t to = from = before;
@@ -415,7 +426,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
   uint8_t* const probs_atom = ones_atom + kAtomBytes;
   float* const reference = reinterpret_cast<float*>(probs_atom + 2 * kAtomBytes); // [N] m of a column
   float* const factor = reference + N;                                            // [N]
-  int* const settled = reinterpret_cast<int*>(factor + N);                        // [N] the reference holds: some token lies above 2^-40
+  int* const settled = reinterpret_cast<int*>(factor + N);                        // [N] tile that set the reference: some token above 2^-40
   float* const by_warp = factor + 2 * N;                                          // [4][N]
   float* const spread = by_warp + 4 * N;                                        // [softmax warps][32]
   bf16** const output_at = reinterpret_cast<bf16**>(spread + 32 * kSoftmaxWarps); // [N]
@@ -855,7 +866,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         const uint32_t at = member * a.group_inverse >> 16;
         output_at[member] = a.output + size_t(m.first_row + at) * a.output_stride + size_t(m.head * group + member - at * group) * D;
         reference[member] = 0.F;
-        settled[member] = int(member) >= m.used;
+        settled[member] = int(member) >= m.used ? -1 : INT32_MAX;
       }
       together();
       if (m.tiles == 0) {                                        // rows that see nothing
@@ -919,9 +930,10 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
           if (!moved && lane < uint32_t(C)) {
             const uint32_t column = column0 + lane;
             ask = largest > kHighBits;                           // NaN too
-            if (!settled[column] && seen_low <= int(column) && int(column) < seen_high) {
+            // what other warps find in the same tile does not count: the answer is the same whoever comes first
+            if (settled[column] >= tile_count && seen_low <= int(column) && int(column) < seen_high) {
               if (largest < kLowBits) ask = true;
-              else settled[column] = 1;
+              else settled[column] = tile_count;
             }
             if (ask) s.move[tile_count & 3] = 1;
           }
@@ -979,11 +991,11 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
             const float highest = fmaxf(fmaxf(by_warp[member], by_warp[N + member]), fmaxf(by_warp[2 * N + member], by_warp[3 * N + member]));
             const float before = reference[member];
             // A column that has not settled has had no token before this tile, and one that sees none here keeps its reference.
-            const bool had = settled[member] != 0, has = highest != -INFINITY;
+            const bool had = settled[member] <= tile_count, has = highest != -INFINITY;
             const float now = !has ? before : had ? fmaxf(before, highest) : highest;
             reference[member] = now;
             factor[member] = !has ? 1.F : had ? exp2_approx(before - now) : 0.F;
-            settled[member] = had || has;
+            if (!had && has) settled[member] = tile_count;
           }
           together();
 #pragma unroll

@@ -215,6 +215,21 @@ def test_bad_pages_are_left_out(gw):
     assert (np.abs(f64(got[:1]) - exact) <= 2.0 ** -7 * (np.abs(exact) + size)).all()
 
 
+def test_more_work_than_can_be_counted_is_left_out(gw):
+    """40 sequences of 2^30 tokens by their lengths (the table has a page each): 2^31 tiles and more over 8 heads."""
+    batch = Batch([(1, 100)] * 40, 128, 29)
+    host = random_cache(batch, 8, 128, 30)
+    q = queries(40, 8, 128, 31)
+    long = batch.device(gw)
+    y = torch.full_like(q, 7.0)
+    long.context_lengths.fill_(2 ** 30)
+    gw.paged_attention(to_device(gw, host), long, q, 0.1, y=y)
+    assert gw.kernel_error() == 0xa2ffffff and (y == 7.0).all()
+    long.context_lengths.fill_(2 ** 30 + 1)
+    gw.paged_attention(to_device(gw, host), long, q, 0.1, y=y)
+    assert gw.kernel_error() >> 24 == 0xa2 and (y == 7.0).all()
+
+
 def test_captured_replayed_with_other_lengths_and_beside_another(gw):
     """One graph serves later steps: lengths and pages are read on the device.  Two graphs with scratch of their own run at once."""
     steps = [[(1, 40), (1, 700), (1, 3)], [(1, 41), (1, 1900), (1, 300)], [(1, 1), (1, 2), (0, 0)]]
