@@ -9,9 +9,9 @@
 //   y_i = n_i cos a - n_j sin a,  y_j = n_j cos a + n_i sin a,  a = position * f,  n = x * rsqrt(mean(x^2) + eps) * w
 //
 // The angle in turns, position * (f / 2 pi), is formed as the sum of two FP32 numbers, exact to 2^-28 up to position 2^24 (in 64
-// bits beyond), and reduced to [-1/2, 1/2]: in 32 bits position 250000 at f = 1 would be off by 0.01 rad.  What is left goes to the
-// hardware's sine and cosine (absolute error 2^-21, against BF16's 2^-9 and E4M3's 2^-4 at the end); everything else is FP32 and is
-// rounded once.
+// bits beyond), and reduced to [-1/2, 1/2], again as two numbers: in 32 bits position 250000 at f = 1 would be off by 0.01 rad.  Its
+// sine and cosine are FP32-exact; the hardware's, 2^-21 off, would let a key in ten thousand fall to the next code of E4M3.  They are
+// computed once for all heads that a warp or block takes.  Everything else is FP32 and is rounded once.
 #include <algorithm>
 #include <string>
 
@@ -90,29 +90,48 @@ constexpr double kTurn = 0.15915494309189535;       // 1 / 2 pi
 constexpr int kNear = 1 << 24;
 
 __device__ __forceinline__ bool is_near(int position) { return uint32_t(position + kNear) <= 2u * kNear; }
-__device__ __forceinline__ float near_turns(float frequency, float position) {
+// turns as the sum of two numbers
+__device__ __forceinline__ float2 near_turns(float frequency, float position) {
   constexpr float high = float(kTurn), low = float(kTurn - double(high));
   const float f = frequency * high, f_rest = fmaf(frequency, low, fmaf(frequency, high, -f));        // turns per position
-  const float whole = position * f;
-  return (whole - rintf(whole)) + fmaf(position, f_rest, fmaf(position, f, -whole));
+  const float whole = position * f, part = whole - rintf(whole), rest = fmaf(position, f_rest, fmaf(position, f, -whole));
+  const float sum = part + rest, of_rest = sum - part;
+  return make_float2(sum, (part - (sum - of_rest)) + (rest - of_rest));
 }
-__device__ __forceinline__ float far_turns(float frequency, int position) {
-  const double turns = double(frequency) * kTurn * double(position);
-  return float(turns - rint(turns));
+__device__ __forceinline__ float2 far_turns(float frequency, int position) {
+  double turns = double(frequency) * kTurn * double(position);
+  turns -= rint(turns);
+  const float sum = float(turns);
+  return make_float2(sum, float(turns - double(sum)));
 }
-__device__ __forceinline__ void sine_cosine(float turns, float& s, float& c) { __sincosf(turns * 6.283185307179586F, &s, &c); }
+__device__ __forceinline__ void sine_cosine(float2 turns, float& s, float& c) {
+  float sine, cosine;
+  sincospif(2.F * turns.x, &sine, &cosine);
+  const float more = turns.y * 6.283185307179586F;
+  s = fmaf(more, cosine, sine);
+  c = fmaf(-more, sine, cosine);
+}
 
 template <int V>
 __device__ __forceinline__ void angles(const float* frequencies, int position, float* s, float* c) {
   constexpr int E = 4 * V;
+  if (is_near(position)) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) s[e] = near_turns(frequencies[e], float(position));
-  if (!is_near(position)) {
+    for (int e = 0; e < E; ++e) {
+      const float2 turns = near_turns(frequencies[e], float(position));
+      s[e] = turns.x;
+      c[e] = turns.y;
+    }
+  } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) s[e] = far_turns(frequencies[e], position);
+    for (int e = 0; e < E; ++e) {
+      const float2 turns = far_turns(frequencies[e], position);
+      s[e] = turns.x;
+      c[e] = turns.y;
+    }
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e) sine_cosine(s[e], s[e], c[e]);
+  for (int e = 0; e < E; ++e) sine_cosine(make_float2(s[e], c[e]), s[e], c[e]);
 }
 
 __device__ __forceinline__ void turn(float& a, float& b, float s, float c) {
