@@ -23,7 +23,8 @@
 //   warps 1, 3  one thread each issues tcgen05.mma: S of the tiles, as far ahead as there is room, and O += P V.  One thread for
 //               both spent half of its time in barriers, with nothing left in the tensor pipe's queue.
 //   warp 2      zeroes rows of V that no query may see: a page's slots behind its last token may hold anything, NaN included, and
-//               0 * NaN is NaN
+//               0 * NaN is NaN.  In rows that some queries see and others do not it zeroes what is NaN; the softmax warps write NaN to
+//               the results of those that see it.
 //   warps 4..   softmax: for every 32 lanes two warps (four at 64 columns), each with its share of the columns.  After an item's last
 //               tile they bring the next item's queries to shared memory, so that its first scores are computed while they write the
 //               results of the one before.
@@ -58,6 +59,7 @@ constexpr int kChunkBytes = kTokens * 128;
 constexpr int kAtomBytes = 512;              // scale atom: 128 rows x 4 blocks of 32 elements
 constexpr uint32_t kHighBits = (127u + 40u) << 23, kLowBits = (127u - 40u) << 23;
 constexpr int kItems = 4;                    // items that the walk is ahead at most
+constexpr int kNans = 32;                    // places with NaN that are kept for an item
 constexpr int kScaleTiles = 16;              // tiles whose scales are kept: more than the ring and the score buffers can hold
 
 struct Attention {
@@ -76,7 +78,7 @@ struct Attention {
 // A piece of an item, as the producer tells the other warps; tiles of -1 end them.
 struct Item {
   int begin, end, tiles, first_tile;           // token tiles of the piece, of the item; where the item's begin in the sequence
-  int low, high;                               // the tokens that it reads
+  int low, high, all_low, all_high;            // the tokens that it reads, and those that all of its queries see
   int used, token_rows, first_row, position0;  // columns with a query, query rows, the first one, its position
   int head, whole;
 };
@@ -86,6 +88,9 @@ struct Shared {
   uint64_t scores_full[2], scores_empty[2], probs_full[2], probs_empty[2], checked, query_full, sums_full, softmax, drained, drained_sums;
   float2 scales[kScaleTiles][8];               // {key, value} of a tile's pages; a value scale below 0: no page
   Item items[kItems];
+  // NaN among the values that not every query of an item sees: {token, dimension / 16 << 16 | which of the 16}
+  uint2 nans[kItems][kNans];
+  int nan_count[kItems], nan_from[kItems];     // all found; the first token of those that did not fit
   int move[4];                                 // of the last tiles: some warp asks for the reference to be moved
   uint32_t tensor_memory;
   // units of all blocks, the block's range of them, and the item that has the first
@@ -108,7 +113,7 @@ struct Layout {
   static constexpr int kFloats = 7 * N + 32 * kSoftmaxWarps;      // as laid out in the kernel
   static constexpr int kSmall = kAtoms * kAtomBytes + kFloats * 4 + 8 * N;
   static constexpr int kAlignment = 1024;
-  static constexpr int kStatic = 3072;                            // at least what is declared in the kernel
+  static constexpr int kStatic = 4096;                            // at least what is declared in the kernel
   static constexpr int kRoom = 227 * 1024 - kStatic - kAlignment - 2 * kQueryBytes - kProbBytes - kSmall;
   static constexpr int kRings = kRoom / kChunkBytes > 16 ? 16 : kRoom / kChunkBytes;          // chunks
   static constexpr int kKeyRing = (kRings + 1) / 2, kValueRing = kRings / 2;
@@ -314,10 +319,18 @@ __device__ __forceinline__ void two_parts(float a, float b, uint16_t& hi, uint16
 }
 
 // whether a token tile has tokens outside [low, high)
-__device__ __forceinline__ bool needs_clearing(int token_tile, int low, int high) {
+__device__ __forceinline__ bool has_others(int token_tile, int low, int high) {
   const int start = token_tile * kTokens;
   return low > start || high < start + kTokens;
 }
+
+// 0xff in the bytes that are NaN in E4M3
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {
+  const uint32_t high = ((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  return (high >> 7) * 255u;
+}
+// a bit for each byte of 0xff
+__device__ __forceinline__ uint32_t one_bits(uint32_t bytes) { return (bytes & 1) | (bytes >> 7 & 2) | (bytes >> 14 & 4) | (bytes >> 21 & 8); }
 
 // matrix descriptor of rows of 128 bytes, 128-byte swizzle, read across the rows: 8 rows of the sum are 1024 bytes apart
 __device__ __forceinline__ uint64_t across_desc(uint32_t address) { return ptx::smem_desc_sw128(address) | uint64_t(1024 >> 4) << 16; }
@@ -499,6 +512,8 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       if (lane == 0) {
         Item& m = s.items[n % kItems];
         m.tiles = -1;                                            // the end
+        s.nan_count[n % kItems] = 0;
+        s.nan_from[n % kItems] = INT32_MAX;
         if (more) {
           m.begin = w.begin;
           m.end = w.end;
@@ -506,10 +521,12 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
           m.first_tile = w.work.first_token_tile(w.tile);
           m.low = w.work.low(w.tile);
           m.high = w.work.high(w.tile);
+          m.position0 = w.work.base + w.tile * int(a.per_tile);
           m.token_rows = min(int(a.per_tile), w.rows.count - w.tile * int(a.per_tile));
           m.used = m.token_rows * int(a.group);
           m.first_row = w.rows.first + w.tile * int(a.per_tile);
-          m.position0 = w.work.base + w.tile * int(a.per_tile);
+          m.all_low = a.window ? max(0, m.position0 + m.token_rows - int(a.window)) : 0;
+          m.all_high = max(0, m.position0 + 1);
           m.head = w.head;
           m.whole = w.begin == 0 && w.end == w.tiles;
           if (w.begin == 0 && w.end < w.tiles)
@@ -645,14 +662,14 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
 #pragma unroll 1
       for (int n = 0; wait(&s.items_full[n % kItems], n / kItems & 1, 0xb2000000u); ++n) {
         const Item& m = s.items[n % kItems];
-        const int begin = m.begin, end = m.end, tiles = m.tiles, first_tile = m.first_tile, low = m.low, high = m.high;
+        const int begin = m.begin, end = m.end, tiles = m.tiles, first_tile = m.first_tile, all_low = m.all_low, all_high = m.all_high;
         ptx::mbar_arrive(&s.items_empty[n % kItems]);
         if (tiles < 0) break;
         if (tiles == 0) continue;
 #pragma unroll 1
         for (int t = begin; t < end; ++t) {
           // once the chunk is there, the warp that zeroes has finished with what was in its place before
-          const bool clear = needs_clearing(first_tile + t, low, high);
+          const bool clear = has_others(first_tile + t, all_low, all_high);
           const auto ready = [&]() {
             wait(&s.v_full[slot], parity, 0xa5100000u | slot);
             return clear ? wait(&s.v_cleared[slot], parity, 0xaf000000u | slot) : error == 0;
@@ -694,7 +711,8 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
     }
     __syncwarp();
   } else if (warp == 2) {
-    // ----- rows of V that no query of an item sees; every chunk is waited for, so that this warp is never a lap of the ring away
+    // ----- V where not every query of an item sees it: rows that none sees are zeroed, and so are NaN in the others, whose places
+    // are kept for those queries that do see them.  Every chunk is waited for, so that this warp is never a lap of the ring away.
     int slot = 0;
     uint32_t parity = 0;
 #pragma unroll 1
@@ -703,9 +721,8 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       error = __reduce_max_sync(0xffffffffu, error);
       if (error) break;
       const Item& m = s.items[n % kItems];
-      const int begin = m.begin, end = m.end, tiles = m.tiles, first_tile = m.first_tile, low = m.low, high = m.high;
+      const int begin = m.begin, end = m.end, tiles = m.tiles, first_tile = m.first_tile, low = m.low, high = m.high, all_low = m.all_low, all_high = m.all_high;
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&s.items_empty[n % kItems]);
       if (tiles < 0) break;
 #pragma unroll 1
       for (int i = 0; i < CH * (end - begin); ++i) {
@@ -713,11 +730,30 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         wait(&s.v_full[slot], parity, 0xa9000000u | slot);
         error = __reduce_max_sync(0xffffffffu, error);
         if (error) break;
-        if (needs_clearing(tile, low, high)) {
+        if (has_others(tile, all_low, all_high)) {
+          // rows of the tile: none sees them up to `first` and from `last` on, all between `all_first` and `all_last`
           uint4* rows = reinterpret_cast<uint4*>(v_ring + slot * kChunkBytes);
+          const int first = min(max(low - start, 0), kTokens), last = min(max(high - start, first), kTokens);
+          const int all_first = min(max(all_low - start, first), last), all_last = min(max(all_high - start, all_first), last);
 #pragma unroll 1
-          for (int k = lane; k < kTokens * 8; k += 32)
-            if (start + k / 8 < low || start + k / 8 >= high) rows[k] = make_uint4(0, 0, 0, 0);
+          for (int k = lane; k < first * 8; k += 32) rows[k] = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+          for (int k = last * 8 + lane; k < kTokens * 8; k += 32) rows[k] = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+          for (int k = first * 8 + lane; k < (last - (all_last - all_first)) * 8; k += 32) {
+            const int unit = k < all_first * 8 ? k : k + (all_last - all_first) * 8;
+            const uint4 codes = rows[unit];
+            const uint4 nan = make_uint4(nan_bytes(codes.x), nan_bytes(codes.y), nan_bytes(codes.z), nan_bytes(codes.w));
+            if ((nan.x | nan.y | nan.z | nan.w) != 0) {
+              rows[unit] = make_uint4(codes.x & ~nan.x, codes.y & ~nan.y, codes.z & ~nan.z, codes.w & ~nan.w);
+              const int at = atomicAdd_block(&s.nan_count[n % kItems], 1), place = (unit % 8) ^ (unit / 8 % 8);       // 128-byte swizzle
+              if (at < kNans)
+                s.nans[n % kItems][at] = make_uint2(start + unit / 8, uint32_t(i % CH * 8 + place) << 16 | one_bits(nan.x) | one_bits(nan.y) << 4 |
+                                                                   one_bits(nan.z) << 8 | one_bits(nan.w) << 12);
+              else
+                atomicMin_block(&s.nan_from[n % kItems], start + unit / 8);
+            }
+          }
           ptx::fence_proxy_async_smem();
           __syncwarp();
         }
@@ -730,6 +766,8 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
           parity ^= 1;
         }
       }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&s.items_empty[n % kItems]);
       if (error) break;
     }
   } else {
@@ -852,6 +890,29 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
             }
           }
           ++scored_items;
+          const int nans = s.nan_count[n % kItems];
+          if (nans != 0) {                                       // to the queries that see them
+            together();                                          // behind what was written above
+            const int listed = min(nans, kNans), from = s.nan_from[n % kItems];
+#pragma unroll 1
+            for (int column = warp - kFirstSoftmaxWarp; column < used; column += kSoftmaxWarps) {
+              const int position = m.position0 + int(column * a.group_inverse >> 16);
+              bf16* const to = output_at[column];
+              float* const to_partial = a.partial + (size_t(place) * N + column) * D;
+              const auto spoil = [&](int d) {
+                if (whole) to[d] = __float2bfloat16_rn(__int_as_float(0x7fc00000));
+                else to_partial[d] = __int_as_float(0x7fc00000);
+              };
+#pragma unroll 1
+              for (int i = 0; i < listed; ++i) {
+                const uint2 at = s.nans[n % kItems][i];
+                const bool seen = int(at.x) <= position && (a.window == 0 || position - int(at.x) < int(a.window));
+                if (seen && lane < 16 && (at.y >> lane & 1)) spoil(int(at.y >> 16) * 16 + lane);
+              }
+              if (from <= position)
+                for (int d = lane; d < D; d += 32) spoil(d);
+            }
+          }
         }
         // The sums were read: the next item's first product may overwrite them once it has the probabilities that this thread
         // publishes later.  What the item had in shared memory is free.

@@ -880,9 +880,13 @@ def paged_attention(cache: KvCache, batch: SequenceBatch, query: torch.Tensor, s
     if batch.device_index != device or dim != cache.head_dim or rows < batch.rows:
         raise _lib.GewellInvalidArgument("queries have the cache's head width and the batch's rows; all lie on one device")
     y, out_stride = _output(query, rows, heads, dim, y, device)
+    if window < 0:
+        raise _lib.GewellInvalidArgument("a window of 0 (all tokens) or more is wanted")
     lib = _library()
     if scratch is None:
         scratch = torch.empty(lib.gw_paged_attention_scratch_bytes(cache._ref, batch._ref, heads), dtype=torch.uint8, device=query.device)
+        if stream is not None:                        # not to be taken by the current stream's next tensors before that stream is done
+            scratch.record_stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream)))
     elif scratch.dtype is not torch.uint8 or scratch.get_device() != device or not scratch.is_contiguous():
         raise _lib.GewellInvalidArgument("scratch is contiguous uint8 on the cache's device")
     _check(lib.gw_paged_attention_bf16(cache._ref, batch._ref, query.data_ptr(), stride, heads, scale, window, y.data_ptr(), out_stride,

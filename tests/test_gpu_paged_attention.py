@@ -215,6 +215,48 @@ def test_bad_pages_are_left_out(gw):
     assert (np.abs(f64(got[:1]) - exact) <= 2.0 ** -7 * (np.abs(exact) + size)).all()
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(4, 2, 128, 16), (16, 2, 512, 64), (8, 8, 256, 128)])
+@pytest.mark.parametrize("sequences,window", [([(5, 90)], 0), ([(3, 400), (6, 33), (2, 2)], 20), ([(200, 300)], 0), ([(150, 700), (64, 64)], 100),
+                                              ([(4, 9000)], 0)])
+def test_nan_values_reach_the_queries_that_see_them_and_no_others(gw, heads, kv_heads, dim, page, sequences, window):
+    """One or several elements of a token, among the step's own tokens and before them."""
+    batch = Batch(sequences, page, 40)
+    host = random_cache(batch, kv_heads, dim, 41)
+    rng = np.random.default_rng(42)
+    codes = host[1][0]
+    for s, (n, length) in enumerate(sequences):
+        for token in {length - 1, length - n // 2 - 1, max(0, length - n - 3), max(0, length - 2)}:
+            at = codes[int(batch.table[s, token // page]), int(rng.integers(kv_heads)), token % page]
+            at[rng.choice(dim, int(rng.choice([1, 3, 10])), replace=False)] = rng.choice([0x7f, 0xff])
+    q = queries(batch.rows, heads, dim, 43)
+    got = f64(gw.paged_attention(to_device(gw, host), batch.device(gw), q, dim ** -0.5, window=window))
+    assert gw.kernel_error() == 0
+    seen_any = False
+    for s, (n, length) in enumerate(sequences):
+        k, v = (sequence_values(batch, c, s) for c in host)
+        low = int(batch.row_offsets[s])
+        for i in sorted({0, n // 2 - 1, n // 2, n - 2, n - 1, n // 3} & set(range(n))):
+            exact, size = oat.attention(f64(q[low + i:low + i + 1]), k, v, dim ** -0.5, length - n + i, window)
+            nan = np.isnan(exact)
+            seen_any |= bool(nan.any()) and not nan.all()
+            assert (np.isnan(got[low + i:low + i + 1]) == nan).all(), f"sequence {s} row {i}"
+            error = np.abs(got[low + i:low + i + 1] - exact)
+            assert (error[~nan] <= (2.0 ** -7 * (np.abs(exact) + size))[~nan]).all()
+    assert seen_any
+
+
+def test_many_nan_values(gw):
+    """More places than are kept: rows in front of the first of them are as they were, rows behind the last are NaN."""
+    batch = Batch([(60, 200)], 16, 44)
+    host = random_cache(batch, 1, 256, 45)
+    for token in range(170, 180):
+        host[1][0][int(batch.table[0, token // 16]), 0, token % 16] = 0x7f
+    q = queries(60, 4, 256, 46)
+    got = f64(gw.paged_attention(to_device(gw, host), batch.device(gw), q, 256 ** -0.5))
+    assert gw.kernel_error() == 0
+    assert not np.isnan(got[:30]).any() and np.isnan(got[30:]).all()
+
+
 def test_more_work_than_can_be_counted_is_left_out(gw):
     """40 sequences of 2^30 tokens by their lengths (the table has a page each): 2^31 tiles and more over 8 heads."""
     batch = Batch([(1, 100)] * 40, 128, 29)
@@ -228,6 +270,35 @@ def test_more_work_than_can_be_counted_is_left_out(gw):
     long.context_lengths.fill_(2 ** 30 + 1)
     gw.paged_attention(to_device(gw, host), long, q, 0.1, y=y)
     assert gw.kernel_error() >> 24 == 0xa2 and (y == 7.0).all()
+
+
+def test_refusals_of_the_wrapper(gw):
+    batch = Batch([(2, 40)], 16, 50)
+    cache = to_device(gw, random_cache(batch, 2, 128, 51))
+    held, q = batch.device(gw), queries(2, 4, 128, 52)
+    strided = torch.zeros((2, 8, 128), dtype=torch.bfloat16).cuda()[:, ::2]
+    for bad in (dict(window=-1), dict(scale=float("nan")), dict(query=q.float()), dict(query=q[:1]), dict(query=strided), dict(query=q.cpu()),
+                dict(y=torch.empty((2, 4, 64), dtype=torch.bfloat16).cuda()), dict(y=q.cpu()), dict(query=queries(2, 3, 128, 1)),
+                dict(query=queries(2, 4, 256, 1)), dict(scratch=torch.empty(16, dtype=torch.uint8).cuda()),
+                dict(scratch=torch.empty(1 << 22, dtype=torch.int8).cuda())):
+        with pytest.raises(gw.GewellInvalidArgument):
+            gw.paged_attention(cache, held, **{**dict(query=q, scale=0.1), **bad})
+
+
+def test_on_another_stream(gw):
+    """Scratch that the call allocates is not handed out again while the other stream still uses it."""
+    batch = Batch([(1, 4000)] * 4, 64, 53)
+    host = random_cache(batch, 2, 256, 54)
+    cache, held, q = to_device(gw, host), batch.device(gw), queries(4, 16, 256, 55)
+    plain = gw.paged_attention(cache, held, q, 0.06)
+    torch.cuda.synchronize()
+    for stream in (torch.cuda.Stream(), torch.cuda.Stream().cuda_stream):
+        results = []
+        for _ in range(6):
+            results.append(gw.paged_attention(cache, held, q, 0.06, stream=stream, y=torch.empty_like(q)))
+            torch.full((1 << 22,), 255, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        assert all(torch.equal(r, plain) for r in results)
 
 
 def test_captured_replayed_with_other_lengths_and_beside_another(gw):
