@@ -75,6 +75,20 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
+// As above, with a hint that the thread may sleep for a microsecond at a time, so that it leaves the issue slots to others.
+__device__ __forceinline__ bool mbar_wait_suspended(uint64_t* bar, uint32_t parity, uint64_t limit_ns = 2000000000ull) {
+  uint64_t start = 0;
+  while (true) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(smem_u32(bar)), "r"(parity), "r"(1000u) : "memory");
+    if (done) return true;
+    const uint64_t now = global_timer_ns();
+    if (start == 0) start = now;
+    if (now - start > limit_ns) return false;
+  }
+}
+
 // Warp-level wait: one lane polls (backing off with nanosleep between polls so
 // that waiting warps leave the issue slots and the barrier unit to the warps
 // that are doing work), the outcome is broadcast.  All 32 lanes must call it.
