@@ -221,7 +221,8 @@ __device__ __forceinline__ bool position_in_batch(const gw_sequences& b, uint32_
 constexpr int kNormWarps = 4;
 
 // A warp takes heads of one row, queries and keys in one line, the next head's values on their way meanwhile; the row's angles are
-// computed once.
+// computed once.  Bound by HBM: 4096 rows of 18 heads of 512, 151 MB, 30 us (77% of a copy's rate; 28 with the hardware's sines).
+// With a task for each head, and angles in 64 bits, it took 74 us; eight rows, 2 us in a graph.
 template <int LPH, int V, bool WHOLE>
 __global__ void __launch_bounds__(32 * kNormWarps, V == 1 ? 8 : 6) qk_norm_rotary_kernel(NormRotary a) {
   constexpr int E = 4 * V, kSide = 32 / LPH;
@@ -432,8 +433,12 @@ __device__ __forceinline__ uint32_t largest_of(const uint32_t* words, uint32_t c
 constexpr int kMostItems = 16;         // of a block
 
 // A cluster of one to eight blocks takes the call's tokens of one page, a token at a time for LPH lanes, for a few KV heads one
-// after the other: the angles are computed once, the next head's values are on their way while a head is rounded.  Of every head
-// each warp sends all blocks the scale that its tokens and the page's codes want; the largest is the page's.
+// after the other (items: first the heads' keys, then their values): the angles are computed once, the next item's values are on their way
+// while an item is normed, and its codes are written while the next one's are.  For every item the last warp of a block sends all
+// blocks the scale that the block's tokens and the page's codes want; the largest is the page's.
+// Bound by issue and by that chain: 4096 rows of 4 heads of 512 in pages of 128, 50 MB, 27 us in a graph (1.9 TB/s), 5 us of it until the
+// first item is loaded; one row of each of 64 sequences, 16 heads of 256, 3.4 us; 12 us for 9 sequences of up to 700 rows, 8 heads of 128.
+// A block for a page, with the tokens of a page in eight rounds and everything computed twice, took 33.6 us for the first.
 template <int LPH, int V, int W, bool WHOLE>
 __global__ void __launch_bounds__(32 * W, (V == 1 || W == 16 ? 32 : 20) / W) kv_append_kernel(Append a) {
   constexpr int E = 4 * V, kSide = 32 / LPH;
@@ -661,7 +666,9 @@ uint32_t heads_each(uint32_t count, uint64_t units, uint64_t wanted) {
 
 cudaError_t launch_norm_rotary(NormRotary a, cudaStream_t stream) {
   const uint32_t lanes = a.width <= 64 ? 8 : a.width <= 128 ? 16 : 32, side = 32 / lanes, heads = a.query.heads + a.key.heads;
-  a.per_task = side * heads_each((heads + side - 1) / side, a.rows, 148 * 48);
+  // Warps for 24 to an SM, then more heads a warp.  4096 rows of 18 heads of 512: 28 / 29 / 32 us with one / two / four warps a row; 1025 rows
+  // of 32 heads of 128: 8.7 / 7.0 / 7.3 us with three / five / seven.
+  a.per_task = side * heads_each((heads + side - 1) / side, a.rows, 148 * 24);
   a.tasks = (heads + a.per_task - 1) / a.per_task;
   const uint64_t tasks = uint64_t(a.rows) * a.tasks;
   if (tasks > 0xffffffffull - 64) return cudaErrorInvalidValue;

@@ -37,6 +37,13 @@
 // A thread waits on a barrier for every phase of it, or for none: with one ring for K and V the thread of S could ask for a phase
 // while the one before, of V, was still open, and a parity cannot tell that from the phase being complete.
 // Every wait is bounded; a role that gives up reports it, all leave, and tensor memory is released.
+//
+// Measured (a call, join included).  24 rows on up to 32,000 tokens, 4 KV heads of 512: 264 us, the rate of a copy from HBM.  One row on
+// 32,749 tokens, 2 heads of 512: 27 us against 10 us of HBM, most of it the first tile's way and the second launch.  64 rows in windows of 1024,
+// 16 heads of 256: 106 us against 81.  Drafts and prompts are bound by the softmax warps, 2400 cycles a tile at 32 columns, 3400 to 4100
+// at 64 (about 400 instructions a warp; their chain of latencies, four warps a scheduler, does not fill the issue slots): 80 rows on up to 9000
+// tokens, 8 heads of 128, 64 us; 2048 rows in windows of 1024, 8 heads of 256, 104 us; 4096 rows on 16,384 tokens, 2 heads of 512, 2184 us,
+// 880 TFLOP/s, where the 64 products of a tile also read 393 KB of shared memory, 3100 cycles.
 #include <algorithm>
 #include <string>
 
@@ -1106,7 +1113,8 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
 }
 
 // Joins the pieces of the items that are divided between blocks: block x looks after the item that block x of the attention kernel
-// begins and does not end.  WPC warps share a column, each with every WPC-th piece.
+// begins and does not end.  WPC warps share a column, each with every WPC-th piece: eight where a block has few columns, so that the pieces'
+// latencies overlap.  Bound by latency: 3 to 5 us, 74 pieces of 8 columns of 512 or one or two of 64.
 template <int D, int WPC>
 __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_constant__ Attention a, uint32_t blocks, uint32_t columns) {
   constexpr int E = D / 32;

@@ -390,7 +390,7 @@ typedef struct gw_kv_cache {
  * of the sequence with the most.  A position below 0 (a context shorter than its rows, as batches are padded) is no token: nothing
  * is appended for it, and it sees nothing.  Offsets outside 0 .. rows, sequences of more than max_rows rows or 2^30 tokens, positions
  * behind the page table and page numbers outside the cache are not followed: those tokens are left out and gw_debug_kernel_error() reports
- * 0xa....... . */
+ * 0xa1...... (a page) or 0xa2...... (a sequence; 0xa2ffffff: a step of attention of 2^31 tiles of 128 tokens or more, which is not begun). */
 typedef struct gw_sequences {
   const int32_t* row_offsets;     /* [sequences + 1] */
   const int32_t* context_lengths; /* [sequences] */
