@@ -955,9 +955,10 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         const int ahead = (m.first_tile + t) * kTokens + int(row) - m.position0;       // of the lane's token, to the first query
         wait(&s.scales_full[entry], tile_count / kScaleTiles & 1, 0xac000000u);
         const float2 scales = s.scales[entry][row >> a.page_shift];
-        // The columns that see the lane's token: query row i where ahead <= i < ahead + window.  Most tiles are open: seen from every column.
+        // The columns that see the lane's token: query row i where ahead <= i < ahead + window.  Most tiles are open: seen from every
+        // column with a query (the others' queries are zeros, and nobody reads what becomes of them).
         const int tile_ahead = ahead - int(row);
-        const bool open = __all_sync(0xffffffffu, scales.y >= 0.F) && used == N && tile_ahead + kTokens <= 1 &&
+        const bool open = __all_sync(0xffffffffu, scales.y >= 0.F) && tile_ahead + kTokens <= 1 &&
                           (a.window == 0 || tile_ahead + int(a.window) >= token_rows);
         uint32_t seen_from = 0, seen_span = N;                   // column0 + j - from < span, unsigned
         int seen_low = 0, seen_high = N;                         // columns that may see any of the warp's tokens
@@ -983,68 +984,72 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         // stays: a move scales what is in the sums.
 #pragma unroll 1
         for (bool moved = false;; moved = true) {
-          float p[C];
-          tmem_load_columns<C>(scores, reinterpret_cast<uint32_t*>(p));
-          ptx::tmem_load_wait();
-          uint32_t bits[C];
+          if (int(column0) < used) {
+            float p[C];
+            tmem_load_columns<C>(scores, reinterpret_cast<uint32_t*>(p));
+            ptx::tmem_load_wait();
+            uint32_t bits[C];
 #pragma unroll
-          for (int j = 0; j < C; ++j) {
-            p[j] = exp2_approx(fmaf(p[j], scale, -reference[column0 + j]));
-            if (!open) p[j] = uint32_t(j) - seen_from < seen_span ? p[j] : 0.F;
-            bits[j] = __reduce_max_sync(0xffffffffu, __float_as_uint(p[j] * value_scale));          // over the warp's tokens
-          }
-          const uint32_t largest = pick<C>(bits, lane);          // lane j: of column j
-          const uint32_t exponent = max(largest >> 23, 8u);      // below, the factor would not be finite
-          bool ask = false;
-          if (!moved && lane < uint32_t(C)) {
-            const uint32_t column = column0 + lane;
-            ask = largest > kHighBits;                           // NaN too
-            // what other warps find in the same tile does not count: the answer is the same whoever comes first
-            if (settled[column] >= tile_count && seen_low <= int(column) && int(column) < seen_high) {
-              if (largest < kLowBits) ask = true;
-              else settled[column] = tile_count;
+            for (int j = 0; j < C; ++j) {
+              p[j] = exp2_approx(fmaf(p[j], scale, -reference[column0 + j]));
+              if (!open) p[j] = uint32_t(j) - seen_from < seen_span ? p[j] : 0.F;
+              bits[j] = __reduce_max_sync(0xffffffffu, __float_as_uint(p[j] * value_scale));          // over the warp's tokens
             }
-            if (ask) s.move[tile_count & 3] = 1;
-          }
-          ask = __any_sync(0xffffffffu, ask);
-          if (!moved && lane == 0) ptx::mbar_arrive(&s.checked);
-          // P: the warp's 32 tokens of a column share a power of two, 2^-7 of that of the largest
-          my_spread[lane] = __uint_as_float((261 - exponent) << 23);
-          if (lane < uint32_t(C)) {
-            const uint32_t column = column0 + lane;
-            my_atom[column % 32 * 16 + column / 32 * 4 + quadrant] = uint8_t(exponent - 7);
-          }
-          __syncwarp();
-          // 16 bytes at a time where the warp has them: half the accesses to shared memory of 8
-          constexpr int STEP = C % 16 == 0 ? 16 : 8;
-#pragma unroll
-          for (int j = 0; j < C; j += STEP) {
-            uint32_t hi[STEP / 4], lo[STEP / 4];
-#pragma unroll
-            for (int i = 0; i < STEP; i += 4) {
-              const float4 up = *reinterpret_cast<const float4*>(my_spread + j + i);
-              uint16_t h0, l0, h1, l1;
-              // in this order: the factor of a column that sees none of these tokens is 2^126, and 0 stays 0
-              two_parts<1>(p[j + i] * value_scale * up.x, p[j + i + 1] * value_scale * up.y, h0, l0);
-              two_parts<1>(p[j + i + 2] * value_scale * up.z, p[j + i + 3] * value_scale * up.w, h1, l1);
-              hi[i / 4] = pack4(h0, h1);
-              lo[i / 4] = pack4(l0, l1);
+            const uint32_t largest = pick<C>(bits, lane);          // lane j: of column j
+            const uint32_t exponent = max(largest >> 23, 8u);      // below, the factor would not be finite
+            bool ask = false;
+            if (!moved && lane < uint32_t(C)) {
+              const uint32_t column = column0 + lane;
+              ask = largest > kHighBits && int(column) < used;     // NaN too
+              // what other warps find in the same tile does not count: the answer is the same whoever comes first
+              if (settled[column] >= tile_count && seen_low <= int(column) && int(column) < seen_high) {
+                if (largest < kLowBits) ask = true;
+                else settled[column] = tile_count;
+              }
+              if (ask) s.move[tile_count & 3] = 1;
             }
-            const uint32_t byte = column0 + j;
-            uint8_t* const to_hi = my_probs + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15);
-            uint8_t* const to_lo = my_probs + ((((byte >> 4) + 4) ^ (row & 7)) << 4) + (byte & 15);
-            if constexpr (STEP == 16) {
-              *reinterpret_cast<uint4*>(to_hi) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-              *reinterpret_cast<uint4*>(to_lo) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            } else {
-              *reinterpret_cast<uint2*>(to_hi) = make_uint2(hi[0], hi[1]);
-              *reinterpret_cast<uint2*>(to_lo) = make_uint2(lo[0], lo[1]);
+            ask = __any_sync(0xffffffffu, ask);
+            if (!moved && lane == 0) ptx::mbar_arrive(&s.checked);
+            // P: the warp's 32 tokens of a column share a power of two, 2^-7 of that of the largest
+            my_spread[lane] = __uint_as_float((261 - exponent) << 23);
+            if (lane < uint32_t(C)) {
+              const uint32_t column = column0 + lane;
+              my_atom[column % 32 * 16 + column / 32 * 4 + quadrant] = uint8_t(exponent - 7);
             }
-          }
-          if (!added && !ask) {
-            added = true;
+            __syncwarp();
+            // 16 bytes at a time where the warp has them: half the accesses to shared memory of 8
+            constexpr int STEP = C % 16 == 0 ? 16 : 8;
 #pragma unroll
-            for (int j = 0; j < C; ++j) total[j] += p[j];
+            for (int j = 0; j < C; j += STEP) {
+              uint32_t hi[STEP / 4], lo[STEP / 4];
+#pragma unroll
+              for (int i = 0; i < STEP; i += 4) {
+                const float4 up = *reinterpret_cast<const float4*>(my_spread + j + i);
+                uint16_t h0, l0, h1, l1;
+                // in this order: the factor of a column that sees none of these tokens is 2^126, and 0 stays 0
+                two_parts<1>(p[j + i] * value_scale * up.x, p[j + i + 1] * value_scale * up.y, h0, l0);
+                two_parts<1>(p[j + i + 2] * value_scale * up.z, p[j + i + 3] * value_scale * up.w, h1, l1);
+                hi[i / 4] = pack4(h0, h1);
+                lo[i / 4] = pack4(l0, l1);
+              }
+              const uint32_t byte = column0 + j;
+              uint8_t* const to_hi = my_probs + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15);
+              uint8_t* const to_lo = my_probs + ((((byte >> 4) + 4) ^ (row & 7)) << 4) + (byte & 15);
+              if constexpr (STEP == 16) {
+                *reinterpret_cast<uint4*>(to_hi) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(to_lo) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+              } else {
+                *reinterpret_cast<uint2*>(to_hi) = make_uint2(hi[0], hi[1]);
+                *reinterpret_cast<uint2*>(to_lo) = make_uint2(lo[0], lo[1]);
+              }
+            }
+            if (!added && !ask) {
+              added = true;
+#pragma unroll
+              for (int j = 0; j < C; ++j) total[j] += p[j];
+            }
+          } else if (!moved && lane == 0) {                      // no queries
+            ptx::mbar_arrive(&s.checked);
           }
           if (moved) break;
           wait(&s.checked, tile_count & 1, 0xad000000u);
