@@ -221,7 +221,7 @@ __device__ __forceinline__ bool position_in_batch(const gw_sequences& b, uint32_
 constexpr int kNormWarps = 4;
 
 // A warp takes heads of one row, queries and keys in one line, the next head's values on their way meanwhile; the row's angles are
-// computed once.  Bound by HBM: 4096 rows of 18 heads of 512, 151 MB, 30 us (77% of a copy's rate; 28 with the hardware's sines).
+// computed once.  Bound by HBM: 4096 rows of 18 heads of 512, 151 MB, 29 us (80% of a copy's rate; 27 with the hardware's sines).
 // With a task for each head, and angles in 64 bits, it took 74 us; eight rows, 2 us in a graph.
 template <int LPH, int V, bool WHOLE>
 __global__ void __launch_bounds__(32 * kNormWarps, V == 1 ? 8 : 6) qk_norm_rotary_kernel(NormRotary a) {

@@ -38,12 +38,12 @@
 // while the one before, of V, was still open, and a parity cannot tell that from the phase being complete.
 // Every wait is bounded; a role that gives up reports it, all leave, and tensor memory is released.
 //
-// Measured (a call, join included).  24 rows on up to 32,000 tokens, 4 KV heads of 512: 264 us, the rate of a copy from HBM.  One row on
+// Measured (a call, join included).  24 rows on up to 32,000 tokens, 4 KV heads of 512: 270 us, the rate of a copy from HBM.  One row on
 // 32,749 tokens, 2 heads of 512: 27 us against 10 us of HBM, most of it the first tile's way and the second launch.  64 rows in windows of 1024,
-// 16 heads of 256: 106 us against 81.  Drafts and prompts are bound by the softmax warps, 2400 cycles a tile at 32 columns, 3400 to 4100
+// 16 heads of 256: 108 us against 81.  Drafts and prompts are bound by the softmax warps, 2400 cycles a tile at 32 columns, 3400 to 4100
 // at 64 (about 400 instructions a warp; their chain of latencies, four warps a scheduler, does not fill the issue slots): 80 rows on up to 9000
-// tokens, 8 heads of 128, 64 us; 2048 rows in windows of 1024, 8 heads of 256, 104 us; 4096 rows on 16,384 tokens, 2 heads of 512, 2184 us,
-// 880 TFLOP/s, where the 64 products of a tile also read 393 KB of shared memory, 3100 cycles.
+// tokens, 8 heads of 128, 64 us; 2048 rows in windows of 1024, 8 heads of 256, 104 us; 4096 rows on 16,384 tokens, 2 heads of 512, 2200 us,
+// 870 TFLOP/s, where the 64 products of a tile also read 393 KB of shared memory, 3100 cycles.
 #include <algorithm>
 #include <string>
 
@@ -66,7 +66,7 @@ constexpr int kChunkBytes = kTokens * 128;
 constexpr int kAtomBytes = 512;              // scale atom: 128 rows x 4 blocks of 32 elements
 constexpr uint32_t kHighBits = (127u + 40u) << 23, kLowBits = (127u - 40u) << 23;
 constexpr int kItems = 4;                    // items that the walk is ahead at most
-constexpr int kNans = 32;                    // places with NaN that are kept for an item
+constexpr int kNans = 30;                    // places with NaN that are kept for an item
 constexpr int kScaleTiles = 16;              // tiles whose scales are kept: more than the ring and the score buffers can hold
 
 struct Attention {

@@ -415,7 +415,7 @@ gw_status gw_kv_cache_append(const gw_kv_cache* cache, const gw_sequences* batch
  * output = sum softmax(scale * q . k) v over what it sees, BF16; a row that sees nothing is 0.  Scores, softmax and sums in FP32;
  * products of the codes themselves: queries and probabilities enter as two E4M3 parts with a shared power of two for every 32
  * elements, which hold 8 significant bits.  A NaN in a cached value reaches the queries that see it and no others (of those, all
- * elements where more than 32 groups of 16 of the tokens that only some queries of a tile see hold NaN).  query and output: rows of [heads, head_dim] with strides in elements, 16-byte aligned, strides divisible by 8.
+ * elements where more than 30 groups of 16 of the tokens that only some queries of a tile see hold NaN).  query and output: rows of [heads, head_dim] with strides in elements, 16-byte aligned, strides divisible by 8.
  * heads / kv_heads at most 64.  scratch: gw_paged_attention_scratch_bytes bytes, 256-byte aligned (not kept between calls). */
 size_t gw_paged_attention_scratch_bytes(const gw_kv_cache* cache, const gw_sequences* batch, uint32_t heads);
 gw_status gw_paged_attention_bf16(const gw_kv_cache* cache, const gw_sequences* batch, const void* query_bf16,
