@@ -386,3 +386,26 @@ def test_a_layer_from_its_projections_to_its_output(gw, heads, kv_heads, dim):
         assert_rows(seen, turned, held, host, dim ** -0.5, 0)
         exact = f64(seen.flatten(1)) @ f64(wo).T
         assert (np.abs(f64(out) - exact) <= 2.0 ** -8 * np.abs(exact) + 2.0 ** -18 * (np.abs(f64(seen.flatten(1))) @ np.abs(f64(wo)).T)).all()
+
+
+def test_pages_behind_four_gigabytes(gw):
+    """The same step on the last pages of a large cache and on a small one gives the same codes, scales and results."""
+    page, dim, kv_heads, rows, sequences = 128, 512, 4, 70, [(70, 70), (1, 1)]
+    many = (1 << 32) // (page * dim * kv_heads) + 3
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GB")
+    g = torch.Generator().manual_seed(60)
+    q, k, v = (torch.randn((rows + 1, h, dim), generator=g).bfloat16().cuda() for h in (8, kv_heads, kv_heads))
+    results = []
+    for pages, table in ((2, [[0], [1]]), (many, [[many - 1], [many - 3]])):
+        cache = gw.KvCache(*(torch.empty((pages, kv_heads, page, dim), dtype=torch.uint8, device="cuda") for _ in range(2)),
+                           *(torch.empty((pages, kv_heads), device="cuda") for _ in range(2)))
+        batch = gw.SequenceBatch(torch.tensor([0, rows, rows + 1], dtype=torch.int32).cuda(), torch.tensor([n for _, n in sequences], dtype=torch.int32).cuda(),
+                                 torch.tensor(table, dtype=torch.int32).cuda(), rows + 1, rows)
+        gw.kv_cache_append(cache, batch, k, v)
+        out = gw.paged_attention(cache, batch, q, dim ** -0.5)
+        at = [t[0] for t in table]
+        results.append([out, cache.k_scales[at], cache.v_scales[at], cache.k_data[at[0], :, :rows].clone(), cache.v_data[at[0], :, :rows].clone(),
+                        cache.k_data[at[1], :, 0].clone(), cache.v_data[at[1], :, 0].clone()])
+    assert gw.kernel_error() == 0
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and not torch.isnan(results[0][0]).any()
