@@ -880,8 +880,8 @@ def paged_attention(cache: KvCache, batch: SequenceBatch, query: torch.Tensor, s
     if batch.device_index != device or dim != cache.head_dim or rows < batch.rows:
         raise _lib.GewellInvalidArgument("queries have the cache's head width and the batch's rows; all lie on one device")
     y, out_stride = _output(query, rows, heads, dim, y, device)
-    if window < 0:
-        raise _lib.GewellInvalidArgument("a window of 0 (all tokens) or more is wanted")
+    if not 0 <= window < 1 << 32:
+        raise _lib.GewellInvalidArgument("a window of 0 (all tokens) to 2^32 - 1 is wanted")
     lib = _library()
     if scratch is None:
         scratch = torch.empty(lib.gw_paged_attention_scratch_bytes(cache._ref, batch._ref, heads), dtype=torch.uint8, device=query.device)

@@ -277,7 +277,7 @@ def test_refusals_of_the_wrapper(gw):
     cache = to_device(gw, random_cache(batch, 2, 128, 51))
     held, q = batch.device(gw), queries(2, 4, 128, 52)
     strided = torch.zeros((2, 8, 128), dtype=torch.bfloat16).cuda()[:, ::2]
-    for bad in (dict(window=-1), dict(scale=float("nan")), dict(query=q.float()), dict(query=q[:1]), dict(query=strided), dict(query=q.cpu()),
+    for bad in (dict(window=-1), dict(window=(1 << 32) + 5), dict(scale=float("nan")), dict(query=q.float()), dict(query=q[:1]), dict(query=strided), dict(query=q.cpu()),
                 dict(y=torch.empty((2, 4, 64), dtype=torch.bfloat16).cuda()), dict(y=q.cpu()), dict(query=queries(2, 3, 128, 1)),
                 dict(query=queries(2, 4, 256, 1)), dict(scratch=torch.empty(16, dtype=torch.uint8).cuda()),
                 dict(scratch=torch.empty(1 << 22, dtype=torch.int8).cuda())):
