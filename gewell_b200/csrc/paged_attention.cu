@@ -862,7 +862,9 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
             factor[member] = v == 0.F ? 0.F : rcp_approx_ftz(v);
             if (!whole) {
               float* const totals = a.partial + size_t(gridDim.x) * 2 * N * D + size_t(place) * 2 * N;
-              totals[member] = reference[member];
+              // The reference of a column that sees nothing of this piece is 0 and says nothing: it must not be the largest of the join,
+              // before which scores far below 0 would all vanish.
+              totals[member] = v == 0.F ? -INFINITY : reference[member];
               totals[N + member] = v;
             }
           }
@@ -1135,7 +1137,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_consta
     for (uint32_t p = lane; p < pieces; p += 32) highest = fmaxf(highest, totals[size_t(place(p)) * 2 * columns + column]);
 #pragma unroll
     for (int m = 16; m; m /= 2) highest = fmaxf(highest, __shfl_xor_sync(0xffffffffu, highest, m));
-    float sum[E] = {}, total = 0.F;
+    float sum[E] = {}, total = 0.F;                          // a piece of which the column sees nothing has -infinity, and no weight
 #pragma unroll 4
     for (uint32_t p = share; p < pieces; p += WPC) {
       const float* const at = totals + size_t(place(p)) * 2 * columns + column;

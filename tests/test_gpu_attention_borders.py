@@ -1,0 +1,108 @@
+"""Attention over a paged 8-bit cache where it is easily wrong, against its definition in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import attention as oat
+from tests.attention_helpers import VALUES, Batch, f64, random_cache, sequence_values, to_device
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def gw():
+    import gewell_b200
+    return gewell_b200
+
+
+def queries(rows, heads, dim, seed, std=1.0):
+    return (torch.randn((rows, heads, dim), generator=torch.Generator().manual_seed(seed)) * std).bfloat16().cuda()
+
+
+def bound_of(q, k, v_codes, v_scales, scale, begin, exact, size):
+    """What the arithmetic of one row may be off by: q [heads, D], k [kv heads, tokens, D] and the codes [kv heads, tokens, D] and
+    scales [kv heads, tokens] of the values that it sees, the first of them token `begin`; exact, size = sum p |v| [heads, D].
+
+    A query element: x = hi + lo / 16 in blocks of 32 that are scaled to a loudest of 2^7 to 2^8.  With eight significant bits it is exact
+    from 2^-6 on; below, half a step of lo is 2^-10 / 16 = 2^-14, 2^-21 of the loudest.  A score adds D / 16 products of 32 terms in
+    FP32, each sum off by 2^-22 of sum |q k| at most and each of its terms by 2^-24 of the largest; its scaling (three factors, one fma)
+    by 2^-22 of it.  All that together is e, and a probability over the sum of them changes by exp(2 e) - 1.
+    A probability in two parts: half a step of each is 2^-4 of it, 2^-8 together; 2^-11 for the half-precision value that is cut; below
+    the normal codes half a step of lo, 2^-10, with the largest p * scale of the 32 tokens of a block at 2^7 or more: 2^-17 of that.
+    The sums: tokens / 16 products of 32 terms as above, tokens additions of 2^-24, 2^-21 for exp2 and the reciprocal.
+    The result: half a step of BF16, 2^-8."""
+    heads, group, tokens, dim = q.shape[0], q.shape[0] // k.shape[0], k.shape[1], q.shape[1]
+    out = np.zeros(exact.shape)
+    block = (begin + np.arange(tokens)) // 32 - begin // 32
+    for h in range(heads):
+        keys, codes, scales = k[h // group], np.abs(v_codes[h // group]), v_scales[h // group]
+        terms = np.abs(keys * q[h])
+        scores = keys @ q[h] * scale
+        e = 2.0 ** -21 * abs(scale) * np.abs(q[h]).max() * np.abs(keys).sum(axis=1).max()
+        e += dim / 16 * abs(scale) * (2.0 ** -22 * terms.sum(axis=1).max() + 32 * 2.0 ** -24 * terms.max())
+        e += 2.0 ** -22 * np.abs(scores).max()
+        p = np.exp(scores - scores.max())
+        p = p / p.sum() * scales
+        loudest = np.zeros(block[-1] + 1)
+        np.maximum.at(loudest, block, p)
+        lost = 2.0 ** -17 * (loudest[block] @ codes)
+        part = 2.0 ** -8 + 2.0 ** -11 + np.expm1(2 * e) + tokens / 16 * 32 * 2.0 ** -24 + tokens * 2.0 ** -24 + 2.0 ** -21
+        out[h] = (2.0 ** -8 * np.abs(exact[h]) + part * size[h] + lost) * (1 + 2.0 ** -8)
+    return out
+
+
+def assert_rows(got, q, batch, cache, scale, window=0, rows_of=None, share=None, what=""):
+    """Rows (default: all) against the definition; `share`: what the bound may be of sum p |v|, at most, in the median."""
+    got, shares = f64(got), []
+    for s, (n, length) in enumerate(batch.sequences):
+        if n == 0:
+            continue
+        k = sequence_values(batch, cache[0], s)
+        pages = batch.table[s, :-(-length // batch.page_tokens)]
+        codes = VALUES[cache[1][0][pages]].transpose(1, 0, 2, 3).reshape(k.shape[0], -1, k.shape[2])[:, :length]
+        scales = np.repeat(cache[1][1][pages].astype(np.float64).T, batch.page_tokens, axis=1)[:, :length]
+        v = codes * scales[..., None]
+        for i in range(n) if rows_of is None else sorted({r % n for r in rows_of}):
+            row, position = int(batch.row_offsets[s]) + i, length - n + i
+            exact, size = oat.attention(f64(q[row:row + 1]), k, v, scale, position, window)
+            seen = slice(max(0, position - window + 1) if window else 0, position + 1)
+            bound = bound_of(f64(q[row]), k[:, seen], codes[:, seen], scales[:, seen], scale, seen.start, exact[0], size[0])
+            error = np.abs(got[row] - exact[0])
+            assert (error <= bound).all(), f"{what} sequence {s} row {i}: {float(np.nanmax(error / bound))} of the bound"
+            shares.append(np.median(bound / size[0]))
+    assert share is None or np.median(shares) <= share, np.median(shares)
+
+
+@pytest.mark.parametrize("level", [80.0, 100.0, 300.0, 1000.0])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(8, 2, 128, 16), (4, 2, 256, 64), (8, 2, 512, 128)])
+@pytest.mark.parametrize("sequences,window", [([(5, 130)], 0), ([(16, 400), (1, 257), (3, 129)], 0), ([(40, 300), (5, 131)], 100), ([(300, 700)], 90),
+                                              ([(140, 140)], 0)])
+def test_scores_far_below_zero_in_pieces_that_some_rows_do_not_see(gw, level, heads, kv_heads, dim, page, sequences, window):
+    """All logits of all rows near -level.  There are fewer units of work than blocks, so every token tile of an item is a piece of its
+    own, and at a causal or window border rows of the item see nothing of it."""
+    batch = Batch(sequences, page, 61)
+    host = random_cache(batch, kv_heads, dim, 62, spread=0.0)
+    codes, scales = host[0]
+    one = int(np.flatnonzero(VALUES == 1.0 / float(np.nanmax(scales)))[0])
+    codes[..., :32] = one
+    q = queries(batch.rows, heads, dim, 63, 0.1)
+    q[..., :32] = -level / 32
+    got = gw.paged_attention(to_device(gw, host), batch.device(gw), q, 1.0, window=window)
+    assert gw.kernel_error() == 0
+    assert_rows(got, q, batch, host, 1.0, window, rows_of=[0, 1, 2, 3, 4, 15, 39, 63, 64, 120, 127, 128, 139, 200, 299], share=0.05)
+
+
+def test_a_piece_without_pages_takes_no_weight_from_scores_far_below_zero(gw):
+    """A whole tile whose page is missing, as a piece of its own."""
+    batch = Batch([(1, 300)], 128, 64)
+    host = random_cache(batch, 1, 128, 65, garbage=False, spread=0.0)
+    host[0][0][..., :32] = int(np.flatnonzero(VALUES == 1.0 / float(host[0][1].max()))[0])
+    q = queries(1, 4, 128, 66, 0.1)
+    q[..., :32] = -300.0 / 32
+    k, v = (np.delete(sequence_values(batch, c, 0), np.arange(128, 256), axis=1) for c in host)
+    batch.table[0, 1] = -1
+    got = gw.paged_attention(to_device(gw, host), batch.device(gw), q, 1.0)
+    assert gw.kernel_error() >> 24 == 0xa1
+    exact, size = oat.attention(f64(q), k, v, 1.0, 171)
+    # of logits near 300: 2^-21 * 9.4 * 132 + 8 * (2^-22 * 300 + 2^-19 * 9.4) + 2^-22 * 300 stays below 2^-9, twice in the exponent
+    assert (np.abs(f64(got) - exact) <= 2.0 ** -8 * np.abs(exact) + (2.0 ** -8 + 2.0 ** -8 + 2.0 ** -10) * size).all()
