@@ -97,7 +97,8 @@ struct Shared {
   Item items[kItems];
   // NaN among the values that not every query of an item sees: {token, dimension / 16 << 16 | which of the 16}
   uint2 nans[kItems][kNans];
-  int nan_count[kItems], nan_from[kItems];     // all found; the first token of those that did not fit
+  int nan_count[kItems];                       // all found
+  uint32_t nan_rows[kItems][2];                // a bit for each query row that sees any of those that did not fit
   int move[4];                                 // of the last tiles: some warp asks for the reference to be moved
   uint32_t tensor_memory;
   // units of all blocks, the block's range of them, and the item that has the first
@@ -339,6 +340,9 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {
 // a bit for each byte of 0xff
 __device__ __forceinline__ uint32_t one_bits(uint32_t bytes) { return (bytes & 1) | (bytes >> 7 & 2) | (bytes >> 14 & 4) | (bytes >> 21 & 8); }
 
+// the bits below `count`, of an item's at most 64 query rows
+__device__ __forceinline__ uint64_t rows_below(int count) { return count <= 0 ? 0 : count >= 64 ? ~0ull : (1ull << count) - 1; }
+
 // matrix descriptor of rows of 128 bytes, 128-byte swizzle, read across the rows: 8 rows of the sum are 1024 bytes apart
 __device__ __forceinline__ uint64_t across_desc(uint32_t address) { return ptx::smem_desc_sw128(address) | uint64_t(1024 >> 4) << 16; }
 
@@ -521,7 +525,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
         Item& m = s.items[n % kItems];
         m.tiles = -1;                                            // the end
         s.nan_count[n % kItems] = 0;
-        s.nan_from[n % kItems] = INT32_MAX;
+        s.nan_rows[n % kItems][0] = s.nan_rows[n % kItems][1] = 0;
         if (more) {
           m.begin = w.begin;
           m.end = w.end;
@@ -729,7 +733,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
       error = __reduce_max_sync(0xffffffffu, error);
       if (error) break;
       const Item& m = s.items[n % kItems];
-      const int begin = m.begin, end = m.end, tiles = m.tiles, first_tile = m.first_tile, low = m.low, high = m.high, all_low = m.all_low, all_high = m.all_high;
+      const int begin = m.begin, end = m.end, tiles = m.tiles, first_tile = m.first_tile, low = m.low, high = m.high, all_low = m.all_low, all_high = m.all_high, position0 = m.position0;
       __syncwarp();
       if (tiles < 0) break;
 #pragma unroll 1
@@ -755,11 +759,15 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
             if ((nan.x | nan.y | nan.z | nan.w) != 0) {
               rows[unit] = make_uint4(codes.x & ~nan.x, codes.y & ~nan.y, codes.z & ~nan.z, codes.w & ~nan.w);
               const int at = atomicAdd_block(&s.nan_count[n % kItems], 1), place = (unit % 8) ^ (unit / 8 % 8);       // 128-byte swizzle
-              if (at < kNans)
+              if (at < kNans) {
                 s.nans[n % kItems][at] = make_uint2(start + unit / 8, uint32_t(i % CH * 8 + place) << 16 | one_bits(nan.x) | one_bits(nan.y) << 4 |
                                                                    one_bits(nan.z) << 8 | one_bits(nan.w) << 12);
-              else
-                atomicMin_block(&s.nan_from[n % kItems], start + unit / 8);
+              } else {
+                const int ahead = start + unit / 8 - position0;    // rows from here on see the token, up to a window behind it
+                const uint64_t seen = rows_below(a.window ? ahead + int(a.window) : 64) & ~rows_below(ahead);
+                atomicOr_block(&s.nan_rows[n % kItems][0], uint32_t(seen));
+                atomicOr_block(&s.nan_rows[n % kItems][1], uint32_t(seen >> 32));
+              }
             }
           }
           ptx::fence_proxy_async_smem();
@@ -903,10 +911,11 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
           const int nans = s.nan_count[n % kItems];
           if (nans != 0) {                                       // to the queries that see them
             together();                                          // behind what was written above
-            const int listed = min(nans, kNans), from = s.nan_from[n % kItems];
+            const int listed = min(nans, kNans);
+            const uint64_t spoilt = s.nan_rows[n % kItems][0] | uint64_t(s.nan_rows[n % kItems][1]) << 32;
 #pragma unroll 1
             for (int column = warp - kFirstSoftmaxWarp; column < used; column += kSoftmaxWarps) {
-              const int position = m.position0 + int(column * a.group_inverse >> 16);
+              const int in_tile = int(column * a.group_inverse >> 16), position = m.position0 + in_tile;
               bf16* const to = output_at[column];
               float* const to_partial = a.partial + (size_t(place) * N + column) * D;
               const auto spoil = [&](int d) {
@@ -919,7 +928,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
                 const bool seen = int(at.x) <= position && (a.window == 0 || position - int(at.x) < int(a.window));
                 if (seen && lane < 16 && (at.y >> lane & 1)) spoil(int(at.y >> 16) * 16 + lane);
               }
-              if (from <= position)
+              if (spoilt >> in_tile & 1)
                 for (int d = lane; d < D; d += 32) spoil(d);
             }
           }

@@ -106,3 +106,26 @@ def test_a_piece_without_pages_takes_no_weight_from_scores_far_below_zero(gw):
     exact, size = oat.attention(f64(q), k, v, 1.0, 171)
     # of logits near 300: 2^-21 * 9.4 * 132 + 8 * (2^-22 * 300 + 2^-19 * 9.4) + 2^-22 * 300 stays below 2^-9, twice in the exponent
     assert (np.abs(f64(got) - exact) <= 2.0 ** -8 * np.abs(exact) + (2.0 ** -8 + 2.0 ** -8 + 2.0 ** -10) * size).all()
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 1, 256), (4, 4, 128), (2, 1, 512), (16, 2, 256)])
+@pytest.mark.parametrize("window", [0, 5, 40, 64, 100])
+@pytest.mark.parametrize("tokens", [(100,), (139,), (140, 141), (90, 91, 92, 150), tuple(range(135, 145)), (60, 145, 199)])
+def test_tokens_of_nan_reach_the_rows_that_see_them(gw, heads, kv_heads, dim, window, tokens):
+    """Whole tokens of NaN, more places than are kept for an item: at both ends of windows, and in windows shorter than a tile's rows."""
+    sequences = [(60, 200)]
+    batch = Batch(sequences, 16, 67)
+    host = random_cache(batch, kv_heads, dim, 68)
+    for token in tokens:
+        host[1][0][int(batch.table[0, token // 16]), :, token % 16] = 0x7f
+    q = queries(60, heads, dim, 69)
+    got = f64(gw.paged_attention(to_device(gw, host), batch.device(gw), q, dim ** -0.5, window=window))
+    assert gw.kernel_error() == 0
+    k, v = (sequence_values(batch, c, 0) for c in host)
+    for i in range(60):
+        position = 140 + i
+        sees = any(t <= position and (window == 0 or position - t < window) for t in tokens)
+        assert np.isnan(got[i]).all() if sees else not np.isnan(got[i]).any(), f"row {i}"
+        if not sees and i % 7 == 0:
+            exact, size = oat.attention(f64(q[i:i + 1]), k, v, dim ** -0.5, position, window)
+            assert (np.abs(got[i] - exact[0]) <= 2.0 ** -7 * (np.abs(exact[0]) + size[0])).all()
