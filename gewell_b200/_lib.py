@@ -74,7 +74,8 @@ class KvCache(ctypes.Structure):
 class Sequences(ctypes.Structure):
     """gw_sequences: rows, lengths and pages of a step's sequences."""
     _fields_ = [("row_offsets", c_void_p), ("context_lengths", c_void_p), ("page_table", c_void_p),
-                ("page_table_stride", c_uint32), ("sequences", c_uint32), ("rows", c_uint32), ("max_rows", c_uint32)]
+                ("page_table_stride", c_uint32), ("sequences", c_uint32), ("rows", c_uint32), ("max_rows", c_uint32),
+                ("page_table_entries", c_uint32)]
 
 
 class ExpertWeights(ctypes.Structure):

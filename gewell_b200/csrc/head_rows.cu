@@ -337,7 +337,7 @@ __device__ __forceinline__ Segment segment_at(const Append& a, uint32_t sequence
   const uint32_t ordinal = uint32_t(first) / page_tokens + which;
   const int low = max(first, int(ordinal * page_tokens)), high = min(int64_t(s.context), int64_t(ordinal + 1) * page_tokens);
   Segment g{s.first + low - begin, high - low, int(uint32_t(low) % page_tokens), low, -1};
-  if (ordinal < a.batch.page_table_stride) {
+  if (ordinal < a.batch.page_table_entries) {
     const int page = a.batch.page_table[size_t(sequence) * a.batch.page_table_stride + ordinal];
     if (page >= 0 && uint32_t(page) < a.cache.pages) g.page = page;
   }
@@ -782,6 +782,7 @@ gw_status gw_kv_cache_append(const gw_kv_cache* cache, const gw_sequences* batch
   }
   a.cache = *cache;
   a.batch = *batch;
+  a.batch.page_table_entries = page_entries(*batch);
   a.key = heads_of(*key);
   a.value = heads_of(*value);
   a.positions = positions;

@@ -22,11 +22,16 @@ inline gw_status check_cache(const gw_kv_cache* c, const char* what) {
   return GW_OK;
 }
 
+// Entries of a sequence's row of the page table.
+inline uint32_t page_entries(const gw_sequences& b) { return b.page_table_entries != 0 ? b.page_table_entries : b.page_table_stride; }
+
 inline gw_status check_batch(const gw_sequences* b, const char* what) {
   if (!b) return fail(GW_INVALID_ARGUMENT, std::string(what) + " requires a batch");
   if (b->rows == 0 || b->sequences == 0) return GW_OK;
   if (!b->row_offsets || !b->context_lengths || !b->page_table || b->page_table_stride == 0)
     return fail(GW_INVALID_ARGUMENT, std::string(what) + " requires row offsets, context lengths and a page table");
+  if (b->page_table_entries > b->page_table_stride)
+    return fail(GW_INVALID_ARGUMENT, std::string(what) + " requires page table entries within a row's stride");
   if (b->max_rows == 0 || b->max_rows > b->rows || b->rows > (1u << 24) || b->sequences > (1u << 20) || b->page_table_stride > (1u << 24))
     return fail(GW_INVALID_ARGUMENT, std::string(what) + " requires max_rows of 1 to rows, at most 2^24 rows, 2^20 sequences and 2^24 page table entries");
   return GW_OK;

@@ -312,7 +312,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // Entry of the page table as it is (-1 behind its end).  Nothing is asked of the value here: a warp that looks at it waits for it.
 __device__ __forceinline__ int page_entry(const Attention& a, uint32_t sequence, int token) {
   const uint32_t ordinal = uint32_t(token) >> a.page_shift;
-  return ordinal < a.batch.page_table_stride ? a.batch.page_table[size_t(sequence) * a.batch.page_table_stride + ordinal] : -1;
+  return ordinal < a.batch.page_table_entries ? a.batch.page_table[size_t(sequence) * a.batch.page_table_stride + ordinal] : -1;
 }
 __device__ __forceinline__ uint32_t pack4(uint16_t low, uint16_t high) { return uint32_t(low) | uint32_t(high) << 16; }
 
@@ -1268,7 +1268,9 @@ gw_status gw_paged_attention_bf16(const gw_kv_cache* cache, const gw_sequences* 
       !encode_tensor_map_2d(&v_map, cache->v_data, cache->head_dim, rows, cache->page_tokens, &error, 0))
     return fail(GW_CUDA_ERROR, "paged attention: " + error);
   const size_t floats = align_up(partial_floats(blocks, columns, cache->head_dim) * sizeof(float), 256);
-  const Attention a{*cache, *batch, static_cast<const bf16*>(query_bf16), static_cast<bf16*>(output_bf16), query_stride, output_stride,
+  gw_sequences sequences = *batch;
+  sequences.page_table_entries = page_entries(*batch);
+  const Attention a{*cache, sequences, static_cast<const bf16*>(query_bf16), static_cast<bf16*>(output_bf16), query_stride, output_stride,
                     heads, group, (65536 + group - 1) / group, columns / group, window > (1u << 30) ? 0 : window, uint32_t(__builtin_ctz(cache->page_tokens)), scale,
                     static_cast<float*>(scratch), reinterpret_cast<int4*>(static_cast<uint8_t*>(scratch) + floats)};
   const cudaStream_t s = as_stream(stream);

@@ -775,8 +775,10 @@ class SequenceBatch:
             raise _lib.GewellInvalidArgument("row_offsets has one entry more than there are sequences, page_table a row for each")
         self.row_offsets, self.context_lengths, self.page_table = row_offsets, context_lengths, page_table
         self.rows, self.max_rows, self.device_index = rows, max_rows, row_offsets.get_device()
-        stride = page_table.stride(0) if count > 1 else max(1, page_table.shape[1])
-        self._struct = _lib.Sequences(_ptr(row_offsets), _ptr(context_lengths), _ptr(page_table), stride, count, rows, max_rows)
+        # a view of a wider table has fewer entries than its stride; one without any is no table
+        entries = page_table.shape[1]
+        self._struct = _lib.Sequences(_ptr(row_offsets), _ptr(context_lengths), _ptr(page_table) if entries else 0,
+                                      page_table.stride(0) if count > 1 else entries, count, rows, max_rows, entries)
         self._ref = ctypes.byref(self._struct)
 
 

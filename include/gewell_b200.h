@@ -394,8 +394,9 @@ typedef struct gw_kv_cache {
 typedef struct gw_sequences {
   const int32_t* row_offsets;     /* [sequences + 1] */
   const int32_t* context_lengths; /* [sequences] */
-  const int32_t* page_table;      /* [sequences, page_table_stride] */
+  const int32_t* page_table;      /* rows of page_table_entries, page_table_stride apart */
   uint32_t page_table_stride, sequences, rows, max_rows;
+  uint32_t page_table_entries;    /* of a sequence, at most the stride; 0: as many as the stride */
 } gw_sequences;
 
 /* Keys and values of the step's rows into their pages, keys normed and rotated and values normed on the way (each as its

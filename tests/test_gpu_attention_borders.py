@@ -129,3 +129,33 @@ def test_tokens_of_nan_reach_the_rows_that_see_them(gw, heads, kv_heads, dim, wi
         if not sees and i % 7 == 0:
             exact, size = oat.attention(f64(q[i:i + 1]), k, v, dim ** -0.5, position, window)
             assert (np.abs(got[i] - exact[0]) <= 2.0 ** -7 * (np.abs(exact[0]) + size[0])).all()
+
+
+def test_a_view_of_a_wider_page_table(gw):
+    """Positions behind a view's last column are behind the table, whatever the wider table holds there."""
+    batch = Batch([(1, 100), (20, 90)], 16, 73)
+    host = random_cache(batch, 1, 128, 74, garbage=False)
+    q = queries(batch.rows, 2, 128, 75)
+    columns, sequences = batch.table.shape[1], len(batch.sequences)
+    wide = torch.zeros((sequences, columns + 7), dtype=torch.int32).cuda()
+    whole = batch.device(gw)
+    wide[:, 4:4 + columns] = whole.page_table
+    offsets, lengths = whole.row_offsets, whole.context_lengths
+    view = gw.SequenceBatch(offsets, lengths, wide[:, 4:4 + columns], batch.rows, batch.max_rows)
+    assert torch.equal(gw.paged_attention(to_device(gw, host), view, q, 0.1), gw.paged_attention(to_device(gw, host), whole, q, 0.1))
+    assert gw.kernel_error() == 0
+    short = gw.SequenceBatch(offsets, lengths, whole.page_table[:, :5].contiguous(), batch.rows, batch.max_rows)
+    want = gw.paged_attention(to_device(gw, host), short, q, 0.1)
+    assert gw.kernel_error() >> 24 == 0xa1
+    short = gw.SequenceBatch(offsets, lengths, wide[:, 4:9], batch.rows, batch.max_rows)
+    assert torch.equal(gw.paged_attention(to_device(gw, host), short, q, 0.1), want)
+    assert gw.kernel_error() >> 24 == 0xa1
+    # and the append writes to none of the pages behind the view
+    x = torch.ones((batch.rows, 1, 128), dtype=torch.bfloat16).cuda()
+    cache = to_device(gw, host)
+    before = cache.k_data.clone()
+    gw.kv_cache_append(cache, short, x, x)
+    assert gw.kernel_error() >> 24 == 0xa1
+    changed = (cache.k_data != before).flatten(1).any(dim=1).cpu().numpy()
+    assert not changed[batch.table[0, 5:7]].any() and not changed[batch.table[1, 5]]
+    assert changed[batch.table[1, 4]]                                # tokens 70 .. 79
