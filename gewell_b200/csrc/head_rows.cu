@@ -345,13 +345,15 @@ __device__ __forceinline__ Segment segment_at(const Append& a, uint32_t sequence
   return g;
 }
 
-// Segment `wanted` of all sequences, found by a scan over their counts.
+// Segment `wanted` of all sequences, found by a scan over their counts.  The first block scans them all and reports those that cannot be
+// followed: a block for the last ones need not be there.
 template <int THREADS>
 __device__ __forceinline__ Segment find_segment(const Append& a, uint32_t wanted) {
   constexpr int WARPS = THREADS / 32;
   __shared__ uint32_t totals[WARPS];
   __shared__ Segment found;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const bool reports = blockIdx.x == 0 && blockIdx.y == 0;
   if (threadIdx.x == 0) found.page = -1;
   uint32_t before = 0;
   for (uint32_t base = 0; base < a.batch.sequences; base += THREADS) {
@@ -359,7 +361,7 @@ __device__ __forceinline__ Segment find_segment(const Append& a, uint32_t wanted
     SequenceRows rows{0, 0, 0, false};
     if (s < a.batch.sequences) {
       rows = sequence_rows(a.batch, s);
-      if (rows.bad && blockIdx.x == 0) report(0xa2000000u | (s & 0xffffffu));
+      if (rows.bad && reports) report(0xa2000000u | (s & 0xffffffu));
     }
     const uint32_t mine = segments_of(rows, a.cache.page_tokens);
     uint32_t sum = mine;
@@ -379,7 +381,7 @@ __device__ __forceinline__ Segment find_segment(const Append& a, uint32_t wanted
     if (wanted >= low && wanted - low < mine) found = segment_at(a, s, rows, wanted - low);
     before += all;
     __syncthreads();
-    if (wanted < before) break;
+    if (wanted < before && !reports) break;
   }
   return found;
 }
