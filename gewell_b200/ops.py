@@ -743,6 +743,23 @@ def _stream_on(device: int, stream) -> int:
     return _raw_stream(device) if stream is None and _raw_stream is not None else _stream(stream)
 
 
+def _allocated(make, device: int, stream, returned: bool):
+    """make(), a tensor that a call on `stream` writes first.  Another stream than the current one gets it from its own memory: a block
+    that the current stream has freed may still be read there.  What is `returned` the current stream's work may read in turn, so its
+    block is not handed out again before that is done."""
+    handle = None if stream is None else _stream(stream)
+    if handle is None or handle == _stream_on(device, None):
+        return make()
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(handle, device) if handle > 1 else torch.cuda.default_stream(device)     # 1: the legacy handle of it
+    current = torch.cuda.current_stream(device)
+    with torch.cuda.stream(stream):
+        made = make()
+    if returned:
+        made.record_stream(current)
+    return made
+
+
 class KvCache:
     """A paged cache of keys and values in 8 bits over the caller's tensors: E4M3 codes [pages, kv_heads, page_tokens,
     head_dim] (torch.uint8 or torch.float8_e4m3fn) and FP32 scales [pages, kv_heads], contiguous."""
@@ -791,10 +808,10 @@ def _layout(x: torch.Tensor, device: int):
     return rows, heads, dim, stride[0] if rows > 1 else heads * dim
 
 
-def _output(x: torch.Tensor, rows: int, heads: int, dim: int, y, device: int):
+def _output(x: torch.Tensor, rows: int, heads: int, dim: int, y, device: int, stream):
     """(y, its row stride); a new tensor for None."""
     if y is None:
-        return torch.empty_like(x, memory_format=torch.contiguous_format), heads * dim
+        return _allocated(lambda: torch.empty_like(x, memory_format=torch.contiguous_format), device, stream, True), heads * dim
     at = _layout(y, device)
     if at[:3] != (rows, heads, dim):
         raise _lib.GewellInvalidArgument("the output has its input's shape")
@@ -832,14 +849,14 @@ def qk_norm_rotary(query: torch.Tensor, key, query_weight, key_weight, positions
     where nothing is rotated)."""
     device = _on_current(query.get_device())
     rows, heads, dim, stride = _layout(query, device)
-    query_out, out_stride = _output(query, rows, heads, dim, query_out, device)
+    query_out, out_stride = _output(query, rows, heads, dim, query_out, device, stream)
     q = _lib.HeadRows(query.data_ptr(), stride, query_out.data_ptr(), out_stride, _head_weight(query_weight, dim, device), heads, 1)
     k = None
     if key is not None:
         key_rows, kv_heads, key_dim, stride = _layout(key, device)
         if key_rows != rows or key_dim != dim:
             raise _lib.GewellInvalidArgument("queries and keys have the same rows and head width")
-        key_out, out_stride = _output(key, rows, kv_heads, dim, key_out, device)
+        key_out, out_stride = _output(key, rows, kv_heads, dim, key_out, device, stream)
         k = ctypes.byref(_lib.HeadRows(key.data_ptr(), stride, key_out.data_ptr(), out_stride, _head_weight(key_weight, dim, device), kv_heads, 1))
     _check(_library().gw_qk_norm_rotary_bf16(ctypes.byref(q), k, rows, dim, _positions(positions, rows, device),
                                              _rotary(frequencies, interleaved, device), epsilon, _stream_on(device, stream)))
@@ -865,7 +882,7 @@ def kv_cache_append(cache: KvCache, batch: SequenceBatch, key: torch.Tensor, val
         q_rows, heads, q_dim, stride = _layout(query, device)
         if q_dim != dim or q_rows < rows:
             raise _lib.GewellInvalidArgument("queries have the cache's head width and the batch's rows")
-        query_out, out_stride = _output(query, q_rows, heads, dim, query_out, device)
+        query_out, out_stride = _output(query, q_rows, heads, dim, query_out, device, stream)
         q = ctypes.byref(_lib.HeadRows(query.data_ptr(), stride, query_out.data_ptr(), out_stride, _head_weight(query_weight, dim, device), heads, 1))
     _check(_library().gw_kv_cache_append(cache._ref, batch._ref, made[0], made[1], q, _positions(positions, rows, device),
                                          _rotary(frequencies, interleaved, device), epsilon, _stream_on(device, stream)))
@@ -881,14 +898,13 @@ def paged_attention(cache: KvCache, batch: SequenceBatch, query: torch.Tensor, s
     rows, heads, dim, stride = _layout(query, device)
     if batch.device_index != device or dim != cache.head_dim or rows < batch.rows:
         raise _lib.GewellInvalidArgument("queries have the cache's head width and the batch's rows; all lie on one device")
-    y, out_stride = _output(query, rows, heads, dim, y, device)
+    y, out_stride = _output(query, rows, heads, dim, y, device, stream)
     if not 0 <= window < 1 << 32:
         raise _lib.GewellInvalidArgument("a window of 0 (all tokens) to 2^32 - 1 is wanted")
     lib = _library()
     if scratch is None:
-        scratch = torch.empty(lib.gw_paged_attention_scratch_bytes(cache._ref, batch._ref, heads), dtype=torch.uint8, device=query.device)
-        if stream is not None:                        # not to be taken by the current stream's next tensors before that stream is done
-            scratch.record_stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream)))
+        size = lib.gw_paged_attention_scratch_bytes(cache._ref, batch._ref, heads)
+        scratch = _allocated(lambda: torch.empty(size, dtype=torch.uint8, device=query.device), device, stream, False)
     elif scratch.dtype is not torch.uint8 or scratch.get_device() != device or not scratch.is_contiguous():
         raise _lib.GewellInvalidArgument("scratch is contiguous uint8 on the cache's device")
     _check(lib.gw_paged_attention_bf16(cache._ref, batch._ref, query.data_ptr(), stride, heads, scale, window, y.data_ptr(), out_stride,

@@ -159,3 +159,65 @@ def test_a_view_of_a_wider_page_table(gw):
     changed = (cache.k_data != before).flatten(1).any(dim=1).cpu().numpy()
     assert not changed[batch.table[0, 5:7]].any() and not changed[batch.table[1, 5]]
     assert changed[batch.table[1, 4]]                                # tokens 70 .. 79
+
+
+@pytest.mark.parametrize("kind", ["attention", "norm", "append"])
+@pytest.mark.parametrize("number", [False, True])
+def test_results_on_another_stream_are_not_in_memory_that_is_still_read(gw, kind, number):
+    """A tensor that the current stream has yet to read, freed, is not where a call on another stream puts its results or scratch; and
+    results of such a call that the current stream has yet to read are not where the next call on that stream puts its own."""
+    batch = Batch([(1, 300)] * 5, 32, 76)
+    cache = to_device(gw, random_cache(batch, 2, 256, 77, garbage=False))
+    held, q = batch.device(gw), queries(5, 8, 256, 78)
+    k = queries(5, 2, 256, 79)
+    positions = torch.arange(5, dtype=torch.int32).cuda()
+
+    def call(stream=None):
+        if kind == "attention":
+            return gw.paged_attention(cache, held, q, 0.06, stream=stream)
+        if kind == "norm":
+            return gw.qk_norm_rotary(q, None, None, None, positions, None, stream=stream)[0]
+        return gw.kv_cache_append(cache, held, k, k, query=q, stream=stream)
+    plain = call()
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    given = other.cuda_stream if number else other
+    # the caching allocator hands a block of the same size out again; several, as others may lie free
+    sizes = [q.numel() * 2] * 50
+    if kind == "attention":
+        sizes += [gw.lib.gw_paged_attention_scratch_bytes(cache._ref, held._ref, 8)] * 4
+    taken = [torch.full((n,), 9, dtype=torch.uint8, device="cuda") for n in sizes]
+    read = [torch.zeros_like(t) for t in taken]
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
+    for t, r in zip(taken, read):
+        r.copy_(t)
+    del taken, t
+    got = call(given)
+    other.synchronize()
+    assert torch.equal(got, plain)
+    torch.cuda.synchronize()
+    assert all((r == 9).all() for r in read)
+    kept = torch.zeros_like(got)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
+    kept.copy_(got)
+    del got                                             # the current stream has yet to read it
+    with torch.cuda.stream(other):
+        for _ in range(4):
+            torch.full((q.numel(),), 3.0, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    assert torch.equal(kept, plain)
+
+
+@pytest.mark.parametrize("number", [0, 1])
+def test_the_default_stream_by_its_number(gw, number):
+    batch = Batch([(1, 300)] * 3, 32, 83)
+    cache = to_device(gw, random_cache(batch, 2, 128, 84, garbage=False))
+    held, q = batch.device(gw), queries(3, 8, 128, 85)
+    plain = gw.paged_attention(cache, held, q, 0.06)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        got = gw.paged_attention(cache, held, q, 0.06, stream=number)
+    torch.cuda.synchronize()
+    assert torch.equal(got, plain) and torch.equal(gw.paged_attention(cache, held, q, 0.06, stream=number), plain)
