@@ -201,7 +201,7 @@ struct NormRotary {
   Heads query, key;                    // key.heads == 0: none
   uint32_t rows, width, per_task, tasks;       // heads of a row that a task takes, tasks of a row
   const int32_t* positions;            // or NULL: those of the batch
-  gw_sequences batch;
+  gw_sequences batch;                  // sequences == 0: every row counts; else rows of no sequence are left as they are
   Rotary rotary;
   float epsilon;
 };
@@ -247,8 +247,8 @@ __global__ void __launch_bounds__(32 * kNormWarps, V == 1 ? 8 : 6) qk_norm_rotar
   Raw<V> next_lo, next_hi;
   load(first + group, next_lo, next_hi);
   int position = 0;
+  if (a.batch.sequences && !position_in_batch(a.batch, row, position)) return;
   if (a.positions != nullptr) position = a.positions[row];
-  else if (a.batch.sequences && !position_in_batch(a.batch, row, position)) return;
   float s[E], c[E];
   {
     float frequencies[E];

@@ -3,6 +3,9 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import attention as oat
+from tests.attention_helpers import f64
+
 pytestmark = pytest.mark.gpu
 
 
@@ -40,3 +43,22 @@ def test_a_bad_sequence_behind_many_good_ones_is_reported(gw, dim, page, most, k
     assert gw.kernel_error() == 0xa2000000 | (count - 1)
     written = cache.k_data[:, 0, 0].any(dim=1)
     assert written[:-1].all() and not written[-1]
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_query_rows_of_no_sequence_stay(gw, given):
+    """Rows behind the last sequence, and of one that cannot be followed, are left as they are, wherever the positions come from."""
+    heads, dim, rows = 3, 128, 9
+    x = torch.randn((rows, heads, dim), generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    k = x[:, :1].contiguous()
+    positions = torch.tensor([5, 0, 1, 2, 9, 9, 9, 9, 9], dtype=torch.int32)
+    f = torch.tensor([1e4 ** (-i / 64) for i in range(64)], dtype=torch.float32)
+    for lengths, good, error in (([6, 3], [0, 1, 2, 3], 0), ([6, 2 ** 30 + 1], [0], 0xa2000001)):
+        y = torch.full_like(x, 7.0)
+        gw.kv_cache_append(small_cache(gw, 2, dim), batch_of(gw, [0, 1, 4], lengths, [[0], [1]], rows, 3), k, k, frequencies=f.cuda(),
+                           positions=positions.cuda() if given else None, query=x, query_out=y)
+        assert gw.kernel_error() == error
+        rest = [r for r in range(rows) if r not in good]
+        assert (y[rest] == 7.0).all()
+        exact = oat.head_norm_rotary(f64(x)[good], None, True, positions.numpy()[good], f.numpy())
+        assert (np.abs(f64(y)[good] - exact) <= 2.0 ** -8 * np.abs(exact) + 2.0 ** -19 * np.abs(exact).max(axis=-1, keepdims=True)).all()
