@@ -373,7 +373,8 @@ gw_status gw_qk_norm_rotary_bf16(const gw_head_rows* query, const gw_head_rows* 
 
 /* A paged cache of keys and values in 8 bits, in the caller's memory: E4M3 codes [pages, kv_heads, page_tokens, head_dim]
  * (16-byte aligned) and an FP32 scale for every page and head [pages, kv_heads], for keys and for values.  What a code stands for
- * is code * scale; attention takes value scales below 2^-64 for 2^-64, and none may be below 0.  page_tokens 16, 32, 64 or 128;
+ * is code * scale; attention takes value scales below 2^-64 for 2^-64, and none may be below 0.  Queries that see a token of a page
+ * whose value scale is NaN, infinite or below 0 get NaN.  page_tokens 16, 32, 64 or 128;
  * head_dim 128, 256 or 512; pages * kv_heads * page_tokens below 2^31. */
 typedef struct gw_kv_cache {
   void* k_data;

@@ -221,3 +221,26 @@ def test_the_default_stream_by_its_number(gw, number):
         got = gw.paged_attention(cache, held, q, 0.06, stream=number)
     torch.cuda.synchronize()
     assert torch.equal(got, plain) and torch.equal(gw.paged_attention(cache, held, q, 0.06, stream=number), plain)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf"), -2.0 ** -7])
+@pytest.mark.parametrize("window", [0, 30])
+def test_value_scales_that_are_no_numbers(gw, bad, window):
+    """The scale of a page that is NaN, infinite or negative makes the rows NaN that see any token of the page, and no others: it is no
+    missing page.  The others need not have the bits that they have without it: a NaN asks for another reference for all rows of
+    its tile, exp2(score - reference) is then another number, and its rounding to two parts falls elsewhere (2^-8 of it, in the bound)."""
+    batch = Batch([(60, 200), (1, 50)], 16, 70)
+    host = random_cache(batch, 2, 128, 71)
+    clean = [tuple(a.copy() for a in part) for part in host]
+    host[1][1][int(batch.table[0, 9]), 1] = bad                    # tokens 144 .. 159 of the first sequence, second head
+    q = queries(batch.rows, 4, 128, 72)
+    got = gw.paged_attention(to_device(gw, host), batch.device(gw), q, 0.1, window=window)
+    assert gw.kernel_error() == 0
+    sees = [140 + i >= 144 and (window == 0 or 140 + i - 159 < window) for i in range(60)]
+    assert 0 < sum(sees) and torch.isnan(got[:60][sees][:, 2:]).all()
+    rest = [i for i in range(60) if not sees[i]]
+    assert_rows(got, q, batch, clean, 0.1, window, rows_of=rest)
+    assert not torch.isnan(got[:, :2]).any()
+    other = got.clone()
+    other[:60, 2:][sees] = gw.paged_attention(to_device(gw, clean), batch.device(gw), q, 0.1, window=window)[:60, 2:][sees]
+    assert_rows(other, q, batch, clean, 0.1, window, rows_of=range(0, 60, 7))
