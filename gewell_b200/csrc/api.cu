@@ -133,10 +133,12 @@ uint32_t gw_debug_kernel_error(void) {
   if (cudaDeviceSynchronize() != cudaSuccess) return 0xFFFFFFFEu;
   cudaMemcpy(&value, word, sizeof(value), cudaMemcpyDeviceToHost);
   if (value != 0) zero_now(word, sizeof(value));
-  // the allocation-free linear reports into a word of its own (it may not use the allocated one)
-  const uint32_t built_in = take_static_scratch_error();
-  const uint32_t append = take_head_rows_error(), attention = take_paged_attention_error();
-  return value != 0 ? value : built_in != 0 ? built_in : append != 0 ? append : attention;
+  // Entry points without a set-up call report into words of their own (they may not use the allocated one).  A word that is not
+  // returned is not cleared: its report is the next call's.
+  if (value == 0) value = take_static_scratch_error();
+  if (value == 0) value = take_head_rows_error();
+  if (value == 0) value = take_paged_attention_error();
+  return value;
 }
 
 uint64_t gw_debug_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }

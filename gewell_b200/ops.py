@@ -56,7 +56,8 @@ def _check(status: int) -> None:
 
 def kernel_error() -> int:
     """Error word written by the bounded waits of the tensor-core kernels
-    (0 = none).  Synchronises the device and clears the word."""
+    (0 = none).  Synchronises the device and clears the word; reports of
+    operators with words of their own come one a call, until 0."""
     return int(_library().gw_debug_kernel_error())
 
 

@@ -745,8 +745,10 @@ gw_status gw_moe_ep_combine(gw_moe_workspace* workspace, uint32_t rows, const in
                             const int32_t* dest_row0, void* const* peer_down, uint32_t capacity_rows,
                             void* output_bf16, void* stream);
 
-/* Last kernel-reported error word of this process's device (0 = none); set by
- * bounded waits inside the tensor-core kernels.  Synchronises the device. */
+/* A kernel-reported error word of this process's device (0 = none); set by
+ * bounded waits inside the tensor-core kernels.  Synchronises the device.
+ * Clears the word that it returns; kernels that have words of their own may
+ * have reported too, so a caller that wants all calls until it gets 0. */
 uint32_t gw_debug_kernel_error(void);
 
 #ifdef __cplusplus

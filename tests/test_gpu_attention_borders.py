@@ -244,3 +244,16 @@ def test_value_scales_that_are_no_numbers(gw, bad, window):
     other = got.clone()
     other[:60, 2:][sees] = gw.paged_attention(to_device(gw, clean), batch.device(gw), q, 0.1, window=window)[:60, 2:][sees]
     assert_rows(other, q, batch, clean, 0.1, window, rows_of=range(0, 60, 7))
+
+
+def test_reports_of_two_operators_are_both_read(gw):
+    batch = Batch([(1, 20), (1, 40)], 16, 80)
+    host = random_cache(batch, 1, 128, 81, garbage=False)
+    broken = Batch([(1, 20), (1, 40)], 16, 80)
+    broken.table[0, 1] = -1
+    x = queries(2, 1, 128, 82)
+    gw.kv_cache_append(to_device(gw, host), broken.device(gw), x, x)
+    broken = Batch([(1, 20), (1, 40)], 16, 80)
+    broken.table[1, 1] = -1
+    gw.paged_attention(to_device(gw, host), broken.device(gw), x, 0.1)
+    assert sorted([gw.kernel_error(), gw.kernel_error()]) == [0xa1000000, 0xa1000001] and gw.kernel_error() == 0
