@@ -13,6 +13,7 @@
 // sine and cosine are FP32-exact; the hardware's, 2^-21 off, would let a key in ten thousand fall to the next code of E4M3.  They are
 // computed once for all heads that a warp or block takes.  Everything else is FP32 and is rounded once.
 #include <algorithm>
+#include <atomic>
 #include <string>
 
 #include "common.cuh"
@@ -24,6 +25,7 @@ using namespace gw;
 namespace {
 
 __device__ uint32_t g_head_rows_error;       // first report since it was last taken
+std::atomic<bool> g_append_ran[kMaxDeviceSlots];       // on a GPU: else the word is 0, and reading it would load the module
 
 __device__ __forceinline__ void report(uint32_t code) { atomicCAS(&g_head_rows_error, 0u, code); }
 
@@ -721,6 +723,7 @@ cudaError_t launch_append(Append a, cudaStream_t stream) {
 }  // namespace
 
 uint32_t gw::take_head_rows_error() {
+  if (!g_append_ran[current_device_slot()]) return 0;
   uint32_t value = 0;
   if (cudaMemcpyFromSymbol(&value, g_head_rows_error, sizeof(value)) != cudaSuccess) return 0xFFFFFFFDu;
   const uint32_t none = 0;
@@ -790,6 +793,7 @@ gw_status gw_kv_cache_append(const gw_kv_cache* cache, const gw_sequences* batch
   a.positions = positions;
   a.epsilon = epsilon;
   const cudaStream_t s = as_stream(stream);
+  g_append_ran[current_device_slot()] = true;
   if (query) GW_CUDA_CHECK(launch_norm_rotary(q, s), "cache append (queries)");
   const bool whole = a.rotary.kind == kWhole;
   const auto launch = width == 128   ? (whole ? &launch_append<16, 1, true> : &launch_append<16, 1, false>)

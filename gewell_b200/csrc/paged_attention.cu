@@ -45,6 +45,7 @@
 // tokens, 8 heads of 128, 64 us; 2048 rows in windows of 1024, 8 heads of 256, 104 us; 4096 rows on 16,384 tokens, 2 heads of 512, 2200 us,
 // 870 TFLOP/s, where the 64 products of a tile also read 393 KB of shared memory, 3100 cycles.
 #include <algorithm>
+#include <atomic>
 #include <string>
 
 #include "attention_work.h"
@@ -59,6 +60,7 @@ using namespace gw;
 namespace {
 
 __device__ uint32_t g_attention_error;       // first report since it was last taken
+std::atomic<bool> g_attention_ran[kMaxDeviceSlots];       // on a GPU: else the word is 0, and reading it would load the module
 
 __host__ __device__ constexpr int softmax_warps(int columns) { return columns <= 32 ? 8 : 16; }
 constexpr int kFirstSoftmaxWarp = 4;
@@ -1234,6 +1236,7 @@ cudaError_t launch_columns(uint32_t columns, const Attention& a, const CUtensorM
 }  // namespace
 
 uint32_t gw::take_paged_attention_error() {
+  if (!g_attention_ran[current_device_slot()]) return 0;
   uint32_t value = 0;
   if (cudaMemcpyFromSymbol(&value, g_attention_error, sizeof(value)) != cudaSuccess) return 0xFFFFFFFDu;
   const uint32_t none = 0;
@@ -1279,6 +1282,7 @@ gw_status gw_paged_attention_bf16(const gw_kv_cache* cache, const gw_sequences* 
   const Attention a{*cache, sequences, static_cast<const bf16*>(query_bf16), static_cast<bf16*>(output_bf16), query_stride, output_stride,
                     heads, group, (65536 + group - 1) / group, columns / group, window > (1u << 30) ? 0 : window, uint32_t(__builtin_ctz(cache->page_tokens)), scale,
                     static_cast<float*>(scratch), reinterpret_cast<int4*>(static_cast<uint8_t*>(scratch) + floats)};
+  g_attention_ran[current_device_slot()] = true;
   const cudaStream_t s = as_stream(stream);
   GW_CUDA_CHECK((cache->head_dim == 128   ? launch_columns<128>(columns, a, k_map, v_map, blocks, s)
                  : cache->head_dim == 256 ? launch_columns<256>(columns, a, k_map, v_map, blocks, s)

@@ -257,3 +257,31 @@ def test_reports_of_two_operators_are_both_read(gw):
     broken.table[1, 1] = -1
     gw.paged_attention(to_device(gw, host), broken.device(gw), x, 0.1)
     assert sorted([gw.kernel_error(), gw.kernel_error()]) == [0xa1000000, 0xa1000001] and gw.kernel_error() == 0
+
+
+def test_reading_the_error_word_loads_no_kernels(tmp_path):
+    """A process that has run none of these operators, perhaps with all memory taken, reads the word without their modules: what the first
+    read takes is the word's own allocation, one granule of 2 MiB."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = ("import torch, gewell_b200 as gw; torch.zeros(1).cuda(); torch.cuda.synchronize(); before = torch.cuda.mem_get_info()[0]; "
+            "assert gw.kernel_error() == 0; print(before - torch.cuda.mem_get_info()[0])")
+    done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
+    assert int(done.stdout.split()[-1]) <= 2 << 20
+
+
+def test_a_replayed_graph_reports(gw):
+    batch = Batch([(1, 40)], 16, 86)
+    cache, held, q = to_device(gw, random_cache(batch, 1, 128, 87, garbage=False)), batch.device(gw), queries(1, 2, 128, 88)
+    gw.paged_attention(cache, held, q, 0.1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gw.kv_cache_append(cache, held, q[:, :1], q[:, :1])
+        gw.paged_attention(cache, held, q, 0.1)
+    graph.replay()
+    assert gw.kernel_error() == 0
+    held.page_table.fill_(-1)
+    graph.replay()
+    assert gw.kernel_error() == 0xa1000000 and gw.kernel_error() == 0xa1000000 and gw.kernel_error() == 0
