@@ -8,6 +8,7 @@ memory and the current stream.  Every call goes through libgewell_b200.so.
 from __future__ import annotations
 
 import ctypes
+import operator
 from dataclasses import dataclass
 
 import torch
@@ -761,6 +762,13 @@ def _allocated(make, device: int, stream, returned: bool):
     return made
 
 
+def _u32(value, name: str) -> int:
+    value = operator.index(value)
+    if not 0 <= value < 1 << 32:
+        raise _lib.GewellInvalidArgument(f"{name}: 0 to 2^32 - 1 are wanted")
+    return value
+
+
 class KvCache:
     """A paged cache of keys and values in 8 bits over the caller's tensors: E4M3 codes [pages, kv_heads, page_tokens,
     head_dim] (torch.uint8 or torch.float8_e4m3fn) and FP32 scales [pages, kv_heads], contiguous."""
@@ -793,10 +801,11 @@ class SequenceBatch:
             raise _lib.GewellInvalidArgument("row_offsets has one entry more than there are sequences, page_table a row for each")
         self.row_offsets, self.context_lengths, self.page_table = row_offsets, context_lengths, page_table
         self.rows, self.max_rows, self.device_index = rows, max_rows, row_offsets.get_device()
+        rows, max_rows = _u32(rows, "rows"), _u32(max_rows, "max_rows")
         # a view of a wider table has fewer entries than its stride; one without any is no table
         entries = page_table.shape[1]
         self._struct = _lib.Sequences(_ptr(row_offsets), _ptr(context_lengths), _ptr(page_table) if entries else 0,
-                                      page_table.stride(0) if count > 1 else entries, count, rows, max_rows, entries)
+                                      _u32(page_table.stride(0), "the page table's stride") if count > 1 else entries, count, rows, max_rows, entries)
         self._ref = ctypes.byref(self._struct)
 
 
@@ -832,7 +841,7 @@ def _rotary(frequencies, interleaved: bool, device: int):
         return None
     if frequencies.dtype is not torch.float32 or frequencies.dim() != 1 or frequencies.stride(0) != 1 or frequencies.get_device() != device:
         raise _lib.GewellInvalidArgument("inverse frequencies are FP32 [width / 2]")
-    return ctypes.byref(_lib.Rotary(frequencies.data_ptr(), 2 * frequencies.shape[0], interleaved))
+    return ctypes.byref(_lib.Rotary(frequencies.data_ptr(), _u32(2 * frequencies.shape[0], "rotated width"), interleaved))
 
 
 def _positions(positions, rows: int, device: int) -> int:

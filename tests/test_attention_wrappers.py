@@ -32,3 +32,19 @@ def test_more_entries_than_a_stride_are_refused():
     assert status == _lib.GW_INVALID_ARGUMENT and b"entries" in lib.gw_last_error()
     status = lib.gw_paged_attention_bf16(ctypes.byref(cache), ctypes.byref(batch), P, 2048, 8, 0.1, 0, P, 2048, P, 1 << 40, None)
     assert status == _lib.GW_INVALID_ARGUMENT and b"entries" in lib.gw_last_error()
+
+
+@pytest.mark.parametrize("rows,max_rows", [(-1, 1), (2, -1), ((1 << 32) + 2, 1), (2, (1 << 32) + 1), (1 << 40, 1)])
+def test_row_counts_that_32_bits_do_not_hold_are_refused(rows, max_rows):
+    import gewell_b200 as gw
+    with pytest.raises(gw.GewellInvalidArgument):
+        sequence_batch(torch.zeros((2, 4), dtype=torch.int32), rows, max_rows)
+
+
+def test_strides_that_32_bits_do_not_hold_are_refused():
+    """A page table 2^32 + 4 entries apart (of the meta device: no memory)."""
+    import gewell_b200 as gw
+    far = torch.empty_strided((2, 4), ((1 << 32) + 4, 1), dtype=torch.int32, device="meta")
+    offsets, lengths = torch.zeros(3, dtype=torch.int32, device="meta"), torch.zeros(2, dtype=torch.int32, device="meta")
+    with pytest.raises(gw.GewellInvalidArgument):
+        gw.SequenceBatch(offsets, lengths, far, 2, 1)
