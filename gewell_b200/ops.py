@@ -769,6 +769,11 @@ def _u32(value, name: str) -> int:
     return value
 
 
+def _packed(t: torch.Tensor) -> bool:
+    """Neighbouring elements along the last dimension; a single one has no stride."""
+    return t.stride(-1) == 1 or t.shape[-1] <= 1
+
+
 class KvCache:
     """A paged cache of keys and values in 8 bits over the caller's tensors: E4M3 codes [pages, kv_heads, page_tokens,
     head_dim] (torch.uint8 or torch.float8_e4m3fn) and FP32 scales [pages, kv_heads], contiguous."""
@@ -794,7 +799,7 @@ class SequenceBatch:
 
     def __init__(self, row_offsets: torch.Tensor, context_lengths: torch.Tensor, page_table: torch.Tensor, rows: int, max_rows: int):
         for name, t, dim in (("row_offsets", row_offsets, 1), ("context_lengths", context_lengths, 1), ("page_table", page_table, 2)):
-            if t.dtype != torch.int32 or t.dim() != dim or t.stride(-1) != 1 or t.device != row_offsets.device:
+            if t.dtype != torch.int32 or t.dim() != dim or not _packed(t) or t.device != row_offsets.device:
                 raise _lib.GewellInvalidArgument(f"{name}: int32 with neighbouring elements, all three on one device")
         count = context_lengths.shape[0]
         if row_offsets.shape[0] != count + 1 or page_table.shape[0] != count or page_table.stride(0) < page_table.shape[1]:
@@ -839,7 +844,7 @@ def _head_weight(weight, dim: int, device: int) -> int:
 def _rotary(frequencies, interleaved: bool, device: int):
     if frequencies is None:
         return None
-    if frequencies.dtype is not torch.float32 or frequencies.dim() != 1 or frequencies.stride(0) != 1 or frequencies.get_device() != device:
+    if frequencies.dtype is not torch.float32 or frequencies.dim() != 1 or not _packed(frequencies) or frequencies.get_device() != device:
         raise _lib.GewellInvalidArgument("inverse frequencies are FP32 [width / 2]")
     return ctypes.byref(_lib.Rotary(frequencies.data_ptr(), _u32(2 * frequencies.shape[0], "rotated width"), interleaved))
 
@@ -847,7 +852,7 @@ def _rotary(frequencies, interleaved: bool, device: int):
 def _positions(positions, rows: int, device: int) -> int:
     if positions is None:
         return 0
-    if positions.dtype is not _I32 or positions.dim() != 1 or positions.shape[0] < rows or positions.stride(0) != 1 or positions.get_device() != device:
+    if positions.dtype is not _I32 or positions.dim() != 1 or positions.shape[0] < rows or not _packed(positions) or positions.get_device() != device:
         raise _lib.GewellInvalidArgument("positions are int32 [rows]")
     return positions.data_ptr()
 

@@ -48,3 +48,17 @@ def test_strides_that_32_bits_do_not_hold_are_refused():
     offsets, lengths = torch.zeros(3, dtype=torch.int32, device="meta"), torch.zeros(2, dtype=torch.int32, device="meta")
     with pytest.raises(gw.GewellInvalidArgument):
         gw.SequenceBatch(offsets, lengths, far, 2, 1)
+
+
+def test_a_single_element_has_no_stride():
+    """Views of one element of something wider are as good as any other."""
+    import gewell_b200 as gw
+    i32, wide = torch.int32, torch.arange(12, dtype=torch.int32).reshape(3, 4)
+    offsets = torch.zeros(4, dtype=i32)
+    held = gw.SequenceBatch(offsets, torch.ones(3, dtype=i32), wide[:, 1:2], 3, 1)._struct
+    assert (held.page_table_stride, held.page_table_entries) == (4, 1)
+    gw.SequenceBatch(offsets, torch.ones(3, dtype=i32), torch.empty_strided((3, 1), (1, 0), dtype=i32), 3, 1)
+    gw.SequenceBatch(offsets[:2], torch.ones(8, dtype=i32)[::8], wide[:1], 1, 1)
+    for bad in (wide.t(), wide[:, ::2]):
+        with pytest.raises(gw.GewellInvalidArgument):
+            gw.SequenceBatch(offsets, torch.ones(3, dtype=i32), bad[:3], 3, 1)

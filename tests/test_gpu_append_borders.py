@@ -62,3 +62,14 @@ def test_query_rows_of_no_sequence_stay(gw, given):
         assert (y[rest] == 7.0).all()
         exact = oat.head_norm_rotary(f64(x)[good], None, True, positions.numpy()[good], f.numpy())
         assert (np.abs(f64(y)[good] - exact) <= 2.0 ** -8 * np.abs(exact) + 2.0 ** -19 * np.abs(exact).max(axis=-1, keepdims=True)).all()
+
+
+def test_single_elements_of_wider_tensors(gw):
+    """One row at a position, one pair and one sequence, each a view with another stride."""
+    x = torch.randn((1, 2, 128), generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    position, f = torch.tensor([9, 0, 0, 0], dtype=torch.int32).cuda(), torch.tensor([0.25, 0.0, 0.0], dtype=torch.float32).cuda()
+    got, _ = gw.qk_norm_rotary(x, None, None, None, position[::4], f[::3])
+    want, _ = gw.qk_norm_rotary(x, None, None, None, position[:1], f[:1])
+    exact = oat.head_norm_rotary(f64(x), None, True, np.array([9]), np.array([0.25]))
+    assert torch.equal(got, want)
+    assert (np.abs(f64(got) - exact) <= 2.0 ** -8 * np.abs(exact) + 2.0 ** -19 * np.abs(exact).max(axis=-1, keepdims=True)).all()
