@@ -153,9 +153,9 @@ __device__ __forceinline__ void rotate(const Rotary& r, float* lo, float* hi, co
     for (int e = 0; e < E; ++e) turn(lo[e], hi[e], s[e], c[e]);
   } else if (r.kind == kNeighbours) {
 #pragma unroll
-    for (int e = 0; e < E / 2; ++e) {
-      turn(lo[2 * e], lo[2 * e + 1], s[e], c[e]);
-      turn(hi[2 * e], hi[2 * e + 1], s[E / 2 + e], c[E / 2 + e]);
+    for (int e = 0; e < E / 2; ++e) {                        // 0 times an infinity behind the width would reach its neighbour
+      if (at + 2 * e < r.width) turn(lo[2 * e], lo[2 * e + 1], s[e], c[e]);
+      if (half + at + 2 * e < r.width) turn(hi[2 * e], hi[2 * e + 1], s[E / 2 + e], c[E / 2 + e]);
     }
   } else if (r.kind == kPart) {
     __syncwarp();

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import attention as oat
-from tests.attention_helpers import f64
+from tests.attention_helpers import VALUES, f64
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +73,23 @@ def test_single_elements_of_wider_tensors(gw):
     exact = oat.head_norm_rotary(f64(x), None, True, np.array([9]), np.array([0.25]))
     assert torch.equal(got, want)
     assert (np.abs(f64(got) - exact) <= 2.0 ** -8 * np.abs(exact) + 2.0 ** -19 * np.abs(exact).max(axis=-1, keepdims=True)).all()
+
+
+@pytest.mark.parametrize("dim,width", [(128, 64), (256, 20), (512, 16), (128, 2)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("rows", [1, 3, 30])
+def test_odd_values_behind_the_rotated_width_stay_where_they_are(gw, dim, width, interleaved, rows):
+    """An infinity or NaN among the elements that are not turned changes none of its neighbours."""
+    x = torch.zeros((rows, 1, dim), dtype=torch.bfloat16)
+    x[:, 0, width:] = 3.0
+    x[:, 0, :width] = 1.0
+    x[:, 0, width], x[:, 0, width + 6], x[:, 0, dim - 1] = float("inf"), float("nan"), float("-inf")
+    cache = small_cache(gw, 2, dim, 32)
+    f = torch.ones(width // 2, dtype=torch.float32).cuda()
+    gw.kv_cache_append(cache, batch_of(gw, [0, rows], [rows], [[1]], rows, rows), x.cuda(), x.cuda(), normalize_key=False, normalize_value=False,
+                       frequencies=f, interleaved=interleaved)
+    assert gw.kernel_error() == 0 and float(cache.k_scales[1]) == 2.0 ** -7
+    got = VALUES[cache.k_data[1, 0, :rows].cpu().numpy()] * 2.0 ** -7
+    wanted = np.full((rows, dim - width), 3.0)
+    wanted[:, 0], wanted[:, 6], wanted[:, -1] = 3.5, np.nan, -3.5           # infinities become the largest code
+    np.testing.assert_array_equal(got[:, width:], wanted)
