@@ -8,8 +8,8 @@
 //
 //   y_i = n_i cos a - n_j sin a,  y_j = n_j cos a + n_i sin a,  a = position * f,  n = x * rsqrt(mean(x^2) + eps) * w
 //
-// The angle in turns, position * (f / 2 pi), is formed as the sum of two FP32 numbers, exact to 2^-28 up to position 2^24 (in 64
-// bits beyond), and reduced to [-1/2, 1/2], again as two numbers: in 32 bits position 250000 at f = 1 would be off by 0.01 rad.  Its
+// The angle in turns, position * (f / 2 pi), is formed as the sum of two FP32 numbers, exact to 2^-28 up to position 2^24 (beyond,
+// of two in 64 bits), and reduced to [-1/2, 1/2], again as two numbers: in 32 bits position 250000 at f = 1 would be off by 0.01 rad.  Its
 // sine and cosine are FP32-exact; the hardware's, 2^-21 off, would let a key in ten thousand fall to the next code of E4M3.  They are
 // computed once for all heads that a warp or block takes.  Everything else is FP32 and is rounded once.
 #include <algorithm>
@@ -88,7 +88,7 @@ __device__ __forceinline__ void load_frequencies(const Rotary& r, uint32_t lane_
   }
 }
 
-constexpr double kTurn = 0.15915494309189535;       // 1 / 2 pi
+constexpr double kTurn = 0.15915494309189535, kTurnRest = -9.839338337591243e-18;       // 1 / 2 pi, and what the first lacks of it
 constexpr int kNear = 1 << 24;
 
 __device__ __forceinline__ bool is_near(int position) { return uint32_t(position + kNear) <= 2u * kNear; }
@@ -101,8 +101,12 @@ __device__ __forceinline__ float2 near_turns(float frequency, float position) {
   return make_float2(sum, (part - (sum - of_rest)) + (rest - of_rest));
 }
 __device__ __forceinline__ float2 far_turns(float frequency, int position) {
-  double turns = double(frequency) * kTurn * double(position);
+  // the angle and its turns as the sum of two numbers each: the angle has up to 55 bits, and 2^28 turns leave 25 of 53 behind the point
+  const double angle = double(frequency) * double(position), angle_rest = fma(double(frequency), double(position), -angle);
+  double turns = angle * kTurn;
+  const double rest = fma(angle, kTurn, -turns) + fma(angle, kTurnRest, angle_rest * kTurn);
   turns -= rint(turns);
+  turns += rest;
   const float sum = float(turns);
   return make_float2(sum, float(turns - double(sum)));
 }

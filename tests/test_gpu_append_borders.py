@@ -1,4 +1,7 @@
 """Append to the paged cache and head norms where they are easily wrong."""
+import math
+from fractions import Fraction
+
 import numpy as np
 import pytest
 import torch
@@ -93,3 +96,44 @@ def test_odd_values_behind_the_rotated_width_stay_where_they_are(gw, dim, width,
     wanted = np.full((rows, dim - width), 3.0)
     wanted[:, 0], wanted[:, 6], wanted[:, -1] = 3.5, np.nan, -3.5           # infinities become the largest code
     np.testing.assert_array_equal(got[:, width:], wanted)
+
+
+PI = Fraction(314159265358979323846264338327950288419716939937510582097494459, 10 ** 62)
+
+
+def sine_cosine(position, frequency):
+    """Of position * frequency (FP32), reduced in whole numbers."""
+    angle = position * Fraction(frequency)
+    rest = angle - round(angle / (2 * PI)) * 2 * PI
+    return math.sin(rest), math.cos(rest)
+
+
+@pytest.mark.parametrize("low,high", [(0, 1 << 12), (1 << 19, 1 << 20), ((1 << 24) - 1000, 1 << 24), ((1 << 24) + 1, (1 << 24) + 1000), ((1 << 31) - 1000, (1 << 31) - 1)])
+@pytest.mark.parametrize("dim,width,interleaved", [(128, 128, False), (128, 128, True), (128, 64, False), (512, 512, False)])
+def test_sines_are_as_exact_as_fp32(gw, low, high, dim, width, interleaved):
+    """Pairs that nearly cancel: (sin a, cos a) turned by a has a first element of 2^-9 or less, and the error of the sines is seen next to its
+    rounding to BF16.
+
+    A sine or cosine is off by a unit of 2^-24 (sincospif), the angle's rest by 2^-28 turns, 2^-25 rad, and the correction by it by half a unit:
+    2 * 2^-24 in all, of both elements n of the pair; each of those is rounded once (2^-24), and so is their first product.  The norm's
+    factor is common to both and cancels with them.  What the hardware's sines leave is 2^-21 of each element."""
+    rng = np.random.default_rng(7)
+    rows, pairs = 96, width // 2
+    positions = rng.integers(low, high, rows)
+    positions[0] = high - 1
+    f = np.array([1e4 ** (-i / pairs) for i in range(pairs)], dtype=np.float32)
+    f[::7] = 1.0
+    turned = np.array([[sine_cosine(int(p), float(v)) for v in f] for p in positions])
+    first = np.arange(0, width, 2) if interleaved else np.arange(pairs)
+    second = first + 1 if interleaved else first + pairs
+    x = np.zeros((rows, 1, dim))
+    x[:, 0, first], x[:, 0, second] = turned[..., 0], turned[..., 1]
+    held = torch.from_numpy(x).bfloat16().cuda()
+    got, _ = gw.qk_norm_rotary(held, None, None, None, torch.from_numpy(positions).int().cuda(), torch.from_numpy(f).cuda(), interleaved=interleaved)
+    n = oat.head_norm_rotary(f64(held), None, True, None, None)
+    a, b = n[:, 0, first], n[:, 0, second]
+    exact = a * turned[..., 1] - b * turned[..., 0]
+    error = np.abs(f64(got)[:, 0, first] - exact)
+    bound = 2.0 ** -8 * np.abs(exact) + 4 * 2.0 ** -24 * (np.abs(a) + np.abs(b))
+    assert (np.abs(exact) < 2.0 ** -13).sum() > 50
+    assert (error <= bound).all(), float((error / bound).max())
