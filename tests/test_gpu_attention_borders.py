@@ -92,6 +92,17 @@ def test_scores_far_below_zero_in_pieces_that_some_rows_do_not_see(gw, level, he
     assert_rows(got, q, batch, host, 1.0, window, rows_of=[0, 1, 2, 3, 4, 15, 39, 63, 64, 120, 127, 128, 139, 200, 299], share=0.05)
 
 
+@pytest.mark.parametrize("std,scale", [(12.0, -1.0), (40.0, 1.0), (300.0, 0.5)])
+def test_sharp_scores_within_what_the_arithmetic_allows(gw, std, scale):
+    """The bound stays well below the values: any finite output would not pass."""
+    batch = Batch([(1, 600), (3, 333), (70, 400)], 32, 64)
+    host = random_cache(batch, 2, 128, 65, spread=0.0)
+    q = queries(batch.rows, 8, 128, 66, std)
+    got = gw.paged_attention(to_device(gw, host), batch.device(gw), q, scale)
+    assert gw.kernel_error() == 0
+    assert_rows(got, q, batch, host, scale, rows_of=[0, 1, 2, 35, 69], share=0.25)
+
+
 def test_a_piece_without_pages_takes_no_weight_from_scores_far_below_zero(gw):
     """A whole tile whose page is missing, as a piece of its own."""
     batch = Batch([(1, 300)], 128, 64)
