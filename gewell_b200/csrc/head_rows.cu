@@ -91,7 +91,7 @@ __device__ __forceinline__ void load_frequencies(const Rotary& r, uint32_t lane_
 constexpr double kTurn = 0.15915494309189535, kTurnRest = -9.839338337591243e-18;       // 1 / 2 pi, and what the first lacks of it
 constexpr int kNear = 1 << 24;
 
-__device__ __forceinline__ bool is_near(int position) { return uint32_t(position + kNear) <= 2u * kNear; }
+__device__ __forceinline__ bool is_near(int position) { return uint32_t(position) + kNear <= 2u * kNear; }
 // turns as the sum of two numbers
 __device__ __forceinline__ float2 near_turns(float frequency, float position) {
   constexpr float high = float(kTurn), low = float(kTurn - double(high));
@@ -676,7 +676,7 @@ cudaError_t launch_norm_rotary(NormRotary a, cudaStream_t stream) {
   const uint32_t lanes = a.width <= 64 ? 8 : a.width <= 128 ? 16 : 32, side = 32 / lanes, heads = a.query.heads + a.key.heads;
   // Warps for 24 to an SM, then more heads a warp.  4096 rows of 18 heads of 512: 28 / 29 / 32 us with one / two / four warps a row; 1025 rows
   // of 32 heads of 128: 8.7 / 7.0 / 7.3 us with three / five / seven.
-  a.per_task = side * heads_each((heads + side - 1) / side, a.rows, 148 * 24);
+  a.per_task = side * heads_each((heads + side - 1) / side, a.rows, sm_count() * 24);
   a.tasks = (heads + a.per_task - 1) / a.per_task;
   const uint64_t tasks = uint64_t(a.rows) * a.tasks;
   if (tasks > 0xffffffffull - 64) return cudaErrorInvalidValue;
@@ -703,7 +703,7 @@ cudaError_t launch_append(Append a, cudaStream_t stream) {
   // Few parts of the heads: what a block does before its first item takes 5 us.  4096 rows of 4 heads of 512 in pages of 128, 264 blocks of
   // 512 threads for each part: 26 / 30 / 41 us with one / two / four parts; 9 sequences of up to 700 rows, 8 heads of 128 in pages of 16,
   // 204 blocks of 256: 15 / 14 / 11 / 12 with one / two / three / six.
-  a.each = std::min<uint32_t>(kMostItems, heads_each(2 * heads, bound * blocks, most > 8 * kSide ? 148 : 148 * 4));
+  a.each = std::min<uint32_t>(kMostItems, heads_each(2 * heads, bound * blocks, most > 8 * kSide ? sm_count() : sm_count() * 4));
   const dim3 grid(uint32_t(bound) * blocks, (2 * heads + a.each - 1) / a.each);
   if (most <= 4 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 4, WHOLE>, grid, 128, stream, a);
   if (most <= 8 * kSide) return launch_pdl(kv_append_kernel<LPH, V, 8, WHOLE>, grid, 256, stream, a);

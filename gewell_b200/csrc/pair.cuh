@@ -43,9 +43,6 @@ __device__ __forceinline__ uint32_t cluster_address(const void* local, uint32_t 
 __device__ __forceinline__ void store_cluster(uint32_t cluster_address, const uint32_t* v) {
   asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_address), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
-__device__ __forceinline__ void store_cluster(uint32_t cluster_address, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_address), "f"(v) : "memory");
-}
 // Plain (CTA-scope release) form on purpose: measured on B200, the .release.cluster form of this arrive
 // cost the scale-loader warps about 1000 cycles per stage.  What the arrival publishes is tensor memory
 // written by tcgen05.st, which tcgen05.wait::st and the tcgen05 fences on both sides order.
