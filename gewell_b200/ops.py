@@ -749,8 +749,8 @@ def _allocated(make, device: int, stream, returned: bool):
     """make(), a tensor that a call on `stream` writes first.  Another stream than the current one gets it from its own memory: a block
     that the current stream has freed may still be read there.  What is `returned` the current stream's work may read in turn, so its
     block is not handed out again before that is done."""
-    handle = None if stream is None else _stream(stream)
-    if handle is None or handle == _stream_on(device, None):
+    handle = _stream(stream)
+    if handle == _stream_on(device, None):
         return make()
     if not isinstance(stream, torch.cuda.Stream):
         stream = torch.cuda.ExternalStream(handle, device) if handle > 1 else torch.cuda.default_stream(device)     # 1: the legacy handle of it
@@ -767,11 +767,6 @@ def _u32(value, name: str) -> int:
     if not 0 <= value < 1 << 32:
         raise _lib.GewellInvalidArgument(f"{name}: 0 to 2^32 - 1 are wanted")
     return value
-
-
-def _packed(t: torch.Tensor) -> bool:
-    """Neighbouring elements along the last dimension; a single one has no stride."""
-    return t.stride(-1) == 1 or t.shape[-1] <= 1
 
 
 class KvCache:
@@ -799,7 +794,7 @@ class SequenceBatch:
 
     def __init__(self, row_offsets: torch.Tensor, context_lengths: torch.Tensor, page_table: torch.Tensor, rows: int, max_rows: int):
         for name, t, dim in (("row_offsets", row_offsets, 1), ("context_lengths", context_lengths, 1), ("page_table", page_table, 2)):
-            if t.dtype != torch.int32 or t.dim() != dim or not _packed(t) or t.device != row_offsets.device:
+            if t.dtype != torch.int32 or t.dim() != dim or (t.stride(-1) != 1 and t.shape[-1] > 1) or t.device != row_offsets.device:
                 raise _lib.GewellInvalidArgument(f"{name}: int32 with neighbouring elements, all three on one device")
         count = context_lengths.shape[0]
         if row_offsets.shape[0] != count + 1 or page_table.shape[0] != count or page_table.stride(0) < page_table.shape[1]:
@@ -826,6 +821,8 @@ def _layout(x: torch.Tensor, device: int):
 def _output(x: torch.Tensor, rows: int, heads: int, dim: int, y, device: int, stream):
     """(y, its row stride); a new tensor for None."""
     if y is None:
+        if stream is None:
+            return torch.empty_like(x, memory_format=torch.contiguous_format), heads * dim
         return _allocated(lambda: torch.empty_like(x, memory_format=torch.contiguous_format), device, stream, True), heads * dim
     at = _layout(y, device)
     if at[:3] != (rows, heads, dim):
@@ -844,15 +841,20 @@ def _head_weight(weight, dim: int, device: int) -> int:
 def _rotary(frequencies, interleaved: bool, device: int):
     if frequencies is None:
         return None
-    if frequencies.dtype is not torch.float32 or frequencies.dim() != 1 or not _packed(frequencies) or frequencies.get_device() != device:
+    if frequencies.dtype is not torch.float32 or frequencies.dim() != 1 or frequencies.get_device() != device or (
+            frequencies.stride(0) != 1 and frequencies.shape[0] > 1):
         raise _lib.GewellInvalidArgument("inverse frequencies are FP32 [width / 2]")
-    return ctypes.byref(_lib.Rotary(frequencies.data_ptr(), _u32(2 * frequencies.shape[0], "rotated width"), interleaved))
+    width = 2 * frequencies.shape[0]
+    if width >= 1 << 32:
+        raise _lib.GewellInvalidArgument("inverse frequencies: a width of 32 bits is wanted")
+    return ctypes.byref(_lib.Rotary(frequencies.data_ptr(), width, interleaved))
 
 
 def _positions(positions, rows: int, device: int) -> int:
     if positions is None:
         return 0
-    if positions.dtype is not _I32 or positions.dim() != 1 or positions.shape[0] < rows or not _packed(positions) or positions.get_device() != device:
+    if positions.dtype is not _I32 or positions.dim() != 1 or positions.shape[0] < rows or positions.get_device() != device or (
+            positions.stride(0) != 1 and positions.shape[0] > 1):
         raise _lib.GewellInvalidArgument("positions are int32 [rows]")
     return positions.data_ptr()
 
@@ -919,7 +921,10 @@ def paged_attention(cache: KvCache, batch: SequenceBatch, query: torch.Tensor, s
     lib = _library()
     if scratch is None:
         size = lib.gw_paged_attention_scratch_bytes(cache._ref, batch._ref, heads)
-        scratch = _allocated(lambda: torch.empty(size, dtype=torch.uint8, device=query.device), device, stream, False)
+        if stream is None:
+            scratch = torch.empty(size, dtype=torch.uint8, device=query.device)
+        else:
+            scratch = _allocated(lambda: torch.empty(size, dtype=torch.uint8, device=query.device), device, stream, False)
     elif scratch.dtype is not torch.uint8 or scratch.get_device() != device or not scratch.is_contiguous():
         raise _lib.GewellInvalidArgument("scratch is contiguous uint8 on the cache's device")
     _check(lib.gw_paged_attention_bf16(cache._ref, batch._ref, query.data_ptr(), stride, heads, scale, window, y.data_ptr(), out_stride,
