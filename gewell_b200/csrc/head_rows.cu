@@ -215,11 +215,16 @@ struct NormRotary {
 // Position of a row in its sequence; false: no sequence has it.
 __device__ __forceinline__ bool position_in_batch(const gw_sequences& b, uint32_t row, int& position) {
   uint32_t low = 0, high = b.sequences;                    // the last sequence that starts at or before the row
-  while (low + 1 < high) {
-    const uint32_t middle = (low + high) / 2;
-    if (b.row_offsets[middle] <= int(row)) low = middle; else high = middle;
+  // In a decode step sequence r has row r alone: asked first, as the loads of a search wait for one another.
+  SequenceRows s{0, 0, 0, false};
+  if (row < high) s = sequence_rows(b, row);
+  if (int(row) < s.first || int(row) >= s.first + s.count) {
+    while (low + 1 < high) {
+      const uint32_t middle = (low + high) / 2;
+      if (b.row_offsets[middle] <= int(row)) low = middle; else high = middle;
+    }
+    s = sequence_rows(b, low);
   }
-  const SequenceRows s = sequence_rows(b, low);
   position = s.context - s.count + int(row) - s.first;
   return int(row) >= s.first && int(row) < s.first + s.count;
 }
@@ -252,15 +257,14 @@ __global__ void __launch_bounds__(32 * kNormWarps, V == 1 ? 8 : 6) qk_norm_rotar
   };
   Raw<V> next_lo, next_hi;
   load(first + group, next_lo, next_hi);
+  // on their way during the search, whose loads wait for one another
+  float s[E], c[E];
+  load_frequencies<V, WHOLE>(a.rotary, at, half, inside, c);
+  const int given = a.positions != nullptr ? a.positions[row] : 0;
   int position = 0;
   if (a.batch.sequences && !position_in_batch(a.batch, row, position)) return;
-  if (a.positions != nullptr) position = a.positions[row];
-  float s[E], c[E];
-  {
-    float frequencies[E];
-    load_frequencies<V, WHOLE>(a.rotary, at, half, inside, frequencies);
-    angles<V>(frequencies, position, s, c);
-  }
+  if (a.positions != nullptr) position = given;
+  angles<V>(c, position, s, c);
   const float inverse_width = 1.F / float(a.width);
 #pragma unroll 1
   for (uint32_t at_head = first; at_head < last; at_head += kSide) {
