@@ -296,3 +296,72 @@ def test_a_replayed_graph_reports(gw):
     held.page_table.fill_(-1)
     graph.replay()
     assert gw.kernel_error() == 0xa1000000 and gw.kernel_error() == 0xa1000000 and gw.kernel_error() == 0
+
+
+@pytest.mark.parametrize("window", [0, 70])
+def test_more_sequences_than_threads_of_a_block(gw, window):
+    """The search for a block's first unit goes over the sequences in several rounds."""
+    rng = np.random.default_rng(89)
+    lengths = rng.integers(1, 300, 1500)
+    sequences = [(int(min(rng.integers(0, 3), n)), int(n)) for n in lengths]
+    batch = Batch(sequences, 64, 90)
+    host = random_cache(batch, 1, 128, 91, spread=1.0)
+    q = queries(batch.rows, 4, 128, 92)
+    got = gw.paged_attention(to_device(gw, host), batch.device(gw), q, 0.1, window=window)
+    assert gw.kernel_error() == 0
+    for s in range(1500):
+        if s % 9 and s not in (639, 640, 641, 1279, 1280, 1281, 1499):
+            batch.sequences[s] = (0, 0)                                # not looked at
+    assert_rows(got, q, batch, host, 0.1, window)
+
+
+@pytest.mark.parametrize("dim", [128, 256, 512])
+@pytest.mark.parametrize("group,rows", [(1, 1), (16, 1), (2, 16), (32, 1), (8, 4), (64, 1), (13, 3), (64, 5), (1, 200)])
+@pytest.mark.parametrize("window", [0, 60])
+def test_every_width_of_a_block_with_every_head(gw, dim, group, rows, window):
+    """Scales that are no powers of two, too."""
+    batch = Batch([(rows, max(rows, 300)), (1, 5), (rows, max(rows, 129))], 32, 93)
+    host = random_cache(batch, 2, dim, 94, spread=1.0)
+    for part in host:
+        part[1][:] *= np.random.default_rng(95).uniform(0.5, 2.0, part[1].shape).astype(np.float32)
+    q = queries(batch.rows, 2 * group, dim, 96)
+    got = gw.paged_attention(to_device(gw, host), batch.device(gw), q, dim ** -0.5, window=window)
+    assert gw.kernel_error() == 0
+    assert_rows(got, q, batch, host, dim ** -0.5, window, rows_of=[0, 1, rows - 1, rows // 2])
+
+
+@pytest.mark.parametrize("what", ["query nan", "query infinity", "key", "key scale"])
+@pytest.mark.parametrize("window", [0, 30])
+def test_odd_keys_and_queries_reach_the_rows_that_see_them(gw, what, window):
+    batch = Batch([(60, 200), (3, 150)], 16, 97)
+    host = random_cache(batch, 2, 128, 98)
+    clean = [tuple(a.copy() for a in part) for part in host]
+    q = queries(batch.rows, 8, 128, 99)
+    odd = torch.zeros((batch.rows, 8), dtype=torch.bool)
+    if what == "key":
+        host[0][0][int(batch.table[0, 9]), 1, 6, 17] = 0xff           # token 150
+        odd[[i for i in range(60) if 140 + i >= 150 and (window == 0 or 140 + i - 150 < window)], 4:] = True
+    elif what == "key scale":
+        host[0][1][int(batch.table[0, 9]), 1] = float("nan")           # tokens 144 .. 159
+        odd[[i for i in range(60) if 140 + i >= 144 and (window == 0 or 140 + i - 159 < window)], 4:] = True
+    else:
+        q[20, 3, 50] = float("nan") if what == "query nan" else float("-inf")
+        odd[20, 3] = True
+    got = gw.paged_attention(to_device(gw, host), batch.device(gw), q, 0.1, window=window)
+    assert gw.kernel_error() == 0
+    got = got.cpu()
+    assert torch.equal(torch.isnan(got).any(dim=2), odd) and torch.equal(torch.isnan(got).all(dim=2), odd)
+    # the others against the definition without what is odd; in the place of the odd ones what a clean call gives
+    q = torch.nan_to_num(q, 0.0, 0.0, 0.0)
+    want = gw.paged_attention(to_device(gw, clean), batch.device(gw), q, 0.1, window=window).cpu()
+    got[odd] = want[odd]
+    assert_rows(got, q, batch, clean, 0.1, window, rows_of=[0, 3, 4, 9, 10, 19, 20, 21, 30, 45, 59])
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,rows", [(8, 2, 128, 1), (16, 2, 512, 3), (4, 4, 256, 90)])
+def test_results_in_the_place_of_the_queries(gw, heads, kv_heads, dim, rows):
+    batch = Batch([(rows, 2000), (1, 300), (rows, 700)], 64, 100)
+    cache = to_device(gw, random_cache(batch, kv_heads, dim, 101, garbage=False))
+    held, q = batch.device(gw), queries(batch.rows, heads, dim, 102)
+    want = gw.paged_attention(cache, held, q, dim ** -0.5)
+    assert gw.paged_attention(cache, held, q, dim ** -0.5, y=q) is q and torch.equal(q, want)
