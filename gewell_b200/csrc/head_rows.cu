@@ -233,7 +233,8 @@ constexpr int kNormWarps = 4;
 
 // A warp takes heads of one row, queries and keys in one line, the next head's values on their way meanwhile; the row's angles are
 // computed once.  Bound by HBM: 4096 rows of 18 heads of 512, 151 MB, 29 us (80% of a copy's rate; 27 with the hardware's sines).
-// With a task for each head, and angles in 64 bits, it took 74 us; eight rows, 2 us in a graph.
+// With a task for each head, and angles in 64 bits, it took 74 us; eight rows, 2 us in a graph.  Rotation of a part in halves goes through
+// shared memory, sines for each head: 1025 rows of 32 heads of 128, 9.5 us in a graph, 6.6 as neighbouring pairs.
 template <int LPH, int V, bool WHOLE>
 __global__ void __launch_bounds__(32 * kNormWarps, V == 1 ? 8 : 6) qk_norm_rotary_kernel(NormRotary a) {
   constexpr int E = 4 * V, kSide = 32 / LPH;
@@ -449,7 +450,7 @@ constexpr int kMostItems = 16;         // of a block
 // while an item is normed, and its codes are written while the next one's are.  For every item the last warp of a block sends all
 // blocks the scale that the block's tokens and the page's codes want; the largest is the page's.
 // Bound by issue and by that chain: 4096 rows of 4 heads of 512 in pages of 128, 50 MB, 27 us in a graph (1.9 TB/s), 5 us of it until the
-// first item is loaded; one row of each of 64 sequences, 16 heads of 256, 3.4 us; 12 us for 9 sequences of up to 700 rows, 8 heads of 128.
+// first item is loaded; one row of each of 64 sequences, 16 heads of 256, 3.5 us; 12 us for 9 sequences of up to 700 rows, 8 heads of 128.
 // A block for a page, with the tokens of a page in eight rounds and everything computed twice, took 33.6 us for the first.
 template <int LPH, int V, int W, bool WHOLE>
 __global__ void __launch_bounds__(32 * W, (V == 1 || W == 16 ? 32 : 20) / W) kv_append_kernel(Append a) {

@@ -16,7 +16,8 @@
 // That also takes the running maximum out of the loop.  The reference m of a column only has to keep FP32 sums in range: it is 0
 // at first, and moves to the maximum so far (with the sums rescaled) only when a probability times its value scale exceeds 2^40, or
 // when a column's first tokens all lie below 2^-40.  (Value scales below 2^-64 are taken for 2^-64, so that no probability passes
-// 2^104 unseen.)
+// 2^104 unseen.)  What falls below the codes of a block, 2^-17 of its largest probability and less, is missing in O and not in the sum: 31
+// such tokens are 2^-12 of that one, next to a result that is rounded to 2^-8.
 //
 //   warp 0      TMA: chunks of [128 tokens x 128 bytes] into a ring for K and one for V, page by page; the pages' scales, and what the softmax
 //               warps need to know of an item
@@ -38,12 +39,13 @@
 // while the one before, of V, was still open, and a parity cannot tell that from the phase being complete.
 // Every wait is bounded; a role that gives up reports it, all leave, and tensor memory is released.
 //
-// Measured (a call, join included).  24 rows on up to 32,000 tokens, 4 KV heads of 512: 270 us, the rate of a copy from HBM.  One row on
+// Measured (calls back to back, join included).  24 rows on up to 32,000 tokens, 4 KV heads of 512: 264 to 276 us from one GPU to another,
+// the rate of a copy from HBM.  One row on
 // 32,749 tokens, 2 heads of 512: 27 us against 10 us of HBM, most of it the first tile's way and the second launch.  64 rows in windows of 1024,
-// 16 heads of 256: 108 us against 81.  Drafts and prompts are bound by the softmax warps, 2400 cycles a tile at 32 columns, 3400 to 4100
+// 16 heads of 256: 104 to 112 us against 81.  Drafts and prompts are bound by the softmax warps, 2400 cycles a tile at 32 columns, 3400 to 4100
 // at 64 (about 400 instructions a warp; their chain of latencies, four warps a scheduler, does not fill the issue slots): 80 rows on up to 9000
-// tokens, 8 heads of 128, 64 us; 2048 rows in windows of 1024, 8 heads of 256, 104 us; 4096 rows on 16,384 tokens, 2 heads of 512, 2200 us,
-// 870 TFLOP/s, where the 64 products of a tile also read 393 KB of shared memory, 3100 cycles.
+// tokens, 8 heads of 128, 63 us; 2048 rows in windows of 1024, 8 heads of 256, 104 us; 4096 rows on 16,384 tokens, 2 heads of 512, 2240 to
+// 2270 us, 850 TFLOP/s (1970 us in a few passes, before the power limit lowers the clock), where the 64 products of a tile also read 393 KB of shared memory, 3100 cycles.
 #include <algorithm>
 #include <atomic>
 #include <string>
@@ -500,7 +502,7 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
   find_start<kThreads>(a, s);                                    // ends with __syncthreads()
   ptx::tc_fence_after_sync();
   const uint32_t tmem = s.tensor_memory;
-  // Waiting threads sleep: polls took the issue slots of the softmax warps (4096 rows on 16384 tokens 2205 -> 2105 us).
+  // Waiting threads sleep: polls took the issue slots of the softmax warps (4096 rows on 16,384 tokens 2312 -> 2184 us on one GPU).
   // What a role gave up on, reported at the end.  A thread whose wait ran out waits no more, but goes on to the end; the roles of one
   // warp or thread leave at once.
   uint32_t error = 0;

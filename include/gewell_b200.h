@@ -356,7 +356,7 @@ typedef struct gw_head_rows {
 } gw_head_rows;
 
 /* Rotation by position: pair i of the first `width` elements of a head turns by position * inverse_frequencies[i]
- * (FP32 [width / 2] on the device; zeros leave pairs as they are).  Pairs are (i, i + width / 2), or (2 i, 2 i + 1) where
+ * (FP32 [width / 2] on the device; zeros leave finite pairs as they are).  Pairs are (i, i + width / 2), or (2 i, 2 i + 1) where
  * `interleaved`; elements behind `width` stay.  The angle is exact up to the rounding of its remainder, also far into a context. */
 typedef struct gw_rotary {
   const float* inverse_frequencies;
@@ -367,15 +367,15 @@ typedef struct gw_rotary {
 /* Norm of every query and key head and their rotation, one launch: y = rotate(x * rsqrt(mean(x^2) + epsilon) * weight) in
  * FP32, rounded to BF16 once.  (The norms that Executor::project_qkv of the reference ends with, models/gemma4/31b/sm120/
  * executor.cuh:1218-1247, and the rotation behind them.)  key NULL: queries alone; rotary NULL: no rotation.  positions: int32
- * [rows], at least 0.  head_dim divisible by 8, at most 512.  output may be input (same stride).  rows == 0 is a no-op. */
+ * [rows], at least 0.  head_dim divisible by 8, beyond 256 by 16, at most 512.  output may be input (same stride).  rows == 0 is a no-op. */
 gw_status gw_qk_norm_rotary_bf16(const gw_head_rows* query, const gw_head_rows* key, uint32_t rows, uint32_t head_dim,
                                  const int32_t* positions, const gw_rotary* rotary, float epsilon, void* stream);
 
 /* A paged cache of keys and values in 8 bits, in the caller's memory: E4M3 codes [pages, kv_heads, page_tokens, head_dim]
  * (16-byte aligned) and an FP32 scale for every page and head [pages, kv_heads], for keys and for values.  What a code stands for
- * is code * scale; attention takes value scales below 2^-64 for 2^-64, and none may be below 0.  Queries that see a token of a page
- * whose value scale is NaN, infinite or below 0 get NaN.  page_tokens 16, 32, 64 or 128;
- * head_dim 128, 256 or 512; pages * kv_heads * page_tokens below 2^31. */
+ * is code * scale; attention takes value scales below 2^-64 for 2^-64, may lose small probabilities above 2^60, and none may be
+ * below 0.  Queries that see a token of a page whose value scale is NaN, infinite or below 0 get NaN.  page_tokens 16, 32, 64 or
+ * 128; head_dim 128, 256 or 512; pages * kv_heads * page_tokens below 2^31. */
 typedef struct gw_kv_cache {
   void* k_data;
   void* v_data;
@@ -406,7 +406,7 @@ typedef struct gw_sequences {
  * again to the new scale; a page that the call begins at its first slot starts anew.  Codes round to nearest even; infinities become
  * the largest code.  Slots behind a page's last token are not touched.  A page belongs to one sequence of the step (pages that
  * several sequences share may only be full ones).
- * query (or NULL) is normed and rotated into its output as by gw_qk_norm_rotary_bf16.  positions (or NULL): int32 [rows] for the
+ * query (or NULL) is normed and rotated into its output as by gw_qk_norm_rotary_bf16 (rows of no sequence are left as they are).  positions (or NULL): int32 [rows] for the
  * rotation in place of the positions in the sequences.  rotary NULL: no rotation. */
 gw_status gw_kv_cache_append(const gw_kv_cache* cache, const gw_sequences* batch, const gw_head_rows* key,
                              const gw_head_rows* value, const gw_head_rows* query, const int32_t* positions,
@@ -417,7 +417,8 @@ gw_status gw_kv_cache_append(const gw_kv_cache* cache, const gw_sequences* batch
  * output = sum softmax(scale * q . k) v over what it sees, BF16; a row that sees nothing is 0.  Scores, softmax and sums in FP32;
  * products of the codes themselves: queries and probabilities enter as two E4M3 parts with a shared power of two for every 32
  * elements, which hold 8 significant bits.  A NaN in a cached value reaches the queries that see it and no others (of those, all
- * elements where more than 30 groups of 16 of the tokens that only some queries of a tile see hold NaN).  query and output: rows of [heads, head_dim] with strides in elements, 16-byte aligned, strides divisible by 8.
+ * elements where more than 30 groups of 16 of the tokens that only some queries of a tile see hold NaN).  query and output: rows of
+ * [heads, head_dim] with strides in elements, 16-byte aligned, strides divisible by 8; output may be query (same stride).
  * heads / kv_heads at most 64.  scratch: gw_paged_attention_scratch_bytes bytes, 256-byte aligned (not kept between calls). */
 size_t gw_paged_attention_scratch_bytes(const gw_kv_cache* cache, const gw_sequences* batch, uint32_t heads);
 gw_status gw_paged_attention_bf16(const gw_kv_cache* cache, const gw_sequences* batch, const void* query_bf16,
