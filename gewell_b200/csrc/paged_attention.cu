@@ -40,12 +40,12 @@
 // Every wait is bounded; a role that gives up reports it, all leave, and tensor memory is released.
 //
 // Measured (calls back to back, join included).  24 rows on up to 32,000 tokens, 4 KV heads of 512: 264 to 276 us from one GPU to another,
-// the rate of a copy from HBM.  One row on
-// 32,749 tokens, 2 heads of 512: 27 us against 10 us of HBM, most of it the first tile's way and the second launch.  64 rows in windows of 1024,
-// 16 heads of 256: 104 to 112 us against 81.  Drafts and prompts are bound by the softmax warps, 2400 cycles a tile at 32 columns, 3400 to 4100
+// the rate of a copy from HBM.  One row on 32,749 tokens, 2 heads of 512: 27 us against 10 us of HBM, most of it the first tile's way and the
+// second launch.  64 rows in windows of 1024, 16 heads of 256: 104 to 112 us against 81.  Drafts and prompts are bound by the softmax warps, 2400 cycles a tile at 32 columns, 3400 to 4100
 // at 64 (about 400 instructions a warp; their chain of latencies, four warps a scheduler, does not fill the issue slots): 80 rows on up to 9000
 // tokens, 8 heads of 128, 63 us; 2048 rows in windows of 1024, 8 heads of 256, 104 us; 4096 rows on 16,384 tokens, 2 heads of 512, 2240 to
-// 2270 us, 850 TFLOP/s (1970 us in a few passes, before the power limit lowers the clock), where the 64 products of a tile also read 393 KB of shared memory, 3100 cycles.
+// 2270 us, 850 TFLOP/s (1970 us in a few passes, before the power limit lowers the clock), where the 64 products of a tile also read 393 KB
+// of shared memory, 3100 cycles.
 #include <algorithm>
 #include <atomic>
 #include <string>
@@ -590,8 +590,10 @@ __global__ void __launch_bounds__(Layout<D, N>::kThreads, 1) paged_attention_ker
           else if (entry != -2) atomicCAS(&g_attention_error, 0u, 0xa1000000u | (w.sequence & 0xffffffu));
           bring(&k_map, row, issued[0], KEYS, s.k_full, s.k_empty, k_ring);
           // A value scale that is no finite number, or below 0, makes the scores of its page NaN: the softmax warps mask what a query does
-          // not see, and 0 times the scale itself would reach the others.  Asked here, where it costs nothing (there 16 sequences of drafts took 69.7 us instead of 62.8).
-          if (uint32_t(entry) < a.cache.pages && !(scales.y >= 0.F && scales.y <= 3.4028234e38F)) scales = make_float2(__int_as_float(0x7fc00000), 1.F);
+          // not see, and 0 times the scale itself would reach the others.  Asked here, where it costs nothing (there 16 sequences of drafts
+          // took 69.7 us instead of 62.8).
+          if (uint32_t(entry) < a.cache.pages && !(scales.y >= 0.F && scales.y <= 3.4028234e38F))
+            scales = make_float2(__int_as_float(0x7fc00000), 1.F);
           if (lane < boxes) s.scales[tile_count % kScaleTiles][lane] = scales;
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive(&s.scales_full[tile_count % kScaleTiles]);

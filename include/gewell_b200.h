@@ -406,7 +406,8 @@ typedef struct gw_sequences {
  * again to the new scale; a page that the call begins at its first slot starts anew.  Codes round to nearest even; infinities become
  * the largest code.  Slots behind a page's last token are not touched.  A page belongs to one sequence of the step (pages that
  * several sequences share may only be full ones).
- * query (or NULL) is normed and rotated into its output as by gw_qk_norm_rotary_bf16 (rows of no sequence are left as they are).  positions (or NULL): int32 [rows] for the
+ * query (or NULL) is normed and rotated into its output as by gw_qk_norm_rotary_bf16; rows of no sequence are left as they are.
+ * positions (or NULL): int32 [rows] for the
  * rotation in place of the positions in the sequences.  rotary NULL: no rotation. */
 gw_status gw_kv_cache_append(const gw_kv_cache* cache, const gw_sequences* batch, const gw_head_rows* key,
                              const gw_head_rows* value, const gw_head_rows* query, const int32_t* positions,
